@@ -281,6 +281,77 @@ int cq_silu_mul_full(const void* gate_f16, const void* up_f16, void* out_f16, lo
                      cq_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * 4-bit KV cache (the reference keeps fp16 keys and values, llama/modeling_llama_quant.py:371-419).
+ * A row is one slot of one KV head: D codes of 4 bits (the even column of a byte in its low half) and
+ * for every `group` columns a pair (scale, minimum) fp16; a column stands for scale * code + minimum.
+ *   minimum = min x, scale = fp16((max x - minimum) / 15), code = rint((x - minimum) / scale) in 0..15
+ * (0 where the scale is 0; a group with an infinite or NaN column is NaN as a whole).
+ * Codes are (sequences, n_kv_heads, slots, D / 2) bytes, scales (sequences, n_kv_heads, slots,
+ * D / group, 2) fp16, all 16-byte aligned and contiguous.  head_dim 64 or 128, group 32 or 64, slots a
+ * multiple of 32.  Calls that write the cache or its workspace must not overlap other calls on it.
+ * ---------------------------------------------------------------------- */
+typedef struct cq_kv4 {
+  int32_t sequences, n_kv_heads, slots, head_dim, group;
+  void *k_codes, *k_scales, *v_codes, *v_scales;
+} cq_kv4;
+/* Whether the fields describe a cache that the calls below take. */
+int cq_kv4_check(const cq_kv4* cache);
+/* `tokens` new rows per sequence: k, v (sequences * tokens, KV, D) fp16 go into the slots first[s] + i (device int64; rows
+ * whose slot lies outside the cache are left out).  With tables (table_rows, D / 2) q (sequences * tokens, n_heads, D) and k
+ * are rotated at positions[t] first, as by cq_rope_cache, each product and sum rounded, then to fp16; q goes to q_out (may be
+ * q itself; n_heads 0: no queries).  A token whose position lies outside the tables is not rotated and its row not written.
+ * cos_table NULL: nothing is rotated. */
+int cq_kv4_write(const cq_kv4* cache, const void* q_f16, void* q_out_f16, const void* k_f16, const void* v_f16,
+                 const float* cos_table, const float* sin_table, const long long* positions, int table_rows,
+                 const long long* first, int tokens, int n_heads, cq_stream_t stream);
+/* The values of the slots first[s] .. first[s] + count - 1: k, v (sequences, count, KV, D) fp16, rounded once; zeros outside
+ * the cache. */
+int cq_kv4_read(const cq_kv4* cache, const long long* first, int count, void* k_f16, void* v_f16, cq_stream_t stream);
+/* Attention of one query per sequence: out (sequences, n_heads, D) = softmax(scale * q . k_j) . v_j over the visible slots
+ * j < n = length[s] (device int64, bounded by the cache): all of them (window 0), or those with j < sinks or j >= n - window.
+ * Nothing visible: zeros.  weights, weights_out (sequences, KV, slots) fp32, both or neither, possibly the same:
+ * weights_out = weights + the sum over the head's queries of their softmax weights for j < n, and 0 from n on.
+ * workspace: device memory of cq_kv4_attend_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls that can
+ * overlap. */
+size_t cq_kv4_attend_workspace_bytes(const cq_kv4* cache, int n_heads, int with_weights);
+int cq_kv4_attend(const cq_kv4* cache, const void* q_f16, const long long* length, void* out_f16, int n_heads, int window,
+                  int sinks, float scale, const float* weights, float* weights_out, void* workspace, cq_stream_t stream);
+/* One decode step: cq_kv4_write of one token per sequence at slot length[s], then cq_kv4_attend over n = length[s] + 1 slots
+ * (q is not changed; the new slot's weight starts at 0; the caller counts length up). */
+int cq_kv4_step(const cq_kv4* cache, const void* q_f16, const void* k_f16, const void* v_f16, const float* cos_table,
+                const float* sin_table, const long long* positions, int table_rows, const long long* length, void* out_f16,
+                int n_heads, int window, int sinks, float scale, const float* weights, float* weights_out, void* workspace,
+                cq_stream_t stream);
+/* Thins the cache out to `keep` slots a head: of the n = length[s] slots the first `sinks`, the last `recent` and of those
+ * between the ones with the largest weights (sequences, KV, from->slots) (of equal ones the lowest slot, NaN above all) stay,
+ * in their order; all of them where n <= keep.  Their rows go to the first slots of `to` (zeros up to `keep`), which has the
+ * same shape up to its slots, and is `from` itself or shares no memory with it; their numbers to kept (sequences, KV, keep)
+ * int32 (-1 behind them), their weights to weights_out (sequences, KV, keep) (0 behind them), min(n, keep) to length_out.
+ * workspace: only where to is from, cq_kv4_evict_workspace_bytes(from, keep) bytes, 16-byte aligned. */
+size_t cq_kv4_evict_workspace_bytes(const cq_kv4* cache, int keep);
+int cq_kv4_evict(const cq_kv4* from, const cq_kv4* to, const float* weights, float* weights_out, const long long* length,
+                 long long* length_out, int keep, int sinks, int recent, int* kept, void* workspace, cq_stream_t stream);
+
+/* Attention of prompts: q (sequences, queries, n_heads, D), k and v (sequences, keys, n_kv_heads, D) fp16 with the given
+ * strides in elements (the columns of a head are contiguous; addresses and strides multiples of 16 bytes).  Query i stands at
+ * position p = i + keys - queries and sees the keys j <= p with j < lengths[s] (device int64; NULL: keys), with a window only
+ * those with j < sinks or j > p - window.  out (sequences, queries, n_heads, D) contiguous, lse (sequences, n_heads, queries)
+ * fp32 = ln of the sum of exp(scale * q . k_j).  A row at or beyond its sequence's length, or that sees no key: zeros and
+ * -infinity.  head_dim 64 or 128. */
+typedef struct cq_prompt {
+  int32_t sequences, queries, keys, n_heads, n_kv_heads, head_dim, window, sinks;
+  int64_t q_strides[3], k_strides[3], v_strides[3];      /* sequence, token, head */
+  float scale;
+} cq_prompt;
+int cq_attn_prefill(const cq_prompt* shape, const void* q_f16, const void* k_f16, const void* v_f16, const long long* lengths,
+                    void* out_f16, float* lse, cq_stream_t stream);
+/* The weight that each key received from the last `observe` positions of its sequence (of those that are among the queries):
+ * weights (sequences, n_kv_heads, keys) fp32 = sum over them and the head's queries of exp(scale * q . k_j - lse); 0 where no
+ * such query sees the key. */
+int cq_attn_prefill_weights(const cq_prompt* shape, const void* q_f16, const void* k_f16, const float* lse,
+                            const long long* lengths, int observe, float* weights, cq_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Tile-layout prepared layer: the format of the tcgen05 (UMMA + tensor memory) kernels.
  * 128-row tiles; a granule is 128 rows x 128 compact columns; cherry columns travel in the same
  * stream as fp16 items of 16 columns.  Same role as cq_layer above, different kernel family.

@@ -20,7 +20,8 @@ ROOT = os.path.dirname(HERE)
 
 LIB = os.path.join(HERE, "libcherryq.so")
 CUDA_SOURCES = ["cq_api.cu", "cq_layout.cu", "cq_matvec.cu", "cq_rowvec.cu", "cq_pack.cu", "cq_fakequant.cu", "cq_legacy_f32.cu",
-                "cq_tile_layout.cu", "cq_prefill.cu", "cq_model_ops.cu", "cq_attn.cu", "cq_peer.cu"]
+                "cq_tile_layout.cu", "cq_prefill.cu", "cq_model_ops.cu", "cq_attn.cu", "cq_peer.cu", "cq_kv4.cu", "cq_kv4_attn.cu",
+                "cq_attn_prompt.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "--shared", "-Xcompiler", "-fPIC", "-Xptxas", "-v", "--fmad=true",
@@ -48,6 +49,7 @@ def cuda_sources():
 def build_lib(force: bool = False, verbose: bool = False) -> str:
     srcs = cuda_sources()
     deps = srcs + [os.path.join(CSRC, "cq_common.cuh"), os.path.join(CSRC, "cq_tile.cuh"), os.path.join(CSRC, "cq_attn.cuh"),
+                   os.path.join(CSRC, "cq_kv4.cuh"),
                    os.path.join(ROOT, "include", "cherryq.h")]
     if not force and _newer(LIB, deps):
         return LIB
@@ -74,9 +76,9 @@ def build_ext(force: bool = False, verbose: bool = False) -> str:
     import torch
     from torch.utils import cpp_extension as ce
 
-    src = os.path.join(CSRC, "quant_cuda_ext.cpp")
+    srcs = [os.path.join(CSRC, "quant_cuda_ext.cpp"), os.path.join(CSRC, "kv4_ext.cpp")]
     out = ext_path()
-    if not force and _newer(out, [src, os.path.join(ROOT, "include", "cherryq.h")]) and os.path.exists(LIB):
+    if not force and _newer(out, srcs + [os.path.join(CSRC, "kv4_ext.h"), os.path.join(ROOT, "include", "cherryq.h")]) and os.path.exists(LIB):
         return out
     build_lib(force=False, verbose=verbose)
     inc = ce.include_paths() + [sysconfig.get_paths()["include"], "/usr/local/cuda/include",
@@ -85,7 +87,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> str:
     cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-DTORCH_EXTENSION_NAME=quant_cuda",
            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     cmd += [f"-I{p}" for p in inc]
-    cmd += [src, "-o", out, f"-L{HERE}", "-lcherryq", f"-L{tlib}", "-ltorch", "-ltorch_cpu", "-lc10",
+    cmd += srcs + ["-o", out, f"-L{HERE}", "-lcherryq", f"-L{tlib}", "-ltorch", "-ltorch_cpu", "-lc10",
             "-ltorch_python", "-lc10_cuda", "-ltorch_cuda",
             "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"]
     res = subprocess.run(cmd, capture_output=True, text=True)

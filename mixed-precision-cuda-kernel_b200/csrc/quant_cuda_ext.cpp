@@ -28,6 +28,7 @@
 #include <vector>
 
 #include "cherryq.h"
+#include "kv4_ext.h"
 
 namespace {
 
@@ -900,6 +901,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("silu_mul", &silu_mul, "silu(gate) * up", py::arg("gate"), py::arg("up"), py::arg("full") = false);
   m.def("attn_decode_step", &attn_decode_step, "rotary embedding, KV cache write and attention of a decode step");
   m.def("attn_decode", &attn_decode, "single-query attention over the KV cache");
+  register_kv4(m);
   m.def("poll", []() { check_status(cq_poll(current_stream()), "poll"); });
   m.def("device_timed_out", &device_timed_out);
   m.def("row_layers_matvec", &row_layers_matvec, "one launch for row-tile layers sharing an activation row");
