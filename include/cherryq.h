@@ -313,7 +313,7 @@ int cq_kv4_read(const cq_kv4* cache, const long long* first, int count, void* k_
  * weights_out = weights + the sum over the head's queries of their softmax weights for j < n, and 0 from n on.
  * workspace: device memory of cq_kv4_attend_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls that can
  * overlap. */
-size_t cq_kv4_attend_workspace_bytes(const cq_kv4* cache, int n_heads, int with_weights);
+size_t cq_kv4_attend_workspace_bytes(const cq_kv4* cache, int n_heads, int window, int sinks, int with_weights);
 int cq_kv4_attend(const cq_kv4* cache, const void* q_f16, const long long* length, void* out_f16, int n_heads, int window,
                   int sinks, float scale, const float* weights, float* weights_out, void* workspace, cq_stream_t stream);
 /* One decode step: cq_kv4_write of one token per sequence at slot length[s], then cq_kv4_attend over n = length[s] + 1 slots

@@ -20,10 +20,10 @@
 //     query (for the codes in the upper half of a byte) leaves fp16;
 //   * a warp takes 32 slots a turn from a ring of its own in shared memory that cp.async fills (two turns), and keeps its own
 //     running maximum, sum and weighted values; nothing waits for another warp until the end;
-//   * several CTAs share a KV head's slots as one cluster, and meet in distributed shared memory: no partial results in
-//     global memory, no counters, nothing that two calls on one cache could confuse.
+//   * several CTAs share a KV head's slots.  Where clusters of them fill the chip they meet in distributed shared memory, else
+//     their sums go to the workspace and a small kernel joins them: no counters, nothing that two calls on one cache could confuse.
 #include <algorithm>
-#include <cstdlib>
+#include <cmath>
 #include <type_traits>
 
 #include "cq_kv4.cuh"
@@ -36,7 +36,7 @@ constexpr int AT_SLOTS = 32;                 // slots of a turn
 constexpr int AT_SM_WARPS = 16;              // warps an SM holds (128 registers a thread)
 constexpr int AT_STAGES = 2;
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LIFT = 15.f;                 // weights are 2^15 times the exponentials: fp16 then reaches down to 2^-39 of the largest
+constexpr float HEADROOM = 8.f, LIFT = 7.f;  // weights are 2^7 times the exponentials, at most 2^15, and fp16 reaches down to 2^-31 of them
 
 __device__ __forceinline__ int held(const long long* length, int b, int more, int slots) {
   const long long n = length[b];
@@ -77,6 +77,12 @@ __device__ __forceinline__ uint32_t hadd2(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// (x & MASK) | y in one instruction
+template <uint32_t MASK> __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t y) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "n"(MASK), "r"(y));
   return d;
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t at) {
@@ -142,7 +148,7 @@ struct NewRow {
 template <int D, int NG, int WARPS, bool STEP, bool WEIGHTS>
 __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_kernel(
     const __half* __restrict__ q, const cq_kv4 cache, const NewRow fresh, const long long* __restrict__ length, __half* __restrict__ out,
-    float* __restrict__ scores, float2* __restrict__ stats, int H, int chunks, int window, int sinks, float scale) {
+    float* __restrict__ scores, float2* __restrict__ stats, float* __restrict__ part, int H, int chunks, int window, int sinks, float scale) {
   using T = Turn<D, NG>;
   constexpr int THREADS = WARPS * 32, GROUP = D / NG, NW = D / 32, WG = GROUP / 32;     // words of a key per lane, of a group
   constexpr int VW = D / 64, LANES = D / 16;                                            // words of a value per lane; lanes of a row
@@ -153,14 +159,16 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
   __shared__ float s_m[WARPS][AT_HEADS], s_l[WARPS][AT_HEADS];
   __shared__ __align__(16) float s_part[AT_HEADS][D];
   __shared__ float s_pm[AT_HEADS], s_pl[AT_HEADS];
+  __shared__ uint32_t s_const[4];
   __shared__ __align__(16) uint32_t s_row[2][D / 8], s_pairs[2][NG];                    // the new row: codes and scales of key, value
   const int kvh = blockIdx.y / chunks, chunk = blockIdx.y - kvh * chunks, b = blockIdx.z;
-  const int split = blockIdx.x, nsplit = gridDim.x;        // (a cluster is the CTAs of one row of the grid)
+  const int split = blockIdx.x, nsplit = gridDim.x;        // (a cluster, where there is one, is the CTAs of one row of the grid)
   const int G = H / cache.n_kv_heads, heads = min(AT_HEADS, G - chunk * AT_HEADS);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g8 = lane >> 2, t4 = lane & 3;
   const size_t head0 = (size_t)b * H + (size_t)kvh * G + chunk * AT_HEADS, row0 = ((size_t)b * cache.n_kv_heads + kvh) * cache.slots;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Visible vis(held(length, b, STEP ? 1 : 0, cache.slots), window, sinks);
+  if (tid < 3) s_const[tid] = tid == 0 ? 0x64006400u : (tid == 1 ? 0x2C002C00u : 0xD400D400u);
 
   const uint32_t my_ring = (uint32_t)__cvta_generic_to_shared(ring) + warp * (AT_STAGES * T::BYTES);
   const int stride = nsplit * WARPS;
@@ -184,8 +192,8 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   int v = split * WARPS + warp;
-  fetch(v, 0);
-  fetch(v + stride, 1);
+#pragma unroll
+  for (int i = 0; i < AT_STAGES; ++i) fetch(v + i * stride, i);
 
   // queries: rotated, scaled by a power of two, to shared memory; D / 16 lanes a head
   const long long pos = STEP && fresh.cos_t ? fresh.positions[b] : 0;
@@ -236,6 +244,11 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
   }
   __syncthreads();
 
+  // Numbers of the values' conversion: 1024 (a code in the lowest bits adds itself), 1 / 16 and -64.  Read back from shared
+  // memory because the compiler, if it knows them, makes two instructions of one, an immediate in each.
+  const uint32_t consts = (uint32_t)__cvta_generic_to_shared(s_const);
+  const uint32_t magic = lds32(consts), sixteenth = lds32(consts + 4), minus64 = lds32(consts + 8);
+
   // B operands of the first product: head g8; word i holds columns 32 i + 8 t4 .. + 7
   uint32_t qb[NW][4], qs[2];
   float sums[NG] = {};
@@ -245,10 +258,10 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
     const uint32_t h[4] = {w.x, w.y, w.z, w.w};            // columns (0 1) (2 3) (4 5) (6 7)
     qb[i][0] = __byte_perm(h[0], h[2], 0x5410);            // 0, 4
     qb[i][1] = __byte_perm(h[1], h[3], 0x5410);            // 2, 6
-    const __half2 sixteenth = __float2half2_rn(0.0625f);
-    __half2 odd = __hmul2(__halves2half2(__ushort_as_half(h[0] >> 16), __ushort_as_half(h[2] >> 16)), sixteenth);
+    const __half2 part16 = __float2half2_rn(0.0625f);
+    __half2 odd = __hmul2(__halves2half2(__ushort_as_half(h[0] >> 16), __ushort_as_half(h[2] >> 16)), part16);
     qb[i][2] = *reinterpret_cast<uint32_t*>(&odd);         // 1, 5
-    odd = __hmul2(__halves2half2(__ushort_as_half(h[1] >> 16), __ushort_as_half(h[3] >> 16)), sixteenth);
+    odd = __hmul2(__halves2half2(__ushort_as_half(h[1] >> 16), __ushort_as_half(h[3] >> 16)), part16);
     qb[i][3] = *reinterpret_cast<uint32_t*>(&odd);         // 3, 7
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -272,15 +285,15 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
   }
   const float unit[2] = {s_unit[2 * t4] * scale * LOG2E, s_unit[2 * t4 + 1] * scale * LOG2E};      // heads 2 t4, 2 t4 + 1
 
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {}, lifted[2] = {-LIFT, -LIFT};
   float o[4 * VW][4] = {};                   // MMA j: rows g8, g8 + 8 are the columns (16 or 8) g8 + 2 j, + 1; heads 2 t4, + 1
   // Where this lane's words lie in a turn.  (A row's bytes start at a multiple of its length, so that the turned order of its
   // pieces is an exclusive or with the address; what is added beyond is a constant of the instruction.)
   constexpr int R = T::ROW;
   const int row_k = T::slot(g8 >> 1, g8 & 1), row_v = T::slot(t4, 0), row_step = T::slot(0, 1);
   const uint32_t off_k = T::piece(row_k, 0) + 4 * t4;
-  const uint32_t off_v[2] = {T::CODES + (D == 128 ? T::piece(row_v, g8 >> 1) + 8 * (g8 & 1) : T::piece(row_v, g8 >> 2) + 4 * (g8 & 3)),
-                             T::CODES + (D == 128 ? T::piece(row_v + row_step, g8 >> 1) + 8 * (g8 & 1) : T::piece(row_v + row_step, g8 >> 2) + 4 * (g8 & 3))};
+  const int word_v = D == 128 ? 8 * (g8 & 1) : 4 * (g8 & 3), piece_v = g8 / (D == 128 ? 2 : 4);
+  const uint32_t off_v[2] = {(uint32_t)(T::CODES + T::piece(row_v, piece_v) + word_v), (uint32_t)(T::CODES + T::piece(row_v + row_step, piece_v) + word_v)};
   const uint32_t off_ks = 2 * T::CODES + row_k * (4 * NG), off_vs = 2 * T::CODES + T::SCALES + (row_v * NG + g8 * (D / 8) / GROUP) * 4;
   auto take = [&](uint32_t at, int base, auto all) {
     constexpr bool ALL = decltype(all)::value;             // every slot of the turn is visible
@@ -323,26 +336,28 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
         else if (WEIGHTS && 2 * t4 + (e & 1) < heads) scores[(head0 + 2 * t4 + (e & 1)) * cache.slots + slot] = s[u][e];
       }
     }
-    // a whole number at or above the maximum, so that most turns leave it as it is and sums are rescaled exactly
-    float ref[2], keep[2];
+    // The reference of the weights is a whole number, so that sums are rescaled exactly, and is only raised when a score is 2^8
+    // above it: the lanes' own maxima are enough to see that none is.
+    float top[2];
+    bool above = false;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float top = fmaxf(fmaxf(s[0][e], s[0][e + 2]), fmaxf(s[1][e], s[1][e + 2]));
-#pragma unroll
-      for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      top = fmaxf(m[e], ceilf(top));
-      ref[e] = top == -INFINITY ? 0.f : top;
-      keep[e] = ex2(m[e] - ref[e]);
-      m[e] = top;
+      top[e] = fmaxf(fmaxf(s[0][e], s[0][e + 2]), fmaxf(s[1][e], s[1][e + 2]));
+      above |= top[e] > m[e] + HEADROOM;
     }
-    if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+    if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        l[e] *= keep[e];
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], d));
+        const float now = fmaxf(m[e], ceilf(top[e])), keep = ex2(m[e] - (now == -INFINITY ? 0.f : now));
+        m[e] = now;
+        lifted[e] = (now == -INFINITY ? 0.f : now) - LIFT;
+        l[e] *= keep;
 #pragma unroll
         for (int j = 0; j < 4 * VW; ++j) {
-          o[j][e] *= keep[e];
-          o[j][e + 2] *= keep[e];
+          o[j][e] *= keep;
+          o[j][e + 2] *= keep;
         }
       }
     }
@@ -351,7 +366,7 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
       float w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        w[e] = ex2(s[u][e] - (ref[e & 1] - LIFT));
+        w[e] = ex2(s[u][e] - lifted[e & 1]);
         l[e & 1] += w[e];
       }
       const uint32_t p0 = transposed(pair_of(w[0], w[1])), p1 = transposed(pair_of(w[2], w[3]));
@@ -378,11 +393,10 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t x = __byte_perm(vw[h][0][i], vw[h][1][i], y ? 0x7632 : 0x5410), z = x >> 8;
-            const uint32_t magic = 0x64006400u;            // 1024 in both halves: a code in the lowest bits adds itself
-            a[h][0] = hfma2(hadd2((x & 0x000F000Fu) | magic, 0xE400E400u), sc[h], mn[h]);
-            a[h][1] = hfma2(hfma2((x & 0x00F000F0u) | magic, 0x2C002C00u, 0xD400D400u), sc[h], mn[h]);
-            a[h][2] = hfma2(hadd2((z & 0x000F000Fu) | magic, 0xE400E400u), sc[h], mn[h]);
-            a[h][3] = hfma2(hfma2((z & 0x00F000F0u) | magic, 0x2C002C00u, 0xD400D400u), sc[h], mn[h]);
+            a[h][0] = hfma2(hadd2(and_or<0x000F000Fu>(x, magic), 0xE400E400u), sc[h], mn[h]);
+            a[h][1] = hfma2(hfma2(and_or<0x00F000F0u>(x, magic), sixteenth, minus64), sc[h], mn[h]);
+            a[h][2] = hfma2(hadd2(and_or<0x000F000Fu>(z, magic), 0xE400E400u), sc[h], mn[h]);
+            a[h][3] = hfma2(hfma2(and_or<0x00F000F0u>(z, magic), sixteenth, minus64), sc[h], mn[h]);
           }
           at_mma(o[4 * i + 2 * y], a[0][0], a[0][1], a[1][0], a[1][1], p0, p1);
           at_mma(o[4 * i + 2 * y + 1], a[0][2], a[0][3], a[1][2], a[1][3], p0, p1);
@@ -393,7 +407,7 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
   int stage = 0;
 #pragma unroll 1
   for (; v < vis.turns; v += stride) {
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    asm volatile("cp.async.wait_group %0;" ::"n"(AT_STAGES - 1) : "memory");
     __syncwarp();
     const uint32_t at = my_ring + stage * T::BYTES;
     const int base = vis.base(v);
@@ -410,8 +424,8 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
     if (vis.whole(base)) take(at, base, std::true_type());
     else take(at, base, std::false_type());
     __syncwarp();
-    fetch(v + 2 * stride, stage);
-    stage ^= 1;
+    fetch(v + AT_STAGES * stride, stage);
+    stage = stage == AT_STAGES - 1 ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncwarp();
@@ -468,6 +482,8 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
       const float inv = vis.n ? 1.f / s_pl[g] : 0.f;
       *reinterpret_cast<uint2*>(out + (head0 + g) * D + c) =
           vis.n ? make_uint2(pair_of(sum.x * inv, sum.y * inv), pair_of(sum.z * inv, sum.w * inv)) : make_uint2(0, 0);
+    } else if (part) {
+      *reinterpret_cast<float4*>(part + (((head0 + g) * nsplit + split) * (D + 4) + 4 + c)) = sum;
     } else {
       *reinterpret_cast<float4*>(&s_part[g][c]) = sum;
     }
@@ -476,10 +492,14 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
     if (WEIGHTS && tid < heads) stats[head0 + tid] = make_float2((s_pm[tid] == -INFINITY ? 0.f : s_pm[tid]) - LIFT, s_pl[tid]);
     return;
   }
+  if (part) {
+    if (tid < heads) *reinterpret_cast<float2*>(part + ((head0 + tid) * nsplit + split) * (D + 4)) = make_float2(s_pm[tid], s_pl[tid]);
+    return;
+  }
   cluster_barrier();
   // every CTA joins its share of the columns, two a thread
   const uint32_t pm = (uint32_t)__cvta_generic_to_shared(s_pm), pl = (uint32_t)__cvta_generic_to_shared(s_pl);
-  const uint32_t part = (uint32_t)__cvta_generic_to_shared(s_part);
+  const uint32_t parts = (uint32_t)__cvta_generic_to_shared(s_part);
   const int pairs = heads * D / 2, mine = (pairs + nsplit - 1) / nsplit;
   for (int i = split * mine + tid; i < min(pairs, (split + 1) * mine); i += THREADS) {
     const int g = i / (D / 2), c = 2 * (i % (D / 2));
@@ -490,13 +510,46 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
       const float mr = ld_cluster(in_cta(pm + 4 * g, r)), lr = ld_cluster(in_cta(pl + 4 * g, r));
       const float f = mr == -INFINITY ? (lr == 0.f ? 0.f : 1.f) : ex2(mr - top);
       tot += f * lr;
-      x += f * ld_cluster(in_cta(part + 4 * (g * D + c), r));
-      y += f * ld_cluster(in_cta(part + 4 * (g * D + c + 1), r));
+      x += f * ld_cluster(in_cta(parts + 4 * (g * D + c), r));
+      y += f * ld_cluster(in_cta(parts + 4 * (g * D + c + 1), r));
     }
     *reinterpret_cast<uint32_t*>(out + (head0 + g) * D + c) = vis.n ? pair_of(x / tot, y / tot) : 0u;
     if (WEIGHTS && c == 0) stats[head0 + g] = make_float2((top == -INFINITY ? 0.f : top) - LIFT, tot);
   }
   cluster_barrier();                                       // (nobody leaves while its sums are read)
+}
+
+// The parts of a query head's sums in the workspace, [head][part][maximum, sum, -, -, D values]: a warp per head.
+template <int D>
+__global__ void __launch_bounds__(AT_THREADS) kv4_join_kernel(const float* __restrict__ part, int nsplit, long long heads, __half* __restrict__ out, float2* __restrict__ stats) {
+  constexpr int CPL = D / 32;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long long head = (long long)blockIdx.x * (AT_THREADS / 32) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (head >= heads) return;
+  const float* mine = part + head * nsplit * (D + 4);
+  const float2 ml = lane < nsplit ? *reinterpret_cast<const float2*>(mine + lane * (D + 4)) : make_float2(-INFINITY, 0.f);      // (at most 32 parts)
+  float top = ml.x;
+  for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - top);
+  float tot = f * ml.y, sum[CPL] = {};
+  for (int d = 16; d; d /= 2) tot += __shfl_xor_sync(0xffffffffu, tot, d);
+#pragma unroll 8
+  for (int r = 0; r < nsplit; ++r) {
+    const float fr = __shfl_sync(0xffffffffu, f, r);
+#pragma unroll
+    for (int i = 0; i < CPL; i += 2) {
+      const float2 x = *reinterpret_cast<const float2*>(mine + r * (D + 4) + 4 + CPL * lane + i);
+      sum[i] = __fmaf_rn(fr, x.x, sum[i]);
+      sum[i + 1] = __fmaf_rn(fr, x.y, sum[i + 1]);
+    }
+  }
+  const bool none = tot == 0.f;                            // no slot is visible (a visible one's weight is not 0)
+#pragma unroll
+  for (int i = 0; i < CPL; i += 2)
+    *reinterpret_cast<uint32_t*>(out + head * D + CPL * lane + i) = none ? 0u : pair_of(sum[i] / tot, sum[i + 1] / tot);
+  if (stats && lane == 0) stats[head] = make_float2((top == -INFINITY ? 0.f : top) - LIFT, tot);
 }
 
 // weights_out = weights + the sum of the weights of the head's queries; 0 from slot n on.  A new slot (more) has none before.
@@ -525,31 +578,56 @@ __global__ void __launch_bounds__(AT_THREADS) kv4_weights_kernel(const float* __
   weights_out[at] = w;
 }
 
+// The CTAs of a call: their warps, how many share a head's slots, and whether those are clusters.
+struct Shape {
+  int warps, splits;
+  bool cluster;
+};
+constexpr int AT_MAX_SPLITS = 32;            // (a lane each where they are joined)
+Shape shape_of(const cq_kv4* cache, int n_heads, int window, int sinks) {
+  const int B = cache->sequences, KV = cache->n_kv_heads, chunks = (n_heads / KV + AT_HEADS - 1) / AT_HEADS, sms = cq_sm_count();
+  const long long tasks = (long long)B * KV * chunks;
+  const long long most = window ? std::min<long long>(cache->slots, (long long)window + sinks + AT_SLOTS) : cache->slots;
+  const int turns = (int)((most + AT_SLOTS - 1) / AT_SLOTS);
+  // The least time by a model (us): waves of CTAs, each its start and the turns of a warp, which take longer the fuller the SM
+  // is; joins as clusters (of 2, 4 or 8, which GPCs hold without a rest: 40 heads of 9984 slots with clusters of 7 33 us, with
+  // 7 unclustered CTAs 24.6) or through the workspace.  Over 29 shapes (1 to 64 sequences, 1 to 40 KV heads, 128 to 131072
+  // slots), each timed with every plan, the plans it takes are 2 % slower than the best ones on average, 15 % at most.
+  // (16 sequences of 64 heads on 8 KV heads, 4096 slots: 16 warps, one CTA a head 26.1 us, 4 warps 31.2; 1 sequence of 65536:
+  // 18 CTAs of 8 warps 31.2, clusters of 8 of 16 warps 42; 32 heads of 512 slots in 32 sequences: 4 warps 30.7, 16 68.6.)
+  Shape best = {4, 1, false};
+  double least = 0;
+  for (int w : {4, 8, 16})
+    for (int n = 1; n <= AT_MAX_SPLITS; ++n) {
+      if (n > 1 && (long long)(n - 1) * w >= turns) break;
+      const long long ctas = tasks * n;
+      const double waves = (double)ctas / (sms * (AT_SM_WARPS / w)), whole = std::ceil(waves);
+      const double part = w == 4 ? 0.37 : (w == 8 ? 0.73 : 0.87), filled = std::max(1.0, part * whole + (1 - part) * waves);
+      const int per_sm = (int)std::min<long long>(AT_SM_WARPS, w * ((ctas + sms - 1) / sms));
+      const double turn = (1.43 + 0.85 * std::max(0, per_sm - 4) / 12) * (cache->head_dim == 64 ? 0.47 : 1.0);
+      const double body = filled * (((turns + n * w - 1) / (n * w)) * turn + 1.4 + 0.05 * w);
+      const bool cluster = n == 2 || n == 4 || n == 8;
+      const double t = body + (n == 1 ? 0.0 : (cluster ? 1.65 + 0.15 * n : 8.7 + 0.05 * n));
+      if (least == 0 || t < least) {
+        least = t;
+        best = {w, n, n > 1 && cluster};
+      }
+    }
+  return best;
+}
+size_t sums_bytes(const cq_kv4* cache, int n_heads, const Shape& s) {
+  return s.splits > 1 && !s.cluster ? (size_t)cache->sequences * n_heads * s.splits * (cache->head_dim + 4) * 4 : 0;
+}
+
 int attend(const cq_kv4* cache, const void* q, const NewRow& fresh, const long long* length, void* out, int n_heads, int window, int sinks,
            float scale, const float* weights, float* weights_out, void* workspace, cudaStream_t stream) {
   const int B = cache->sequences, KV = cache->n_kv_heads, D = cache->head_dim, NG = D / cache->group, more = fresh.k ? 1 : 0;
   const int chunks = (n_heads / KV + AT_HEADS - 1) / AT_HEADS;
-  float2* stats = weights ? (float2*)workspace : nullptr;
+  const Shape s = shape_of(cache, n_heads, window, sinks);
+  float* part = s.splits > 1 && !s.cluster ? (float*)workspace : nullptr;
+  float2* stats = weights ? (float2*)((uint8_t*)workspace + sums_bytes(cache, n_heads, s)) : nullptr;
   float* scores = weights ? (float*)(stats + (size_t)B * n_heads) : nullptr;
-  // CTAs of 16 warps, one on an SM, or of 4, four on an SM, and how many share a head's slots
-  const long long tasks = (long long)B * KV * chunks;
-  const int most = window ? std::min(cache->slots, window + sinks) : cache->slots, turns = (most + AT_SLOTS - 1) / AT_SLOTS + (window ? 1 : 0);
-  const int sms = cq_sm_count();
-  int warps = 16, splits = 1;
-  double best = 0;
-  for (int w = 16; w >= 4; w -= 12)
-    for (int n : {1, 2, 3, 4, 5, 6, 7, 8, 16}) {
-      if (n > 1 && (n - 1) * w >= turns) break;
-      const long long ctas = tasks * n, slots = (long long)sms * (AT_SM_WARPS / w), waves = (ctas + slots - 1) / slots;
-      const double t = (double)waves * ((turns + n * w - 1) / (n * w)) * 1.0 + 3.0 * waves + (n > 1 ? 1.0 : 0.0);
-      if (best == 0 || t < best) {
-        best = t;
-        warps = w;
-        splits = n;
-      }
-    }
-  if (getenv("KVW")) { warps = atoi(getenv("KVW")); splits = atoi(getenv("KVS")); }
-  using Kernel = void (*)(const __half*, const cq_kv4, const NewRow, const long long*, __half*, float*, float2*, int, int, int, int, float);
+  using Kernel = void (*)(const __half*, const cq_kv4, const NewRow, const long long*, __half*, float*, float2*, float*, int, int, int, int, float);
   auto pick = [&](auto width, auto groups) -> Kernel {
     constexpr int W = decltype(width)::value, N = decltype(groups)::value;
     auto sized = [&](auto w) -> Kernel {
@@ -557,28 +635,33 @@ int attend(const cq_kv4* cache, const void* q, const NewRow& fresh, const long l
       if (weights) return more ? kv4_attend_kernel<W, N, C, true, true> : kv4_attend_kernel<W, N, C, false, true>;
       return more ? kv4_attend_kernel<W, N, C, true, false> : kv4_attend_kernel<W, N, C, false, false>;
     };
-    return warps == 16 ? sized(std::integral_constant<int, 16>()) : (warps == 8 ? sized(std::integral_constant<int, 8>()) : sized(std::integral_constant<int, 4>()));
+    return s.warps == 16 ? sized(std::integral_constant<int, 16>()) : (s.warps == 8 ? sized(std::integral_constant<int, 8>()) : sized(std::integral_constant<int, 4>()));
   };
   using std::integral_constant;
   const Kernel fn = D == 128 ? (NG == 4 ? pick(integral_constant<int, 128>(), integral_constant<int, 4>()) : pick(integral_constant<int, 128>(), integral_constant<int, 2>()))
                              : (NG == 2 ? pick(integral_constant<int, 64>(), integral_constant<int, 2>()) : pick(integral_constant<int, 64>(), integral_constant<int, 1>()));
-  const int smem = warps * AT_STAGES * AT_SLOTS * (D + 8 * NG);
+  const int smem = s.warps * AT_STAGES * AT_SLOTS * (D + 8 * NG);
   CQ_CUDA_TRY(cq_grant_smem((const void*)fn, smem));
-  if (splits > 8) CQ_CUDA_TRY(cudaFuncSetAttribute((const void*)fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(splits, KV * chunks, B);
-  cfg.blockDim = dim3(warps * 32);
+  cfg.gridDim = dim3(s.splits, KV * chunks, B);
+  cfg.blockDim = dim3(s.warps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = splits;
+  attr[1].val.clusterDim.x = s.splits;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = splits > 1 ? 2 : 1;
-  CQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, (const __half*)q, *cache, fresh, length, (__half*)out, scores, stats, n_heads, chunks, window, sinks, scale));
+  cfg.numAttrs = s.cluster ? 2 : 1;
+  CQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, (const __half*)q, *cache, fresh, length, (__half*)out, scores, stats, part, n_heads, chunks, window, sinks,
+                                 scale));
+  if (part) {
+    const long long heads = (long long)B * n_heads;
+    CQ_CUDA_TRY(kv4_launch(D == 128 ? kv4_join_kernel<128> : kv4_join_kernel<64>, dim3((unsigned)((heads + 7) / 8)), dim3(AT_THREADS), 0, stream,
+                           (const float*)part, s.splits, heads, (__half*)out, stats));
+  }
   if (weights)
     CQ_CUDA_TRY(kv4_launch(kv4_weights_kernel, dim3((cache->slots + AT_THREADS - 1) / AT_THREADS, KV, B), dim3(AT_THREADS), 0, stream,
                            (const float*)scores, (const float2*)stats, length, more, weights, weights_out, n_heads, KV, cache->slots, window,
@@ -598,10 +681,10 @@ int check(const cq_kv4* cache, const void* q, const long long* length, const voi
 
 }  // namespace
 
-extern "C" size_t cq_kv4_attend_workspace_bytes(const cq_kv4* cache, int n_heads, int with_weights) {
-  if (cq_kv4_check(cache) != CQ_OK || n_heads < 1) return 0;
+extern "C" size_t cq_kv4_attend_workspace_bytes(const cq_kv4* cache, int n_heads, int window, int sinks, int with_weights) {
+  if (cq_kv4_check(cache) != CQ_OK || n_heads < 1 || n_heads % cache->n_kv_heads || window < 0 || sinks < 0) return 0;
   const size_t heads = (size_t)cache->sequences * n_heads;
-  return (with_weights ? heads * 8 + heads * cache->slots * 4 : 0) + 256;
+  return sums_bytes(cache, n_heads, shape_of(cache, n_heads, window, sinks)) + (with_weights ? heads * 8 + heads * cache->slots * 4 : 0) + 16;
 }
 
 extern "C" int cq_kv4_attend(const cq_kv4* cache, const void* q, const long long* length, void* out, int n_heads, int window, int sinks,

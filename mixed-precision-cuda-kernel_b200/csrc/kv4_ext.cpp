@@ -166,8 +166,8 @@ struct KVCache4 {
     return {weights->const_data_ptr<float>(), out.data_ptr<float>()};
   }
 
-  torch::Tensor workspace(int H, bool weights) const {
-    return torch::empty({(int64_t)cq_kv4_attend_workspace_bytes(&c, H, weights)}, k_codes.options());
+  torch::Tensor workspace(int H, int64_t window, int64_t sinks, bool weights) const {
+    return torch::empty({(int64_t)cq_kv4_attend_workspace_bytes(&c, H, (int)window, (int)sinks, weights)}, k_codes.options());
   }
 
   torch::Tensor attend(const torch::Tensor& q, const torch::Tensor& length, int64_t window, int64_t sinks, const OptTensor& weights,
@@ -178,7 +178,7 @@ struct KVCache4 {
     const long long* n = whole_numbers(length, "length", c.sequences, device);
     const auto w = check_weights(weights, weights_out);
     auto out = torch::empty_like(q);
-    auto ws = workspace(H, w.first);
+    auto ws = workspace(H, window, sinks, w.first);
     check_status(cq_kv4_attend(&c, q.const_data_ptr(), n, out.data_ptr(), H, (int)window, (int)sinks,
                                (float)scale.value_or(1.0 / std::sqrt((double)c.head_dim)), w.first, w.second, ws.data_ptr(), use()),
                  "KVCache4.attend");
@@ -197,7 +197,7 @@ struct KVCache4 {
     const long long* n = whole_numbers(length, "length", c.sequences, device);
     const auto w = check_weights(weights, weights_out);
     auto out = torch::empty_like(q);
-    auto ws = workspace(H, w.first);
+    auto ws = workspace(H, window, sinks, w.first);
     check_status(cq_kv4_step(&c, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), table ? cos->const_data_ptr<float>() : nullptr,
                              table ? sin->const_data_ptr<float>() : nullptr, table ? (const long long*)positions->const_data_ptr() : nullptr,
                              table, n, out.data_ptr(), H, (int)window, (int)sinks,

@@ -45,7 +45,7 @@ def test_cache_fields(lib, field, value, code):
     assert lib.cq_kv4_read(C.byref(c), at, 1, at, at, None) == code
     assert lib.cq_kv4_attend(C.byref(c), at, at, at, 4, 0, 0, C.c_float(1.0), None, None, at, None) == code
     assert lib.cq_kv4_evict(C.byref(c), C.byref(cache()), at, at, at, at, 8, 0, 0, at, at, None) == code
-    assert lib.cq_kv4_evict_workspace_bytes(C.byref(c), 8) == 0 and lib.cq_kv4_attend_workspace_bytes(C.byref(c), 4, 1) == 0
+    assert lib.cq_kv4_evict_workspace_bytes(C.byref(c), 8) == 0 and lib.cq_kv4_attend_workspace_bytes(C.byref(c), 4, 0, 0, 1) == 0
 
 
 def test_cache_calls(lib):
