@@ -66,8 +66,14 @@ __device__ __forceinline__ uint32_t pair_of(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+// 16 bytes that are read once: they leave L2 first
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "l"(policy) : "memory");
+}
+__device__ __forceinline__ uint64_t evict_first() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
 }
 __device__ __forceinline__ uint32_t hadd2(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -172,6 +178,7 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
 
   const uint32_t my_ring = (uint32_t)__cvta_generic_to_shared(ring) + warp * (AT_STAGES * T::BYTES);
   const int stride = nsplit * WARPS;
+  const uint64_t policy = evict_first();
   auto fetch = [&](int v, int stage) {
     if (v < vis.turns) {
       const int base = vis.base(v);
@@ -181,12 +188,12 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
 #pragma unroll
       for (int i = 0; i < T::CODES / 512; ++i) {
         const int p = lane + 32 * i, at = T::piece(p / (T::ROW / 16), p % (T::ROW / 16));
-        copy16(to + at, kc + 16 * p);
-        copy16(to + T::CODES + at, vc + 16 * p);
+        copy16(to + at, kc + 16 * p, policy);
+        copy16(to + T::CODES + at, vc + 16 * p, policy);
       }
       if (NG == 4 || lane < 8 * NG) {
-        copy16(to + 2 * T::CODES + 16 * lane, (const uint8_t*)cache.k_scales + (row0 + base) * (4 * NG) + 16 * lane);
-        copy16(to + 2 * T::CODES + T::SCALES + 16 * lane, (const uint8_t*)cache.v_scales + (row0 + base) * (4 * NG) + 16 * lane);
+        copy16(to + 2 * T::CODES + 16 * lane, (const uint8_t*)cache.k_scales + (row0 + base) * (4 * NG) + 16 * lane, policy);
+        copy16(to + 2 * T::CODES + T::SCALES + 16 * lane, (const uint8_t*)cache.v_scales + (row0 + base) * (4 * NG) + 16 * lane, policy);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -553,29 +560,38 @@ __global__ void __launch_bounds__(AT_THREADS) kv4_join_kernel(const float* __res
 }
 
 // weights_out = weights + the sum of the weights of the head's queries; 0 from slot n on.  A new slot (more) has none before.
+// Four slots a thread.
 __global__ void __launch_bounds__(AT_THREADS) kv4_weights_kernel(const float* __restrict__ scores, const float2* __restrict__ stats,
                                                                  const long long* __restrict__ length, int more, const float* weights,
                                                                  float* weights_out, int H, int KV, int slots, int window, int sinks) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int slot = blockIdx.x * AT_THREADS + threadIdx.x, kv = blockIdx.y, b = blockIdx.z, G = H / KV;
+  const int slot = 4 * (blockIdx.x * AT_THREADS + threadIdx.x), kv = blockIdx.y, b = blockIdx.z, G = H / KV;
   if (slot >= slots) return;
-  const int n = held(length, b, more, slots);
+  const Visible vis(held(length, b, more, slots), window, sinks);
   const size_t at = ((size_t)b * KV + kv) * slots + slot;
-  float w = 0.f;
-  if (slot < n) {
-    if (!(more && slot == length[b])) w = weights[at];
-    if (!window || slot < sinks || slot >= n - window) {
-      float sum = 0.f;
-      for (int g = 0; g < G; ++g) {
-        const size_t head = (size_t)b * H + kv * G + g;
-        const float2 ml = stats[head];
-        sum += exp2f(scores[head * slots + slot] - ml.x) / ml.y;
-      }
-      w += sum;
+  float sum[4] = {};
+  if (slot < vis.n && (slot < vis.first || slot + 3 >= vis.from)) {
+    const size_t head0 = (size_t)b * H + (size_t)kv * G;
+#pragma unroll 8
+    for (int g = 0; g < G; ++g) {
+      const float2 ml = stats[head0 + g];
+      const float4 s = *reinterpret_cast<const float4*>(scores + (head0 + g) * slots + slot);
+      const float inv = 1.f / ml.y;
+      sum[0] += ex2(s.x - ml.x) * inv;
+      sum[1] += ex2(s.y - ml.x) * inv;
+      sum[2] += ex2(s.z - ml.x) * inv;
+      sum[3] += ex2(s.w - ml.x) * inv;
     }
   }
-  weights_out[at] = w;
+  const long long fresh = more ? length[b] : -1;
+  const float4 old = slot < vis.n ? *reinterpret_cast<const float4*>(weights + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+  const float before[4] = {old.x, old.y, old.z, old.w};
+  float w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    w[e] = slot + e < vis.n ? (slot + e == fresh ? 0.f : before[e]) + (vis.sees(slot + e) ? sum[e] : 0.f) : 0.f;
+  *reinterpret_cast<float4*>(weights_out + at) = make_float4(w[0], w[1], w[2], w[3]);
 }
 
 // The CTAs of a call: their warps, how many share a head's slots, and whether those are clusters.
@@ -626,7 +642,7 @@ int attend(const cq_kv4* cache, const void* q, const NewRow& fresh, const long l
   const Shape s = shape_of(cache, n_heads, window, sinks);
   float* part = s.splits > 1 && !s.cluster ? (float*)workspace : nullptr;
   float2* stats = weights ? (float2*)((uint8_t*)workspace + sums_bytes(cache, n_heads, s)) : nullptr;
-  float* scores = weights ? (float*)(stats + (size_t)B * n_heads) : nullptr;
+  float* scores = weights ? (float*)(stats + ((size_t)B * n_heads + 1) / 2 * 2) : nullptr;
   using Kernel = void (*)(const __half*, const cq_kv4, const NewRow, const long long*, __half*, float*, float2*, float*, int, int, int, int, float);
   auto pick = [&](auto width, auto groups) -> Kernel {
     constexpr int W = decltype(width)::value, N = decltype(groups)::value;
@@ -663,7 +679,7 @@ int attend(const cq_kv4* cache, const void* q, const NewRow& fresh, const long l
                            (const float*)part, s.splits, heads, (__half*)out, stats));
   }
   if (weights)
-    CQ_CUDA_TRY(kv4_launch(kv4_weights_kernel, dim3((cache->slots + AT_THREADS - 1) / AT_THREADS, KV, B), dim3(AT_THREADS), 0, stream,
+    CQ_CUDA_TRY(kv4_launch(kv4_weights_kernel, dim3((cache->slots + 4 * AT_THREADS - 1) / (4 * AT_THREADS), KV, B), dim3(AT_THREADS), 0, stream,
                            (const float*)scores, (const float2*)stats, length, more, weights, weights_out, n_heads, KV, cache->slots, window,
                            sinks));
   return CQ_OK;
@@ -675,7 +691,7 @@ int check(const cq_kv4* cache, const void* q, const long long* length, const voi
   if (rc != CQ_OK) return rc;
   if (!q || !length || !out || window < 0 || sinks < 0 || (!weights != !weights_out) || !workspace) return CQ_ERR_BAD_ARG;
   if (n_heads < 1 || n_heads % cache->n_kv_heads || (n_heads + 7ll * cache->n_kv_heads) / 8 > 65535) return CQ_ERR_BAD_SHAPE;
-  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15) return CQ_ERR_BAD_ARG;
+  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)weights | (uintptr_t)weights_out | (uintptr_t)workspace) & 15) return CQ_ERR_BAD_ARG;
   return CQ_OK;
 }
 
@@ -684,7 +700,7 @@ int check(const cq_kv4* cache, const void* q, const long long* length, const voi
 extern "C" size_t cq_kv4_attend_workspace_bytes(const cq_kv4* cache, int n_heads, int window, int sinks, int with_weights) {
   if (cq_kv4_check(cache) != CQ_OK || n_heads < 1 || n_heads % cache->n_kv_heads || window < 0 || sinks < 0) return 0;
   const size_t heads = (size_t)cache->sequences * n_heads;
-  return sums_bytes(cache, n_heads, shape_of(cache, n_heads, window, sinks)) + (with_weights ? heads * 8 + heads * cache->slots * 4 : 0) + 16;
+  return sums_bytes(cache, n_heads, shape_of(cache, n_heads, window, sinks)) + (with_weights ? heads * 8 + heads * cache->slots * 4 + 16 : 0) + 16;
 }
 
 extern "C" int cq_kv4_attend(const cq_kv4* cache, const void* q, const long long* length, void* out, int n_heads, int window, int sinks,
