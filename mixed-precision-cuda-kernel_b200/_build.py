@@ -49,7 +49,7 @@ def cuda_sources():
 def build_lib(force: bool = False, verbose: bool = False) -> str:
     srcs = cuda_sources()
     deps = srcs + [os.path.join(CSRC, "cq_common.cuh"), os.path.join(CSRC, "cq_tile.cuh"), os.path.join(CSRC, "cq_attn.cuh"),
-                   os.path.join(CSRC, "cq_kv4.cuh"),
+                   os.path.join(CSRC, "cq_kv4.cuh"), os.path.join(CSRC, "cq_umma.cuh"),
                    os.path.join(ROOT, "include", "cherryq.h")]
     if not force and _newer(LIB, deps):
         return LIB

@@ -10,6 +10,7 @@
 #include <algorithm>
 
 #include "cq_kv4.cuh"
+#include "cq_umma.cuh"
 
 namespace {
 
@@ -159,6 +160,344 @@ __global__ void __launch_bounds__(PR_THREADS) prompt_kernel(const __grid_constan
   }
 }
 
+// ------------------------------------------------------------------ on tcgen05
+// A CTA takes two tiles of 128 queries of a head, one for each group of four softmax warps, and goes through the keys 128 at a
+// time.  S = Q . K^T and O += P . V are tcgen05.mma of one CTA (128 x 128 x 16 a step), all accumulators in tensor memory:
+// S of the two tiles, O of the two tiles, 512 columns; P takes the place of its S, as fp16, and is the A operand from there.
+// While the softmax warps of one tile take exponentials, the tensor core works on the other tile.
+//   warps 0-3, 4-7  softmax of a tile, a thread a query: row maximum, exponentials, row sum, P; O / sum at the end
+//   warp 8          TMA of Q, K, V (128-byte swizzle, boxes of 64 columns x 128 rows; what lies outside reads as zeros)
+//   warp 9          issues the MMAs; owns the tensor memory
+// The reference of a row's exponentials is a whole number and only raised when a score is 2^8 above it, so that O is rescaled
+// (tensor memory -> registers -> tensor memory) a few times in the first tiles and hardly ever afterwards.  P is rounded to
+// fp16 (2^-11 of each weight; the row sum is of the unrounded ones, in fp32).
+constexpr int UM_THREADS = 320, UM_TILE = 128, UM_STAGES = 4, UM_CHUNK = 64 * 128 * 2;      // bytes of 64 columns of a tile
+constexpr int W_LOAD = 8, W_MMA = 9;
+constexpr float HEADROOM = 8.f, LIFT = 7.f;      // weights are 2^7 times the exponentials, at most 2^15
+
+// the key tiles that the queries at positions pmin .. pmax (both inside the length n) of a CTA see
+struct KeyTiles {
+  int ns = 0, wt0 = 0, count = 0;
+  __device__ __forceinline__ KeyTiles(const cq_prompt& s, int pmin, int pmax) {
+    if (pmax < pmin) return;
+    const int from = s.window ? max(0, pmin - s.window + 1) : 0, first = s.window ? min(s.sinks, from) : 0;
+    ns = (first + UM_TILE - 1) / UM_TILE;
+    wt0 = from / UM_TILE;
+    if (ns >= wt0) ns = wt0 = 0;
+    count = ns + pmax / UM_TILE + 1 - wt0;
+  }
+  __device__ __forceinline__ int base(int i) const { return UM_TILE * (i < ns ? i : i - ns + wt0); }
+};
+// whether any of the queries pmin .. pmax sees a key of the tile; whether all of them see all of it
+__device__ __forceinline__ bool tile_seen(const cq_prompt& s, int base, int pmin, int pmax) {
+  return pmin <= pmax && base <= pmax && (!s.window || base < s.sinks || base + UM_TILE - 1 > pmin - s.window);
+}
+__device__ __forceinline__ bool tile_whole(const cq_prompt& s, int base, int pmin, int pmax, int n) {
+  const int last = base + UM_TILE - 1;
+  return last <= pmin && last < n && (!s.window || last < s.sinks || base > pmax - s.window);
+}
+
+__device__ __forceinline__ uint64_t two(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 apart(uint64_t a) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct PromptMaps {
+  CUtensorMap q, k, v;
+  int one[3][2];             // 0 where the heads (0) or sequences (1) of q, k, v are all the same rows
+};
+
+template <int D>
+__global__ void __launch_bounds__(UM_THREADS, 1) prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ PromptMaps maps,
+                                                                    __half* __restrict__ out, float* __restrict__ lse, uint32_t* __restrict__ status) {
+  using namespace umma;
+  constexpr int CH = D / 64, TILE_BYTES = CH * UM_CHUNK;
+  extern __shared__ __align__(1024) uint8_t um_smem[];
+  __shared__ __align__(8) uint64_t s_bar[2 + 2 * UM_STAGES + 6];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_gone;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t smem = (smem_at(um_smem) + 1023u) & ~1023u, s_q = smem, s_kv = smem + 2 * TILE_BYTES;
+  const uint32_t bars = smem_at(s_bar);
+  const uint32_t q_full = bars;
+  auto kv_full = [&](int st) { return bars + 8 * (1 + st); };
+  auto kv_free = [&](int st) { return bars + 8 * (1 + UM_STAGES + st); };
+  auto s_full = [&](int t) { return bars + 8 * (1 + 2 * UM_STAGES + t); };
+  auto p_full = [&](int t) { return bars + 8 * (3 + 2 * UM_STAGES + t); };
+  auto o_done = [&](int t) { return bars + 8 * (5 + 2 * UM_STAGES + t); };
+  const uint32_t drained = bars + 8 * (7 + 2 * UM_STAGES);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) {
+    bar_init(q_full, 1);
+    bar_init(drained, 1);
+    for (int i = 0; i < UM_STAGES; ++i) {
+      bar_init(kv_full(i), 1);
+      bar_init(kv_free(i), 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      bar_init(s_full(t), 1);
+      bar_init(p_full(t), 128);
+      bar_init(o_done(t), 1);
+    }
+    s_gone = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == W_MMA) alloc(&s_tmem, 512);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = s_tmem;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  const cq_prompt& s = a.s;
+  const int nq = (s.queries + 2 * UM_TILE - 1) / (2 * UM_TILE);
+  const int qb = nq - 1 - blockIdx.x / s.n_heads, h = blockIdx.x % s.n_heads, b = blockIdx.y;      // (the longest rows first)
+  const int q0 = qb * 2 * UM_TILE, off = s.keys - s.queries, n = length_of(a, b), kvh = h / (s.n_heads / s.n_kv_heads);
+  const int pmin = q0 + off, pmax = min(n, min(q0 + 2 * UM_TILE, s.queries) + off) - 1;
+  const KeyTiles tiles(s, pmin, pmax);
+  auto tile_pmin = [&](int t) { return pmin + UM_TILE * t; };
+  auto tile_pmax = [&](int t) { return min(pmax, pmin + UM_TILE * t + UM_TILE - 1); };
+  auto seen = [&](int t, int i) { return tile_seen(s, tiles.base(i), tile_pmin(t), tile_pmax(t)); };
+
+  if (warp == W_LOAD) {
+    if (lane == 0 && tiles.count) {
+      bar_expect(q_full, 2 * TILE_BYTES);
+      for (int t = 0; t < 2; ++t)
+        for (int c = 0; c < CH; ++c)
+          tma(s_q + t * TILE_BYTES + c * UM_CHUNK, &maps.q, 64 * c, q0 + UM_TILE * t, h * maps.one[0][0], b * maps.one[0][1], q_full);
+      int sent = 0;
+      for (int i = 0; i < 2 * tiles.count; ++i) {          // keys, values, keys, values ...
+        const int st = i % UM_STAGES, use = i / UM_STAGES;
+        if (use && !bar_wait(kv_free(st), (use - 1) & 1, &s_gone, status)) break;
+        bar_expect(kv_full(st), TILE_BYTES);
+        const int which = i & 1 ? 2 : 1;
+        for (int c = 0; c < CH; ++c)
+          tma(s_kv + st * TILE_BYTES + c * UM_CHUNK, which == 1 ? &maps.k : &maps.v, 64 * c, tiles.base(i / 2), kvh * maps.one[which][0],
+              b * maps.one[which][1], kv_full(st));
+        ++sent;
+      }
+      if (s_gone) {                                        // copies in flight end before the CTA does
+        bar_wait(q_full, 0, &s_gone, nullptr);
+        for (int i = max(0, sent - UM_STAGES); i < sent; ++i)
+          for (int k = 0; k < 1000 && !bar_try(kv_full(i % UM_STAGES), (i / UM_STAGES) & 1); ++k) {}
+      }
+    }
+  } else if (warp == W_MMA) {
+    constexpr uint32_t SHAPE_S = shape_of(128, 128, false), SHAPE_O = shape_of(128, D, true);
+    int used[2] = {0, 0};                                  // tiles of keys that a query tile has taken
+    bool ok = true;
+    auto scores = [&](int t, int i) {
+      if (lane == 0) {
+        const uint32_t kt = s_kv + (2 * i % UM_STAGES) * TILE_BYTES, qt = s_q + t * TILE_BYTES;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t at = (k / 4) * UM_CHUNK + (k % 4) * 32;
+          mma_ss(tmem + 128 * t, operand(qt + at, 0), operand(kt + at, 0), SHAPE_S, k > 0);
+        }
+        commit(s_full(t));
+      }
+    };
+    if (tiles.count) {
+      ok = bar_wait_warp(q_full, 0, &s_gone, status) && bar_wait_warp(kv_full(0), 0, &s_gone, status);
+      if (ok) {
+        fence_after();
+        for (int t = 0; t < 2; ++t)
+          if (seen(t, 0)) scores(t, 0);
+        if (lane == 0) commit(kv_free(0));
+      }
+      for (int i = 0; i < tiles.count && ok; ++i) {
+        const int vi = 2 * i + 1, ki = 2 * i + 2, sv = vi % UM_STAGES;
+        const bool next = i + 1 < tiles.count;
+        ok = bar_wait_warp(kv_full(sv), (vi / UM_STAGES) & 1, &s_gone, status);
+        if (ok && next) ok = bar_wait_warp(kv_full(ki % UM_STAGES), (ki / UM_STAGES) & 1, &s_gone, status);
+        if (!ok) break;
+        const int base = tiles.base(i);
+        if (base + UM_TILE > n && n < s.keys) {
+          // Rows behind the sequence's end may hold anything, and 0 times NaN is NaN.
+          uint8_t* vt = um_smem + (s_kv + sv * TILE_BYTES - smem_at(um_smem));
+          for (int r = n - base; r < UM_TILE; ++r)
+            for (int c = lane; c < CH * 8; c += 32) *reinterpret_cast<uint4*>(vt + (c / 8) * UM_CHUNK + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+          fence_async();
+          __syncwarp();
+        }
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (seen(t, i)) {
+            ok = bar_wait_warp(p_full(t), used[t] & 1, &s_gone, status);
+            if (!ok) break;
+            fence_after();
+            if (lane == 0) {
+              const uint32_t vt = s_kv + sv * TILE_BYTES;
+#pragma unroll
+              for (int k = 0; k < UM_TILE / 16; ++k)
+                mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, operand(vt + k * 2048, UM_CHUNK), SHAPE_O, used[t] > 0 || k > 0);
+              commit(o_done(t));
+            }
+            ++used[t];
+          }
+          if (next && seen(t, i + 1)) scores(t, i + 1);
+        }
+        if (ok && lane == 0) {
+          commit(kv_free(sv));
+          if (next) commit(kv_free(ki % UM_STAGES));
+        }
+        __syncwarp();
+      }
+      // nothing is in flight when the tensor memory is given back and the CTA ends
+      if (lane == 0) commit(drained);
+      for (int k = 0; k < 100000 && !bar_try(drained, 0); ++k) {}
+      __syncwarp();
+    }
+  } else {
+    const int t = warp >> 2, r = tid & 127, p = tile_pmin(t) + r, q = q0 + UM_TILE * t + r;
+    const int hi = min(p, n - 1), lo = s.window ? p - s.window + 1 : 0;
+    const uint32_t at_s = tmem + 128 * t + ((uint32_t)(warp & 3) << 21), at_o = at_s - 128 * t + 256 + 128 * t;
+    const float scale2 = s.scale * LOG2E;
+    float ref = -INFINITY;
+    uint64_t sum = 0;                                      // two partial sums
+    int used = 0;
+    bool ok = true;
+    for (int i = 0; i < tiles.count; ++i) {
+      if (!seen(t, i)) continue;
+      const int base = tiles.base(i);
+      ok = bar_wait_warp(s_full(t), used & 1, &s_gone, status);
+      if (!ok) break;
+      fence_after();
+      uint32_t x[128];
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) load32(at_s + c, x + c);
+      wait_load<128>(x);
+      if (!tile_whole(s, base, tile_pmin(t), tile_pmax(t), n)) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c) {
+          const int key = base + c;
+          if (!(key <= hi && (key >= lo || key < s.sinks))) x[c] = 0xFF800000u;
+        }
+      }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 128; c += 4)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(x[c + e]));
+      const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+      const bool above = most > ref + HEADROOM;
+      if (__any_sync(0xffffffffu, above)) {
+        const float now = above ? ceilf(most) : ref, keep = above ? (ref == -INFINITY ? 0.f : ex2(ref - now)) : 1.f;
+        ref = now;
+        sum = fma2(sum, two(keep, keep), 0ull);
+        if (used) {
+          if (!(ok = bar_wait_warp(o_done(t), (used - 1) & 1, &s_gone, status))) break;
+          fence_after();
+#pragma unroll
+          for (int c = 0; c < D; c += 16) {
+            uint32_t y[16];
+            load16(at_o + c, y);
+            wait_load<16>(y);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * keep);
+            store16(at_o + c, y);
+          }
+        }
+      }
+      const float minus = LIFT - (ref == -INFINITY ? 0.f : ref);
+      const uint64_t scale22 = two(scale2, scale2), minus2 = two(minus, minus);
+#pragma unroll
+      for (int c = 0; c < 128; c += 32) {
+        uint32_t pr[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float2 y = apart(fma2(two(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])), scale22, minus2));
+          y.x = ex2(y.x);
+          y.y = ex2(y.y);
+          sum = add2(sum, two(y.x, y.y));
+          pr[e] = half_pair(y.x, y.y);
+        }
+        store16(at_s + c / 2, pr);
+      }
+      wait_store();
+      fence_before();
+      bar_arrive(p_full(t));
+      ++used;
+    }
+    const float2 parts = apart(sum);
+    const float total = parts.x + parts.y;
+    const bool row = q < s.queries, empty = !used || p >= n || (ref == -INFINITY && total == 0.f);
+    if (ok && used) ok = bar_wait_warp(o_done(t), (used - 1) & 1, &s_gone, status);
+    fence_after();
+    const float inv = empty ? 0.f : 1.f / total;
+    __half* to = out + (((size_t)b * s.queries + q) * s.n_heads + h) * D;
+#pragma unroll
+    for (int c = 0; c < D; c += 32) {
+      uint32_t y[32];
+      if (used && ok) {
+        load32(at_o + c, y);
+        wait_load<32>(y);
+      }
+      if (!row) continue;
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = half_pair(__uint_as_float(y[e + 2 * k]) * inv, __uint_as_float(y[e + 2 * k + 1]) * inv);
+        *reinterpret_cast<uint4*>(to + c + e) = !ok ? make_uint4(~0u, ~0u, ~0u, ~0u) : (empty ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]));
+      }
+    }
+    if (row) lse[((size_t)b * s.n_heads + h) * s.queries + q] = !ok ? NAN : empty ? -INFINITY : ((ref == -INFINITY ? 0.f : ref) - LIFT + log2f(total)) * LN2;
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == W_MMA) {
+    fence_after();
+    dealloc(tmem, 512);
+  }
+}
+
+// Tensor map of q, k or v (sequence, token, head strides in halves): boxes of 64 columns x 128 tokens.  A broadcast sequence or
+// head (stride 0) is one of them, addressed with the coordinate 0 (one[]).  False where the map cannot describe the tensor.
+bool map_of(CUtensorMap* map, const void* at, const int64_t (&strides)[3], int sequences, int tokens, int heads, int D, int (&one)[2]) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = []() -> Encode {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      (void)cudaGetLastError();
+      return nullptr;
+    }
+    return (Encode)fn;
+  }();
+  if (!encode || (tokens > 1 && strides[1] < 8)) return false;
+  one[0] = heads > 1 && strides[2] != 0;
+  one[1] = sequences > 1 && strides[0] != 0;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)tokens, one[0] ? (cuuint64_t)heads : 1, one[1] ? (cuuint64_t)sequences : 1};
+  const cuuint64_t steps[3] = {tokens > 1 ? (cuuint64_t)strides[1] * 2 : (cuuint64_t)D * 2, one[0] ? (cuuint64_t)strides[2] * 2 : (cuuint64_t)D * 2,
+                               one[1] ? (cuuint64_t)strides[0] * 2 : (cuuint64_t)D * 2};
+  const cuuint32_t box[4] = {64, UM_TILE, 1, 1}, each[4] = {1, 1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(at), dims, steps, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // 64 keys of a KV head, all its query heads and observed queries one after another
 template <int D>
 __global__ void __launch_bounds__(PR_THREADS) prompt_weights_kernel(const __grid_constant__ PromptArgs a, const float* __restrict__ lse, int observe,
@@ -214,7 +553,7 @@ __global__ void __launch_bounds__(PR_THREADS) prompt_weights_kernel(const __grid
 }
 
 int check(const cq_prompt* s, const void* q, const void* k, const void* v) {
-  if (!s || !q || !k || (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) || s->window < 0 || s->sinks < 0) return CQ_ERR_BAD_ARG;
+  if (!s || !q || !k || (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) || s->window < 0 || s->sinks < 0 || !(s->scale > 0.f)) return CQ_ERR_BAD_ARG;
   if (s->sequences < 1 || s->sequences > 65535 || s->queries < 1 || s->keys < s->queries || s->keys > (1 << 24) || s->n_kv_heads < 1 ||
       s->n_heads < 1 || s->n_heads > 65535 || s->n_heads % s->n_kv_heads)
     return CQ_ERR_BAD_SHAPE;
@@ -227,14 +566,26 @@ int check(const cq_prompt* s, const void* q, const void* k, const void* v) {
 }  // namespace
 
 extern "C" int cq_attn_prefill(const cq_prompt* shape, const void* q, const void* k, const void* v, const long long* lengths, void* out,
-                               float* lse, cq_stream_t stream) {
+                               float* lse, uint32_t* status_word, cq_stream_t stream) {
   const int rc = check(shape, q, k, v);
   if (rc != CQ_OK) return rc;
   if (!v || !out || !lse || ((uintptr_t)out & 15)) return CQ_ERR_BAD_ARG;
   const PromptArgs a = {*shape, (const __half*)q, (const __half*)k, (const __half*)v, lengths};
-  auto fn = shape->head_dim == 128 ? prompt_kernel<128> : prompt_kernel<64>;
-  CQ_CUDA_TRY(kv4_launch(fn, dim3((shape->queries + PR_TILE - 1) / PR_TILE, shape->n_heads, shape->sequences), dim3(PR_THREADS), 0,
-                         (cudaStream_t)stream, a, (__half*)out, lse));
+  const int D = shape->head_dim, B = shape->sequences;
+  PromptMaps maps;
+  if (map_of(&maps.q, q, shape->q_strides, B, shape->queries, shape->n_heads, D, maps.one[0]) &&
+      map_of(&maps.k, k, shape->k_strides, B, shape->keys, shape->n_kv_heads, D, maps.one[1]) &&
+      map_of(&maps.v, v, shape->v_strides, B, shape->keys, shape->n_kv_heads, D, maps.one[2])) {
+    auto fn = D == 128 ? prompt_umma_kernel<128> : prompt_umma_kernel<64>;
+    const int smem = (2 + UM_STAGES) * (D / 64) * UM_CHUNK + 1024;
+    CQ_CUDA_TRY(cq_grant_smem((const void*)fn, smem));
+    const unsigned blocks = (unsigned)((shape->queries + 2 * UM_TILE - 1) / (2 * UM_TILE)) * shape->n_heads;
+    CQ_CUDA_TRY(kv4_launch(fn, dim3(blocks, B), dim3(UM_THREADS), smem, (cudaStream_t)stream, a, maps, (__half*)out, lse, status_word));
+    return CQ_OK;
+  }
+  auto fn = D == 128 ? prompt_kernel<128> : prompt_kernel<64>;
+  CQ_CUDA_TRY(kv4_launch(fn, dim3((shape->queries + PR_TILE - 1) / PR_TILE, shape->n_heads, B), dim3(PR_THREADS), 0, (cudaStream_t)stream, a,
+                         (__half*)out, lse));
   return CQ_OK;
 }
 

@@ -262,6 +262,7 @@ cq_prompt prompt_of(const torch::Tensor& q, const torch::Tensor& k, int64_t wind
   s.window = (int)window;
   s.sinks = (int)sinks;
   s.scale = (float)scale.value_or(1.0 / std::sqrt((double)s.head_dim));
+  TORCH_CHECK(s.scale > 0.f, "scale must be positive");
   *n = lengths.has_value() ? whole_numbers(*lengths, "lengths", s.sequences, q.device()) : nullptr;
   return s;
 }
@@ -276,7 +277,7 @@ std::pair<torch::Tensor, torch::Tensor> attn_prefill(const torch::Tensor& q, con
   auto out = torch::empty(q.sizes(), q.options());
   auto lse = torch::empty({s.sequences, s.n_heads, s.queries}, q.options().dtype(torch::kFloat32));
   check_status(cq_attn_prefill(&s, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), n, out.data_ptr(), lse.data_ptr<float>(),
-                               (cq_stream_t)c10::cuda::getCurrentCUDAStream().stream()),
+                               device_status(q.device()), (cq_stream_t)c10::cuda::getCurrentCUDAStream().stream()),
                "attn_prefill");
   return {out, lse};
 }

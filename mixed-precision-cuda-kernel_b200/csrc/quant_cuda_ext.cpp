@@ -756,6 +756,10 @@ bool device_timed_out(int device_index) {
 
 }  // namespace
 
+uint32_t* device_status(const c10::Device& device) {
+  return (uint32_t*)(scratch_for(device).data_ptr<uint8_t>() + cq_scratch_bytes());
+}
+
 // ---- element-wise kernels of the decode harness
 std::vector<torch::Tensor> rmsnorm(torch::Tensor x, c10::optional<torch::Tensor> residual, torch::Tensor weight,
                                    double eps, bool return_sum) {
