@@ -173,7 +173,8 @@ __global__ void __launch_bounds__(PR_THREADS) prompt_kernel(const __grid_constan
 // fp16 (2^-11 of each weight; the row sum is of the unrounded ones, in fp32).
 constexpr int UM_THREADS = 320, UM_TILE = 128, UM_STAGES = 4, UM_CHUNK = 64 * 128 * 2;      // bytes of 64 columns of a tile
 constexpr int W_LOAD = 8, W_MMA = 9;
-constexpr float HEADROOM = 8.f, LIFT = 7.f;      // weights are 2^7 times the exponentials, at most 2^15
+constexpr int POLY_OF_8 = 1;                      // of eight pairs of exponentials, how many are polynomials
+constexpr float HEADROOM = 8.f, LIFT = 7.f, LOWEST = -4.f;      // weights are 2^7 times the exponentials, at most 2^15
 
 // the key tiles that the queries at positions pmin .. pmax (both inside the length n) of a CTA see
 struct KeyTiles {
@@ -217,10 +218,49 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x of two numbers up to 2^7 on the multiply-add pipe: x = n + f with a whole n and |f| <= 1/2, by adding and taking away
+// 1.5 * 2^23, then 2^f by the polynomial of degree 4 whose largest relative error is the least (2.6e-6; coefficients by
+// Remez's exchange) and 2^n as a bit pattern.  Below 2^-126: 2^-126.  NaN stays NaN.
+__device__ __forceinline__ uint64_t power2(float2 x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+  const uint64_t v = two(x.x, x.y), big = two(12582912.f, 12582912.f), less = two(-12582912.f, -12582912.f);
+  const uint64_t t = add2(v, big), f = fma2(add2(t, less), two(-1.f, -1.f), v);
+  uint64_t p = fma2(f, two(0.009570102207362652f, 0.009570102207362652f), two(0.05591785907745361f, 0.05591785907745361f));
+  p = fma2(p, f, two(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f, two(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(p, f, two(0.9999992847442627f, 0.9999992847442627f));
+  const float2 n = apart(t);
+  return mul2(p, two(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3F800000u), __uint_as_float((__float_as_uint(n.y) << 23) + 0x3F800000u)));
+}
+// whether the condition holds in any of the 256 threads of a query tile, and a barrier between them; the barrier alone
+__device__ __forceinline__ bool any_of_tile(int id, bool here) {
+  int any;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 256, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+               : "=r"(any) : "r"((int)here), "r"(id) : "memory");
+  return any != 0;
+}
+__device__ __forceinline__ void tile_sync(int id) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// which of the 32 keys from `first` on a query sees that sees lo .. hi and those below `sinks`: a bit each
+__device__ __forceinline__ uint32_t below32(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }
+__device__ __forceinline__ uint32_t visible32(int first, int lo, int hi, int sinks) {
+  return below32(hi + 1 - first) & (~below32(lo - first) | below32(sinks - first));
 }
 
 struct PromptMaps {
@@ -228,28 +268,53 @@ struct PromptMaps {
   int one[3][2];             // 0 where the heads (0) or sequences (1) of q, k, v are all the same rows
 };
 
+// The work of a CTA: every gridDim.x-th block of 256 queries of a head, the longest first, forwards and backwards in turn.
+struct PromptItem {
+  int b, h, kvh, q0, n, pmin, pmax;          // positions of the queries that are inside the length
+  __device__ __forceinline__ PromptItem(const PromptArgs& a, int item) {
+    const cq_prompt& s = a.s;
+    const int nq = (s.queries + 2 * UM_TILE - 1) / (2 * UM_TILE), per = s.n_heads * s.sequences, qb = nq - 1 - item / per;
+    const int rest = item % per;
+    b = rest / s.n_heads;
+    h = rest - b * s.n_heads;
+    kvh = h / (s.n_heads / s.n_kv_heads);
+    q0 = qb * 2 * UM_TILE;
+    n = length_of(a, b);
+    pmin = q0 + s.keys - s.queries;
+    pmax = min(n, min(q0 + 2 * UM_TILE, s.queries) + s.keys - s.queries) - 1;
+  }
+  __device__ __forceinline__ int lowest(int t) const { return pmin + UM_TILE * t; }
+  __device__ __forceinline__ int highest(int t) const { return min(pmax, pmin + UM_TILE * t + UM_TILE - 1); }
+  __device__ __forceinline__ static int at(int round, int items) {
+    const int i = round * (int)gridDim.x + (int)(round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    return i < items ? i : -1;
+  }
+};
+
 template <int D>
 __global__ void __launch_bounds__(UM_THREADS, 1) prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ PromptMaps maps,
-                                                                    __half* __restrict__ out, float* __restrict__ lse, uint32_t* __restrict__ status) {
+                                                                    __half* __restrict__ out, float* __restrict__ lse, int items,
+                                                                    uint32_t* __restrict__ status) {
   using namespace umma;
   constexpr int CH = D / 64, TILE_BYTES = CH * UM_CHUNK;
   extern __shared__ __align__(1024) uint8_t um_smem[];
-  __shared__ __align__(8) uint64_t s_bar[2 + 2 * UM_STAGES + 6];
+  __shared__ __align__(8) uint64_t s_bar[3 + 2 * UM_STAGES + 6];
   __shared__ uint32_t s_tmem;
   __shared__ int s_gone;
+  __shared__ float s_row[2][2][128];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t smem = (smem_at(um_smem) + 1023u) & ~1023u, s_q = smem, s_kv = smem + 2 * TILE_BYTES;
   const uint32_t bars = smem_at(s_bar);
-  const uint32_t q_full = bars;
-  auto kv_full = [&](int st) { return bars + 8 * (1 + st); };
-  auto kv_free = [&](int st) { return bars + 8 * (1 + UM_STAGES + st); };
-  auto s_full = [&](int t) { return bars + 8 * (1 + 2 * UM_STAGES + t); };
-  auto p_full = [&](int t) { return bars + 8 * (3 + 2 * UM_STAGES + t); };
-  auto o_done = [&](int t) { return bars + 8 * (5 + 2 * UM_STAGES + t); };
-  const uint32_t drained = bars + 8 * (7 + 2 * UM_STAGES);
+  const uint32_t q_full = bars, q_free = bars + 8, drained = bars + 16;
+  auto kv_full = [&](int st) { return bars + 8 * (3 + st); };
+  auto kv_free = [&](int st) { return bars + 8 * (3 + UM_STAGES + st); };
+  auto s_full = [&](int t) { return bars + 8 * (3 + 2 * UM_STAGES + t); };
+  auto p_full = [&](int t) { return bars + 8 * (5 + 2 * UM_STAGES + t); };
+  auto o_done = [&](int t) { return bars + 8 * (7 + 2 * UM_STAGES + t); };
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     bar_init(q_full, 1);
+    bar_init(q_free, 1);
     bar_init(drained, 1);
     for (int i = 0; i < UM_STAGES; ++i) {
       bar_init(kv_full(i), 1);
@@ -269,200 +334,233 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_umma_kernel(const __grid
   fence_after();
   const uint32_t tmem = s_tmem;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-
   const cq_prompt& s = a.s;
-  const int nq = (s.queries + 2 * UM_TILE - 1) / (2 * UM_TILE);
-  const int qb = nq - 1 - blockIdx.x / s.n_heads, h = blockIdx.x % s.n_heads, b = blockIdx.y;      // (the longest rows first)
-  const int q0 = qb * 2 * UM_TILE, off = s.keys - s.queries, n = length_of(a, b), kvh = h / (s.n_heads / s.n_kv_heads);
-  const int pmin = q0 + off, pmax = min(n, min(q0 + 2 * UM_TILE, s.queries) + off) - 1;
-  const KeyTiles tiles(s, pmin, pmax);
-  auto tile_pmin = [&](int t) { return pmin + UM_TILE * t; };
-  auto tile_pmax = [&](int t) { return min(pmax, pmin + UM_TILE * t + UM_TILE - 1); };
-  auto seen = [&](int t, int i) { return tile_seen(s, tiles.base(i), tile_pmin(t), tile_pmax(t)); };
 
-  if (warp == W_LOAD) {
-    if (lane == 0 && tiles.count) {
-      bar_expect(q_full, 2 * TILE_BYTES);
-      for (int t = 0; t < 2; ++t)
-        for (int c = 0; c < CH; ++c)
-          tma(s_q + t * TILE_BYTES + c * UM_CHUNK, &maps.q, 64 * c, q0 + UM_TILE * t, h * maps.one[0][0], b * maps.one[0][1], q_full);
-      int sent = 0;
-      for (int i = 0; i < 2 * tiles.count; ++i) {          // keys, values, keys, values ...
-        const int st = i % UM_STAGES, use = i / UM_STAGES;
-        if (use && !bar_wait(kv_free(st), (use - 1) & 1, &s_gone, status)) break;
-        bar_expect(kv_full(st), TILE_BYTES);
-        const int which = i & 1 ? 2 : 1;
-        for (int c = 0; c < CH; ++c)
-          tma(s_kv + st * TILE_BYTES + c * UM_CHUNK, which == 1 ? &maps.k : &maps.v, 64 * c, tiles.base(i / 2), kvh * maps.one[which][0],
-              b * maps.one[which][1], kv_full(st));
-        ++sent;
+  if (warp >= W_LOAD) {
+    if (warp == W_LOAD && lane == 0) {
+      int loaded = 0, sent = 0;                            // query blocks, tiles of keys and values
+      bool ok = true;
+      for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
+        const PromptItem w(a, item);
+        const KeyTiles tiles(s, w.pmin, w.pmax);
+        if (!tiles.count) continue;
+        if (loaded && !(ok = bar_wait(q_free, (loaded - 1) & 1, &s_gone, status))) break;
+        bar_expect(q_full, 2 * TILE_BYTES);
+        for (int t = 0; t < 2; ++t)
+          for (int c = 0; c < CH; ++c)
+            tma(s_q + t * TILE_BYTES + c * UM_CHUNK, &maps.q, 64 * c, w.q0 + UM_TILE * t, w.h * maps.one[0][0], w.b * maps.one[0][1], q_full);
+        ++loaded;
+        for (int i = 0; i < 2 * tiles.count; ++i, ++sent) {      // keys, values, keys, values ...
+          const int st = sent % UM_STAGES, use = sent / UM_STAGES;
+          if (use && !(ok = bar_wait(kv_free(st), (use - 1) & 1, &s_gone, status))) break;
+          bar_expect(kv_full(st), TILE_BYTES);
+          const int which = i & 1 ? 2 : 1;
+          for (int c = 0; c < CH; ++c)
+            tma(s_kv + st * TILE_BYTES + c * UM_CHUNK, which == 1 ? &maps.k : &maps.v, 64 * c, tiles.base(i / 2), w.kvh * maps.one[which][0],
+                w.b * maps.one[which][1], kv_full(st));
+        }
       }
-      if (s_gone) {                                        // copies in flight end before the CTA does
-        bar_wait(q_full, 0, &s_gone, nullptr);
+      if (!ok) {                                           // copies in flight end before the CTA does
+        for (int k = 0; loaded && k < 1000 && !bar_try(q_full, (loaded - 1) & 1); ++k) {}
         for (int i = max(0, sent - UM_STAGES); i < sent; ++i)
           for (int k = 0; k < 1000 && !bar_try(kv_full(i % UM_STAGES), (i / UM_STAGES) & 1); ++k) {}
       }
-    }
-  } else if (warp == W_MMA) {
-    constexpr uint32_t SHAPE_S = shape_of(128, 128, false), SHAPE_O = shape_of(128, D, true);
-    int used[2] = {0, 0};                                  // tiles of keys that a query tile has taken
-    bool ok = true;
-    auto scores = [&](int t, int i) {
-      if (lane == 0) {
-        const uint32_t kt = s_kv + (2 * i % UM_STAGES) * TILE_BYTES, qt = s_q + t * TILE_BYTES;
+    } else if (warp == W_MMA) {
+      constexpr uint32_t SHAPE_S = shape_of(128, 128, false), SHAPE_O = shape_of(128, D, true);
+      int taken[2] = {0, 0};                               // tiles of keys that a query tile has taken, in all items
+      int blocks = 0, sent = 0;
+      bool ok = true;
+      for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
+        const PromptItem w(a, item);
+        const KeyTiles tiles(s, w.pmin, w.pmax);
+        if (!tiles.count) continue;
+        auto seen = [&](int t, int i) { return tile_seen(s, tiles.base(i), w.lowest(t), w.highest(t)); };
+        auto scores = [&](int t, int i) {
+          if (elected()) {
+            const uint32_t kt = s_kv + ((sent + 2 * i) % UM_STAGES) * TILE_BYTES, qt = s_q + t * TILE_BYTES;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t at = (k / 4) * UM_CHUNK + (k % 4) * 32;
-          mma_ss(tmem + 128 * t, operand(qt + at, 0), operand(kt + at, 0), SHAPE_S, k > 0);
-        }
-        commit(s_full(t));
-      }
-    };
-    if (tiles.count) {
-      ok = bar_wait_warp(q_full, 0, &s_gone, status) && bar_wait_warp(kv_full(0), 0, &s_gone, status);
-      if (ok) {
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t at = (k / 4) * UM_CHUNK + (k % 4) * 32;
+              mma_ss(tmem + 128 * t, operand(qt + at, 0), operand(kt + at, 0), SHAPE_S, k > 0);
+            }
+            commit(s_full(t));
+          }
+          __syncwarp();
+        };
+        bool first[2] = {true, true};
+        ok = bar_wait_warp(q_full, blocks & 1, &s_gone, status) && bar_wait_warp(kv_full(sent % UM_STAGES), (sent / UM_STAGES) & 1, &s_gone, status);
+        if (!ok) break;
+        ++blocks;
         fence_after();
         for (int t = 0; t < 2; ++t)
           if (seen(t, 0)) scores(t, 0);
-        if (lane == 0) commit(kv_free(0));
-      }
-      for (int i = 0; i < tiles.count && ok; ++i) {
-        const int vi = 2 * i + 1, ki = 2 * i + 2, sv = vi % UM_STAGES;
-        const bool next = i + 1 < tiles.count;
-        ok = bar_wait_warp(kv_full(sv), (vi / UM_STAGES) & 1, &s_gone, status);
-        if (ok && next) ok = bar_wait_warp(kv_full(ki % UM_STAGES), (ki / UM_STAGES) & 1, &s_gone, status);
-        if (!ok) break;
-        const int base = tiles.base(i);
-        if (base + UM_TILE > n && n < s.keys) {
-          // Rows behind the sequence's end may hold anything, and 0 times NaN is NaN.
-          uint8_t* vt = um_smem + (s_kv + sv * TILE_BYTES - smem_at(um_smem));
-          for (int r = n - base; r < UM_TILE; ++r)
-            for (int c = lane; c < CH * 8; c += 32) *reinterpret_cast<uint4*>(vt + (c / 8) * UM_CHUNK + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
-          fence_async();
-          __syncwarp();
-        }
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (seen(t, i)) {
-            ok = bar_wait_warp(p_full(t), used[t] & 1, &s_gone, status);
-            if (!ok) break;
-            fence_after();
-            if (lane == 0) {
-              const uint32_t vt = s_kv + sv * TILE_BYTES;
-#pragma unroll
-              for (int k = 0; k < UM_TILE / 16; ++k)
-                mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, operand(vt + k * 2048, UM_CHUNK), SHAPE_O, used[t] > 0 || k > 0);
-              commit(o_done(t));
-            }
-            ++used[t];
-          }
-          if (next && seen(t, i + 1)) scores(t, i + 1);
-        }
-        if (ok && lane == 0) {
-          commit(kv_free(sv));
-          if (next) commit(kv_free(ki % UM_STAGES));
+        if (elected()) {
+          commit(kv_free(sent % UM_STAGES));
+          if (tiles.count == 1) commit(q_free);
         }
         __syncwarp();
+        for (int i = 0; i < tiles.count && ok; ++i) {
+          const int vi = sent + 2 * i + 1, ki = vi + 1, sv = vi % UM_STAGES;
+          const bool next = i + 1 < tiles.count;
+          ok = bar_wait_warp(kv_full(sv), (vi / UM_STAGES) & 1, &s_gone, status);
+          if (ok && next) ok = bar_wait_warp(kv_full(ki % UM_STAGES), (ki / UM_STAGES) & 1, &s_gone, status);
+          if (!ok) break;
+          const int base = tiles.base(i);
+          if (base + UM_TILE > w.n && w.n < s.keys) {
+            // Rows behind the sequence's end may hold anything, and 0 times NaN is NaN.
+            uint8_t* vt = um_smem + (s_kv + sv * TILE_BYTES - smem_at(um_smem));
+            for (int r = w.n - base; r < UM_TILE; ++r)
+              for (int c = lane; c < CH * 8; c += 32) *reinterpret_cast<uint4*>(vt + (c / 8) * UM_CHUNK + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+            fence_async();
+            __syncwarp();
+          }
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (seen(t, i)) {
+              ok = bar_wait_warp(p_full(t), taken[t] & 1, &s_gone, status);
+              if (!ok) break;
+              fence_after();
+              if (elected()) {
+                const uint32_t vt = s_kv + sv * TILE_BYTES;
+#pragma unroll
+                for (int k = 0; k < UM_TILE / 16; ++k)
+                  mma_ts(tmem + 256 + 128 * t, tmem + 128 * t + 8 * k, operand(vt + k * 2048, UM_CHUNK), SHAPE_O, !first[t] || k > 0);
+                commit(o_done(t));
+              }
+              __syncwarp();
+              first[t] = false;
+              ++taken[t];
+            }
+            if (next && seen(t, i + 1)) scores(t, i + 1);
+          }
+          if (ok && elected()) {
+            commit(kv_free(sv));
+            if (next) commit(kv_free(ki % UM_STAGES));
+            if (i + 2 == tiles.count) commit(q_free);      // the last scores of these queries are on their way
+          }
+          __syncwarp();
+        }
+        sent += 2 * tiles.count;
       }
       // nothing is in flight when the tensor memory is given back and the CTA ends
-      if (lane == 0) commit(drained);
+      if (elected()) commit(drained);
       for (int k = 0; k < 100000 && !bar_try(drained, 0); ++k) {}
       __syncwarp();
     }
   } else {
-    const int t = warp >> 2, r = tid & 127, p = tile_pmin(t) + r, q = q0 + UM_TILE * t + r;
-    const int hi = min(p, n - 1), lo = s.window ? p - s.window + 1 : 0;
-    const uint32_t at_s = tmem + 128 * t + ((uint32_t)(warp & 3) << 21), at_o = at_s - 128 * t + 256 + 128 * t;
+    const int t = warp >> 2, r = tid & 127;
+    const uint32_t at_s = tmem + 128 * t + ((uint32_t)(warp & 3) << 21), at_o = at_s + 256;
     const float scale2 = s.scale * LOG2E;
-    float ref = -INFINITY;
-    uint64_t sum = 0;                                      // two partial sums
-    int used = 0;
+    const uint64_t scale22 = two(scale2, scale2);
+    int taken = 0;                                         // tiles of keys, in all items
     bool ok = true;
-    for (int i = 0; i < tiles.count; ++i) {
-      if (!seen(t, i)) continue;
-      const int base = tiles.base(i);
-      ok = bar_wait_warp(s_full(t), used & 1, &s_gone, status);
-      if (!ok) break;
-      fence_after();
-      uint32_t x[128];
+    for (int round = 0, item; (item = PromptItem::at(round, items)) >= 0; ++round) {
+      const PromptItem w(a, item);
+      const KeyTiles tiles(s, w.pmin, w.pmax);
+      const int p = w.lowest(t) + r, q = w.q0 + UM_TILE * t + r;
+      const int hi = min(p, w.n - 1), lo = s.window ? p - s.window + 1 : 0;
+      float ref = -INFINITY;
+      uint64_t sum = 0;                                    // two partial sums
+      bool first = true;
+      for (int i = 0; i < tiles.count && ok; ++i) {
+        const int base = tiles.base(i);
+        if (!tile_seen(s, base, w.lowest(t), w.highest(t))) continue;
+        ok = bar_wait_warp(s_full(t), taken & 1, &s_gone, status);
+        if (!ok) break;
+        fence_after();
+        const bool whole = tile_whole(s, base, w.lowest(t), w.highest(t), w.n);
+        // Exponentials with the reference as it is, the maximum on the way: where it shows that the reference has to rise (or a
+        // first guess of 0 was too high), the tile is taken again, once.  P leaves the registers when that is known.
+        uint32_t pr[64];
+        uint64_t here;
+        for (;;) {
+          const float minus = LIFT - (ref == -INFINITY ? 0.f : ref);
+          const uint64_t minus2 = two(minus, minus);
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          here = 0;
 #pragma unroll
-      for (int c = 0; c < 128; c += 32) load32(at_s + c, x + c);
-      wait_load<128>(x);
-      if (!tile_whole(s, base, tile_pmin(t), tile_pmax(t), n)) {
+          for (int c0 = 0; c0 < 128; c0 += 64) {
+            uint32_t x[64];
+            load32(at_s + c0, x);
+            load32(at_s + c0 + 32, x + 32);
+            wait_load<32>(x);
+            wait_load<32>(x + 32);
+            if (!whole) {
 #pragma unroll
-        for (int c = 0; c < 128; ++c) {
-          const int key = base + c;
-          if (!(key <= hi && (key >= lo || key < s.sinks))) x[c] = 0xFF800000u;
-        }
-      }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+              for (int g = 0; g < 64; g += 32) {
+                const uint32_t vis = visible32(base + c0 + g, lo, hi, s.sinks);
 #pragma unroll
-      for (int c = 0; c < 128; c += 4)
+                for (int c = 0; c < 32; ++c) x[g + c] = vis >> c & 1u ? x[g + c] : 0xFF800000u;
+              }
+            }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], __uint_as_float(x[c + e]));
-      const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
-      const bool above = most > ref + HEADROOM;
-      if (__any_sync(0xffffffffu, above)) {
-        const float now = above ? ceilf(most) : ref, keep = above ? (ref == -INFINITY ? 0.f : ex2(ref - now)) : 1.f;
-        ref = now;
-        sum = fma2(sum, two(keep, keep), 0ull);
-        if (used) {
-          if (!(ok = bar_wait_warp(o_done(t), (used - 1) & 1, &s_gone, status))) break;
-          fence_after();
+            for (int e = 0; e < 32; ++e) {
+              const float2 f = apart(fma2(two(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale22, minus2));
+              const uint64_t z = e % 8 < POLY_OF_8 ? power2(f) : two(ex2(f.x), ex2(f.y));
+              here = add2(here, z);
+              const float2 g = apart(z);
+              pr[c0 / 2 + e] = half_pair(g.x, g.y);
+              top[e % 4] = max3(top[e % 4], __uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+            }
+          }
+          const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale2;
+          const bool unset = ref == -INFINITY;
+          const bool again = most > (unset ? 0.f : ref) + HEADROOM || (unset && most < LOWEST && most != -INFINITY);
+          if (!__any_sync(0xffffffffu, again)) {
+            if (unset && most != -INFINITY) ref = 0.f;
+            break;
+          }
+          const float now = again ? ceilf(most) : ref, keep = again && !unset ? ex2(ref - now) : 1.f;
+          ref = now;
+          sum = mul2(sum, two(keep, keep));
+          if (!first) {
+            if (!(ok = bar_wait_warp(o_done(t), (taken - 1) & 1, &s_gone, status))) break;
+            fence_after();
 #pragma unroll
-          for (int c = 0; c < D; c += 16) {
-            uint32_t y[16];
-            load16(at_o + c, y);
-            wait_load<16>(y);
+            for (int c = 0; c < D; c += 16) {
+              uint32_t y[16];
+              load16(at_o + c, y);
+              wait_load<16>(y);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * keep);
-            store16(at_o + c, y);
+              for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * keep);
+              store16(at_o + c, y);
+            }
           }
         }
+        if (!ok) break;
+        sum = add2(sum, here);
+        store32(at_s, pr);
+        store32(at_s + 32, pr + 32);
+        wait_store();
+        fence_before();
+        bar_arrive(p_full(t));
+        first = false;
+        ++taken;
       }
-      const float minus = LIFT - (ref == -INFINITY ? 0.f : ref);
-      const uint64_t scale22 = two(scale2, scale2), minus2 = two(minus, minus);
+      const float2 parts = apart(sum);
+      const float total = parts.x + parts.y;
+      const bool row = q < s.queries, empty = first || p >= w.n || (ref == -INFINITY && total == 0.f);
+      if (ok && !first) ok = bar_wait_warp(o_done(t), (taken - 1) & 1, &s_gone, status);
+      fence_after();
+      const float inv = empty ? 0.f : 1.f / total;
+      __half* to = out + (((size_t)w.b * s.queries + q) * s.n_heads + w.h) * D;
 #pragma unroll
-      for (int c = 0; c < 128; c += 32) {
-        uint32_t pr[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float2 y = apart(fma2(two(__uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1])), scale22, minus2));
-          y.x = ex2(y.x);
-          y.y = ex2(y.y);
-          sum = add2(sum, two(y.x, y.y));
-          pr[e] = half_pair(y.x, y.y);
+      for (int c = 0; c < D; c += 32) {
+        uint32_t y[32];
+        if (!first && ok) {
+          load32(at_o + c, y);
+          wait_load<32>(y);
         }
-        store16(at_s + c / 2, pr);
+        if (!row) continue;
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+          uint32_t v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = half_pair(__uint_as_float(y[e + 2 * k]) * inv, __uint_as_float(y[e + 2 * k + 1]) * inv);
+          *reinterpret_cast<uint4*>(to + c + e) = !ok ? make_uint4(~0u, ~0u, ~0u, ~0u) : (empty ? make_uint4(0, 0, 0, 0) : make_uint4(v[0], v[1], v[2], v[3]));
+        }
       }
-      wait_store();
-      fence_before();
-      bar_arrive(p_full(t));
-      ++used;
+      if (row) lse[((size_t)w.b * s.n_heads + w.h) * s.queries + q] = !ok ? NAN : (empty ? -INFINITY : ((ref == -INFINITY ? 0.f : ref) - LIFT + log2f(total)) * LN2);
     }
-    const float2 parts = apart(sum);
-    const float total = parts.x + parts.y;
-    const bool row = q < s.queries, empty = !used || p >= n || (ref == -INFINITY && total == 0.f);
-    if (ok && used) ok = bar_wait_warp(o_done(t), (used - 1) & 1, &s_gone, status);
-    fence_after();
-    const float inv = empty ? 0.f : 1.f / total;
-    __half* to = out + (((size_t)b * s.queries + q) * s.n_heads + h) * D;
-#pragma unroll
-    for (int c = 0; c < D; c += 32) {
-      uint32_t y[32];
-      if (used && ok) {
-        load32(at_o + c, y);
-        wait_load<32>(y);
-      }
-      if (!row) continue;
-#pragma unroll
-      for (int e = 0; e < 32; e += 8) {
-        uint32_t w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = half_pair(__uint_as_float(y[e + 2 * k]) * inv, __uint_as_float(y[e + 2 * k + 1]) * inv);
-        *reinterpret_cast<uint4*>(to + c + e) = !ok ? make_uint4(~0u, ~0u, ~0u, ~0u) : (empty ? make_uint4(0, 0, 0, 0) : make_uint4(w[0], w[1], w[2], w[3]));
-      }
-    }
-    if (row) lse[((size_t)b * s.n_heads + h) * s.queries + q] = !ok ? NAN : empty ? -INFINITY : ((ref == -INFINITY ? 0.f : ref) - LIFT + log2f(total)) * LN2;
   }
   fence_before();
   __syncthreads();
@@ -579,8 +677,10 @@ extern "C" int cq_attn_prefill(const cq_prompt* shape, const void* q, const void
     auto fn = D == 128 ? prompt_umma_kernel<128> : prompt_umma_kernel<64>;
     const int smem = (2 + UM_STAGES) * (D / 64) * UM_CHUNK + 1024;
     CQ_CUDA_TRY(cq_grant_smem((const void*)fn, smem));
-    const unsigned blocks = (unsigned)((shape->queries + 2 * UM_TILE - 1) / (2 * UM_TILE)) * shape->n_heads;
-    CQ_CUDA_TRY(kv4_launch(fn, dim3(blocks, B), dim3(UM_THREADS), smem, (cudaStream_t)stream, a, maps, (__half*)out, lse, status_word));
+    const long long items = (long long)((shape->queries + 2 * UM_TILE - 1) / (2 * UM_TILE)) * shape->n_heads * B;
+    if (items > INT32_MAX) return CQ_ERR_BAD_SHAPE;
+    CQ_CUDA_TRY(kv4_launch(fn, dim3((unsigned)std::min<long long>(items, cq_sm_count())), dim3(UM_THREADS), smem, (cudaStream_t)stream, a, maps,
+                           (__half*)out, lse, (int)items, status_word));
     return CQ_OK;
   }
   auto fn = D == 128 ? prompt_kernel<128> : prompt_kernel<64>;

@@ -24,9 +24,10 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
   return ok != 0;
 }
+// (Inlined: a function call does not go with setmaxnreg.)
 // Bounded wait: after two seconds of the device's clock (or at once where another wait of the CTA ran out) it gives up, notes
 // that in *gone and in the status word, and returns false; the CTA then runs on to its end.
-__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* gone, uint32_t* status) {
+__device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* gone, uint32_t* status) {
   unsigned long long t0 = 0;
   for (uint32_t it = 0; it < (1u << 26); ++it) {
     if (bar_try(bar, parity)) return true;
@@ -49,6 +50,12 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 // the same by a whole warp: all of its lanes go the same way
 __device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int* gone, uint32_t* status) {
   return __all_sync(0xffffffffu, bar_wait(bar, parity, gone, status));
+}
+// one lane of a converged warp; what it alone does with values that are the same in all lanes stays on the uniform datapath
+__device__ __forceinline__ bool elected() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -84,6 +91,7 @@ __device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t wide) {
 }
 #define CQ_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
 #define CQ_I8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+#define CQ_B8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
 // 32 columns of this warp's lanes
 __device__ __forceinline__ void load32(uint32_t at, uint32_t* r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -103,9 +111,9 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t* r) {
 }
 // Results of load32 may be used from here on: waits for them, and keeps the compiler from using them before.
 template <int N> __device__ __forceinline__ void wait_load(uint32_t* r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+  static_assert(N == 16 || N == 32, "");
+  if constexpr (N == 16) asm volatile("tcgen05.wait::ld.sync.aligned;" : CQ_B8(r, 0), CQ_B8(r, 8)::"memory");
+  else asm volatile("tcgen05.wait::ld.sync.aligned;" : CQ_B8(r, 0), CQ_B8(r, 8), CQ_B8(r, 16), CQ_B8(r, 24)::"memory");
 }
 __device__ __forceinline__ void wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // a box of a tensor map to shared memory
