@@ -350,7 +350,8 @@ int cq_attn_prefill(const cq_prompt* shape, const void* q_f16, const void* k_f16
  * weights (sequences, n_kv_heads, keys) fp32 = sum over them and the head's queries of exp(scale * q . k_j - lse); 0 where no
  * such query sees the key. */
 int cq_attn_prefill_weights(const cq_prompt* shape, const void* q_f16, const void* k_f16, const float* lse,
-                            const long long* lengths, int observe, float* weights, cq_stream_t stream);
+                            const long long* lengths, int observe, float* weights, uint32_t* status_word,
+                            cq_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Tile-layout prepared layer: the format of the tcgen05 (UMMA + tensor memory) kernels.

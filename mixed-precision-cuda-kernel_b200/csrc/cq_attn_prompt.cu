@@ -570,9 +570,231 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_umma_kernel(const __grid
   }
 }
 
-// Tensor map of q, k or v (sequence, token, head strides in halves): boxes of 64 columns x 128 tokens.  A broadcast sequence or
+// ------------------------------------------------------------------ weights of the keys on tcgen05
+// S^T = K . Q^T of 128 keys (lanes of tensor memory, a thread each) and 128 queries (columns): a key's weight is a sum along
+// its thread's own columns, so nothing is exchanged.  The columns are two blocks of 64 queries, of any two heads and places:
+// queries of a head that are fewer than 128 do not leave a tile half empty.  Bound by the exponentials, one for each pair and
+// 16 a cycle and SM (1024 cycles a tile, its MMAs 540); some of them are polynomials.
+//   warps 0-3, 4-7  every other tile each: sums of exponentials; joined at the end of an item
+//   warp 8          TMA of K, Q;  warp 9  MMAs, four score buffers ahead;  warp 10  the queries' lse
+constexpr int KW_THREADS = 352, KW_Q = 64, KW_BUFFERS = 4;
+constexpr int W_LSE = 10;
+constexpr int KW_POLY_OF_8 = 2;
+
+// An item: 128 keys of a KV head, the queries [first, last) of its heads in blocks of 64
+struct KeysItem {
+  int b, kvh, k0, n, first, last, per_head, blocks, tiles;
+  __device__ __forceinline__ KeysItem(const PromptArgs& a, int item, int observe) {
+    const cq_prompt& s = a.s;
+    const int per = s.n_kv_heads * s.sequences, rest = item % per;
+    k0 = item / per * UM_TILE;
+    b = rest / s.n_kv_heads;
+    kvh = rest - b * s.n_kv_heads;
+    n = length_of(a, b);
+    first = max(max(s.keys - s.queries, n - observe), k0);
+    last = s.window && k0 >= s.sinks ? (int)min((long long)n, min(k0 + UM_TILE, n) - 1 + (long long)s.window) : n;
+    per_head = max(0, last - first + KW_Q - 1) / KW_Q;
+    blocks = per_head * (s.n_heads / s.n_kv_heads);
+    tiles = (blocks + 1) / 2;
+  }
+  __device__ __forceinline__ int head(int block) const { return block / per_head; }
+  __device__ __forceinline__ int place(int block) const { return first + KW_Q * (block % per_head); }
+};
+
+template <int D>
+__global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ PromptMaps maps,
+                                                                    const float* __restrict__ lse, int observe, float* __restrict__ weights, int items,
+                                                                    uint32_t* __restrict__ status) {
+  using namespace umma;
+  constexpr int CH = D / 64, TILE_BYTES = CH * UM_CHUNK;
+  extern __shared__ __align__(1024) uint8_t um_smem[];
+  __shared__ __align__(8) uint64_t s_bar[5 + 5 * KW_BUFFERS];
+  __shared__ __align__(16) float s_lse[KW_BUFFERS][UM_TILE];
+  __shared__ float s_sum[UM_TILE];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_gone;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t smem = (smem_at(um_smem) + 1023u) & ~1023u, s_k = smem, s_q = smem + 2 * TILE_BYTES;
+  const uint32_t bars = smem_at(s_bar), drained = bars;
+  auto k_full = [&](int i) { return bars + 8 * (1 + i); };
+  auto k_free = [&](int i) { return bars + 8 * (3 + i); };
+  auto q_full = [&](int i) { return bars + 8 * (5 + i); };
+  auto q_free = [&](int i) { return bars + 8 * (5 + KW_BUFFERS + i); };
+  auto s_full = [&](int i) { return bars + 8 * (5 + 2 * KW_BUFFERS + i); };
+  auto s_free = [&](int i) { return bars + 8 * (5 + 3 * KW_BUFFERS + i); };
+  auto l_full = [&](int i) { return bars + 8 * (5 + 4 * KW_BUFFERS + i); };
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) {
+    bar_init(drained, 1);
+    for (int i = 0; i < 2; ++i) {
+      bar_init(k_full(i), 1);
+      bar_init(k_free(i), 1);
+    }
+    for (int i = 0; i < KW_BUFFERS; ++i) {
+      bar_init(q_full(i), 1);
+      bar_init(q_free(i), 1);
+      bar_init(s_full(i), 1);
+      bar_init(s_free(i), 128);
+      bar_init(l_full(i), 32);
+    }
+    s_gone = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == W_MMA) alloc(&s_tmem, 512);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = s_tmem;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const cq_prompt& s = a.s;
+  const int off = s.keys - s.queries, G = s.n_heads / s.n_kv_heads;
+
+  if (warp == W_LOAD) {
+    if (lane == 0) {
+      uint32_t loaded = 0, sent = 0;                       // key tiles, query tiles
+      bool ok = true;
+      for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
+        const KeysItem w(a, item, observe);
+        if (!w.tiles) continue;
+        const uint32_t kb = loaded & 1;
+        if (loaded >= 2 && !(ok = bar_wait(k_free(kb), (loaded / 2 - 1) & 1, &s_gone, status))) break;
+        bar_expect(k_full(kb), TILE_BYTES);
+        for (int c = 0; c < CH; ++c)
+          tma(s_k + kb * TILE_BYTES + c * UM_CHUNK, &maps.k, 64 * c, w.k0, w.kvh * maps.one[1][0], w.b * maps.one[1][1], k_full(kb));
+        ++loaded;
+        for (int j = 0; j < w.tiles; ++j, ++sent) {
+          const uint32_t st = sent % KW_BUFFERS, use = sent / KW_BUFFERS;
+          if (use && !(ok = bar_wait(q_free(st), (use - 1) & 1, &s_gone, status))) break;
+          bar_expect(q_full(st), TILE_BYTES);
+          for (int e = 0; e < 2; ++e) {
+            const int block = min(2 * j + e, w.blocks - 1);      // (the last tile may have one block: the other one is not used)
+            for (int c = 0; c < CH; ++c)
+              tma(s_q + st * TILE_BYTES + c * UM_CHUNK + e * (UM_CHUNK / 2), &maps.q, 64 * c, w.place(block) - off,
+                  (w.kvh * G + w.head(block)) * maps.one[0][0], w.b * maps.one[0][1], q_full(st));
+          }
+        }
+      }
+      if (!ok) {                                           // copies in flight end before the CTA does
+        for (uint32_t i = loaded > 2 ? loaded - 2 : 0; i < loaded; ++i)
+          for (int k = 0; k < 1000 && !bar_try(k_full(i & 1), (i / 2) & 1); ++k) {}
+        for (uint32_t i = sent > KW_BUFFERS ? sent - KW_BUFFERS : 0; i < sent; ++i)
+          for (int k = 0; k < 1000 && !bar_try(q_full(i % KW_BUFFERS), (i / KW_BUFFERS) & 1); ++k) {}
+      }
+    }
+  } else if (warp == W_MMA) {
+    constexpr uint32_t SHAPE = shape_of(128, 128, false);
+    uint32_t loaded = 0, sent = 0;
+    bool ok = true;
+    for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
+      const KeysItem w(a, item, observe);
+      if (!w.tiles) continue;
+      const uint32_t kb = loaded & 1;
+      ok = bar_wait_warp(k_full(kb), (loaded / 2) & 1, &s_gone, status);
+      for (int j = 0; j < w.tiles && ok; ++j, ++sent) {
+        const uint32_t st = sent % KW_BUFFERS, use = sent / KW_BUFFERS;
+        ok = bar_wait_warp(q_full(st), use & 1, &s_gone, status) && (!use || bar_wait_warp(s_free(st), (use - 1) & 1, &s_gone, status));
+        if (!ok) break;
+        fence_after();
+        if (elected()) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t at = (k / 4) * UM_CHUNK + (k % 4) * 32;
+            mma_ss(tmem + 128 * st, operand(s_k + kb * TILE_BYTES + at, 0), operand(s_q + st * TILE_BYTES + at, 0), SHAPE, k > 0);
+          }
+          commit(q_free(st));
+          commit(s_full(st));
+        }
+        __syncwarp();
+      }
+      if (ok && elected()) commit(k_free(kb));
+      __syncwarp();
+      ++loaded;
+    }
+    // nothing is in flight when the tensor memory is given back and the CTA ends
+    if (elected()) commit(drained);
+    for (int k = 0; k < 100000 && !bar_try(drained, 0); ++k) {}
+    __syncwarp();
+  } else if (warp == W_LSE) {
+    uint32_t sent = 0;
+    bool ok = true;
+    for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
+      const KeysItem w(a, item, observe);
+      for (int j = 0; j < w.tiles && ok; ++j, ++sent) {
+        const uint32_t st = sent % KW_BUFFERS, use = sent / KW_BUFFERS;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {                      // minus lse in powers of two; what is not a query counts as nothing
+          const int block = 2 * j + e / 2, p = block < w.blocks ? w.place(block) + 32 * (e & 1) + lane : w.last;
+          v[e] = p < w.last ? -LOG2E * lse[((size_t)w.b * s.n_heads + w.kvh * G + w.head(block)) * s.queries + p - off] : -INFINITY;
+        }
+        ok = !use || bar_wait_warp(s_free(st), (use - 1) & 1, &s_gone, status);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s_lse[st][32 * e + lane] = v[e];
+        bar_arrive(l_full(st));
+      }
+    }
+  } else {
+    const int wg = warp >> 2, r = tid & 127;
+    const float scale2 = s.scale * LOG2E;
+    const uint64_t scale22 = two(scale2, scale2);
+    uint32_t seen = 0;                                     // tiles of all items
+    bool ok = true;
+    for (int round = 0, item; (item = PromptItem::at(round, items)) >= 0; ++round) {
+      const KeysItem w(a, item, observe);
+      const int key = w.k0 + r;
+      const int lo = key < w.n ? max(w.first, key) : w.last, hi = min(w.last, s.window && key >= s.sinks ? (int)min((long long)w.last, key + (long long)s.window) : w.last) - 1;
+      uint64_t sum[2] = {};
+      for (int j = 0; j < w.tiles; ++j, ++seen) {
+        if ((j & 1) != wg || !ok) continue;
+        const uint32_t st = seen % KW_BUFFERS, use = seen / KW_BUFFERS;
+        ok = bar_wait_warp(l_full(st), use & 1, &s_gone, status) && bar_wait_warp(s_full(st), use & 1, &s_gone, status);
+        if (!ok) continue;
+        fence_after();
+        const uint32_t at = tmem + 128 * st + ((uint32_t)(warp & 3) << 21);
+#pragma unroll
+        for (int c0 = 0; c0 < 128; c0 += 32) {
+          uint32_t x[32];
+          load32(at + c0, x);
+          wait_load<32>(x);
+          const int block = 2 * j + c0 / 64, p0 = block < w.blocks ? w.place(block) + c0 % 64 : w.last;
+          const bool whole = w.k0 + UM_TILE - 1 <= p0 && p0 + 32 <= w.last && (!s.window || w.k0 + UM_TILE - 1 < s.sinks || p0 + 31 < w.k0 + s.window);
+          if (!whole) {
+            const uint32_t vis = below32(hi + 1 - p0) & ~below32(lo - p0);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) x[c] = vis >> c & 1u ? x[c] : 0xFF800000u;
+          }
+          const ulonglong2* less = reinterpret_cast<const ulonglong2*>(&s_lse[st][c0]);
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            const ulonglong2 m = less[e / 2];
+            const float2 f = apart(fma2(two(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale22, m.x));
+            const float2 g = apart(fma2(two(__uint_as_float(x[2 * e + 2]), __uint_as_float(x[2 * e + 3])), scale22, m.y));
+            sum[0] = add2(sum[0], e % 8 < KW_POLY_OF_8 ? power2(f) : two(ex2(f.x), ex2(f.y)));
+            sum[1] = add2(sum[1], two(ex2(g.x), ex2(g.y)));
+          }
+        }
+        fence_before();
+        bar_arrive(s_free(st));
+      }
+      const float2 parts = apart(add2(sum[0], sum[1]));
+      const float total = ok ? parts.x + parts.y : NAN;
+      if (wg) s_sum[r] = total;
+      asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+      if (!wg && key < s.keys) weights[((size_t)w.b * s.n_kv_heads + w.kvh) * s.keys + key] = total + s_sum[r];
+      asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == W_MMA) {
+    fence_after();
+    dealloc(tmem, 512);
+  }
+}
+
+// Tensor map of q, k or v (sequence, token, head strides in halves): boxes of 64 columns x `rows` tokens.  A broadcast sequence or
 // head (stride 0) is one of them, addressed with the coordinate 0 (one[]).  False where the map cannot describe the tensor.
-bool map_of(CUtensorMap* map, const void* at, const int64_t (&strides)[3], int sequences, int tokens, int heads, int D, int (&one)[2]) {
+bool map_of(CUtensorMap* map, const void* at, const int64_t (&strides)[3], int sequences, int tokens, int heads, int D, int rows, int (&one)[2]) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   static const Encode encode = []() -> Encode {
@@ -591,7 +813,7 @@ bool map_of(CUtensorMap* map, const void* at, const int64_t (&strides)[3], int s
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)tokens, one[0] ? (cuuint64_t)heads : 1, one[1] ? (cuuint64_t)sequences : 1};
   const cuuint64_t steps[3] = {tokens > 1 ? (cuuint64_t)strides[1] * 2 : (cuuint64_t)D * 2, one[0] ? (cuuint64_t)strides[2] * 2 : (cuuint64_t)D * 2,
                                one[1] ? (cuuint64_t)strides[0] * 2 : (cuuint64_t)D * 2};
-  const cuuint32_t box[4] = {64, UM_TILE, 1, 1}, each[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, each[4] = {1, 1, 1, 1};
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(at), dims, steps, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -671,9 +893,9 @@ extern "C" int cq_attn_prefill(const cq_prompt* shape, const void* q, const void
   const PromptArgs a = {*shape, (const __half*)q, (const __half*)k, (const __half*)v, lengths};
   const int D = shape->head_dim, B = shape->sequences;
   PromptMaps maps;
-  if (map_of(&maps.q, q, shape->q_strides, B, shape->queries, shape->n_heads, D, maps.one[0]) &&
-      map_of(&maps.k, k, shape->k_strides, B, shape->keys, shape->n_kv_heads, D, maps.one[1]) &&
-      map_of(&maps.v, v, shape->v_strides, B, shape->keys, shape->n_kv_heads, D, maps.one[2])) {
+  if (map_of(&maps.q, q, shape->q_strides, B, shape->queries, shape->n_heads, D, UM_TILE, maps.one[0]) &&
+      map_of(&maps.k, k, shape->k_strides, B, shape->keys, shape->n_kv_heads, D, UM_TILE, maps.one[1]) &&
+      map_of(&maps.v, v, shape->v_strides, B, shape->keys, shape->n_kv_heads, D, UM_TILE, maps.one[2])) {
     auto fn = D == 128 ? prompt_umma_kernel<128> : prompt_umma_kernel<64>;
     const int smem = (2 + UM_STAGES) * (D / 64) * UM_CHUNK + 1024;
     CQ_CUDA_TRY(cq_grant_smem((const void*)fn, smem));
@@ -690,13 +912,27 @@ extern "C" int cq_attn_prefill(const cq_prompt* shape, const void* q, const void
 }
 
 extern "C" int cq_attn_prefill_weights(const cq_prompt* shape, const void* q, const void* k, const float* lse, const long long* lengths,
-                                       int observe, float* weights, cq_stream_t stream) {
+                                       int observe, float* weights, uint32_t* status_word, cq_stream_t stream) {
   const int rc = check(shape, q, k, nullptr);
   if (rc != CQ_OK) return rc;
   if (!lse || !weights || observe < 1) return CQ_ERR_BAD_ARG;
   const PromptArgs a = {*shape, (const __half*)q, (const __half*)k, nullptr, lengths};
-  auto fn = shape->head_dim == 128 ? prompt_weights_kernel<128> : prompt_weights_kernel<64>;
-  CQ_CUDA_TRY(kv4_launch(fn, dim3((shape->keys + PR_TILE - 1) / PR_TILE, shape->n_kv_heads, shape->sequences), dim3(PR_THREADS), 0,
-                         (cudaStream_t)stream, a, lse, observe, weights));
+  const int D = shape->head_dim, B = shape->sequences;
+  PromptMaps maps;
+  if (map_of(&maps.q, q, shape->q_strides, B, shape->queries, shape->n_heads, D, KW_Q, maps.one[0]) &&
+      map_of(&maps.k, k, shape->k_strides, B, shape->keys, shape->n_kv_heads, D, UM_TILE, maps.one[1])) {
+    maps.v = maps.k;
+    auto fn = D == 128 ? prompt_keys_kernel<128> : prompt_keys_kernel<64>;
+    const int smem = (2 + KW_BUFFERS) * (D / 64) * UM_CHUNK + 1024;
+    CQ_CUDA_TRY(cq_grant_smem((const void*)fn, smem));
+    const long long items = (long long)((shape->keys + UM_TILE - 1) / UM_TILE) * shape->n_kv_heads * B;
+    if (items > INT32_MAX) return CQ_ERR_BAD_SHAPE;
+    CQ_CUDA_TRY(kv4_launch(fn, dim3((unsigned)std::min<long long>(items, cq_sm_count())), dim3(KW_THREADS), smem, (cudaStream_t)stream, a, maps, lse,
+                           observe, weights, (int)items, status_word));
+    return CQ_OK;
+  }
+  auto fn = D == 128 ? prompt_weights_kernel<128> : prompt_weights_kernel<64>;
+  CQ_CUDA_TRY(kv4_launch(fn, dim3((shape->keys + PR_TILE - 1) / PR_TILE, shape->n_kv_heads, B), dim3(PR_THREADS), 0, (cudaStream_t)stream, a, lse,
+                         observe, weights));
   return CQ_OK;
 }

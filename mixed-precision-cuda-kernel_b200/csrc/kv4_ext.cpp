@@ -295,7 +295,7 @@ torch::Tensor attn_prefill_weights(const torch::Tensor& q, const torch::Tensor& 
   auto out = torch::empty({s.sequences, s.n_kv_heads, s.keys}, lse.options());
   check_status(cq_attn_prefill_weights(&s, q.const_data_ptr(), k.const_data_ptr(), lse.const_data_ptr<float>(), n,
                                        (int)std::min<int64_t>(last, s.keys), out.data_ptr<float>(),
-                                       (cq_stream_t)c10::cuda::getCurrentCUDAStream().stream()),
+                                       device_status(q.device()), (cq_stream_t)c10::cuda::getCurrentCUDAStream().stream()),
                "attn_prefill_weights");
   return out;
 }
