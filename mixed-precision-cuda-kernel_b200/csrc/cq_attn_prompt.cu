@@ -576,9 +576,8 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_umma_kernel(const __grid
 // queries of a head that are fewer than 128 do not leave a tile half empty.  Bound by the exponentials, one for each pair and
 // 16 a cycle and SM (1024 cycles a tile, its MMAs 540); some of them are polynomials.
 //   warps 0-3, 4-7  every other tile each: sums of exponentials; joined at the end of an item
-//   warp 8          TMA of K, Q;  warp 9  MMAs, four score buffers ahead;  warp 10  the queries' lse
-constexpr int KW_THREADS = 352, KW_Q = 64, KW_BUFFERS = 4;
-constexpr int W_LSE = 10;
+//   warp 8          TMA of K, Q;  warp 9  MMAs, up to four score buffers ahead
+constexpr int KW_THREADS = 320, KW_Q = 64, KW_BUFFERS = 4;
 constexpr int KW_POLY_OF_8 = 2;
 
 // An item: 128 keys of a KV head, the queries [first, last) of its heads in blocks of 64
@@ -597,8 +596,18 @@ struct KeysItem {
     blocks = per_head * (s.n_heads / s.n_kv_heads);
     tiles = (blocks + 1) / 2;
   }
-  __device__ __forceinline__ int head(int block) const { return block / per_head; }
-  __device__ __forceinline__ int place(int block) const { return first + KW_Q * (block % per_head); }
+};
+// a block's head (of the KV head's) and place in it; steps forward without a division
+struct Block {
+  int head = 0, at = 0;
+  __device__ __forceinline__ void step(const KeysItem& w, int n) {
+    at += n;
+    while (at >= w.per_head) {
+      at -= w.per_head;
+      ++head;
+    }
+  }
+  __device__ __forceinline__ int position(const KeysItem& w) const { return w.first + KW_Q * at; }
 };
 
 template <int D>
@@ -608,8 +617,8 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
   using namespace umma;
   constexpr int CH = D / 64, TILE_BYTES = CH * UM_CHUNK;
   extern __shared__ __align__(1024) uint8_t um_smem[];
-  __shared__ __align__(8) uint64_t s_bar[5 + 5 * KW_BUFFERS];
-  __shared__ __align__(16) float s_lse[KW_BUFFERS][UM_TILE];
+  __shared__ __align__(8) uint64_t s_bar[5 + 4 * KW_BUFFERS];
+  __shared__ __align__(16) float s_lse[4][UM_TILE];
   __shared__ float s_sum[UM_TILE];
   __shared__ uint32_t s_tmem;
   __shared__ int s_gone;
@@ -622,7 +631,6 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
   auto q_free = [&](int i) { return bars + 8 * (5 + KW_BUFFERS + i); };
   auto s_full = [&](int i) { return bars + 8 * (5 + 2 * KW_BUFFERS + i); };
   auto s_free = [&](int i) { return bars + 8 * (5 + 3 * KW_BUFFERS + i); };
-  auto l_full = [&](int i) { return bars + 8 * (5 + 4 * KW_BUFFERS + i); };
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     bar_init(drained, 1);
@@ -635,7 +643,6 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
       bar_init(q_free(i), 1);
       bar_init(s_full(i), 1);
       bar_init(s_free(i), 128);
-      bar_init(l_full(i), 32);
     }
     s_gone = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -662,15 +669,16 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
         for (int c = 0; c < CH; ++c)
           tma(s_k + kb * TILE_BYTES + c * UM_CHUNK, &maps.k, 64 * c, w.k0, w.kvh * maps.one[1][0], w.b * maps.one[1][1], k_full(kb));
         ++loaded;
+        Block block;
         for (int j = 0; j < w.tiles; ++j, ++sent) {
           const uint32_t st = sent % KW_BUFFERS, use = sent / KW_BUFFERS;
           if (use && !(ok = bar_wait(q_free(st), (use - 1) & 1, &s_gone, status))) break;
           bar_expect(q_full(st), TILE_BYTES);
           for (int e = 0; e < 2; ++e) {
-            const int block = min(2 * j + e, w.blocks - 1);      // (the last tile may have one block: the other one is not used)
             for (int c = 0; c < CH; ++c)
-              tma(s_q + st * TILE_BYTES + c * UM_CHUNK + e * (UM_CHUNK / 2), &maps.q, 64 * c, w.place(block) - off,
-                  (w.kvh * G + w.head(block)) * maps.one[0][0], w.b * maps.one[0][1], q_full(st));
+              tma(s_q + st * TILE_BYTES + c * UM_CHUNK + e * (UM_CHUNK / 2), &maps.q, 64 * c, block.position(w) - off,
+                  (w.kvh * G + block.head) * maps.one[0][0], w.b * maps.one[0][1], q_full(st));
+            if (2 * j + e + 1 < w.blocks) block.step(w, 1);      // (the last tile may have one block: it fills the other place, unused)
           }
         }
       }
@@ -714,40 +722,45 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
     if (elected()) commit(drained);
     for (int k = 0; k < 100000 && !bar_try(drained, 0); ++k) {}
     __syncwarp();
-  } else if (warp == W_LSE) {
-    uint32_t sent = 0;
-    bool ok = true;
-    for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
-      const KeysItem w(a, item, observe);
-      for (int j = 0; j < w.tiles && ok; ++j, ++sent) {
-        const uint32_t st = sent % KW_BUFFERS, use = sent / KW_BUFFERS;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {                      // minus lse in powers of two; what is not a query counts as nothing
-          const int block = 2 * j + e / 2, p = block < w.blocks ? w.place(block) + 32 * (e & 1) + lane : w.last;
-          v[e] = p < w.last ? -LOG2E * lse[((size_t)w.b * s.n_heads + w.kvh * G + w.head(block)) * s.queries + p - off] : -INFINITY;
-        }
-        ok = !use || bar_wait_warp(s_free(st), (use - 1) & 1, &s_gone, status);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s_lse[st][32 * e + lane] = v[e];
-        bar_arrive(l_full(st));
-      }
-    }
   } else {
     const int wg = warp >> 2, r = tid & 127;
     const float scale2 = s.scale * LOG2E;
     const uint64_t scale22 = two(scale2, scale2);
-    uint32_t seen = 0;                                     // tiles of all items
+    uint32_t seen = 0;                                     // tiles of all items before this one
     bool ok = true;
     for (int round = 0, item; (item = PromptItem::at(round, items)) >= 0; ++round) {
       const KeysItem w(a, item, observe);
       const int key = w.k0 + r;
-      const int lo = key < w.n ? max(w.first, key) : w.last, hi = min(w.last, s.window && key >= s.sinks ? (int)min((long long)w.last, key + (long long)s.window) : w.last) - 1;
+      // the positions of the queries that see this key
+      const int lo = key < w.n ? max(w.first, key) : w.last;
+      const int hi = min(w.last, s.window && key >= s.sinks ? (int)min((long long)w.last, key + (long long)s.window) : w.last) - 1;
       uint64_t sum[2] = {};
-      for (int j = 0; j < w.tiles; ++j, ++seen) {
-        if ((j & 1) != wg || !ok) continue;
-        const uint32_t st = seen % KW_BUFFERS, use = seen / KW_BUFFERS;
-        ok = bar_wait_warp(l_full(st), use & 1, &s_gone, status) && bar_wait_warp(s_full(st), use & 1, &s_gone, status);
+      // this group's tiles are every other one; their two blocks, and minus the lse (in powers of two) of column r a tile ahead
+      Block block[2];
+      if (wg < w.tiles) {
+        block[0].step(w, 2 * wg);
+        block[1].step(w, 2 * wg + 1);
+      }
+      auto minus_lse = [&](int j) {
+        const Block& mine = block[r >> 6];
+        const int p = mine.position(w) + (r & 63);
+        return 2 * j + (r >> 6) < w.blocks && p < w.last ? -LOG2E * lse[((size_t)w.b * s.n_heads + w.kvh * G + mine.head) * s.queries + p - off] : -INFINITY;
+      };
+      float ahead = wg < w.tiles ? minus_lse(wg) : 0.f;
+      for (int j = wg; j < w.tiles; j += 2) {
+        const uint32_t tile = seen + j, st = tile % KW_BUFFERS, use = tile / KW_BUFFERS;
+        int place[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) place[e] = 2 * j + e < w.blocks ? block[e].position(w) : w.last;
+        float* mine = s_lse[2 * wg + (j >> 1 & 1)];
+        mine[r] = ahead;
+        if (j + 2 < w.tiles) {
+          block[0].step(w, 4);
+          block[1].step(w, 4);
+          ahead = minus_lse(j + 2);
+        }
+        asm volatile("barrier.cta.sync %0, 128;" ::"r"(2 + wg) : "memory");
+        ok = ok && bar_wait_warp(s_full(st), use & 1, &s_gone, status);
         if (!ok) continue;
         fence_after();
         const uint32_t at = tmem + 128 * st + ((uint32_t)(warp & 3) << 21);
@@ -756,14 +769,14 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
           uint32_t x[32];
           load32(at + c0, x);
           wait_load<32>(x);
-          const int block = 2 * j + c0 / 64, p0 = block < w.blocks ? w.place(block) + c0 % 64 : w.last;
+          const int p0 = place[c0 / 64] + c0 % 64;
           const bool whole = w.k0 + UM_TILE - 1 <= p0 && p0 + 32 <= w.last && (!s.window || w.k0 + UM_TILE - 1 < s.sinks || p0 + 31 < w.k0 + s.window);
           if (!whole) {
             const uint32_t vis = below32(hi + 1 - p0) & ~below32(lo - p0);
 #pragma unroll
             for (int c = 0; c < 32; ++c) x[c] = vis >> c & 1u ? x[c] : 0xFF800000u;
           }
-          const ulonglong2* less = reinterpret_cast<const ulonglong2*>(&s_lse[st][c0]);
+          const ulonglong2* less = reinterpret_cast<const ulonglong2*>(mine + c0);
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
             const ulonglong2 m = less[e / 2];
@@ -776,6 +789,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
         fence_before();
         bar_arrive(s_free(st));
       }
+      seen += w.tiles;
       const float2 parts = apart(add2(sum[0], sum[1]));
       const float total = ok ? parts.x + parts.y : NAN;
       if (wg) s_sum[r] = total;
