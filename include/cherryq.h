@@ -348,10 +348,12 @@ int cq_attn_prefill(const cq_prompt* shape, const void* q_f16, const void* k_f16
                     void* out_f16, float* lse, uint32_t* status_word, cq_stream_t stream);
 /* The weight that each key received from the last `observe` positions of its sequence (of those that are among the queries):
  * weights (sequences, n_kv_heads, keys) fp32 = sum over them and the head's queries of exp(scale * q . k_j - lse); 0 where no
- * such query sees the key. */
+ * such query sees the key.  workspace: device memory of cq_attn_prefill_weights_workspace_bytes(...) bytes, not shared by
+ * calls that can overlap. */
+size_t cq_attn_prefill_weights_workspace_bytes(const cq_prompt* shape, int observe);
 int cq_attn_prefill_weights(const cq_prompt* shape, const void* q_f16, const void* k_f16, const float* lse,
-                            const long long* lengths, int observe, float* weights, uint32_t* status_word,
-                            cq_stream_t stream);
+                            const long long* lengths, int observe, float* weights, void* workspace,
+                            uint32_t* status_word, cq_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Tile-layout prepared layer: the format of the tcgen05 (UMMA + tensor memory) kernels.

@@ -8,6 +8,7 @@
 //
 // mma.sync tiles: 64 queries of a head against 64 keys at a time, four warps of 16 queries, a running maximum and sum per row.
 #include <algorithm>
+#include <cmath>
 
 #include "cq_kv4.cuh"
 #include "cq_umma.cuh"
@@ -580,12 +581,13 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_umma_kernel(const __grid
 constexpr int KW_THREADS = 320, KW_Q = 64, KW_BUFFERS = 4;
 constexpr int KW_POLY_OF_8 = 2;
 
-// An item: 128 keys of a KV head, the queries [first, last) of its heads in blocks of 64
+// An item: 128 keys of a KV head, the queries [first, last) of its heads in blocks of 64, and of those one of `parts` parts
 struct KeysItem {
-  int b, kvh, k0, n, first, last, per_head, blocks, tiles;
-  __device__ __forceinline__ KeysItem(const PromptArgs& a, int item, int observe) {
+  int b, kvh, k0, n, first, last, per_head, begin, blocks, tiles, part;
+  __device__ __forceinline__ KeysItem(const PromptArgs& a, int item, int observe, int parts) {
     const cq_prompt& s = a.s;
-    const int per = s.n_kv_heads * s.sequences, rest = item % per;
+    const int per = s.n_kv_heads * s.sequences * parts, rest_p = item % per, rest = rest_p / parts;
+    part = rest_p - rest * parts;
     k0 = item / per * UM_TILE;
     b = rest / s.n_kv_heads;
     kvh = rest - b * s.n_kv_heads;
@@ -593,13 +595,21 @@ struct KeysItem {
     first = max(max(s.keys - s.queries, n - observe), k0);
     last = s.window && k0 >= s.sinks ? (int)min((long long)n, min(k0 + UM_TILE, n) - 1 + (long long)s.window) : n;
     per_head = max(0, last - first + KW_Q - 1) / KW_Q;
-    blocks = per_head * (s.n_heads / s.n_kv_heads);
+    const int all = per_head * (s.n_heads / s.n_kv_heads);
+    begin = (int)((long long)all * part / parts);
+    blocks = (int)((long long)all * (part + 1) / parts) - begin;
     tiles = (blocks + 1) / 2;
   }
 };
 // a block's head (of the KV head's) and place in it; steps forward without a division
 struct Block {
-  int head = 0, at = 0;
+  int head, at;
+  __device__ __forceinline__ explicit Block(const KeysItem& w, int n) : head(0), at(0) {
+    if (w.blocks) {
+      head = (w.begin + n) / w.per_head;
+      at = w.begin + n - head * w.per_head;
+    }
+  }
   __device__ __forceinline__ void step(const KeysItem& w, int n) {
     at += n;
     while (at >= w.per_head) {
@@ -612,7 +622,7 @@ struct Block {
 
 template <int D>
 __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ PromptMaps maps,
-                                                                    const float* __restrict__ lse, int observe, float* __restrict__ weights, int items,
+                                                                    const float* __restrict__ lse, int observe, int parts, float* __restrict__ weights, int items,
                                                                     uint32_t* __restrict__ status) {
   using namespace umma;
   constexpr int CH = D / 64, TILE_BYTES = CH * UM_CHUNK;
@@ -661,7 +671,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
       uint32_t loaded = 0, sent = 0;                       // key tiles, query tiles
       bool ok = true;
       for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
-        const KeysItem w(a, item, observe);
+        const KeysItem w(a, item, observe, parts);
         if (!w.tiles) continue;
         const uint32_t kb = loaded & 1;
         if (loaded >= 2 && !(ok = bar_wait(k_free(kb), (loaded / 2 - 1) & 1, &s_gone, status))) break;
@@ -669,7 +679,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
         for (int c = 0; c < CH; ++c)
           tma(s_k + kb * TILE_BYTES + c * UM_CHUNK, &maps.k, 64 * c, w.k0, w.kvh * maps.one[1][0], w.b * maps.one[1][1], k_full(kb));
         ++loaded;
-        Block block;
+        Block block(w, 0);
         for (int j = 0; j < w.tiles; ++j, ++sent) {
           const uint32_t st = sent % KW_BUFFERS, use = sent / KW_BUFFERS;
           if (use && !(ok = bar_wait(q_free(st), (use - 1) & 1, &s_gone, status))) break;
@@ -694,7 +704,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
     uint32_t loaded = 0, sent = 0;
     bool ok = true;
     for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
-      const KeysItem w(a, item, observe);
+      const KeysItem w(a, item, observe, parts);
       if (!w.tiles) continue;
       const uint32_t kb = loaded & 1;
       ok = bar_wait_warp(k_full(kb), (loaded / 2) & 1, &s_gone, status);
@@ -729,18 +739,14 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
     uint32_t seen = 0;                                     // tiles of all items before this one
     bool ok = true;
     for (int round = 0, item; (item = PromptItem::at(round, items)) >= 0; ++round) {
-      const KeysItem w(a, item, observe);
+      const KeysItem w(a, item, observe, parts);
       const int key = w.k0 + r;
       // the positions of the queries that see this key
       const int lo = key < w.n ? max(w.first, key) : w.last;
       const int hi = min(w.last, s.window && key >= s.sinks ? (int)min((long long)w.last, key + (long long)s.window) : w.last) - 1;
       uint64_t sum[2] = {};
       // this group's tiles are every other one; their two blocks, and minus the lse (in powers of two) of column r a tile ahead
-      Block block[2];
-      if (wg < w.tiles) {
-        block[0].step(w, 2 * wg);
-        block[1].step(w, 2 * wg + 1);
-      }
+      Block block[2] = {Block(w, 2 * wg), Block(w, 2 * wg + 1)};
       auto minus_lse = [&](int j) {
         const Block& mine = block[r >> 6];
         const int p = mine.position(w) + (r & 63);
@@ -794,7 +800,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
       const float total = ok ? parts.x + parts.y : NAN;
       if (wg) s_sum[r] = total;
       asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
-      if (!wg && key < s.keys) weights[((size_t)w.b * s.n_kv_heads + w.kvh) * s.keys + key] = total + s_sum[r];
+      if (!wg && key < s.keys) weights[(((size_t)w.part * s.sequences + w.b) * s.n_kv_heads + w.kvh) * s.keys + key] = total + s_sum[r];
       asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
     }
   }
@@ -804,6 +810,45 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
     fence_after();
     dealloc(tmem, 512);
   }
+}
+
+// the parts' sums, in order
+__global__ void __launch_bounds__(256) prompt_join_kernel(const float* __restrict__ part, int parts, long long n, float* __restrict__ weights) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float sum = 0.f;
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) sum += part[p * n + i];
+  weights[i] = sum;
+}
+// Into how many parts an item's queries are cut, by a model in tiles of 128 x 128 (about 1 us each): an SM's share of all of
+// them, 2 for every item that it takes, more than half of the longest item where the work runs out, 2.5 for joining the parts.  (70B
+// heads, 8192 tokens, a window of 2048 with sinks, whose tile all queries see: 1 part 843 us, 8 484, 16 531; 512 tokens of 8 KV
+// heads 38 and 14; 2048 tokens of 40 heads stay whole, 45 us, 58 in two.)
+int parts_of(const cq_prompt* s, int observe) {
+  const int tiles = (s->keys + UM_TILE - 1) / UM_TILE, G = s->n_heads / s->n_kv_heads, step = (tiles + 255) / 256;
+  double sum = 0, longest = 0;
+  for (int t = 0; t < tiles; t += step) {
+    const long long k0 = (long long)t * UM_TILE, end = std::min<long long>(k0 + UM_TILE, s->keys);
+    const long long first = std::max({(long long)s->keys - s->queries, (long long)s->keys - observe, k0});
+    const long long last = s->window && k0 >= s->sinks ? std::min<long long>(s->keys, end - 1 + s->window) : s->keys;
+    const double n = std::ceil(0.5 * G * ((std::max(0ll, last - first) + KW_Q - 1) / KW_Q));
+    sum += n * step;
+    longest = std::max(longest, n);
+  }
+  const double heads = (double)s->n_kv_heads * s->sequences, sms = cq_sm_count(), share = sum * heads / sms;
+  int best = 1;
+  double least = 0;
+  for (int p = 1; p <= 16; ++p) {
+    const double t = share + 2.0 * tiles * heads * p / sms + 0.6 * longest / p + (p > 1 ? 2.5 : 0.0);
+    if (p == 1 || t < least) {
+      least = t;
+      best = p;
+    }
+  }
+  return best;
 }
 
 // Tensor map of q, k or v (sequence, token, head strides in halves): boxes of 64 columns x `rows` tokens.  A broadcast sequence or
@@ -925,11 +970,17 @@ extern "C" int cq_attn_prefill(const cq_prompt* shape, const void* q, const void
   return CQ_OK;
 }
 
+extern "C" size_t cq_attn_prefill_weights_workspace_bytes(const cq_prompt* s, int observe) {
+  if (!s || s->sequences < 1 || s->queries < 1 || s->keys < s->queries || s->n_kv_heads < 1 || s->n_heads < s->n_kv_heads || observe < 1) return 0;
+  const int parts = parts_of(s, observe);
+  return parts > 1 ? (size_t)parts * s->sequences * s->n_kv_heads * s->keys * sizeof(float) : 16;
+}
+
 extern "C" int cq_attn_prefill_weights(const cq_prompt* shape, const void* q, const void* k, const float* lse, const long long* lengths,
-                                       int observe, float* weights, uint32_t* status_word, cq_stream_t stream) {
+                                       int observe, float* weights, void* workspace, uint32_t* status_word, cq_stream_t stream) {
   const int rc = check(shape, q, k, nullptr);
   if (rc != CQ_OK) return rc;
-  if (!lse || !weights || observe < 1) return CQ_ERR_BAD_ARG;
+  if (!lse || !weights || !workspace || observe < 1) return CQ_ERR_BAD_ARG;
   const PromptArgs a = {*shape, (const __half*)q, (const __half*)k, nullptr, lengths};
   const int D = shape->head_dim, B = shape->sequences;
   PromptMaps maps;
@@ -939,10 +990,14 @@ extern "C" int cq_attn_prefill_weights(const cq_prompt* shape, const void* q, co
     auto fn = D == 128 ? prompt_keys_kernel<128> : prompt_keys_kernel<64>;
     const int smem = (2 + KW_BUFFERS) * (D / 64) * UM_CHUNK + 1024;
     CQ_CUDA_TRY(cq_grant_smem((const void*)fn, smem));
-    const long long items = (long long)((shape->keys + UM_TILE - 1) / UM_TILE) * shape->n_kv_heads * B;
+    const int parts = parts_of(shape, observe);
+    const long long n = (long long)B * shape->n_kv_heads * shape->keys, items = (long long)((shape->keys + UM_TILE - 1) / UM_TILE) * shape->n_kv_heads * B * parts;
     if (items > INT32_MAX) return CQ_ERR_BAD_SHAPE;
     CQ_CUDA_TRY(kv4_launch(fn, dim3((unsigned)std::min<long long>(items, cq_sm_count())), dim3(KW_THREADS), smem, (cudaStream_t)stream, a, maps, lse,
-                           observe, weights, (int)items, status_word));
+                           observe, parts, parts > 1 ? (float*)workspace : weights, (int)items, status_word));
+    if (parts > 1)
+      CQ_CUDA_TRY(kv4_launch(prompt_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (cudaStream_t)stream, (const float*)workspace, parts, n,
+                             weights));
     return CQ_OK;
   }
   auto fn = D == 128 ? prompt_weights_kernel<128> : prompt_weights_kernel<64>;

@@ -293,8 +293,9 @@ torch::Tensor attn_prefill_weights(const torch::Tensor& q, const torch::Tensor& 
   const int64_t last = observe.value_or(s.keys);
   TORCH_CHECK(last > 0, "observe must be positive");
   auto out = torch::empty({s.sequences, s.n_kv_heads, s.keys}, lse.options());
+  auto ws = torch::empty({(int64_t)cq_attn_prefill_weights_workspace_bytes(&s, (int)std::min<int64_t>(last, s.keys))}, lse.options().dtype(torch::kUInt8));
   check_status(cq_attn_prefill_weights(&s, q.const_data_ptr(), k.const_data_ptr(), lse.const_data_ptr<float>(), n,
-                                       (int)std::min<int64_t>(last, s.keys), out.data_ptr<float>(),
+                                       (int)std::min<int64_t>(last, s.keys), out.data_ptr<float>(), ws.data_ptr(),
                                        device_status(q.device()), (cq_stream_t)c10::cuda::getCurrentCUDAStream().stream()),
                "attn_prefill_weights");
   return out;
