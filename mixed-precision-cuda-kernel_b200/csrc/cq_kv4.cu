@@ -7,80 +7,103 @@
 
 namespace {
 
-constexpr int WR_THREADS = 256;
+constexpr int WR_THREADS = 256, WR_TOKENS = 64;      // a block's tokens of one head
 
-// D / 16 lanes a row of q, k or v: rotated (q and k), q to q_out, k and v quantised into their slots.
+// D / 16 lanes a row of q, k or v: rotated (q and k), q to q_out, k and v quantised into their slots.  A block takes one head's
+// rows of 64 tokens, so that nothing is divided but block indices; a lane has two rows' columns in flight.  Bound by memory.
 template <int D, int GROUP>
 __global__ void __launch_bounds__(WR_THREADS) kv4_write_kernel(
     const __half* __restrict__ q, __half* __restrict__ q_out, const __half* __restrict__ k, const __half* __restrict__ v,
     const float* __restrict__ cos_t, const float* __restrict__ sin_t, const long long* __restrict__ positions, int table_rows,
-    const long long* __restrict__ first, cq_kv4 cache, int tokens, int H, long long rows) {
-  constexpr int LANES = D / 16;
+    const long long* __restrict__ first, cq_kv4 cache, int tokens, int H) {
+  constexpr int LANES = D / 16, ROWS = WR_THREADS / LANES, FLIGHT = 2;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int KV = cache.n_kv_heads, per = H + 2 * KV, c = 8 * (threadIdx.x % LANES);
-  const long long stride = (long long)gridDim.x * (WR_THREADS / LANES);
-  // every lane of a warp stays in the loop to its end: the rows' lanes exchange their minima
-  const long long turns = (rows + stride - 1) / stride;
-  for (long long i = 0, row = (long long)blockIdx.x * (WR_THREADS / LANES) + threadIdx.x / LANES; i < turns; ++i, row += stride) {
-    const bool in = row < rows;
-    const long long t = in ? row / per : 0;
-    const int j = in ? (int)(row - t * per) : 0;
-    const bool is_q = j < H, is_k = !is_q && j < H + KV;
-    const __half* src = is_q ? q + (t * H + j) * D : (is_k ? k + (t * KV + j - H) * D : v + (t * KV + j - H - KV) * D);
-    float x[16];
-    kv4_load16(src + c, src + c + D / 2, x);
-    bool there = true;
-    if (cos_t && (is_q || is_k)) {
-      const long long p = positions[t];
-      there = p >= 0 && p < table_rows;
-      if (there) kv4_rotate(x, cos_t + p * (D / 2) + c, sin_t + p * (D / 2) + c);
+  const int KV = cache.n_kv_heads, j = blockIdx.y, b = blockIdx.z, c = 8 * (threadIdx.x % LANES);
+  const bool is_q = j < H, is_k = !is_q && j < H + KV;
+  const int head = is_q ? j : (is_k ? j - H : j - H - KV), heads = is_q ? H : KV;
+  const __half* src = (is_q ? q : (is_k ? k : v)) + ((size_t)b * tokens * heads + head) * D + c;
+  const size_t step = (size_t)heads * D;
+  const long long slot0 = is_q ? 0 : first[b];
+  const size_t row0 = ((size_t)b * KV + head) * cache.slots;
+  uint8_t* codes = (uint8_t*)(is_k ? cache.k_codes : cache.v_codes);
+  uint32_t* scales = (uint32_t*)(is_k ? cache.k_scales : cache.v_scales);
+  const int end = min(tokens, ((int)blockIdx.x + 1) * WR_TOKENS);
+  // every lane stays to the end: a row's lanes exchange their minima
+  for (int t0 = blockIdx.x * WR_TOKENS; t0 < end; t0 += FLIGHT * ROWS) {
+    float x[FLIGHT][16];
+    long long pos[FLIGHT];
+#pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+      const int t = min(t0 + f * ROWS + (int)threadIdx.x / LANES, end - 1);
+      kv4_load16(src + t * step, src + t * step + D / 2, x[f]);
+      pos[f] = cos_t && (is_q || is_k) ? positions[(size_t)b * tokens + t] : -1;
     }
-    uint32_t words[2], pairs[2];
-    kv4_quantise<D, GROUP>(x, words, pairs);
-    if (!in) continue;
-    if (is_q) {
-      *reinterpret_cast<uint4*>(q_out + (t * H + j) * D + c) = kv4_halves(x);
-      *reinterpret_cast<uint4*>(q_out + (t * H + j) * D + c + D / 2) = kv4_halves(x + 8);
-      continue;
+#pragma unroll
+    for (int f = 0; f < FLIGHT; ++f) {
+      const int t = t0 + f * ROWS + threadIdx.x / LANES;
+      const bool turn = pos[f] >= 0 && pos[f] < table_rows;
+      if (turn) kv4_rotate(x[f], cos_t + pos[f] * (D / 2) + c, sin_t + pos[f] * (D / 2) + c);
+      if (is_q) {
+        if (t >= end) continue;
+        __half* to = q_out + ((size_t)(b * (size_t)tokens + t) * H + head) * D + c;
+        *reinterpret_cast<uint4*>(to) = kv4_halves(x[f]);
+        *reinterpret_cast<uint4*>(to + D / 2) = kv4_halves(x[f] + 8);
+        continue;
+      }
+      uint32_t words[2], pairs[2];
+      kv4_quantise<D, GROUP>(x[f], words, pairs);
+      const long long slot = slot0 + t;
+      if (t >= end || (is_k && cos_t && !turn) || slot < 0 || slot >= cache.slots) continue;
+      if (!is_k && cos_t) {                                // (a value's row is left out with its key's)
+        const long long p = positions[(size_t)b * tokens + t];
+        if (p < 0 || p >= table_rows) continue;
+      }
+      const size_t at = row0 + slot;
+      *reinterpret_cast<uint32_t*>(codes + at * (D / 2) + c / 2) = words[0];
+      *reinterpret_cast<uint32_t*>(codes + at * (D / 2) + (c + D / 2) / 2) = words[1];
+      if (c % GROUP == 0) {
+        scales[at * (D / GROUP) + c / GROUP] = pairs[0];
+        if (GROUP != D) scales[at * (D / GROUP) + (c + D / 2) / GROUP] = pairs[1];
+      }
     }
-    const long long b = t / tokens, slot = first[b] + (t - b * tokens);
-    if (!there || slot < 0 || slot >= cache.slots) continue;
-    const size_t at = ((size_t)b * KV + (is_k ? j - H : j - H - KV)) * cache.slots + slot;
-    uint8_t* codes = (uint8_t*)(is_k ? cache.k_codes : cache.v_codes) + at * (D / 2);
-    uint32_t* scales = (uint32_t*)(is_k ? cache.k_scales : cache.v_scales) + at * (D / GROUP);
-    *reinterpret_cast<uint32_t*>(codes + c / 2) = words[0];
-    *reinterpret_cast<uint32_t*>(codes + (c + D / 2) / 2) = words[1];
-    if (c % GROUP == 0) scales[c / GROUP] = pairs[0];
-    if (GROUP != D && c % GROUP == 0) scales[(c + D / 2) / GROUP] = pairs[1];
   }
 }
 
-// One lane per eight columns of a row: k and v (sequence, count, KV, D) fp16.  Slots outside the cache read as zeros.
+// D / 8 lanes a row, eight columns each: k and v (sequence, count, KV, D) fp16.  A block takes a head's rows of 64 tokens.  Slots
+// outside the cache read as zeros.
+template <int D, int GROUP>
 __global__ void __launch_bounds__(WR_THREADS) kv4_read_kernel(cq_kv4 cache, const long long* __restrict__ first, int count,
-                                                              __half* __restrict__ k, __half* __restrict__ v, long long pieces) {
+                                                              __half* __restrict__ k, __half* __restrict__ v) {
+  constexpr int LANES = D / 8, ROWS = WR_THREADS / LANES, FLIGHT = WR_TOKENS / ROWS;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int KV = cache.n_kv_heads, D = cache.head_dim, per = D / 8, groups = D / cache.group;
-  const bool value = blockIdx.y;
+  const int KV = cache.n_kv_heads, b = blockIdx.z, head = blockIdx.y >> 1, w = threadIdx.x % LANES;
+  const bool value = blockIdx.y & 1;
   const uint32_t* codes = (const uint32_t*)(value ? cache.v_codes : cache.k_codes);
   const __half2* scales = (const __half2*)(value ? cache.v_scales : cache.k_scales);
   __half* to = value ? v : k;
-  for (long long i = (long long)blockIdx.x * WR_THREADS + threadIdx.x; i < pieces; i += (long long)gridDim.x * WR_THREADS) {
-    const long long row = i / per, tok = row / KV, b = tok / count;
-    const int w = (int)(i - row * per), head = (int)(row - tok * KV);
-    const long long slot = first[b] + (tok - b * count);
-    uint4 out = make_uint4(0, 0, 0, 0);
-    if (slot >= 0 && slot < cache.slots) {
-      const size_t at = ((size_t)b * KV + head) * cache.slots + slot;
-      const uint32_t word = codes[at * per + w];
-      const float2 sm = __half22float2(scales[at * groups + 8 * w / cache.group]);
-      float x[8];
+  const size_t row0 = ((size_t)b * KV + head) * cache.slots;
+  const long long slot0 = first[b];
+  uint32_t word[FLIGHT];
+  __half2 pair[FLIGHT];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = __fmaf_rn((float)((word >> (4 * e)) & 15u), sm.x, sm.y);
-      out = kv4_halves(x);
-    }
-    *reinterpret_cast<uint4*>(to + 8 * i) = out;
+  for (int f = 0; f < FLIGHT; ++f) {
+    const int t = blockIdx.x * WR_TOKENS + f * ROWS + threadIdx.x / LANES;
+    const long long slot = slot0 + t;
+    const bool in = t < count && slot >= 0 && slot < cache.slots;
+    word[f] = in ? codes[(row0 + slot) * LANES + w] : 0u;
+    pair[f] = in ? scales[(row0 + slot) * (D / GROUP) + 8 * w / GROUP] : __half2half2(__ushort_as_half(0));
+  }
+#pragma unroll
+  for (int f = 0; f < FLIGHT; ++f) {
+    const int t = blockIdx.x * WR_TOKENS + f * ROWS + threadIdx.x / LANES;
+    if (t >= count) break;
+    const float2 sm = __half22float2(pair[f]);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __fmaf_rn((float)((word[f] >> (4 * e)) & 15u), sm.x, sm.y);
+    *reinterpret_cast<uint4*>(to + (((size_t)b * count + t) * KV + head) * D + 8 * w) = kv4_halves(x);
   }
 }
 
@@ -211,37 +234,58 @@ __global__ void __launch_bounds__(SEL_THREADS) kv4_select_kernel(const float* __
   }
 }
 
-// Rows kept[...] of `from` to the first slots of `to`, zeros behind them; a lane per 16 bytes of codes, 4 of scales.
+// Rows kept[...] of a head to its first slots, zeros behind them: 16 bytes of codes a lane, 64 rows a block.  kept null: the
+// rows as they lie.
 struct MoveArgs {
-  const void* src[4];
-  void* dst[4];
-  int bytes[4];              // of a row
+  const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
+  uint8_t *k_codes_to, *k_scales_to, *v_codes_to, *v_scales_to;
   int src_slots, dst_slots, keep;
 };
-__global__ void __launch_bounds__(WR_THREADS) kv4_gather_kernel(MoveArgs a, const int* __restrict__ kept, long long rows) {
+template <int D, int GROUP>
+__global__ void __launch_bounds__(WR_THREADS) kv4_gather_kernel(const MoveArgs a, const int* __restrict__ kept) {
+  constexpr int ROW = D / 2, PIECES = ROW / 16, WORDS = D / GROUP;      // 16-byte pieces of codes, words of scales
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int which = blockIdx.y, per = a.bytes[which] / 4;
-  const uint32_t* src = (const uint32_t*)a.src[which];
-  uint32_t* dst = (uint32_t*)a.dst[which];
-  for (long long i = (long long)blockIdx.x * WR_THREADS + threadIdx.x; i < rows * per; i += (long long)gridDim.x * WR_THREADS) {
-    const long long r = i / per, head = r / a.keep;
-    const int w = (int)(i - r * per), at = kept ? kept[r] : (int)(r - head * a.keep);
-    dst[((size_t)head * a.dst_slots + (r - head * a.keep)) * per + w] = at < 0 ? 0u : src[((size_t)head * a.src_slots + at) * per + w];
+  const size_t head = blockIdx.y + (size_t)gridDim.y * blockIdx.z, from = head * a.src_slots, to = head * a.dst_slots;
+  const int r0 = blockIdx.x * WR_TOKENS;
+  __shared__ int s_at[WR_TOKENS];
+  if (threadIdx.x < WR_TOKENS) {
+    const int r = r0 + threadIdx.x;
+    s_at[threadIdx.x] = r < a.keep ? (kept ? kept[head * a.keep + r] : r) : -1;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < WR_TOKENS * PIECES; i += WR_THREADS) {
+    const int r = i / PIECES, c = 16 * (i % PIECES), at = s_at[r];
+    if (r0 + r >= a.keep) break;
+    uint4 x = make_uint4(0, 0, 0, 0), y = x;
+    if (at >= 0) {
+      x = *reinterpret_cast<const uint4*>(a.k_codes + (from + at) * ROW + c);
+      y = *reinterpret_cast<const uint4*>(a.v_codes + (from + at) * ROW + c);
+    }
+    *reinterpret_cast<uint4*>(a.k_codes_to + (to + r0 + r) * ROW + c) = x;
+    *reinterpret_cast<uint4*>(a.v_codes_to + (to + r0 + r) * ROW + c) = y;
+  }
+  for (int i = threadIdx.x; i < WR_TOKENS * WORDS; i += WR_THREADS) {
+    const int r = i / WORDS, c = 4 * (i % WORDS), at = s_at[r];
+    if (r0 + r >= a.keep) break;
+    *reinterpret_cast<uint32_t*>(a.k_scales_to + (to + r0 + r) * (4 * WORDS) + c) =
+        at < 0 ? 0u : *reinterpret_cast<const uint32_t*>(a.k_scales + (from + at) * (4 * WORDS) + c);
+    *reinterpret_cast<uint32_t*>(a.v_scales_to + (to + r0 + r) * (4 * WORDS) + c) =
+        at < 0 ? 0u : *reinterpret_cast<const uint32_t*>(a.v_scales + (from + at) * (4 * WORDS) + c);
   }
 }
 
-int blocks_for(long long items, int threads, int most) {
-  return (int)std::max<long long>(1, std::min<long long>((items + threads - 1) / threads, most));
-}
-int most_blocks() { return cq_sm_count() * 16; }
+// the instance for a cache's head width and group
+#define KV4_PICK(kernel, c)                                                                \
+  ((c)->head_dim == 128 ? ((c)->group == 32 ? kernel<128, 32> : kernel<128, 64>)           \
+                        : ((c)->group == 32 ? kernel<64, 32> : kernel<64, 64>))
 
 }  // namespace
 
 extern "C" int cq_kv4_check(const cq_kv4* c) {
   if (!c || !c->k_codes || !c->k_scales || !c->v_codes || !c->v_scales) return CQ_ERR_BAD_ARG;
   if (((uintptr_t)c->k_codes | (uintptr_t)c->k_scales | (uintptr_t)c->v_codes | (uintptr_t)c->v_scales) & 15) return CQ_ERR_BAD_ARG;
-  if (c->sequences < 1 || c->sequences > 65535 || c->n_kv_heads < 1 || c->slots < 32 || c->slots % 32 || c->slots > (1 << 30))
+  if (c->sequences < 1 || c->sequences > 65535 || c->n_kv_heads < 1 || c->n_kv_heads > 32767 || c->slots < 32 || c->slots % 32 || c->slots > (1 << 30))
     return CQ_ERR_BAD_SHAPE;
   if ((c->head_dim != 64 && c->head_dim != 128) || (c->group != 32 && c->group != 64)) return CQ_ERR_UNSUPPORTED;
   return CQ_OK;
@@ -255,13 +299,11 @@ extern "C" int cq_kv4_write(const cq_kv4* cache, const void* q, void* q_out, con
   if (!k || !v || !first || tokens < 1 || n_heads < 0 || (n_heads > 0 && (!q || !q_out))) return CQ_ERR_BAD_ARG;
   if (cos_table && (!sin_table || !positions || table_rows < 1)) return CQ_ERR_BAD_ARG;
   if (((uintptr_t)q | (uintptr_t)q_out | (uintptr_t)k | (uintptr_t)v) & 15) return CQ_ERR_BAD_ARG;
-  const long long rows = (long long)cache->sequences * tokens * (n_heads + 2 * cache->n_kv_heads);
-  const bool wide = cache->head_dim == 128, narrow = cache->group == 32;
-  auto fn = wide ? (narrow ? kv4_write_kernel<128, 32> : kv4_write_kernel<128, 64>)
-                 : (narrow ? kv4_write_kernel<64, 32> : kv4_write_kernel<64, 64>);
-  const int blocks = blocks_for(rows * (cache->head_dim / 16), WR_THREADS, most_blocks());
-  CQ_CUDA_TRY(kv4_launch(fn, dim3(blocks), dim3(WR_THREADS), 0, (cudaStream_t)stream, (const __half*)q, (__half*)q_out, (const __half*)k,
-                         (const __half*)v, cos_table, sin_table, positions, table_rows, first, *cache, tokens, n_heads, rows));
+  const long long kinds = n_heads + 2ll * cache->n_kv_heads;
+  if (kinds > 65535) return CQ_ERR_BAD_SHAPE;
+  CQ_CUDA_TRY(kv4_launch(KV4_PICK(kv4_write_kernel, cache), dim3((tokens + WR_TOKENS - 1) / WR_TOKENS, (unsigned)kinds, cache->sequences), dim3(WR_THREADS), 0,
+                         (cudaStream_t)stream, (const __half*)q, (__half*)q_out, (const __half*)k, (const __half*)v, cos_table, sin_table, positions,
+                         table_rows, first, *cache, tokens, n_heads));
   return CQ_OK;
 }
 
@@ -269,9 +311,8 @@ extern "C" int cq_kv4_read(const cq_kv4* cache, const long long* first, int coun
   const int rc = cq_kv4_check(cache);
   if (rc != CQ_OK) return rc;
   if (!first || !k || !v || count < 1 || (((uintptr_t)k | (uintptr_t)v) & 15)) return CQ_ERR_BAD_ARG;
-  const long long pieces = (long long)cache->sequences * count * cache->n_kv_heads * (cache->head_dim / 8);
-  CQ_CUDA_TRY(kv4_launch(kv4_read_kernel, dim3(blocks_for(pieces, WR_THREADS, most_blocks()), 2), dim3(WR_THREADS), 0,
-                         (cudaStream_t)stream, *cache, first, count, (__half*)k, (__half*)v, pieces));
+  CQ_CUDA_TRY(kv4_launch(KV4_PICK(kv4_read_kernel, cache), dim3((count + WR_TOKENS - 1) / WR_TOKENS, 2 * cache->n_kv_heads, cache->sequences),
+                         dim3(WR_THREADS), 0, (cudaStream_t)stream, *cache, first, count, (__half*)k, (__half*)v));
   return CQ_OK;
 }
 
@@ -299,24 +340,21 @@ extern "C" int cq_kv4_evict(const cq_kv4* from, const cq_kv4* to, const float* w
   const int B = from->sequences, KV = from->n_kv_heads, D = from->head_dim;
   CQ_CUDA_TRY(kv4_launch(kv4_select_kernel, dim3(KV, B), dim3(SEL_THREADS), 0, (cudaStream_t)stream, weights, length, length_out, kept,
                          weights_out, KV, from->slots, keep, sinks, recent));
-  const long long rows = (long long)B * KV * keep;
-  MoveArgs move = {}, back = {};
-  const int bytes[4] = {D / 2, 4 * (D / from->group), D / 2, 4 * (D / from->group)};
+  const size_t rows = (size_t)B * KV * keep;
+  const int code = D / 2, scale = 4 * (D / from->group);
   uint8_t* ws = (uint8_t*)workspace;
-  for (int i = 0; i < 4; ++i) {
-    move.src[i] = fp[i];
-    move.dst[i] = in_place ? ws : tp[i];
-    back.src[i] = ws;
-    back.dst[i] = tp[i];
-    move.bytes[i] = back.bytes[i] = bytes[i];
-    if (in_place) ws += rows * bytes[i];
-  }
-  move.src_slots = from->slots;
-  move.dst_slots = in_place ? keep : to->slots;
-  move.keep = back.keep = back.src_slots = keep;
-  back.dst_slots = to->slots;
-  const dim3 grid(blocks_for(rows * (D / 8), WR_THREADS, most_blocks()), 4);
-  CQ_CUDA_TRY(kv4_launch(kv4_gather_kernel, grid, dim3(WR_THREADS), 0, (cudaStream_t)stream, move, (const int*)kept, rows));
-  if (in_place) CQ_CUDA_TRY(kv4_launch(kv4_gather_kernel, grid, dim3(WR_THREADS), 0, (cudaStream_t)stream, back, (const int*)nullptr, rows));
+  // codes in front: they are moved in pieces of 16 bytes, a row of scales may have four
+  uint8_t* mid[4] = {ws, ws + 2 * rows * code, ws + rows * code, ws + rows * (2 * code + scale)};
+  auto args = [](const void* const* f, void* const* t, int src_slots, int dst_slots, int n) {
+    return MoveArgs{(const uint8_t*)f[0], (const uint8_t*)f[1], (const uint8_t*)f[2], (const uint8_t*)f[3], (uint8_t*)t[0], (uint8_t*)t[1],
+                    (uint8_t*)t[2], (uint8_t*)t[3], src_slots, dst_slots, n};
+  };
+  const dim3 grid((keep + WR_TOKENS - 1) / WR_TOKENS, KV, B);
+  void* over[4] = {mid[0], mid[1], mid[2], mid[3]};
+  auto fn = KV4_PICK(kv4_gather_kernel, from);
+  CQ_CUDA_TRY(kv4_launch(fn, grid, dim3(WR_THREADS), 0, (cudaStream_t)stream, args(fp, in_place ? over : tp, from->slots, in_place ? keep : to->slots, keep),
+                         (const int*)kept));
+  if (in_place)
+    CQ_CUDA_TRY(kv4_launch(fn, grid, dim3(WR_THREADS), 0, (cudaStream_t)stream, args(over, tp, keep, to->slots, keep), (const int*)nullptr));
   return CQ_OK;
 }

@@ -54,10 +54,13 @@ __device__ __forceinline__ void kv4_quantise(const float (&x)[16], uint32_t (&wo
     pairs[h] = (uint32_t)__half_as_ushort(s16) | (bad ? 0x7FFF0000u : (uint32_t)__half_as_ushort(__float2half_rn(lo[h])) << 16);
     uint32_t w = 0;
     if (s > 0.f) {
+      // the quotient as the division rounds it, by one residual step after the product with the reciprocal (Markstein)
+      const float inv = __frcp_rn(s);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float u = rintf(__fdiv_rn(__fsub_rn(x[8 * h + e], lo[h]), s));
-        w |= (uint32_t)fminf(u, 15.f) << (4 * e);
+        const float d = __fsub_rn(x[8 * h + e], lo[h]), q = __fmul_rn(d, inv), u = fminf(__fmaf_rn(__fmaf_rn(-q, s, d), inv, q), 15.f);
+        // (rounded to a whole number, half to even, by adding 1.5 * 2^23)
+        w |= (__float_as_uint(__fadd_rn(u, 12582912.f)) & 15u) << (4 * e);
       }
     }
     words[h] = w;

@@ -64,7 +64,7 @@ struct KVCache4 {
     TORCH_CHECK(D == 64 || D == 128, "heads must be 64 or 128 wide, not ", D);
     TORCH_CHECK(groups > 0 && D % groups == 0 && (D / groups == 32 || D / groups == 64), "groups must have 32 or 64 columns");
     TORCH_CHECK(k_codes.size(2) > 0 && k_codes.size(2) % 32 == 0 && k_codes.size(2) <= (1 << 30), "slots must be a multiple of 32");
-    TORCH_CHECK(k_codes.size(0) > 0 && k_codes.size(0) <= 65535 && k_codes.size(1) > 0 && k_codes.size(1) <= 65535, "1 to 65535 sequences and heads");
+    TORCH_CHECK(k_codes.size(0) > 0 && k_codes.size(0) <= 65535 && k_codes.size(1) > 0 && k_codes.size(1) <= 32767, "1 to 65535 sequences, 1 to 32767 KV heads");
     c.sequences = (int)k_codes.size(0);
     c.n_kv_heads = (int)k_codes.size(1);
     c.slots = (int)k_codes.size(2);
