@@ -24,6 +24,12 @@ SwiGLU output, down): four collectives per layer.  Every output element is still
 exactly the single-GPU arithmetic, so the tokens are identical for every group size; all ranks
 draw the full random weight and pack only their rows.
 
+`kv_bits=4` keeps keys and values in 4 bits (`quant_cuda.KVCache4`): prompts go through `attn_prefill`, steps through
+`KVCache4.step`, both with a sliding `window` and the first `sinks` positions visible if asked for.  `kv_budget` bounds the cache: a
+prompt's positions are weighed by its last `kv_observe` queries (`attn_prefill_weights`), every step adds what each slot
+received, and whenever the `kv_budget + kv_slack` slots of a layer are full the heaviest `kv_budget` stay (`KVCache4.evict`; the
+first `sinks` and the last `kv_recent` always do).  Keys keep the rotation of their own positions.
+
 `dense=True` builds the parity twin: the same packed buffers, every projection computed as
 F.linear(x, unpack()) the way the reference's dense mode does (llama/qlinear.py:183-195).
 """
@@ -77,7 +83,8 @@ class CherryDecoder:
 
     def __init__(self, cfg: DecoderConfig, device="cuda", seed: int = 0, dense: bool = False,
                  release_reference_buffers: bool = False, tp_group=None, tp_gather: str = "peer", batch: int = 1,
-                 attention: str = "auto"):
+                 attention: str = "auto", kv_bits: int = 16, kv_group: int = 32, window: int = 0, sinks: int = 0,
+                 kv_budget: int = None, kv_slack: int = 256, kv_recent: int = None, kv_observe: int = 64):
         if not torch.cuda.is_available():
             raise RuntimeError("CherryDecoder needs a CUDA device (there is no CPU path)")
         if batch < 1:
@@ -92,9 +99,22 @@ class CherryDecoder:
         # at 4000 positions 12.5 and 20 at batch 1, 20 and 27 at 4, 50 and 64 at 16, 93 and 194 at 32.
         if attention not in ("auto", "own", "flash"):
             raise ValueError("attention is 'auto', 'own' or 'flash'")
+        if kv_bits not in (4, 16):
+            raise ValueError("kv_bits is 16 or 4")
+        if window < 0 or sinks < 0:
+            raise ValueError("window and sinks must not be negative")
+        if kv_bits == 16 and (window or sinks or kv_budget is not None):
+            raise ValueError("window, sinks and kv_budget need the 4-bit cache (kv_bits=4)")
+        if kv_bits == 4 and (attention == "flash" or cfg.head_dim not in (64, 128)):
+            raise ValueError("the 4-bit cache has its own attention, for heads 64 or 128 wide")
+        self.kv_bits, self.window, self.sinks, self.kv_budget, self.kv_observe = kv_bits, window, sinks, kv_budget, kv_observe
+        if kv_budget is not None:
+            self.kv_recent = kv_budget // 4 if kv_recent is None else kv_recent
+            if not (kv_budget > 0 and kv_slack > 0 and kv_observe > 0 and self.kv_recent >= 0 and sinks + self.kv_recent <= kv_budget):
+                raise ValueError("kv_budget must hold the sinks and the recent positions, and kv_slack and kv_observe be positive")
         self._flash = None
         grouped = cfg.n_heads // cfg.n_kv_heads
-        if attention == "flash" or (attention == "auto" and cfg.max_seq > 1024 and
+        if attention == "flash" or (attention == "auto" and kv_bits == 16 and cfg.max_seq > 1024 and
                                     grouped > (8 if cfg.head_dim in (64, 128) else 1)):
             try:
                 from flash_attn import flash_attn_with_kvcache
@@ -146,8 +166,20 @@ class CherryDecoder:
         inv = 1.0 / (cfg.rope_theta ** (torch.arange(0, hd, 2, device=self.dev, dtype=torch.float32) / hd))
         ang = torch.outer(torch.arange(cfg.max_seq, device=self.dev, dtype=torch.float32), inv)
         self.cos, self.sin = ang.cos(), ang.sin()                      # (max_seq, hd / 2)
-        self.k_cache = torch.zeros(cfg.n_layers, batch, cfg.max_seq, self.kv_local, hd, dtype=torch.float16, device=self.dev)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        if kv_bits == 4:
+            slots = cfg.max_seq if kv_budget is None else kv_budget + kv_slack
+            make = lambda n: self.qc.KVCache4.empty(batch, self.kv_local, n, hd, kv_group, self.dev)
+            self.caches = [make(slots) for _ in range(cfg.n_layers)]
+            self.slots = slots
+            self.zero = torch.zeros(batch, dtype=torch.long, device=self.dev)
+            if kv_budget is not None:
+                self.prompt_cache = make(cfg.max_seq)        # of one layer at a time
+                self.kv_weights = torch.zeros(cfg.n_layers, batch, self.kv_local, self.caches[0].slots, device=self.dev)
+                # slots that hold a position, on the device and on the host
+                self.length, self.length_host = torch.zeros(batch, dtype=torch.long, device=self.dev), 0
+        else:
+            self.k_cache = torch.zeros(cfg.n_layers, batch, cfg.max_seq, self.kv_local, hd, dtype=torch.float16, device=self.dev)
+            self.v_cache = torch.zeros_like(self.k_cache)
         # state of the decode loop, all on the device: next token and position of every sequence
         self.tok = torch.zeros(batch, dtype=torch.long, device=self.dev)
         self.pos = torch.zeros(batch, dtype=torch.long, device=self.dev)
@@ -234,7 +266,9 @@ class CherryDecoder:
         t, nh, kv, hd, nb = h.shape[0], self.h_local, self.kv_local, cfg.head_dim, self.batch
         (q, k, v), h = self._norm_lins(lay, ("q", "k", "v"), h, delta, lay["norm1"])
         q, k, v = q.view(t, nh, hd), k.view(t, kv, hd), v.view(t, kv, hd)
-        if decode and self._flash is None:
+        if self.kv_bits == 4:
+            a = (self._kv4_step if decode else self._kv4_prompt)(li, q, k, v, pos).view(t, nh * hd)
+        elif decode and self._flash is None:
             a = self.qc.attn_decode_step(q, k, v, self.cos, self.sin, pos, self.k_cache[li], self.v_cache[li]).view(t, nh * hd)
         else:
             self.qc.rope_cache(q, k, v, self.cos, self.sin, pos, self.k_cache[li], self.v_cache[li])
@@ -252,6 +286,48 @@ class CherryDecoder:
             return h, lay["down"].forward_swiglu(gate, up)
         act = self.qc.silu_mul(gate, up)
         return h, self._lin_gather(lay["down"], self._gather(act))
+
+    # ------------------------------------------------------------------ 4-bit cache
+    def _kv4_step(self, li: int, q, k, v, pos):
+        weights = None if self.kv_budget is None else self.kv_weights[li]
+        return self.caches[li].step(q, k, v, self.cos, self.sin, pos, pos if self.kv_budget is None else self.length,
+                                    window=self.window, sinks=self.sinks, weights=weights)
+
+    def _kv4_prompt(self, li: int, q, k, v, pos):
+        """Attention of the prompts on their fp16 keys and values; the cache takes them in 4 bits, all or the budget's."""
+        nb, (t, nh, hd), kv = self.batch, q.shape, k.shape[1]
+        cache = self.caches[li] if self.kv_budget is None else self.prompt_cache
+        turned = cache.write(torch.cat([q, k], 1), k, v, self.zero, self.cos, self.sin, pos).view(nb, t // nb, nh + kv, hd)
+        q, k, v = turned[:, :, :nh], turned[:, :, nh:], v.view(nb, t // nb, kv, hd)
+        out, lse = self.qc.attn_prefill(q, k, v, window=self.window, sinks=self.sinks)
+        if self.kv_budget is not None:
+            weights = torch.zeros(nb, kv, cache.slots, device=self.dev)
+            weights[:, :, :t // nb] = self.qc.attn_prefill_weights(q, k, lse, window=self.window, sinks=self.sinks, observe=self.kv_observe)
+            _, left, length = cache.evict(weights, self.zero + t // nb, self.kv_budget, sinks=self.sinks, recent=self.kv_recent,
+                                          out=self.caches[li])
+            self.kv_weights[li, :, :, :self.kv_budget] = left
+            self.length.copy_(length)
+        return out
+
+    def _kv4_evict(self):
+        """Every layer's cache down to the budget; the slots that stay keep their weights."""
+        for li, cache in enumerate(self.caches):
+            _, left, length = cache.evict(self.kv_weights[li], self.length, self.kv_budget, sinks=self.sinks, recent=self.kv_recent)
+            self.kv_weights[li, :, :, :self.kv_budget] = left
+        self.length.copy_(length)
+        self.length_host = self.kv_budget
+
+    def _kv4_room(self):
+        """A free slot for the next position."""
+        if self.kv_budget is not None:
+            if self.length_host == self.slots:
+                self._kv4_evict()
+            self.length_host += 1
+
+    def _kv4_rows(self):
+        """What a step at positions 0, 1 and 2 changes."""
+        rows = [x[:, :, :3] for c in self.caches for x in (c.k_codes, c.k_scales, c.v_codes, c.v_scales)]
+        return rows if self.kv_budget is None else rows + [self.kv_weights, self.length]
 
     def _logits(self, h: torch.Tensor, delta) -> torch.Tensor:
         return F.linear(self._norm(h, delta, self.final_norm)[0], self.lm_head)
@@ -277,6 +353,8 @@ class CherryDecoder:
         self._check_exchange()
         self.pos.fill_(t)
         self.pos_host = t
+        if self.kv_budget is not None:
+            self.length_host = min(t, self.kv_budget)
         self.tok.copy_(logits.argmax(-1))
         return logits
 
@@ -289,6 +367,8 @@ class CherryDecoder:
         logits = self._logits(h, delta)
         self.tok.copy_(logits.argmax(-1))
         self.pos.add_(1)
+        if self.kv_budget is not None:
+            self.length.add_(1)
         return logits
 
     @torch.inference_mode()
@@ -298,8 +378,11 @@ class CherryDecoder:
             raise ValueError("max_seq must be at least 4")
         # the warm-up and the captured step run at positions 0, 1, 2: always inside the cache, whatever
         # the current position is (state and those cache rows are restored below)
-        saved = (self.tok.clone(), self.pos.clone(), self.k_cache[:, :, :3].clone(), self.v_cache[:, :, :3].clone())
+        rows = self._kv4_rows() if self.kv_bits == 4 else [self.k_cache[:, :, :3], self.v_cache[:, :, :3]]
+        saved = [x.clone() for x in (self.tok, self.pos, *rows)]
         self.pos.zero_()
+        if self.kv_budget is not None:
+            self.length.zero_()
         s = torch.cuda.Stream(device=self.dev)
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
@@ -311,7 +394,7 @@ class CherryDecoder:
                 self.graph_logits = self._step()
         torch.cuda.current_stream().wait_stream(s)
         torch.cuda.synchronize()
-        for dst, src in zip((self.tok, self.pos, self.k_cache[:, :, :3], self.v_cache[:, :, :3]), saved):
+        for dst, src in zip((self.tok, self.pos, *rows), saved):
             dst.copy_(src)
 
     @torch.inference_mode()
@@ -326,6 +409,8 @@ class CherryDecoder:
             self.capture()
         for i in range(n_tokens):
             out[i:i + 1].copy_(self.tok)
+            if self.kv_bits == 4:
+                self._kv4_room()
             if use_graph:
                 self.graph.replay()
             else:
