@@ -376,7 +376,11 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
         w[e] = ex2(s[u][e] - lifted[e & 1]);
         l[e & 1] += w[e];
       }
-      const uint32_t p0 = transposed(pair_of(w[0], w[1])), p1 = transposed(pair_of(w[2], w[3]));
+      // the weights' upper 11 bits, and the next 11
+      const uint32_t h0 = pair_of(w[0], w[1]), h1 = pair_of(w[2], w[3]);
+      const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+      const uint32_t p0 = transposed(h0), p1 = transposed(h1);
+      const uint32_t r0 = transposed(pair_of(w[0] - f0.x, w[1] - f0.y)), r1 = transposed(pair_of(w[2] - f1.x, w[3] - f1.y));
       // two slots' words side by side: [slots 0-7 | 8-15]
       uint32_t sc[2], mn[2], vw[2][2][VW];
 #pragma unroll
@@ -407,6 +411,8 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
           }
           at_mma(o[4 * i + 2 * y], a[0][0], a[0][1], a[1][0], a[1][1], p0, p1);
           at_mma(o[4 * i + 2 * y + 1], a[0][2], a[0][3], a[1][2], a[1][3], p0, p1);
+          at_mma(o[4 * i + 2 * y], a[0][0], a[0][1], a[1][0], a[1][1], r0, r1);
+          at_mma(o[4 * i + 2 * y + 1], a[0][2], a[0][3], a[1][2], a[1][3], r0, r1);
         }
     }
   };
