@@ -311,8 +311,8 @@ int cq_kv4_read(const cq_kv4* cache, const long long* first, int count, void* k_
  * j < n = length[s] (device int64, bounded by the cache): all of them (window 0), or those with j < sinks or j >= n - window.
  * Nothing visible: zeros.  weights, weights_out (sequences, KV, slots) fp32, both or neither, possibly the same:
  * weights_out = weights + the sum over the head's queries of their softmax weights for j < n, and 0 from n on.
- * workspace: device memory of cq_kv4_attend_workspace_bytes(...) bytes, 16-byte aligned, not shared by calls that can
- * overlap. */
+ * workspace: device memory of cq_kv4_attend_workspace_bytes(...) bytes (may be NULL where that is 0), 16-byte aligned, not
+ * shared by calls that can overlap. */
 size_t cq_kv4_attend_workspace_bytes(const cq_kv4* cache, int n_heads, int window, int sinks, int with_weights);
 int cq_kv4_attend(const cq_kv4* cache, const void* q_f16, const long long* length, void* out_f16, int n_heads, int window,
                   int sinks, float scale, const float* weights, float* weights_out, void* workspace, cq_stream_t stream);

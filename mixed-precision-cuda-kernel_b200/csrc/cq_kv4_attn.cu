@@ -24,6 +24,7 @@
 //     their sums go to the workspace and a small kernel joins them: no counters, nothing that two calls on one cache could confuse.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <type_traits>
 
 #include "cq_kv4.cuh"
@@ -606,8 +607,8 @@ struct Shape {
   bool cluster;
 };
 constexpr int AT_MAX_SPLITS = 32;            // (a lane each where they are joined)
-Shape shape_of(const cq_kv4* cache, int n_heads, int window, int sinks) {
-  const int B = cache->sequences, KV = cache->n_kv_heads, chunks = (n_heads / KV + AT_HEADS - 1) / AT_HEADS, sms = cq_sm_count();
+Shape plan_of(const cq_kv4* cache, int n_heads, int window, int sinks, int sms) {
+  const int B = cache->sequences, KV = cache->n_kv_heads, chunks = (n_heads / KV + AT_HEADS - 1) / AT_HEADS;
   const long long tasks = (long long)B * KV * chunks;
   const long long most = window ? std::min<long long>(cache->slots, (long long)window + sinks + AT_SLOTS) : cache->slots;
   const int turns = (int)((most + AT_SLOTS - 1) / AT_SLOTS);
@@ -636,6 +637,20 @@ Shape shape_of(const cq_kv4* cache, int n_heads, int window, int sinks) {
       }
     }
   return best;
+}
+// A program's calls are alike from one to the next, and the model takes 1 to 2 us of the host: the last plan of a thread stays.
+Shape shape_of(const cq_kv4* cache, int n_heads, int window, int sinks) {
+  struct Asked {
+    int sequences, n_kv_heads, slots, head_dim, n_heads, window, sinks, sms;
+  };
+  thread_local Asked last = {};
+  thread_local Shape plan = {};
+  const Asked now = {cache->sequences, cache->n_kv_heads, cache->slots, cache->head_dim, n_heads, window, sinks, cq_sm_count()};
+  if (std::memcmp(&now, &last, sizeof(now)) != 0) {
+    plan = plan_of(cache, n_heads, window, sinks, now.sms);
+    last = now;
+  }
+  return plan;
 }
 size_t sums_bytes(const cq_kv4* cache, int n_heads, const Shape& s) {
   return s.splits > 1 && !s.cluster ? (size_t)cache->sequences * n_heads * s.splits * (cache->head_dim + 4) * 4 : 0;
@@ -695,9 +710,10 @@ int check(const cq_kv4* cache, const void* q, const long long* length, const voi
           const float* weights, const float* weights_out, const void* workspace) {
   const int rc = cq_kv4_check(cache);
   if (rc != CQ_OK) return rc;
-  if (!q || !length || !out || window < 0 || sinks < 0 || (!weights != !weights_out) || !workspace) return CQ_ERR_BAD_ARG;
+  if (!q || !length || !out || window < 0 || sinks < 0 || (!weights != !weights_out)) return CQ_ERR_BAD_ARG;
   if (n_heads < 1 || n_heads % cache->n_kv_heads || (n_heads + 7ll * cache->n_kv_heads) / 8 > 65535) return CQ_ERR_BAD_SHAPE;
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)weights | (uintptr_t)weights_out | (uintptr_t)workspace) & 15) return CQ_ERR_BAD_ARG;
+  if (!workspace && cq_kv4_attend_workspace_bytes(cache, n_heads, window, sinks, weights != nullptr)) return CQ_ERR_BAD_ARG;
   return CQ_OK;
 }
 
@@ -706,7 +722,7 @@ int check(const cq_kv4* cache, const void* q, const long long* length, const voi
 extern "C" size_t cq_kv4_attend_workspace_bytes(const cq_kv4* cache, int n_heads, int window, int sinks, int with_weights) {
   if (cq_kv4_check(cache) != CQ_OK || n_heads < 1 || n_heads % cache->n_kv_heads || window < 0 || sinks < 0) return 0;
   const size_t heads = (size_t)cache->sequences * n_heads;
-  return sums_bytes(cache, n_heads, shape_of(cache, n_heads, window, sinks)) + (with_weights ? heads * 8 + heads * cache->slots * 4 + 16 : 0) + 16;
+  return sums_bytes(cache, n_heads, shape_of(cache, n_heads, window, sinks)) + (with_weights ? heads * 8 + heads * cache->slots * 4 + 16 : 0);
 }
 
 extern "C" int cq_kv4_attend(const cq_kv4* cache, const void* q, const long long* length, void* out, int n_heads, int window, int sinks,

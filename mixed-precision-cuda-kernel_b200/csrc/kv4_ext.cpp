@@ -2,6 +2,8 @@
 // quant_cuda_ext.cpp this file holds no device code: it checks the tensors and takes torch's current stream and device.
 #include "kv4_ext.h"
 
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -97,6 +99,13 @@ struct KVCache4 {
     return (cq_stream_t)s.stream();
   }
 
+  // An output or workspace, straight from the allocator: single tokens are bound by the host, and a trip through the
+  // dispatcher for each of them costs more than the rest of a call.  (Not where a dispatch mode watches.)
+  torch::Tensor fresh(c10::IntArrayRef shape, c10::ScalarType type) const {
+    if (c10::impl::TorchDispatchModeTLS::any_modes_set()) return torch::empty(shape, torch::TensorOptions().device(device).dtype(type));
+    return at::detail::empty_cuda(shape, type, device, c10::nullopt);
+  }
+
   // rows (rows, heads, D) fp16; returns the number of heads
   int check_rows(const torch::Tensor& t, const char* name, int64_t rows, int64_t heads) const {
     check_tensor(t, name, torch::kFloat16, device);
@@ -134,7 +143,7 @@ struct KVCache4 {
     const int table = check_tables(cos, sin, positions, rows);
     const long long* at = whole_numbers(first, "first", c.sequences, device);
     OptTensor out;
-    if (q.has_value()) out = torch::empty_like(*q);
+    if (q.has_value()) out = fresh(q->sizes(), torch::kFloat16);
     check_status(cq_kv4_write(&c, H ? q->const_data_ptr() : nullptr, H ? out->data_ptr() : nullptr, k.const_data_ptr(), v.const_data_ptr(),
                               table ? cos->const_data_ptr<float>() : nullptr, table ? sin->const_data_ptr<float>() : nullptr,
                               table ? (const long long*)positions->const_data_ptr() : nullptr, table, at, (int)(rows / c.sequences), H, use()),
@@ -146,7 +155,7 @@ struct KVCache4 {
     const c10::cuda::CUDAGuard guard(device);
     TORCH_CHECK(count > 0 && count <= INT32_MAX, "count must be positive");
     const long long* at = whole_numbers(first, "first", c.sequences, device);
-    auto k = torch::empty({c.sequences, count, c.n_kv_heads, c.head_dim}, k_scales.options()), v = torch::empty_like(k);
+    auto k = fresh({c.sequences, count, c.n_kv_heads, c.head_dim}, torch::kFloat16), v = fresh(k.sizes(), torch::kFloat16);
     check_status(cq_kv4_read(&c, at, (int)count, k.data_ptr(), v.data_ptr(), use()), "KVCache4.read");
     return {k, v};
   }
@@ -166,8 +175,10 @@ struct KVCache4 {
     return {weights->const_data_ptr<float>(), out.data_ptr<float>()};
   }
 
+  // undefined where a call needs none
   torch::Tensor workspace(int H, int64_t window, int64_t sinks, bool weights) const {
-    return torch::empty({(int64_t)cq_kv4_attend_workspace_bytes(&c, H, (int)window, (int)sinks, weights)}, k_codes.options());
+    const int64_t bytes = (int64_t)cq_kv4_attend_workspace_bytes(&c, H, (int)window, (int)sinks, weights);
+    return bytes ? fresh({bytes}, torch::kUInt8) : torch::Tensor();
   }
 
   torch::Tensor attend(const torch::Tensor& q, const torch::Tensor& length, int64_t window, int64_t sinks, const OptTensor& weights,
@@ -177,10 +188,10 @@ struct KVCache4 {
     check_mask(window, sinks);
     const long long* n = whole_numbers(length, "length", c.sequences, device);
     const auto w = check_weights(weights, weights_out);
-    auto out = torch::empty_like(q);
+    auto out = fresh(q.sizes(), torch::kFloat16);
     auto ws = workspace(H, window, sinks, w.first);
     check_status(cq_kv4_attend(&c, q.const_data_ptr(), n, out.data_ptr(), H, (int)window, (int)sinks,
-                               (float)scale.value_or(1.0 / std::sqrt((double)c.head_dim)), w.first, w.second, ws.data_ptr(), use()),
+                               (float)scale.value_or(1.0 / std::sqrt((double)c.head_dim)), w.first, w.second, ws.defined() ? ws.data_ptr() : nullptr, use()),
                  "KVCache4.attend");
     return out;
   }
@@ -196,12 +207,12 @@ struct KVCache4 {
     const int table = check_tables(cos, sin, positions, c.sequences);
     const long long* n = whole_numbers(length, "length", c.sequences, device);
     const auto w = check_weights(weights, weights_out);
-    auto out = torch::empty_like(q);
+    auto out = fresh(q.sizes(), torch::kFloat16);
     auto ws = workspace(H, window, sinks, w.first);
     check_status(cq_kv4_step(&c, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), table ? cos->const_data_ptr<float>() : nullptr,
                              table ? sin->const_data_ptr<float>() : nullptr, table ? (const long long*)positions->const_data_ptr() : nullptr,
                              table, n, out.data_ptr(), H, (int)window, (int)sinks,
-                             (float)scale.value_or(1.0 / std::sqrt((double)c.head_dim)), w.first, w.second, ws.data_ptr(), use()),
+                             (float)scale.value_or(1.0 / std::sqrt((double)c.head_dim)), w.first, w.second, ws.defined() ? ws.data_ptr() : nullptr, use()),
                  "KVCache4.step");
     return out;
   }

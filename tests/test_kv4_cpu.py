@@ -54,7 +54,7 @@ def test_cache_calls(lib):
     f = C.c_float(1.0)
     attend = lambda q=at, n=at, out=at, heads=4, window=0, sinks=0, w=None, wo=None, ws=at: lib.cq_kv4_attend(
         C.byref(c), q, n, out, heads, window, sinks, f, w, wo, ws, None)
-    for bad in (dict(q=None), dict(n=None), dict(out=None), dict(ws=None), dict(window=-1), dict(sinks=-1), dict(w=at), dict(wo=at), dict(q=odd), dict(out=odd)):
+    for bad in (dict(q=None), dict(n=None), dict(out=None), dict(w=at, wo=at, ws=None), dict(window=-1), dict(sinks=-1), dict(w=at), dict(wo=at), dict(q=odd), dict(out=odd)):
         assert attend(**bad) == BAD_ARG, bad
     assert attend(heads=0) == BAD_SHAPE and attend(heads=3) == BAD_SHAPE
     write = lambda q=at, qo=at, k=at, v=at, cos=None, sin=None, pos=None, rows=0, first=at, tokens=1, heads=4: lib.cq_kv4_write(
