@@ -333,7 +333,7 @@ int cq_kv4_evict(const cq_kv4* from, const cq_kv4* to, const float* weights, flo
                  long long* length_out, int keep, int sinks, int recent, int* kept, void* workspace, cq_stream_t stream);
 
 /* Attention of prompts: q (sequences, queries, n_heads, D), k and v (sequences, keys, n_kv_heads, D) fp16 with the given
- * strides in elements (the columns of a head are contiguous; addresses and strides multiples of 16 bytes).  Query i stands at
+ * strides in elements (the columns of a head are contiguous; addresses and strides multiples of 16 bytes; tokens do not share a row).  Query i stands at
  * position p = i + keys - queries and sees the keys j <= p with j < lengths[s] (device int64; NULL: keys), with a window only
  * those with j < sinks or j > p - window.  out (sequences, queries, n_heads, D) contiguous, lse (sequences, n_heads, queries)
  * fp32 = ln of the sum of exp(scale * q . k_j).  A row at or beyond its sequence's length, or that sees no key: zeros and

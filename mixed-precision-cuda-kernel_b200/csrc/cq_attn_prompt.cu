@@ -6,7 +6,8 @@
 //   out_i = sum_j softmax_j(scale q_i . k_j) v_j,  lse_i = ln sum_j exp(scale q_i . k_j)
 //   weights_j = sum of exp(scale q_i . k_j - lse_i) over the observed queries i of the KV head
 //
-// mma.sync tiles: 64 queries of a head against 64 keys at a time, four warps of 16 queries, a running maximum and sum per row.
+// Both are tcgen05 kernels, a persistent CTA on every SM: tiles come by TMA, products are 128 x 128 into tensor memory, and the
+// exponentials bound them.
 #include <algorithm>
 #include <cmath>
 
@@ -15,7 +16,6 @@
 
 namespace {
 
-constexpr int PR_THREADS = 128, PR_TILE = 64;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct PromptArgs {
@@ -24,144 +24,16 @@ struct PromptArgs {
   const long long* lengths;
 };
 
-__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const __half* p) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_at(p)));
-}
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const __half* p) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_at(p)));
-}
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ uint32_t half_pair(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
-}
-// 64 rows of D halves into shared memory (row stride D + 8); rows from `rows` on are zeros
-template <int D>
-__device__ __forceinline__ void load_tile(__half* to, const __half* src, long long stride, int rows) {
-  for (int i = threadIdx.x; i < PR_TILE * (D / 8); i += PR_THREADS) {
-    const int r = i / (D / 8), c = 8 * (i % (D / 8));
-    *reinterpret_cast<uint4*>(to + r * (D + 8) + c) = r < rows ? *reinterpret_cast<const uint4*>(src + r * stride + c) : make_uint4(0, 0, 0, 0);
-  }
-}
-__device__ __forceinline__ bool sees(const cq_prompt& s, int pos, int key, int n) {
-  return key <= pos && key < n && pos < n && (!s.window || key < s.sinks || key > pos - s.window);
 }
 __device__ __forceinline__ int length_of(const PromptArgs& a, int b) {
   if (!a.lengths) return a.s.keys;
   const long long n = a.lengths[b];
   return n < 0 ? 0 : (n > a.s.keys ? a.s.keys : (int)n);
 }
-// scores of this warp's 16 queries (fragments qf) against the 64 keys in shared memory, not scaled
-template <int D>
-__device__ __forceinline__ void scores64(float (&s)[8][4], const uint32_t (&qf)[D / 16][4], const __half* s_k, int lane) {
-#pragma unroll
-  for (int nt = 0; nt < 8; ++nt) {
-    s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-    for (int kc = 0; kc < D / 16; kc += 2) {
-      uint32_t r[4];
-      ldsm4(r, s_k + (8 * nt + (lane & 7)) * (D + 8) + 16 * kc + 8 * (lane >> 3));
-      mma16816(s[nt], qf[kc], r[0], r[1]);
-      mma16816(s[nt], qf[kc + 1], r[2], r[3]);
-    }
-  }
-}
-template <int D>
-__device__ __forceinline__ void query_fragments(uint32_t (&qf)[D / 16][4], const __half* s_q, int warp, int lane) {
-#pragma unroll
-  for (int kc = 0; kc < D / 16; ++kc) ldsm4(qf[kc], s_q + (16 * warp + (lane & 15)) * (D + 8) + 16 * kc + 8 * (lane >> 4));
-}
-
-template <int D>
-__global__ void __launch_bounds__(PR_THREADS) prompt_kernel(const __grid_constant__ PromptArgs a, __half* __restrict__ out, float* __restrict__ lse) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ __align__(16) __half s_k[PR_TILE * (D + 8)], s_v[PR_TILE * (D + 8)];
-  const cq_prompt& s = a.s;
-  const int q0 = blockIdx.x * PR_TILE, h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int kvh = h / (s.n_heads / s.n_kv_heads), off = s.keys - s.queries, n = length_of(a, b);
-  const int rows = min(PR_TILE, s.queries - q0), pmin = q0 + off, pmax = pmin + rows - 1;
-  uint32_t qf[D / 16][4];
-  load_tile<D>(s_k, a.q + b * s.q_strides[0] + (long long)q0 * s.q_strides[1] + h * s.q_strides[2], s.q_strides[1], rows);
-  __syncthreads();
-  query_fragments<D>(qf, s_k, warp, lane);
-  float o[D / 8][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
-  const float scale2 = s.scale * LOG2E;
-  const int r0 = pmin + 16 * warp + (lane >> 2);           // positions r0 and r0 + 8
-  const int end = pmin < n ? min(n, pmax + 1) : 0;
-  for (int k0 = 0; k0 < end; k0 += PR_TILE) {
-    if (s.window && k0 >= s.sinks && k0 + PR_TILE - 1 <= pmin - s.window) continue;
-    __syncthreads();
-    const __half* ks = a.k + b * s.k_strides[0] + (long long)k0 * s.k_strides[1] + kvh * s.k_strides[2];
-    const __half* vs = a.v + b * s.v_strides[0] + (long long)k0 * s.v_strides[1] + kvh * s.v_strides[2];
-    load_tile<D>(s_k, ks, s.k_strides[1], n - k0);
-    load_tile<D>(s_v, vs, s.v_strides[1], n - k0);
-    __syncthreads();
-    float sc[8][4];
-    scores64<D>(sc, qf, s_k, lane);
-    float top[2] = {m[0], m[1]};
-#pragma unroll
-    for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = k0 + 8 * nt + 2 * (lane & 3) + (e & 1);
-        sc[nt][e] = sees(s, r0 + 8 * (e >> 1), key, n) ? sc[nt][e] * scale2 : -INFINITY;
-        top[e >> 1] = fmaxf(top[e >> 1], sc[nt][e]);
-      }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-      const float ref = top[i] == -INFINITY ? 0.f : top[i], keep = exp2f(m[i] - ref);
-      m[i] = top[i];
-      l[i] *= keep;
-#pragma unroll
-      for (int nt = 0; nt < D / 8; ++nt) {
-        o[nt][2 * i] *= keep;
-        o[nt][2 * i + 1] *= keep;
-      }
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-        for (int e = 2 * i; e < 2 * i + 2; ++e) {
-          sc[nt][e] = exp2f(sc[nt][e] - ref);
-          l[i] += sc[nt][e];
-        }
-    }
-#pragma unroll
-    for (int kc = 0; kc < 4; ++kc) {
-      const uint32_t p[4] = {half_pair(sc[2 * kc][0], sc[2 * kc][1]), half_pair(sc[2 * kc][2], sc[2 * kc][3]),
-                             half_pair(sc[2 * kc + 1][0], sc[2 * kc + 1][1]), half_pair(sc[2 * kc + 1][2], sc[2 * kc + 1][3])};
-#pragma unroll
-      for (int nt = 0; nt < D / 8; nt += 2) {
-        uint32_t r[4];
-        ldsm4t(r, s_v + (16 * kc + (lane & 15)) * (D + 8) + 8 * (nt + (lane >> 4)));
-        mma16816(o[nt], p, r[0], r[1]);
-        mma16816(o[nt + 1], p, r[2], r[3]);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    const int r = q0 + 16 * warp + (lane >> 2) + 8 * i;
-    if (r >= s.queries) continue;
-    const bool empty = m[i] == -INFINITY && l[i] == 0.f;
-    const float inv = empty ? 0.f : 1.f / l[i];
-    __half* to = out + (((size_t)b * s.queries + r) * s.n_heads + h) * D + 2 * (lane & 3);
-#pragma unroll
-    for (int nt = 0; nt < D / 8; ++nt)
-      *reinterpret_cast<uint32_t*>(to + 8 * nt) = empty ? 0u : half_pair(o[nt][2 * i] * inv, o[nt][2 * i + 1] * inv);
-    if ((lane & 3) == 0) lse[((size_t)b * s.n_heads + h) * s.queries + r] = empty ? -INFINITY : ((m[i] == -INFINITY ? 0.f : m[i]) + log2f(l[i])) * LN2;
-  }
-}
-
-// ------------------------------------------------------------------ on tcgen05
+// ------------------------------------------------------------------ attention
 // A CTA takes two tiles of 128 queries of a head, one for each group of four softmax warps, and goes through the keys 128 at a
 // time.  S = Q . K^T and O += P . V are tcgen05.mma of one CTA (128 x 128 x 16 a step), all accumulators in tensor memory:
 // S of the two tiles, O of the two tiles, 512 columns; P takes the place of its S, as fp16, and is the A operand from there.
@@ -244,14 +116,6 @@ __device__ __forceinline__ uint64_t power2(float2 x) {
   const float2 n = apart(t);
   return mul2(p, two(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3F800000u), __uint_as_float((__float_as_uint(n.y) << 23) + 0x3F800000u)));
 }
-// whether the condition holds in any of the 256 threads of a query tile, and a barrier between them; the barrier alone
-__device__ __forceinline__ bool any_of_tile(int id, bool here) {
-  int any;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 256, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
-               : "=r"(any) : "r"((int)here), "r"(id) : "memory");
-  return any != 0;
-}
-__device__ __forceinline__ void tile_sync(int id) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -292,8 +156,52 @@ struct PromptItem {
   }
 };
 
+// 32 columns of a row (bit i of `which`: those from 32 i on) whose sum over whole tiles met 0 times a value that is no number, or
+// infinite: again, in fp32, over the keys that it sees.  total2 is log2 of its exponentials' sum.  (A value in a masked place has weight 0, which only then is not enough.  Left
+// out of line: finite values never come here, and it is slow: a dot product a thread.)
 template <int D>
-__global__ void __launch_bounds__(UM_THREADS, 1) prompt_umma_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ PromptMaps maps,
+__device__ __noinline__ void row_again(const PromptArgs& a, int item, int q, float total2, uint32_t which, __half* to) {
+  const PromptItem w(a, item);
+  const cq_prompt& s = a.s;
+  const __half* qr = a.q + w.b * s.q_strides[0] + q * s.q_strides[1] + w.h * s.q_strides[2];
+  const __half* ks = a.k + w.b * s.k_strides[0] + w.kvh * s.k_strides[2];
+  const __half* vs = a.v + w.b * s.v_strides[0] + w.kvh * s.v_strides[2];
+  const int hi = q + s.keys - s.queries, lo = s.window ? hi - s.window + 1 : 0;
+  for (int c = 0; c < D; c += 32) {
+    if (!(which >> (c / 32) & 1u)) continue;
+    float y[32] = {};
+    for (int j = 0; j <= hi; ++j) {
+      if (j >= s.sinks && j < lo) j = lo;
+      const uint4* kr = reinterpret_cast<const uint4*>(ks + j * s.k_strides[1]);
+      float dot = 0.f;
+#pragma unroll 1
+      for (int e = 0; e < D / 8; ++e) {
+        const uint4 x = reinterpret_cast<const uint4*>(qr)[e], z = kr[e];
+        const __half2 *xh = reinterpret_cast<const __half2*>(&x), *zh = reinterpret_cast<const __half2*>(&z);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = __half22float2(xh[i]), g = __half22float2(zh[i]);
+          dot = fmaf(f.x, g.x, fmaf(f.y, g.y, dot));
+        }
+      }
+      const float p = exp2f(dot * (s.scale * LOG2E) - total2);
+#pragma unroll
+      for (int e = 0; e < 32; e += 8) {
+        const uint4 x = *reinterpret_cast<const uint4*>(vs + j * s.v_strides[1] + c + e);
+        const __half* xh = reinterpret_cast<const __half*>(&x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[e + i] = fmaf(p, __half2float(xh[i]), y[e + i]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 32; e += 8)
+      *reinterpret_cast<uint4*>(to + c + e) =
+          make_uint4(half_pair(y[e], y[e + 1]), half_pair(y[e + 2], y[e + 3]), half_pair(y[e + 4], y[e + 5]), half_pair(y[e + 6], y[e + 7]));
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ PromptMaps maps,
                                                                     __half* __restrict__ out, float* __restrict__ lse, int items,
                                                                     uint32_t* __restrict__ status) {
   using namespace umma;
@@ -302,7 +210,6 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_umma_kernel(const __grid
   __shared__ __align__(8) uint64_t s_bar[3 + 2 * UM_STAGES + 6];
   __shared__ uint32_t s_tmem;
   __shared__ int s_gone;
-  __shared__ float s_row[2][2][128];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t smem = (smem_at(um_smem) + 1023u) & ~1023u, s_q = smem, s_kv = smem + 2 * TILE_BYTES;
   const uint32_t bars = smem_at(s_bar);
@@ -544,6 +451,7 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_umma_kernel(const __grid
       fence_after();
       const float inv = empty ? 0.f : 1.f / total;
       __half* to = out + (((size_t)w.b * s.queries + q) * s.n_heads + w.h) * D;
+      uint32_t which = 0;                                  // bit i: a NaN in the 32 columns from 32 i on
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t y[32];
@@ -552,6 +460,11 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_umma_kernel(const __grid
           wait_load<32>(y);
         }
         if (!row) continue;
+        uint64_t all[2] = {};
+#pragma unroll
+        for (int e = 0; e < 16; ++e) all[e & 1] = add2(all[e & 1], two(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1])));
+        const float2 any = apart(add2(all[0], all[1]));
+        if (any.x != any.x || any.y != any.y) which |= 1u << (c / 32);
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
           uint32_t v[4];
@@ -560,7 +473,9 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_umma_kernel(const __grid
           *reinterpret_cast<uint4*>(to + c + e) = !ok ? make_uint4(~0u, ~0u, ~0u, ~0u) : (empty ? make_uint4(0, 0, 0, 0) : make_uint4(v[0], v[1], v[2], v[3]));
         }
       }
-      if (row) lse[((size_t)w.b * s.n_heads + w.h) * s.queries + q] = !ok ? NAN : (empty ? -INFINITY : ((ref == -INFINITY ? 0.f : ref) - LIFT + log2f(total)) * LN2);
+      const float total2 = (ref == -INFINITY ? 0.f : ref) - LIFT + log2f(total);
+      if (row) lse[((size_t)w.b * s.n_heads + w.h) * s.queries + q] = !ok ? NAN : (empty ? -INFINITY : total2 * LN2);
+      if (row && ok && !empty && which && total == total) row_again<D>(a, item, q, total2, which, to);
     }
   }
   fence_before();
@@ -571,7 +486,7 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_umma_kernel(const __grid
   }
 }
 
-// ------------------------------------------------------------------ weights of the keys on tcgen05
+// ------------------------------------------------------------------ weights of the keys
 // S^T = K . Q^T of 128 keys (lanes of tensor memory, a thread each) and 128 queries (columns): a key's weight is a sum along
 // its thread's own columns, so nothing is exchanged.  The columns are two blocks of 64 queries, of any two heads and places:
 // queries of a head that are fewer than 128 do not leave a tile half empty.  Bound by the exponentials, one for each pair and
@@ -776,7 +691,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
           load32(at + c0, x);
           wait_load<32>(x);
           const int p0 = place[c0 / 64] + c0 % 64;
-          const bool whole = w.k0 + UM_TILE - 1 <= p0 && p0 + 32 <= w.last && (!s.window || w.k0 + UM_TILE - 1 < s.sinks || p0 + 31 < w.k0 + s.window);
+          const bool whole = w.k0 + UM_TILE - 1 <= p0 && p0 + 32 <= w.last && (!s.window || w.k0 + UM_TILE - 1 < s.sinks || p0 + 31 - w.k0 < s.window);
           if (!whole) {
             const uint32_t vis = below32(hi + 1 - p0) & ~below32(lo - p0);
 #pragma unroll
@@ -866,7 +781,7 @@ bool map_of(CUtensorMap* map, const void* at, const int64_t (&strides)[3], int s
     }
     return (Encode)fn;
   }();
-  if (!encode || (tokens > 1 && strides[1] < 8)) return false;
+  if (!encode) return false;
   one[0] = heads > 1 && strides[2] != 0;
   one[1] = sequences > 1 && strides[0] != 0;
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)tokens, one[0] ? (cuuint64_t)heads : 1, one[1] ? (cuuint64_t)sequences : 1};
@@ -877,60 +792,6 @@ bool map_of(CUtensorMap* map, const void* at, const int64_t (&strides)[3], int s
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// 64 keys of a KV head, all its query heads and observed queries one after another
-template <int D>
-__global__ void __launch_bounds__(PR_THREADS) prompt_weights_kernel(const __grid_constant__ PromptArgs a, const float* __restrict__ lse, int observe,
-                                                                    float* __restrict__ weights) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ __align__(16) __half s_k[PR_TILE * (D + 8)], s_q[PR_TILE * (D + 8)];
-  __shared__ float s_sum[4][PR_TILE];
-  const cq_prompt& s = a.s;
-  const int k0 = blockIdx.x * PR_TILE, kvh = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int G = s.n_heads / s.n_kv_heads, off = s.keys - s.queries, n = length_of(a, b);
-  load_tile<D>(s_k, a.k + b * s.k_strides[0] + (long long)k0 * s.k_strides[1] + kvh * s.k_strides[2], s.k_strides[1], n - k0);
-  const float scale2 = s.scale * LOG2E;
-  float sum[8][2] = {};
-  // positions of the queries that count: the observed ones from this tile's first key on, and within its last key's window
-  const int first = max(max(off, n - observe), k0);
-  const int last = s.window && k0 >= s.sinks ? min(n, min(k0 + PR_TILE, n) - 1 + s.window) : n;
-  for (int g = 0; g < G; ++g)
-    for (int p0 = first; p0 < last; p0 += PR_TILE) {
-      const int h = kvh * G + g, q0 = p0 - off;
-      __syncthreads();
-      load_tile<D>(s_q, a.q + b * s.q_strides[0] + (long long)q0 * s.q_strides[1] + h * s.q_strides[2], s.q_strides[1], last - p0);
-      __syncthreads();
-      uint32_t qf[D / 16][4];
-      query_fragments<D>(qf, s_q, warp, lane);
-      float sc[8][4];
-      scores64<D>(sc, qf, s_k, lane);
-      float ref[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int p = p0 + 16 * warp + (lane >> 2) + 8 * i;
-        ref[i] = p < last ? lse[((size_t)b * s.n_heads + h) * s.queries + p - off] * LOG2E : 0.f;
-      }
-#pragma unroll
-      for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = k0 + 8 * nt + 2 * (lane & 3) + (e & 1), p = p0 + 16 * warp + (lane >> 2) + 8 * (e >> 1);
-          if (p < last && sees(s, p, key, n)) sum[nt][e & 1] += exp2f(sc[nt][e] * scale2 - ref[e >> 1]);
-        }
-    }
-#pragma unroll
-  for (int nt = 0; nt < 8; ++nt)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      for (int d = 4; d < 32; d *= 2) sum[nt][e] += __shfl_xor_sync(0xffffffffu, sum[nt][e], d);
-      if (lane < 4) s_sum[warp][8 * nt + 2 * lane + e] = sum[nt][e];
-    }
-  __syncthreads();
-  if (threadIdx.x < PR_TILE && k0 + threadIdx.x < s.keys)
-    weights[((size_t)b * s.n_kv_heads + kvh) * s.keys + k0 + threadIdx.x] =
-        (s_sum[0][threadIdx.x] + s_sum[1][threadIdx.x]) + (s_sum[2][threadIdx.x] + s_sum[3][threadIdx.x]);
-}
-
 int check(const cq_prompt* s, const void* q, const void* k, const void* v) {
   if (!s || !q || !k || (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) || s->window < 0 || s->sinks < 0 || !(s->scale > 0.f)) return CQ_ERR_BAD_ARG;
   if (s->sequences < 1 || s->sequences > 65535 || s->queries < 1 || s->keys < s->queries || s->keys > (1 << 24) || s->n_kv_heads < 1 ||
@@ -939,6 +800,7 @@ int check(const cq_prompt* s, const void* q, const void* k, const void* v) {
   if (s->head_dim != 64 && s->head_dim != 128) return CQ_ERR_UNSUPPORTED;
   for (int i = 0; i < 3; ++i)
     if ((s->q_strides[i] | s->k_strides[i] | (v ? s->v_strides[i] : 0)) & 7) return CQ_ERR_BAD_ARG;
+  if ((s->queries > 1 && s->q_strides[1] < 8) || (s->keys > 1 && (s->k_strides[1] < 8 || (v && s->v_strides[1] < 8)))) return CQ_ERR_BAD_ARG;
   return CQ_OK;
 }
 
@@ -952,21 +814,17 @@ extern "C" int cq_attn_prefill(const cq_prompt* shape, const void* q, const void
   const PromptArgs a = {*shape, (const __half*)q, (const __half*)k, (const __half*)v, lengths};
   const int D = shape->head_dim, B = shape->sequences;
   PromptMaps maps;
-  if (map_of(&maps.q, q, shape->q_strides, B, shape->queries, shape->n_heads, D, UM_TILE, maps.one[0]) &&
-      map_of(&maps.k, k, shape->k_strides, B, shape->keys, shape->n_kv_heads, D, UM_TILE, maps.one[1]) &&
-      map_of(&maps.v, v, shape->v_strides, B, shape->keys, shape->n_kv_heads, D, UM_TILE, maps.one[2])) {
-    auto fn = D == 128 ? prompt_umma_kernel<128> : prompt_umma_kernel<64>;
-    const int smem = (2 + UM_STAGES) * (D / 64) * UM_CHUNK + 1024;
-    CQ_CUDA_TRY(cq_grant_smem((const void*)fn, smem));
-    const long long items = (long long)((shape->queries + 2 * UM_TILE - 1) / (2 * UM_TILE)) * shape->n_heads * B;
-    if (items > INT32_MAX) return CQ_ERR_BAD_SHAPE;
-    CQ_CUDA_TRY(kv4_launch(fn, dim3((unsigned)std::min<long long>(items, cq_sm_count())), dim3(UM_THREADS), smem, (cudaStream_t)stream, a, maps,
-                           (__half*)out, lse, (int)items, status_word));
-    return CQ_OK;
-  }
+  if (!map_of(&maps.q, q, shape->q_strides, B, shape->queries, shape->n_heads, D, UM_TILE, maps.one[0]) ||
+      !map_of(&maps.k, k, shape->k_strides, B, shape->keys, shape->n_kv_heads, D, UM_TILE, maps.one[1]) ||
+      !map_of(&maps.v, v, shape->v_strides, B, shape->keys, shape->n_kv_heads, D, UM_TILE, maps.one[2]))
+    return CQ_ERR_UNSUPPORTED;
   auto fn = D == 128 ? prompt_kernel<128> : prompt_kernel<64>;
-  CQ_CUDA_TRY(kv4_launch(fn, dim3((shape->queries + PR_TILE - 1) / PR_TILE, shape->n_heads, B), dim3(PR_THREADS), 0, (cudaStream_t)stream, a,
-                         (__half*)out, lse));
+  const int smem = (2 + UM_STAGES) * (D / 64) * UM_CHUNK + 1024;
+  CQ_CUDA_TRY(cq_grant_smem((const void*)fn, smem));
+  const long long items = (long long)((shape->queries + 2 * UM_TILE - 1) / (2 * UM_TILE)) * shape->n_heads * B;
+  if (items > INT32_MAX / 2) return CQ_ERR_BAD_SHAPE;
+  CQ_CUDA_TRY(kv4_launch(fn, dim3((unsigned)std::min<long long>(items, cq_sm_count())), dim3(UM_THREADS), smem, (cudaStream_t)stream, a, maps,
+                         (__half*)out, lse, (int)items, status_word));
   return CQ_OK;
 }
 
@@ -984,24 +842,20 @@ extern "C" int cq_attn_prefill_weights(const cq_prompt* shape, const void* q, co
   const PromptArgs a = {*shape, (const __half*)q, (const __half*)k, nullptr, lengths};
   const int D = shape->head_dim, B = shape->sequences;
   PromptMaps maps;
-  if (map_of(&maps.q, q, shape->q_strides, B, shape->queries, shape->n_heads, D, KW_Q, maps.one[0]) &&
-      map_of(&maps.k, k, shape->k_strides, B, shape->keys, shape->n_kv_heads, D, UM_TILE, maps.one[1])) {
-    maps.v = maps.k;
-    auto fn = D == 128 ? prompt_keys_kernel<128> : prompt_keys_kernel<64>;
-    const int smem = (2 + KW_BUFFERS) * (D / 64) * UM_CHUNK + 1024;
-    CQ_CUDA_TRY(cq_grant_smem((const void*)fn, smem));
-    const int parts = parts_of(shape, observe);
-    const long long n = (long long)B * shape->n_kv_heads * shape->keys, items = (long long)((shape->keys + UM_TILE - 1) / UM_TILE) * shape->n_kv_heads * B * parts;
-    if (items > INT32_MAX) return CQ_ERR_BAD_SHAPE;
-    CQ_CUDA_TRY(kv4_launch(fn, dim3((unsigned)std::min<long long>(items, cq_sm_count())), dim3(KW_THREADS), smem, (cudaStream_t)stream, a, maps, lse,
-                           observe, parts, parts > 1 ? (float*)workspace : weights, (int)items, status_word));
-    if (parts > 1)
-      CQ_CUDA_TRY(kv4_launch(prompt_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (cudaStream_t)stream, (const float*)workspace, parts, n,
-                             weights));
-    return CQ_OK;
-  }
-  auto fn = D == 128 ? prompt_weights_kernel<128> : prompt_weights_kernel<64>;
-  CQ_CUDA_TRY(kv4_launch(fn, dim3((shape->keys + PR_TILE - 1) / PR_TILE, shape->n_kv_heads, B), dim3(PR_THREADS), 0, (cudaStream_t)stream, a, lse,
-                         observe, weights));
+  if (!map_of(&maps.q, q, shape->q_strides, B, shape->queries, shape->n_heads, D, KW_Q, maps.one[0]) ||
+      !map_of(&maps.k, k, shape->k_strides, B, shape->keys, shape->n_kv_heads, D, UM_TILE, maps.one[1]))
+    return CQ_ERR_UNSUPPORTED;
+  maps.v = maps.k;
+  auto fn = D == 128 ? prompt_keys_kernel<128> : prompt_keys_kernel<64>;
+  const int smem = (2 + KW_BUFFERS) * (D / 64) * UM_CHUNK + 1024;
+  CQ_CUDA_TRY(cq_grant_smem((const void*)fn, smem));
+  const int parts = parts_of(shape, observe);
+  const long long n = (long long)B * shape->n_kv_heads * shape->keys, items = (long long)((shape->keys + UM_TILE - 1) / UM_TILE) * shape->n_kv_heads * B * parts;
+  if (items > INT32_MAX / 2) return CQ_ERR_BAD_SHAPE;
+  CQ_CUDA_TRY(kv4_launch(fn, dim3((unsigned)std::min<long long>(items, cq_sm_count())), dim3(KW_THREADS), smem, (cudaStream_t)stream, a, maps, lse,
+                         observe, parts, parts > 1 ? (float*)workspace : weights, (int)items, status_word));
+  if (parts > 1)
+    CQ_CUDA_TRY(kv4_launch(prompt_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (cudaStream_t)stream, (const float*)workspace, parts, n,
+                           weights));
   return CQ_OK;
 }

@@ -24,7 +24,6 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "=r"(ok) : "r"(bar), "r"(parity), "r"(20000u) : "memory");
   return ok != 0;
 }
-// (Inlined: a function call does not go with setmaxnreg.)
 // Bounded wait: after two seconds of the device's clock (or at once where another wait of the CTA ran out) it gives up, notes
 // that in *gone and in the status word, and returns false; the CTA then runs on to its end.
 __device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* gone, uint32_t* status) {

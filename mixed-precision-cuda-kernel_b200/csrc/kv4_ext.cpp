@@ -253,6 +253,11 @@ void strides_of(const torch::Tensor& t, const char* name, const c10::Device& dev
   TORCH_CHECK(fits, name, " must have contiguous columns and 16-byte aligned rows");
 }
 
+// one row for all tokens (an expanded tensor) is written out: the kernels' copies of tiles need a step from token to token
+torch::Tensor rows_apart(const torch::Tensor& t) {
+  return t.defined() && t.dim() == 4 && t.size(1) > 1 && t.stride(1) == 0 ? t.contiguous() : t;
+}
+
 cq_prompt prompt_of(const torch::Tensor& q, const torch::Tensor& k, int64_t window, int64_t sinks, const OptTensor& lengths,
                     c10::optional<double> scale, const long long** n) {
   cq_prompt s = {};
@@ -278,10 +283,11 @@ cq_prompt prompt_of(const torch::Tensor& q, const torch::Tensor& k, int64_t wind
   return s;
 }
 
-std::pair<torch::Tensor, torch::Tensor> attn_prefill(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, int64_t window,
+std::pair<torch::Tensor, torch::Tensor> attn_prefill(torch::Tensor q, torch::Tensor k, torch::Tensor v, int64_t window,
                                                      int64_t sinks, const OptTensor& lengths, c10::optional<double> scale) {
   const at::cuda::OptionalCUDAGuard guard(device_of(q));
   const long long* n;
+  q = rows_apart(q), k = rows_apart(k), v = rows_apart(v);
   cq_prompt s = prompt_of(q, k, window, sinks, lengths, scale, &n);
   strides_of(v, "v", q.device(), s.v_strides);
   TORCH_CHECK(v.sizes() == k.sizes(), "v must have the shape of k");
@@ -293,10 +299,11 @@ std::pair<torch::Tensor, torch::Tensor> attn_prefill(const torch::Tensor& q, con
   return {out, lse};
 }
 
-torch::Tensor attn_prefill_weights(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& lse, int64_t window, int64_t sinks,
+torch::Tensor attn_prefill_weights(torch::Tensor q, torch::Tensor k, const torch::Tensor& lse, int64_t window, int64_t sinks,
                                    const OptTensor& lengths, c10::optional<int64_t> observe, c10::optional<double> scale) {
   const at::cuda::OptionalCUDAGuard guard(device_of(q));
   const long long* n;
+  q = rows_apart(q), k = rows_apart(k);
   const cq_prompt s = prompt_of(q, k, window, sinks, lengths, scale, &n);
   check_tensor(lse, "lse", torch::kFloat32, q.device());
   TORCH_CHECK(lse.dim() == 3 && lse.size(0) == s.sequences && lse.size(1) == s.n_heads && lse.size(2) == s.queries,

@@ -208,3 +208,45 @@ def test_refusals(qc):
             call()
             pytest.fail(f"call {i} was taken")
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("D,window,sinks", [(128, 0, 0), (64, 0, 0), (128, 70, 3), (64, 70, 0)])
+def test_masked_values_may_be_anything(qc, bad, D, window, sinks):
+    """A value that is no number, or infinite, reaches the rows that see it, in its columns, and no other."""
+    q, k, v = make(2, 300, 340, 4, 2, D, 9)
+    want, lse = qc.attn_prefill(q, k, v, window=window, sinks=sinks)
+    v2 = v.clone()
+    v2[0, 200, 1, 5] = v2[1, 250, 0] = v2[1, 339, 1, D - 1] = bad
+    out, l = qc.attn_prefill(q, k, v2, window=window, sinks=sinks)
+    assert torch.equal(l, lse)
+    m = seen(300, 340, 340, window, sinks)
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[0, :, 2:, 5] |= m[:, 200, None]
+    hit[1, :, :2] |= m[:, 250, None, None]
+    hit[1, :, 2:, D - 1] |= m[:, 339, None]
+    assert not out[hit].isfinite().any() and out[~hit].isfinite().all()
+    if not math.isnan(bad):
+        assert (out[hit] == bad).all()
+    top = float(v.abs().max())
+    ref = reference(q, k, v, None, window, sinks)[0]
+    assert ((out.double() - ref).abs()[~hit] <= 3 * 2.0 ** -11 * top).all()
+    assert torch.equal(out[0, :, :2], want[0, :, :2])
+
+
+def test_rows_shared_by_all_tokens(qc):
+    """An expanded token: every position has the same key and value, or the same query."""
+    q, k, v = make(2, 90, 150, 4, 2, 128, 10)
+    for x, y, z in ((q, k[:, :1].expand(-1, 150, -1, -1), v), (q, k, v[:, 3:4].expand(-1, 150, -1, -1)), (q[:, 2:3].expand(-1, 90, -1, -1), k, v)):
+        assert torch.equal(check(qc, x, y, z, None, 40, 2), qc.attn_prefill(x.contiguous(), y.contiguous(), z.contiguous(), window=40, sinks=2)[0])
+
+
+def test_windows_of_any_size(qc):
+    """A window or sinks up to 2^31 - 1 that leave nothing out."""
+    q, k, v = make(1, 200, 260, 2, 1, 64, 11)
+    want, lse = qc.attn_prefill(q, k, v)
+    w = qc.attn_prefill_weights(q, k, lse)
+    for window, sinks in ((2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (5, 2 ** 31 - 1)):
+        out, l = qc.attn_prefill(q, k, v, window=window, sinks=sinks)
+        assert ((out.double() - want.double()).abs() <= 2.0 ** -10 * float(v.abs().max())).all()
+        assert torch.equal(qc.attn_prefill_weights(q, k, lse, window=window, sinks=sinks), w)
