@@ -156,47 +156,49 @@ struct PromptItem {
   }
 };
 
-// 32 columns of a row (bit i of `which`: those from 32 i on) whose sum over whole tiles met 0 times a value that is no number, or
-// infinite: again, in fp32, over the keys that it sees.  total2 is log2 of its exponentials' sum.  (A value in a masked place has weight 0, which only then is not enough.  Left
-// out of line: finite values never come here, and it is slow: a dot product a thread.)
+// A value in a masked place has the weight 0, and 0 times infinity or NaN is NaN: where a softmax warp wrote a NaN in a row with a
+// finite lse, its columns with one are summed again in fp32 over the keys that the row sees, at the CTA's end, where no other
+// warp waits.  (Finite values never come here.)
 template <int D>
-__device__ __noinline__ void row_again(const PromptArgs& a, int item, int q, float total2, uint32_t which, __half* to) {
-  const PromptItem w(a, item);
+__device__ __noinline__ void rows_again(const PromptArgs& a, int items, __half* out, const float* lse) {
+  constexpr int C = D / 32;                                // columns of a lane
   const cq_prompt& s = a.s;
-  const __half* qr = a.q + w.b * s.q_strides[0] + q * s.q_strides[1] + w.h * s.q_strides[2];
-  const __half* ks = a.k + w.b * s.k_strides[0] + w.kvh * s.k_strides[2];
-  const __half* vs = a.v + w.b * s.v_strides[0] + w.kvh * s.v_strides[2];
-  const int hi = q + s.keys - s.queries, lo = s.window ? hi - s.window + 1 : 0;
-  for (int c = 0; c < D; c += 32) {
-    if (!(which >> (c / 32) & 1u)) continue;
-    float y[32] = {};
-    for (int j = 0; j <= hi; ++j) {
-      if (j >= s.sinks && j < lo) j = lo;
-      const uint4* kr = reinterpret_cast<const uint4*>(ks + j * s.k_strides[1]);
-      float dot = 0.f;
-#pragma unroll 1
-      for (int e = 0; e < D / 8; ++e) {
-        const uint4 x = reinterpret_cast<const uint4*>(qr)[e], z = kr[e];
-        const __half2 *xh = reinterpret_cast<const __half2*>(&x), *zh = reinterpret_cast<const __half2*>(&z);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __syncwarp();
+  for (int round = 0, item; (item = PromptItem::at(round, items)) >= 0; ++round) {
+    const PromptItem w(a, item);
+    const __half* ks = a.k + w.b * s.k_strides[0] + w.kvh * s.k_strides[2] + C * lane;
+    const __half* vs = a.v + w.b * s.v_strides[0] + w.kvh * s.v_strides[2] + C * lane;
+    for (int q = w.q0 + 32 * warp, end = min(q + 32, s.queries); q < end; ++q) {
+      __half* to = out + (((size_t)w.b * s.queries + q) * s.n_heads + w.h) * D + C * lane;
+      const float l = lse[((size_t)w.b * s.n_heads + w.h) * s.queries + q];
+      bool mine = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = __half22float2(xh[i]), g = __half22float2(zh[i]);
-          dot = fmaf(f.x, g.x, fmaf(f.y, g.y, dot));
+      for (int i = 0; i < C; ++i) mine |= __hisnan(to[i]);
+      if (!(fabsf(l) < INFINITY) || !__any_sync(0xffffffffu, mine)) continue;
+      const __half* qr = a.q + w.b * s.q_strides[0] + q * s.q_strides[1] + w.h * s.q_strides[2] + C * lane;
+      float x[C], y[C] = {};
+#pragma unroll
+      for (int i = 0; i < C; ++i) x[i] = __half2float(qr[i]) * (s.scale * LOG2E);
+      const int hi = q + s.keys - s.queries, lo = s.window ? max(0, hi - s.window + 1) : 0;
+      for (int part = 0; part < 2; ++part) {
+        const int from = part ? lo : 0, to_key = part ? hi + 1 : min(s.sinks, lo);
+#pragma unroll 4
+        for (int j = from; j < to_key; ++j) {
+          float dot = 0.f;
+#pragma unroll
+          for (int i = 0; i < C; ++i) dot = fmaf(x[i], __half2float(ks[j * s.k_strides[1] + i]), dot);
+#pragma unroll
+          for (int d = 16; d; d /= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+          const float p = exp2f(dot - l * LOG2E);
+#pragma unroll
+          for (int i = 0; i < C; ++i) y[i] = fmaf(p, __half2float(vs[j * s.v_strides[1] + i]), y[i]);
         }
       }
-      const float p = exp2f(dot * (s.scale * LOG2E) - total2);
 #pragma unroll
-      for (int e = 0; e < 32; e += 8) {
-        const uint4 x = *reinterpret_cast<const uint4*>(vs + j * s.v_strides[1] + c + e);
-        const __half* xh = reinterpret_cast<const __half*>(&x);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[e + i] = fmaf(p, __half2float(xh[i]), y[e + i]);
-      }
+      for (int i = 0; i < C; ++i)
+        if (__hisnan(to[i])) to[i] = __float2half_rn(y[i]);
     }
-#pragma unroll
-    for (int e = 0; e < 32; e += 8)
-      *reinterpret_cast<uint4*>(to + c + e) =
-          make_uint4(half_pair(y[e], y[e + 1]), half_pair(y[e + 2], y[e + 3]), half_pair(y[e + 4], y[e + 5]), half_pair(y[e + 6], y[e + 7]));
   }
 }
 
@@ -210,6 +212,7 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
   __shared__ __align__(8) uint64_t s_bar[3 + 2 * UM_STAGES + 6];
   __shared__ uint32_t s_tmem;
   __shared__ int s_gone;
+  __shared__ int s_nan[W_LOAD];                            // a softmax warp met a NaN in a sum
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t smem = (smem_at(um_smem) + 1023u) & ~1023u, s_q = smem, s_kv = smem + 2 * TILE_BYTES;
   const uint32_t bars = smem_at(s_bar);
@@ -234,6 +237,7 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
       bar_init(o_done(t), 1);
     }
     s_gone = 0;
+    for (int i = 0; i < W_LOAD; ++i) s_nan[i] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == W_MMA) alloc(&s_tmem, 512);
@@ -451,7 +455,6 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
       fence_after();
       const float inv = empty ? 0.f : 1.f / total;
       __half* to = out + (((size_t)w.b * s.queries + q) * s.n_heads + w.h) * D;
-      uint32_t which = 0;                                  // bit i: a NaN in the 32 columns from 32 i on
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t y[32];
@@ -464,7 +467,7 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
 #pragma unroll
         for (int e = 0; e < 16; ++e) all[e & 1] = add2(all[e & 1], two(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1])));
         const float2 any = apart(add2(all[0], all[1]));
-        if (any.x != any.x || any.y != any.y) which |= 1u << (c / 32);
+        if (any.x != any.x || any.y != any.y) s_nan[warp] = 1;
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
           uint32_t v[4];
@@ -473,9 +476,7 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
           *reinterpret_cast<uint4*>(to + c + e) = !ok ? make_uint4(~0u, ~0u, ~0u, ~0u) : (empty ? make_uint4(0, 0, 0, 0) : make_uint4(v[0], v[1], v[2], v[3]));
         }
       }
-      const float total2 = (ref == -INFINITY ? 0.f : ref) - LIFT + log2f(total);
-      if (row) lse[((size_t)w.b * s.n_heads + w.h) * s.queries + q] = !ok ? NAN : (empty ? -INFINITY : total2 * LN2);
-      if (row && ok && !empty && which && total == total) row_again<D>(a, item, q, total2, which, to);
+      if (row) lse[((size_t)w.b * s.n_heads + w.h) * s.queries + q] = !ok ? NAN : (empty ? -INFINITY : ((ref == -INFINITY ? 0.f : ref) - LIFT + log2f(total)) * LN2);
     }
   }
   fence_before();
@@ -484,6 +485,7 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
     fence_after();
     dealloc(tmem, 512);
   }
+  if (warp < W_LOAD && s_nan[warp]) rows_again<D>(a, items, out, lse);
 }
 
 // ------------------------------------------------------------------ weights of the keys

@@ -250,3 +250,14 @@ def test_windows_of_any_size(qc):
         out, l = qc.attn_prefill(q, k, v, window=window, sinks=sinks)
         assert ((out.double() - want.double()).abs() <= 2.0 ** -10 * float(v.abs().max())).all()
         assert torch.equal(qc.attn_prefill_weights(q, k, lse, window=window, sinks=sinks), w)
+
+
+def test_masked_infinities_in_a_long_prompt(qc):
+    """As above over several tiles and items of a CTA: the last token's values are infinite, only its own row sees them."""
+    q, k, v = make(1, 1500, 1500, 40, 40, 128, 12)
+    want, lse = qc.attn_prefill(q, k, v)
+    v[0, 1499] = math.inf
+    out, l = qc.attn_prefill(q, k, v)
+    assert torch.equal(l, lse) and (out[0, 1499] == math.inf).all()
+    assert ((out[0, :1499].double() - want[0, :1499].double()).abs() <= 6 * 2.0 ** -11 * float(v[0, :1499].abs().max())).all()
+    assert torch.equal(out[0, :1408], want[0, :1408])
