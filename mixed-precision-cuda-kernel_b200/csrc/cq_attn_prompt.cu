@@ -181,8 +181,10 @@ __device__ __noinline__ void rows_again(const PromptArgs& a, int items, __half* 
 #pragma unroll
       for (int i = 0; i < C; ++i) x[i] = __half2float(qr[i]) * (s.scale * LOG2E);
       const int hi = q + s.keys - s.queries, lo = s.window ? max(0, hi - s.window + 1) : 0;
-      for (int part = 0; part < 2; ++part) {
-        const int from = part ? lo : 0, to_key = part ? hi + 1 : min(s.sinks, lo);
+      bool done = false;                                   // NaN again: the row sees one
+      for (int from = 0, to_key; from <= hi && !done; from = to_key) {
+        if (from >= s.sinks && from < lo) from = lo;
+        to_key = min(min(from + 128, hi + 1), from < min(s.sinks, lo) ? min(s.sinks, lo) : hi + 1);
 #pragma unroll 4
         for (int j = from; j < to_key; ++j) {
           float dot = 0.f;
@@ -194,6 +196,10 @@ __device__ __noinline__ void rows_again(const PromptArgs& a, int items, __half* 
 #pragma unroll
           for (int i = 0; i < C; ++i) y[i] = fmaf(p, __half2float(vs[j * s.v_strides[1] + i]), y[i]);
         }
+        done = true;
+#pragma unroll
+        for (int i = 0; i < C; ++i) done = done && (y[i] != y[i] || !__hisnan(to[i]));
+        done = __all_sync(0xffffffffu, done);
       }
 #pragma unroll
       for (int i = 0; i < C; ++i)

@@ -32,11 +32,21 @@ def kept4(x, group):
 class Plain:
     """The harness's 4-bit methods as torch expressions; every sequence's cache is a list of rows."""
 
-    def __init__(self, d, group):
+    def __init__(self, d, group, other=None):
         self.d, self.group = d, group
+        self.rows = {}                                  # a layer's q, k, v in the last call on the other side
+        if other is not None:
+            for name in ("_kv4_step", "_kv4_prompt"):
+                setattr(other, name, self.noting(getattr(other, name)))
         self.k, self.v, self.w = ([None] * len(d.caches) for _ in range(3))
         for name in ("_kv4_step", "_kv4_prompt", "_kv4_evict"):
             setattr(d, name, getattr(self, name[5:]))
+
+    def noting(self, method):
+        def call(li, q, k, v, pos):
+            self.rows[li] = q.clone(), k.clone(), v.clone()
+            return method(li, q, k, v, pos)
+        return call
 
     def turn(self, x, pos):
         c, s = self.d.cos[pos][:, None], self.d.sin[pos][:, None]
@@ -60,6 +70,7 @@ class Plain:
         return p.unflatten(1, (kv, -1)).sum(2)
 
     def prompt(self, li, q, k, v, pos):
+        q, k, v = self.rows.get(li, (q, k, v))
         d, B = self.d, self.d.batch
         q, k = self.turn(q, pos), self.turn(k, pos)
         rows = lambda x: x.view(B, -1, *x.shape[1:])
@@ -73,6 +84,7 @@ class Plain:
         return out.reshape(-1, *q.shape[1:]).contiguous()
 
     def step(self, li, q, k, v, pos):
+        q, k, v = self.rows.get(li, (q, k, v))
         q, k = self.turn(q, pos), self.turn(k, pos)
         self.k[li] = torch.cat([self.k[li], kept4(k, self.group)[:, :, None]], 2)
         self.v[li] = torch.cat([self.v[li], kept4(v, self.group)[:, :, None]], 2)
@@ -104,10 +116,12 @@ def test_against_torch_expressions(dec, batch, kv, head_dim, group, options):
     # With evictions one layer: its queries, keys and values follow from the tokens alone and are the same on both sides, so that
     # the weights that are ranked differ in their last bits only.  (Behind a first layer, whose outputs differ by roundings, slots
     # of nearly equal weight are ranked otherwise here and there, and other slots stay.)
+    # Without evictions two layers; the torch expressions take the second layer's rows from the kernels' side, as a last bit there
+    # can be another 4-bit code, which is 1/15 of the group's range.
     cfg = tiny(dec, kv, head_dim, layers=1 if "kv_budget" in options else 2)
     make = lambda: dec.CherryDecoder(cfg, seed=5, batch=batch, kv_bits=4, kv_group=group, **options)
     a, b = make(), make()
-    plain = Plain(b, group)
+    plain = Plain(b, group, a)
     prompt = torch.randint(0, cfg.vocab, (batch, 45), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
     la, lb = a.prefill(prompt), b.prefill(prompt)
     scale = float(lb.float().abs().max())
