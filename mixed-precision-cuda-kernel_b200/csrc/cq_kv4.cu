@@ -330,7 +330,9 @@ extern "C" int cq_kv4_evict(const cq_kv4* from, const cq_kv4* to, const float* w
   if (!weights || !weights_out || !length || !length_out || !kept) return CQ_ERR_BAD_ARG;
   if (from->sequences != to->sequences || from->n_kv_heads != to->n_kv_heads || from->head_dim != to->head_dim || from->group != to->group)
     return CQ_ERR_BAD_SHAPE;
-  if (sinks < 0 || recent < 0 || keep < 1 || keep > to->slots || (long long)sinks + recent > keep) return CQ_ERR_BAD_ARG;
+  if (sinks < 0 || recent < 0 || keep < 1 || keep > to->slots) return CQ_ERR_BAD_ARG;
+  sinks = std::min(sinks, keep);                           // (where more than keep slots are to stay in any case)
+  recent = std::min(recent, keep - sinks);
   const void* fp[4] = {from->k_codes, from->k_scales, from->v_codes, from->v_scales};
   void* tp[4] = {to->k_codes, to->k_scales, to->v_codes, to->v_scales};
   const bool in_place = fp[0] == tp[0];

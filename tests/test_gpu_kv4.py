@@ -387,6 +387,18 @@ def test_evict(qc, n, keep, sinks, recent, D, group, in_place):
             assert torch.equal(mine, was)
 
 
+@pytest.mark.parametrize("n,keep,sinks,recent,want", [(8, 8, 8, 2, range(8)), (5, 9, 16, 2, range(5)), (40, 10, 6, 20, [*range(6), *range(36, 40)]),
+                                                      (40, 10, 16, 4, range(10)), (40, 10, 0, 2 ** 31 - 1, range(30, 40))])
+def test_evict_more_than_keep_to_stay(qc, n, keep, sinks, recent, want):
+    cache = filled(qc, gen(n), 1, 2, 64, 64, 32)
+    w = randn(gen(1), 1, 2, 64).exp()
+    kept, left, now = cache.evict(w, long([n]), keep, sinks=sinks, recent=recent, out=qc.KVCache4.empty(1, 2, 32, 64, 32))
+    want = list(want)
+    assert now.tolist() == [len(want)]
+    for h in range(2):
+        assert kept[0, h].tolist() == want + [-1] * (keep - len(want)) and torch.equal(left[0, h, :len(want)], w[0, h, want])
+
+
 @pytest.mark.parametrize("n,keep", [(70000, 1000), (70001, 69990), (131072, 65536)])
 def test_evict_long(qc, n, keep):
     g = gen(n)
@@ -458,7 +470,7 @@ def test_refusals(qc):
         lambda: c.step(q, k, k, mk(8, 32), mk(8, 32), n, n), lambda: c.step(q, k, k, mk(8, 64, **f16), mk(8, 64, **f16), n, n),
         lambda: c.write(None, mk(3, 2, 128, **f16), mk(3, 2, 128, **f16), n), lambda: c.write(None, k, mk(2, 1, 128, **f16), n),
         lambda: c.write(q[:1], k, k, n), lambda: c.write(None, k, k, n[:1]), lambda: c.read(n, 0), lambda: c.read(n.float(), 1),
-        lambda: c.evict(w, n, 0), lambda: c.evict(w, n, 65), lambda: c.evict(w, n, 8, sinks=5, recent=4), lambda: c.evict(w, n, 8, sinks=-1),
+        lambda: c.evict(w, n, 0), lambda: c.evict(w, n, 65), lambda: c.evict(w, n, 8, sinks=-1),
         lambda: c.evict(w[:1], n, 8), lambda: c.evict(w, n, 8, out=qc.KVCache4.empty(2, 2, 64, 128, 64)),
         lambda: c.evict(w, n, 33, out=qc.KVCache4.empty(2, 2, 32, 128)), lambda: c.evict(w, n, 8, out=qc.KVCache4.empty(1, 2, 64, 128)),
         lambda: qc.KVCache4.empty(1, 1, 0, 128), lambda: qc.KVCache4.empty(1, 1, 32, 96), lambda: qc.KVCache4.empty(1, 1, 32, 128, 128),

@@ -65,7 +65,7 @@ def test_cache_calls(lib):
     assert lib.cq_kv4_read(C.byref(c), at, 0, at, at, None) == BAD_ARG and lib.cq_kv4_read(C.byref(c), at, 1, odd, at, None) == BAD_ARG
     to = cache(k_codes=5 << 20, k_scales=6 << 20, v_codes=7 << 20, v_scales=9 << 20)
     evict = lambda to=to, keep=8, sinks=0, recent=0, w=at, ws=at: lib.cq_kv4_evict(C.byref(c), C.byref(to), w, at, at, at, keep, sinks, recent, at, ws, None)
-    for bad in (dict(keep=0), dict(keep=65), dict(sinks=-1), dict(recent=-1), dict(sinks=5, recent=4), dict(w=None), dict(to=c, ws=None),
+    for bad in (dict(keep=0), dict(keep=65), dict(sinks=-1), dict(recent=-1), dict(w=None), dict(to=c, ws=None),
                 dict(to=cache(k_scales=6 << 20)), dict(to=cache(slots=32))):
         assert evict(**bad) == BAD_ARG, bad
     for bad in (cache(sequences=1), cache(n_kv_heads=4), cache(head_dim=64), cache(group=64)):
