@@ -499,9 +499,13 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
 // its thread's own columns, so nothing is exchanged.  The columns are two blocks of 64 queries, of any two heads and places:
 // queries of a head that are fewer than 128 do not leave a tile half empty.  Bound by the exponentials, one for each pair and
 // 16 a cycle and SM (1024 cycles a tile, its MMAs 540); some of them are polynomials.
-//   warps 0-3, 4-7  every other tile each: sums of exponentials; joined at the end of an item
-//   warp 8          TMA of K, Q;  warp 9  MMAs, up to four score buffers ahead
-constexpr int KW_THREADS = 320, KW_Q = 64, KW_BUFFERS = 4;
+//   warps 0-15  four groups, every fourth tile each: sums of exponentials, joined by the group with an item's last tile
+//   warp 16     TMA of K, Q;  warp 17  MMAs, up to four score buffers ahead
+// (Two groups that met at every item's end were 47.6 us for 2048 tokens of 40 heads of 128 and 490 for 8192 of 64 / 8 heads with
+// window and sinks, four are 37.2 and 366: two warps a scheduler leave most of their instructions' latency open.)
+constexpr int KW_GROUPS = 4, KW_THREADS = 128 * KW_GROUPS + 64, KW_Q = 64, KW_BUFFERS = 4;
+constexpr int KW_LOAD = 4 * KW_GROUPS, KW_MMA = KW_LOAD + 1, KW_SLOTS = 12;
+static_assert(KW_GROUPS == KW_BUFFERS, "a group's tiles come in one buffer");
 constexpr int KW_POLY_OF_8 = 2;
 
 // An item: 128 keys of a KV head, the queries [first, last) of its heads in blocks of 64, and of those one of `parts` parts
@@ -550,9 +554,9 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
   using namespace umma;
   constexpr int CH = D / 64, TILE_BYTES = CH * UM_CHUNK;
   extern __shared__ __align__(1024) uint8_t um_smem[];
-  __shared__ __align__(8) uint64_t s_bar[5 + 4 * KW_BUFFERS];
-  __shared__ __align__(16) float s_lse[4][UM_TILE];
-  __shared__ float s_sum[UM_TILE];
+  __shared__ __align__(8) uint64_t s_bar[5 + 4 * KW_BUFFERS + KW_SLOTS];
+  __shared__ __align__(16) float s_lse[2 * KW_GROUPS][UM_TILE];
+  __shared__ float s_sum[KW_SLOTS][KW_GROUPS][UM_TILE];
   __shared__ uint32_t s_tmem;
   __shared__ int s_gone;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -564,6 +568,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
   auto q_free = [&](int i) { return bars + 8 * (5 + KW_BUFFERS + i); };
   auto s_full = [&](int i) { return bars + 8 * (5 + 2 * KW_BUFFERS + i); };
   auto s_free = [&](int i) { return bars + 8 * (5 + 3 * KW_BUFFERS + i); };
+  auto summed = [&](int i) { return bars + 8 * (5 + 4 * KW_BUFFERS + i); };
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     bar_init(drained, 1);
@@ -577,10 +582,11 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
       bar_init(s_full(i), 1);
       bar_init(s_free(i), 128);
     }
+    for (int i = 0; i < KW_SLOTS; ++i) bar_init(summed(i), 4 * KW_GROUPS);
     s_gone = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == W_MMA) alloc(&s_tmem, 512);
+  if (warp == KW_MMA) alloc(&s_tmem, 512);
   fence_before();
   __syncthreads();
   fence_after();
@@ -589,7 +595,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
   const cq_prompt& s = a.s;
   const int off = s.keys - s.queries, G = s.n_heads / s.n_kv_heads;
 
-  if (warp == W_LOAD) {
+  if (warp == KW_LOAD) {
     if (lane == 0) {
       uint32_t loaded = 0, sent = 0;                       // key tiles, query tiles
       bool ok = true;
@@ -622,7 +628,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
           for (int k = 0; k < 1000 && !bar_try(q_full(i % KW_BUFFERS), (i / KW_BUFFERS) & 1); ++k) {}
       }
     }
-  } else if (warp == W_MMA) {
+  } else if (warp == KW_MMA) {
     constexpr uint32_t SHAPE = shape_of(128, 128, false);
     uint32_t loaded = 0, sent = 0;
     bool ok = true;
@@ -656,37 +662,43 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
     for (int k = 0; k < 100000 && !bar_try(drained, 0); ++k) {}
     __syncwarp();
   } else {
-    const int wg = warp >> 2, r = tid & 127;
+    const uint32_t wg = warp >> 2;
+    const int r = tid & 127;
     const float scale2 = s.scale * LOG2E;
     const uint64_t scale22 = two(scale2, scale2);
-    uint32_t seen = 0;                                     // tiles of all items before this one
+    uint32_t seen = 0, before = 0;                         // tiles, and items with any, before this one
     bool ok = true;
     for (int round = 0, item; (item = PromptItem::at(round, items)) >= 0; ++round) {
       const KeysItem w(a, item, observe, parts);
       const int key = w.k0 + r;
+      if (!w.tiles) {
+        if (!wg && key < s.keys) weights[(((size_t)w.part * s.sequences + w.b) * s.n_kv_heads + w.kvh) * s.keys + key] = 0.f;
+        continue;
+      }
       // the positions of the queries that see this key
       const int lo = key < w.n ? max(w.first, key) : w.last;
       const int hi = min(w.last, s.window && key >= s.sinks ? (int)min((long long)w.last, key + (long long)s.window) : w.last) - 1;
       uint64_t sum[2] = {};
-      // this group's tiles are every other one; their two blocks, and minus the lse (in powers of two) of column r a tile ahead
-      Block block[2] = {Block(w, 2 * wg), Block(w, 2 * wg + 1)};
+      // this group's tiles are every KW_GROUPS-th; their two blocks, and minus the lse (in powers of two) of column r a tile ahead
+      const int own = (wg - seen) % KW_GROUPS;
+      Block block[2] = {Block(w, min(2 * own, w.blocks - 1)), Block(w, min(2 * own + 1, w.blocks - 1))};
       auto minus_lse = [&](int j) {
         const Block& mine = block[r >> 6];
         const int p = mine.position(w) + (r & 63);
         return 2 * j + (r >> 6) < w.blocks && p < w.last ? -LOG2E * lse[((size_t)w.b * s.n_heads + w.kvh * G + mine.head) * s.queries + p - off] : -INFINITY;
       };
-      float ahead = wg < w.tiles ? minus_lse(wg) : 0.f;
-      for (int j = wg; j < w.tiles; j += 2) {
-        const uint32_t tile = seen + j, st = tile % KW_BUFFERS, use = tile / KW_BUFFERS;
+      float ahead = own < w.tiles ? minus_lse(own) : 0.f;
+      for (int j = own; j < w.tiles; j += KW_GROUPS) {
+        const uint32_t st = wg, use = (seen + j) / KW_BUFFERS;
         int place[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) place[e] = 2 * j + e < w.blocks ? block[e].position(w) : w.last;
-        float* mine = s_lse[2 * wg + (j >> 1 & 1)];
+        float* mine = s_lse[2 * wg + (use & 1)];
         mine[r] = ahead;
-        if (j + 2 < w.tiles) {
-          block[0].step(w, 4);
-          block[1].step(w, 4);
-          ahead = minus_lse(j + 2);
+        if (j + KW_GROUPS < w.tiles) {
+          block[0].step(w, 2 * KW_GROUPS);
+          block[1].step(w, 2 * KW_GROUPS);
+          ahead = minus_lse(j + KW_GROUPS);
         }
         asm volatile("barrier.cta.sync %0, 128;" ::"r"(2 + wg) : "memory");
         ok = ok && bar_wait_warp(s_full(st), use & 1, &s_gone, status);
@@ -718,18 +730,27 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
         fence_before();
         bar_arrive(s_free(st));
       }
+      const float2 halves = apart(add2(sum[0], sum[1]));
+      // The group with the item's last tile adds the groups' sums; the others go on.  (Until it has, they come 10 items further at
+      // most: its next tile, 4 on, is not taken, so that the tile 8 on is not made, and what a group goes through without one of
+      // its own is fewer than 4.)
+      const uint32_t slot = before % KW_SLOTS;
+      s_sum[slot][wg][r] = ok ? halves.x + halves.y : NAN;
+      __syncwarp();
+      if (lane == 0) bar_arrive(summed(slot));
       seen += w.tiles;
-      const float2 parts = apart(add2(sum[0], sum[1]));
-      const float total = ok ? parts.x + parts.y : NAN;
-      if (wg) s_sum[r] = total;
-      asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
-      if (!wg && key < s.keys) weights[(((size_t)w.part * s.sequences + w.b) * s.n_kv_heads + w.kvh) * s.keys + key] = total + s_sum[r];
-      asm volatile("barrier.cta.sync 1, 256;" ::: "memory");
+      if ((seen - 1) % KW_GROUPS == wg) {
+        ok = bar_wait_warp(summed(slot), before / KW_SLOTS & 1, &s_gone, status) && ok;
+        float all = s_sum[slot][0][r];
+        for (int g = 1; g < KW_GROUPS; ++g) all += s_sum[slot][g][r];
+        if (key < s.keys) weights[(((size_t)w.part * s.sequences + w.b) * s.n_kv_heads + w.kvh) * s.keys + key] = ok ? all : NAN;
+      }
+      ++before;
     }
   }
   fence_before();
   __syncthreads();
-  if (warp == W_MMA) {
+  if (warp == KW_MMA) {
     fence_after();
     dealloc(tmem, 512);
   }
