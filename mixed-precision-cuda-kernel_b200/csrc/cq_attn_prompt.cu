@@ -18,10 +18,24 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
+// n / d for 0 <= n < 2^31 by one multiplication: m = floor(2^32 (2^shift - d) / d) + 1 with 2^shift >= d.  (Every warp of a CTA works out
+// for itself what an item is; with the compiler's divisions that was a third of a short item's time.)
+struct Divisor {
+  uint32_t d = 1, m = 1, shift = 0;
+  Divisor() = default;
+  explicit Divisor(uint32_t by) : d(by) {
+    while ((1ull << shift) < by) ++shift;
+    m = (uint32_t)((((1ull << shift) - by) << 32) / by + 1);
+  }
+  __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi(m, (uint32_t)n) + (uint32_t)n) >> shift); }
+};
+
 struct PromptArgs {
   cq_prompt s;
   const __half *q, *k, *v;
   const long long* lengths;
+  int group;                                               // query heads of a KV head
+  Divisor by_group, by_heads, by_row, by_parts;            // by_heads, by_row: the heads, and the items, of a block of rows
 };
 
 __device__ __forceinline__ uint32_t half_pair(float a, float b) {
@@ -138,11 +152,11 @@ struct PromptItem {
   int b, h, kvh, q0, n, pmin, pmax;          // positions of the queries that are inside the length
   __device__ __forceinline__ PromptItem(const PromptArgs& a, int item) {
     const cq_prompt& s = a.s;
-    const int nq = (s.queries + 2 * UM_TILE - 1) / (2 * UM_TILE), per = s.n_heads * s.sequences, qb = nq - 1 - item / per;
-    const int rest = item % per;
-    b = rest / s.n_heads;
+    const int nq = (s.queries + 2 * UM_TILE - 1) / (2 * UM_TILE), row = a.by_row(item), qb = nq - 1 - row;
+    const int rest = item - row * (int)a.by_row.d;
+    b = a.by_heads(rest);
     h = rest - b * s.n_heads;
-    kvh = h / (s.n_heads / s.n_kv_heads);
+    kvh = a.by_group(h);
     q0 = qb * 2 * UM_TILE;
     n = length_of(a, b);
     pmin = q0 + s.keys - s.queries;
@@ -511,20 +525,20 @@ constexpr int KW_POLY_OF_8 = 2;
 // An item: 128 keys of a KV head, the queries [first, last) of its heads in blocks of 64, and of those one of `parts` parts
 struct KeysItem {
   int b, kvh, k0, n, first, last, per_head, begin, blocks, tiles, part;
-  __device__ __forceinline__ KeysItem(const PromptArgs& a, int item, int observe, int parts) {
+  __device__ __forceinline__ KeysItem(const PromptArgs& a, int item, int observe) {
     const cq_prompt& s = a.s;
-    const int per = s.n_kv_heads * s.sequences * parts, rest_p = item % per, rest = rest_p / parts;
-    part = rest_p - rest * parts;
-    k0 = item / per * UM_TILE;
-    b = rest / s.n_kv_heads;
+    const int row = a.by_row(item), in_row = item - row * (int)a.by_row.d, rest = a.by_parts(in_row);
+    part = in_row - rest * (int)a.by_parts.d;
+    k0 = row * UM_TILE;
+    b = a.by_heads(rest);
     kvh = rest - b * s.n_kv_heads;
     n = length_of(a, b);
     first = max(max(s.keys - s.queries, n - observe), k0);
     last = s.window && k0 >= s.sinks ? (int)min((long long)n, min(k0 + UM_TILE, n) - 1 + (long long)s.window) : n;
     per_head = max(0, last - first + KW_Q - 1) / KW_Q;
-    const int all = per_head * (s.n_heads / s.n_kv_heads);
-    begin = (int)((long long)all * part / parts);
-    blocks = (int)((long long)all * (part + 1) / parts) - begin;
+    const int all = per_head * a.group, each = a.by_parts(all), more = all - each * (int)a.by_parts.d;
+    begin = part * each + min(part, more);
+    blocks = each + (part < more);
     tiles = (blocks + 1) / 2;
   }
 };
@@ -549,7 +563,7 @@ struct Block {
 
 template <int D>
 __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ PromptMaps maps,
-                                                                    const float* __restrict__ lse, int observe, int parts, float* __restrict__ weights, int items,
+                                                                    const float* __restrict__ lse, int observe, float* __restrict__ weights, int items,
                                                                     uint32_t* __restrict__ status) {
   using namespace umma;
   constexpr int CH = D / 64, TILE_BYTES = CH * UM_CHUNK;
@@ -593,14 +607,14 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
   const uint32_t tmem = s_tmem;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const cq_prompt& s = a.s;
-  const int off = s.keys - s.queries, G = s.n_heads / s.n_kv_heads;
+  const int off = s.keys - s.queries, G = a.group;
 
   if (warp == KW_LOAD) {
     if (lane == 0) {
       uint32_t loaded = 0, sent = 0;                       // key tiles, query tiles
       bool ok = true;
       for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
-        const KeysItem w(a, item, observe, parts);
+        const KeysItem w(a, item, observe);
         if (!w.tiles) continue;
         const uint32_t kb = loaded & 1;
         if (loaded >= 2 && !(ok = bar_wait(k_free(kb), (loaded / 2 - 1) & 1, &s_gone, status))) break;
@@ -612,12 +626,13 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
         for (int j = 0; j < w.tiles; ++j, ++sent) {
           const uint32_t st = sent % KW_BUFFERS, use = sent / KW_BUFFERS;
           if (use && !(ok = bar_wait(q_free(st), (use - 1) & 1, &s_gone, status))) break;
-          bar_expect(q_full(st), TILE_BYTES);
-          for (int e = 0; e < 2; ++e) {
+          const int here = min(2, w.blocks - 2 * j);       // (the last tile may have one block: the other place is not read)
+          bar_expect(q_full(st), here * (TILE_BYTES / 2));
+          for (int e = 0; e < here; ++e) {
             for (int c = 0; c < CH; ++c)
               tma(s_q + st * TILE_BYTES + c * UM_CHUNK + e * (UM_CHUNK / 2), &maps.q, 64 * c, block.position(w) - off,
                   (w.kvh * G + block.head) * maps.one[0][0], w.b * maps.one[0][1], q_full(st));
-            if (2 * j + e + 1 < w.blocks) block.step(w, 1);      // (the last tile may have one block: it fills the other place, unused)
+            block.step(w, 1);
           }
         }
       }
@@ -633,7 +648,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
     uint32_t loaded = 0, sent = 0;
     bool ok = true;
     for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
-      const KeysItem w(a, item, observe, parts);
+      const KeysItem w(a, item, observe);
       if (!w.tiles) continue;
       const uint32_t kb = loaded & 1;
       ok = bar_wait_warp(k_full(kb), (loaded / 2) & 1, &s_gone, status);
@@ -669,7 +684,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
     uint32_t seen = 0, before = 0;                         // tiles, and items with any, before this one
     bool ok = true;
     for (int round = 0, item; (item = PromptItem::at(round, items)) >= 0; ++round) {
-      const KeysItem w(a, item, observe, parts);
+      const KeysItem w(a, item, observe);
       const int key = w.k0 + r;
       if (!w.tiles) {
         if (!wg && key < s.keys) weights[(((size_t)w.part * s.sequences + w.b) * s.n_kv_heads + w.kvh) * s.keys + key] = 0.f;
@@ -707,6 +722,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
         const uint32_t at = tmem + 128 * st + ((uint32_t)(warp & 3) << 21);
 #pragma unroll
         for (int c0 = 0; c0 < 128; c0 += 32) {
+          if (c0 == 64 && 2 * j + 1 == w.blocks) break;
           uint32_t x[32];
           load32(at + c0, x);
           wait_load<32>(x);
@@ -840,8 +856,11 @@ extern "C" int cq_attn_prefill(const cq_prompt* shape, const void* q, const void
   const int rc = check(shape, q, k, v);
   if (rc != CQ_OK) return rc;
   if (!v || !out || !lse || ((uintptr_t)out & 15)) return CQ_ERR_BAD_ARG;
-  const PromptArgs a = {*shape, (const __half*)q, (const __half*)k, (const __half*)v, lengths};
+  PromptArgs a = {*shape, (const __half*)q, (const __half*)k, (const __half*)v, lengths, shape->n_heads / shape->n_kv_heads};
   const int D = shape->head_dim, B = shape->sequences;
+  a.by_group = Divisor(a.group);
+  a.by_heads = Divisor(shape->n_heads);
+  a.by_row = Divisor((uint32_t)shape->n_heads * B);
   PromptMaps maps;
   if (!map_of(&maps.q, q, shape->q_strides, B, shape->queries, shape->n_heads, D, UM_TILE, maps.one[0]) ||
       !map_of(&maps.k, k, shape->k_strides, B, shape->keys, shape->n_kv_heads, D, UM_TILE, maps.one[1]) ||
@@ -868,7 +887,7 @@ extern "C" int cq_attn_prefill_weights(const cq_prompt* shape, const void* q, co
   const int rc = check(shape, q, k, nullptr);
   if (rc != CQ_OK) return rc;
   if (!lse || !weights || !workspace || observe < 1) return CQ_ERR_BAD_ARG;
-  const PromptArgs a = {*shape, (const __half*)q, (const __half*)k, nullptr, lengths};
+  PromptArgs a = {*shape, (const __half*)q, (const __half*)k, nullptr, lengths, shape->n_heads / shape->n_kv_heads};
   const int D = shape->head_dim, B = shape->sequences;
   PromptMaps maps;
   if (!map_of(&maps.q, q, shape->q_strides, B, shape->queries, shape->n_heads, D, KW_Q, maps.one[0]) ||
@@ -881,8 +900,11 @@ extern "C" int cq_attn_prefill_weights(const cq_prompt* shape, const void* q, co
   const int parts = parts_of(shape, observe);
   const long long n = (long long)B * shape->n_kv_heads * shape->keys, items = (long long)((shape->keys + UM_TILE - 1) / UM_TILE) * shape->n_kv_heads * B * parts;
   if (items > INT32_MAX / 2) return CQ_ERR_BAD_SHAPE;
+  a.by_heads = Divisor(shape->n_kv_heads);
+  a.by_row = Divisor((uint32_t)shape->n_kv_heads * B * parts);
+  a.by_parts = Divisor(parts);
   CQ_CUDA_TRY(kv4_launch(fn, dim3((unsigned)std::min<long long>(items, cq_sm_count())), dim3(KW_THREADS), smem, (cudaStream_t)stream, a, maps, lse,
-                         observe, parts, parts > 1 ? (float*)workspace : weights, (int)items, status_word));
+                         observe, parts > 1 ? (float*)workspace : weights, (int)items, status_word));
   if (parts > 1)
     CQ_CUDA_TRY(kv4_launch(prompt_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (cudaStream_t)stream, (const float*)workspace, parts, n,
                            weights));
