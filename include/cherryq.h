@@ -339,14 +339,16 @@ int cq_kv4_evict(const cq_kv4* from, const cq_kv4* to, const float* weights, flo
  * those with j < sinks or j > p - window.  out (sequences, queries, n_heads, D) contiguous, lse (sequences, n_heads, queries)
  * fp32 = ln of the sum of exp(scale * q . k_j).  A row at or beyond its sequence's length, or that sees no key: zeros and
  * -infinity.  head_dim 64 or 128, scale positive.  status_word: device uint32 that receives CQ_ERR_DEVICE_TIMEOUT bits, may be
- * NULL. */
+ * NULL.  workspace: device memory of cq_attn_prefill_workspace_bytes(shape) bytes (0: may be NULL; fewer items than the device
+ * has SMs are cut along their keys), 16-byte aligned, not shared by calls that can overlap. */
 typedef struct cq_prompt {
   int32_t sequences, queries, keys, n_heads, n_kv_heads, head_dim, window, sinks;
   int64_t q_strides[3], k_strides[3], v_strides[3];      /* sequence, token, head */
   float scale;
 } cq_prompt;
+size_t cq_attn_prefill_workspace_bytes(const cq_prompt* shape);
 int cq_attn_prefill(const cq_prompt* shape, const void* q_f16, const void* k_f16, const void* v_f16, const long long* lengths,
-                    void* out_f16, float* lse, uint32_t* status_word, cq_stream_t stream);
+                    void* out_f16, float* lse, void* workspace, uint32_t* status_word, cq_stream_t stream);
 /* The weight that each key received from the last `observe` positions of its sequence (of those that are among the queries):
  * weights (sequences, n_kv_heads, keys) fp32 = sum over them and the head's queries of exp(scale * q . k_j - lse); 0 where no
  * such query sees the key.  workspace: device memory of cq_attn_prefill_weights_workspace_bytes(...) bytes, not shared by

@@ -24,7 +24,7 @@ SYMBOLS = [
     "cq_peer_region_open", "cq_peer_region_close", "cq_peer_allgather",
     "cq_rlayer_init", "cq_rlayer_prepare", "cq_rlayer_unprepare", "cq_rlayer_check", "cq_rlayer_matvec", "cq_rlayers_matvec", "cq_rlayers_matvec_norm", "cq_rlayer_matvec_host", "cq_rlayer_preferred_rows", "cq_rlayer_matvec_gather", "cq_rlayer_matvec_swiglu",
     "cq_kv4_check", "cq_kv4_write", "cq_kv4_read", "cq_kv4_attend_workspace_bytes", "cq_kv4_attend", "cq_kv4_step",
-    "cq_kv4_evict_workspace_bytes", "cq_kv4_evict", "cq_attn_prefill", "cq_attn_prefill_weights", "cq_attn_prefill_weights_workspace_bytes",
+    "cq_kv4_evict_workspace_bytes", "cq_kv4_evict", "cq_attn_prefill", "cq_attn_prefill_workspace_bytes", "cq_attn_prefill_weights", "cq_attn_prefill_weights_workspace_bytes",
 ]
 
 

@@ -10,6 +10,8 @@
 // exponentials bound them.
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
+#include <cstring>
 
 #include "cq_kv4.cuh"
 #include "cq_umma.cuh"
@@ -35,7 +37,8 @@ struct PromptArgs {
   const __half *q, *k, *v;
   const long long* lengths;
   int group;                                               // query heads of a KV head
-  Divisor by_group, by_heads, by_row, by_parts;            // by_heads, by_row: the heads, and the items, of a block of rows
+  Divisor by_group, by_heads, by_row, by_parts;            // (what they divide: PromptItem, KeysItem)
+  int rows = 256, shift = 8, pack = 1;                     // queries of a head in an item (2^shift), heads in it
 };
 
 __device__ __forceinline__ uint32_t half_pair(float a, float b) {
@@ -65,16 +68,21 @@ constexpr float HEADROOM = 8.f, LIFT = 7.f, LOWEST = -4.f;      // weights are 2
 
 // the key tiles that the queries at positions pmin .. pmax (both inside the length n) of a CTA see
 struct KeyTiles {
-  int ns = 0, wt0 = 0, count = 0;
+  int ns = 0, wt0 = 0, count = 0, from = 0;
   __device__ __forceinline__ KeyTiles(const cq_prompt& s, int pmin, int pmax) {
     if (pmax < pmin) return;
-    const int from = s.window ? max(0, pmin - s.window + 1) : 0, first = s.window ? min(s.sinks, from) : 0;
+    const int key = s.window ? max(0, pmin - s.window + 1) : 0, first = s.window ? min(s.sinks, key) : 0;
     ns = (first + UM_TILE - 1) / UM_TILE;
-    wt0 = from / UM_TILE;
+    wt0 = key / UM_TILE;
     if (ns >= wt0) ns = wt0 = 0;
     count = ns + pmax / UM_TILE + 1 - wt0;
   }
-  __device__ __forceinline__ int base(int i) const { return UM_TILE * (i < ns ? i : i - ns + wt0); }
+  __device__ __forceinline__ void cut(int part, const Divisor& parts) {      // to one of as many parts as equal as they can be
+    const int each = parts(count), more = count - each * (int)parts.d;
+    from = part * each + min(part, more);
+    count = each + (part < more);
+  }
+  __device__ __forceinline__ int base(int i) const { return UM_TILE * (i + from < ns ? i + from : i + from - ns + wt0); }
 };
 // whether any of the queries pmin .. pmax sees a key of the tile; whether all of them see all of it
 __device__ __forceinline__ bool tile_seen(const cq_prompt& s, int base, int pmin, int pmax) {
@@ -147,84 +155,107 @@ struct PromptMaps {
   int one[3][2];             // 0 where the heads (0) or sequences (1) of q, k, v are all the same rows
 };
 
-// The work of a CTA: every gridDim.x-th block of 256 queries of a head, the longest first, forwards and backwards in turn.
+// The work of a CTA: every gridDim.x-th item, the longest first, forwards and backwards in turn.
+__device__ __forceinline__ int item_at(int round, int items) {
+  const int i = round * (int)gridDim.x + (int)(round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+  return i < items ? i : -1;
+}
+
+// An item is 256 queries of a head,
+// or where calls have few of them (FEW) one of several parts of such an item's keys, and where they have 128 at most the queries
+// of several heads of a KV head, `rows` places each.
+template <bool FEW>
 struct PromptItem {
   int b, h, kvh, q0, n, pmin, pmax;          // positions of the queries that are inside the length
+  int part = 0, heads = 1;
   __device__ __forceinline__ PromptItem(const PromptArgs& a, int item) {
     const cq_prompt& s = a.s;
-    const int nq = (s.queries + 2 * UM_TILE - 1) / (2 * UM_TILE), row = a.by_row(item), qb = nq - 1 - row;
-    const int rest = item - row * (int)a.by_row.d;
+    const int whole = FEW ? a.by_parts(item) : item, rows = FEW ? a.rows : 2 * UM_TILE;
+    const int row = a.by_row(whole), rest = whole - row * (int)a.by_row.d;
     b = a.by_heads(rest);
-    h = rest - b * s.n_heads;
+    h = rest - b * (int)a.by_heads.d;
     kvh = a.by_group(h);
-    q0 = qb * 2 * UM_TILE;
+    if (FEW) {
+      part = item - whole * (int)a.by_parts.d;
+      const int first = (h - kvh * (int)a.by_group.d) * a.pack;
+      h = kvh * a.group + first;
+      heads = min(a.pack, a.group - first);
+    }
+    q0 = ((FEW ? (s.queries + rows - 1) >> a.shift : (s.queries + rows - 1) / (2 * UM_TILE)) - 1 - row) * rows;
     n = length_of(a, b);
     pmin = q0 + s.keys - s.queries;
-    pmax = min(n, min(q0 + 2 * UM_TILE, s.queries) + s.keys - s.queries) - 1;
+    pmax = min(n, min(q0 + rows, s.queries) + s.keys - s.queries) - 1;
   }
-  __device__ __forceinline__ int lowest(int t) const { return pmin + UM_TILE * t; }
-  __device__ __forceinline__ int highest(int t) const { return min(pmax, pmin + UM_TILE * t + UM_TILE - 1); }
-  __device__ __forceinline__ static int at(int round, int items) {
-    const int i = round * (int)gridDim.x + (int)(round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-    return i < items ? i : -1;
+  // of tile t
+  __device__ __forceinline__ static bool packed(const PromptArgs& a) { return FEW && a.rows <= UM_TILE; }
+  __device__ __forceinline__ int lowest(const PromptArgs& a, int t) const { return packed(a) ? pmin : pmin + UM_TILE * t; }
+  __device__ __forceinline__ int highest(const PromptArgs& a, int t) const {
+    if (packed(a)) return heads * a.rows > UM_TILE * t ? pmax : -1;
+    return min(pmax, pmin + UM_TILE * t + UM_TILE - 1);
   }
+  // of row x of the 256
+  __device__ __forceinline__ int query(const PromptArgs& a, int x) const { return q0 + (packed(a) ? x & (a.rows - 1) : x); }
+  __device__ __forceinline__ int head(const PromptArgs& a, int x) const { return packed(a) ? x >> a.shift : 0; }
 };
 
-// A value in a masked place has the weight 0, and 0 times infinity or NaN is NaN: where a softmax warp wrote a NaN in a row with a
-// finite lse, its columns with one are summed again in fp32 over the keys that the row sees, at the CTA's end, where no other
-// warp waits.  (Finite values never come here.)
+// A value in a masked place has the weight 0, and 0 times infinity or NaN is NaN: where a row with a finite lse has a NaN, a warp
+// sums its columns with one again, in fp32, over the keys that the row sees.  (Finite values never come here.)
 template <int D>
-__device__ __noinline__ void rows_again(const PromptArgs& a, int items, __half* out, const float* lse) {
+__device__ __noinline__ void row_again(const PromptArgs& a, int b, int h, int q, __half* out, const float* lse) {
   constexpr int C = D / 32;                                // columns of a lane
   const cq_prompt& s = a.s;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  __syncwarp();
-  for (int round = 0, item; (item = PromptItem::at(round, items)) >= 0; ++round) {
-    const PromptItem w(a, item);
-    const __half* ks = a.k + w.b * s.k_strides[0] + w.kvh * s.k_strides[2] + C * lane;
-    const __half* vs = a.v + w.b * s.v_strides[0] + w.kvh * s.v_strides[2] + C * lane;
-    for (int q = w.q0 + 32 * warp, end = min(q + 32, s.queries); q < end; ++q) {
-      __half* to = out + (((size_t)w.b * s.queries + q) * s.n_heads + w.h) * D + C * lane;
-      const float l = lse[((size_t)w.b * s.n_heads + w.h) * s.queries + q];
-      bool mine = false;
+  const int lane = threadIdx.x & 31, kvh = h / a.group;
+  __half* to = out + (((size_t)b * s.queries + q) * s.n_heads + h) * D + C * lane;
+  const float l = lse[((size_t)b * s.n_heads + h) * s.queries + q];
+  bool mine = false;
 #pragma unroll
-      for (int i = 0; i < C; ++i) mine |= __hisnan(to[i]);
-      if (!(fabsf(l) < INFINITY) || !__any_sync(0xffffffffu, mine)) continue;
-      const __half* qr = a.q + w.b * s.q_strides[0] + q * s.q_strides[1] + w.h * s.q_strides[2] + C * lane;
-      float x[C], y[C] = {};
+  for (int i = 0; i < C; ++i) mine |= __hisnan(to[i]);
+  if (!(fabsf(l) < INFINITY) || !__any_sync(0xffffffffu, mine)) return;
+  const __half* ks = a.k + b * s.k_strides[0] + kvh * s.k_strides[2] + C * lane;
+  const __half* vs = a.v + b * s.v_strides[0] + kvh * s.v_strides[2] + C * lane;
+  const __half* qr = a.q + b * s.q_strides[0] + q * s.q_strides[1] + h * s.q_strides[2] + C * lane;
+  float x[C], y[C] = {};
 #pragma unroll
-      for (int i = 0; i < C; ++i) x[i] = __half2float(qr[i]) * (s.scale * LOG2E);
-      const int hi = q + s.keys - s.queries, lo = s.window ? max(0, hi - s.window + 1) : 0;
-      bool done = false;                                   // NaN again: the row sees one
-      for (int from = 0, to_key; from <= hi && !done; from = to_key) {
-        if (from >= s.sinks && from < lo) from = lo;
-        to_key = min(min(from + 128, hi + 1), from < min(s.sinks, lo) ? min(s.sinks, lo) : hi + 1);
+  for (int i = 0; i < C; ++i) x[i] = __half2float(qr[i]) * (s.scale * LOG2E);
+  const int hi = q + s.keys - s.queries, lo = s.window ? max(0, hi - s.window + 1) : 0;
+  bool done = false;                                   // NaN again: the row sees one
+  for (int from = 0, to_key; from <= hi && !done; from = to_key) {
+    if (from >= s.sinks && from < lo) from = lo;
+    to_key = min(min(from + 128, hi + 1), from < min(s.sinks, lo) ? min(s.sinks, lo) : hi + 1);
 #pragma unroll 4
-        for (int j = from; j < to_key; ++j) {
-          float dot = 0.f;
+    for (int j = from; j < to_key; ++j) {
+      float dot = 0.f;
 #pragma unroll
-          for (int i = 0; i < C; ++i) dot = fmaf(x[i], __half2float(ks[j * s.k_strides[1] + i]), dot);
+      for (int i = 0; i < C; ++i) dot = fmaf(x[i], __half2float(ks[j * s.k_strides[1] + i]), dot);
 #pragma unroll
-          for (int d = 16; d; d /= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-          const float p = exp2f(dot - l * LOG2E);
+      for (int d = 16; d; d /= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+      const float p = exp2f(dot - l * LOG2E);
 #pragma unroll
-          for (int i = 0; i < C; ++i) y[i] = fmaf(p, __half2float(vs[j * s.v_strides[1] + i]), y[i]);
-        }
-        done = true;
-#pragma unroll
-        for (int i = 0; i < C; ++i) done = done && (y[i] != y[i] || !__hisnan(to[i]));
-        done = __all_sync(0xffffffffu, done);
-      }
-#pragma unroll
-      for (int i = 0; i < C; ++i)
-        if (__hisnan(to[i])) to[i] = __float2half_rn(y[i]);
+      for (int i = 0; i < C; ++i) y[i] = fmaf(p, __half2float(vs[j * s.v_strides[1] + i]), y[i]);
     }
+    done = true;
+#pragma unroll
+    for (int i = 0; i < C; ++i) done = done && (y[i] != y[i] || !__hisnan(to[i]));
+    done = __all_sync(0xffffffffu, done);
+  }
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+    if (__hisnan(to[i])) to[i] = __float2half_rn(y[i]);
+}
+// the rows of a softmax warp, at the CTA's end, where no other warp waits
+template <int D, bool FEW>
+__device__ __noinline__ void rows_again(const PromptArgs& a, int items, __half* out, const float* lse) {
+  const int warp = threadIdx.x >> 5;
+  for (int round = 0, item; (item = item_at(round, items)) >= 0; ++round) {
+    const PromptItem<FEW> w(a, item);
+    for (int x = 32 * warp; x < 32 * warp + 32; ++x)
+      if (w.query(a, x) < a.s.queries && w.head(a, x) < w.heads) row_again<D>(a, w.b, w.h + w.head(a, x), w.query(a, x), out, lse);
   }
 }
 
-template <int D>
+template <int D, bool FEW>
 __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_constant__ PromptArgs a, const __grid_constant__ PromptMaps maps,
-                                                                    __half* __restrict__ out, float* __restrict__ lse, int items,
+                                                                    __half* __restrict__ out, float* __restrict__ lse, float* __restrict__ partial, int items,
                                                                     uint32_t* __restrict__ status) {
   using namespace umma;
   constexpr int CH = D / 64, TILE_BYTES = CH * UM_CHUNK;
@@ -272,15 +303,24 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
     if (warp == W_LOAD && lane == 0) {
       int loaded = 0, sent = 0;                            // query blocks, tiles of keys and values
       bool ok = true;
-      for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
-        const PromptItem w(a, item);
-        const KeyTiles tiles(s, w.pmin, w.pmax);
+      for (int round = 0, item; ok && (item = item_at(round, items)) >= 0; ++round) {
+        const PromptItem<FEW> w(a, item);
+        KeyTiles tiles(s, w.pmin, w.pmax);
+        if (FEW) tiles.cut(w.part, a.by_parts);
         if (!tiles.count) continue;
         if (loaded && !(ok = bar_wait(q_free, (loaded - 1) & 1, &s_gone, status))) break;
-        bar_expect(q_full, 2 * TILE_BYTES);
-        for (int t = 0; t < 2; ++t)
-          for (int c = 0; c < CH; ++c)
-            tma(s_q + t * TILE_BYTES + c * UM_CHUNK, &maps.q, 64 * c, w.q0 + UM_TILE * t, w.h * maps.one[0][0], w.b * maps.one[0][1], q_full);
+        if (w.packed(a)) {
+          bar_expect(q_full, w.heads * a.rows * D * 2);
+          for (int e = 0; e < w.heads; ++e)
+            for (int c = 0; c < CH; ++c)
+              tma(s_q + e * a.rows / UM_TILE * TILE_BYTES + c * UM_CHUNK + e * a.rows % UM_TILE * 128, &maps.q, 64 * c, w.q0, (w.h + e) * maps.one[0][0],
+                  w.b * maps.one[0][1], q_full);
+        } else {
+          bar_expect(q_full, 2 * TILE_BYTES);
+          for (int t = 0; t < 2; ++t)
+            for (int c = 0; c < CH; ++c)
+              tma(s_q + t * TILE_BYTES + c * UM_CHUNK, &maps.q, 64 * c, w.q0 + UM_TILE * t, w.h * maps.one[0][0], w.b * maps.one[0][1], q_full);
+        }
         ++loaded;
         for (int i = 0; i < 2 * tiles.count; ++i, ++sent) {      // keys, values, keys, values ...
           const int st = sent % UM_STAGES, use = sent / UM_STAGES;
@@ -302,11 +342,12 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
       int taken[2] = {0, 0};                               // tiles of keys that a query tile has taken, in all items
       int blocks = 0, sent = 0;
       bool ok = true;
-      for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
-        const PromptItem w(a, item);
-        const KeyTiles tiles(s, w.pmin, w.pmax);
+      for (int round = 0, item; ok && (item = item_at(round, items)) >= 0; ++round) {
+        const PromptItem<FEW> w(a, item);
+        KeyTiles tiles(s, w.pmin, w.pmax);
+        if (FEW) tiles.cut(w.part, a.by_parts);
         if (!tiles.count) continue;
-        auto seen = [&](int t, int i) { return tile_seen(s, tiles.base(i), w.lowest(t), w.highest(t)); };
+        auto seen = [&](int t, int i) { return tile_seen(s, tiles.base(i), w.lowest(a, t), w.highest(a, t)); };
         auto scores = [&](int t, int i) {
           if (elected()) {
             const uint32_t kt = s_kv + ((sent + 2 * i) % UM_STAGES) * TILE_BYTES, qt = s_q + t * TILE_BYTES;
@@ -385,21 +426,22 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
     const uint64_t scale22 = two(scale2, scale2);
     int taken = 0;                                         // tiles of keys, in all items
     bool ok = true;
-    for (int round = 0, item; (item = PromptItem::at(round, items)) >= 0; ++round) {
-      const PromptItem w(a, item);
-      const KeyTiles tiles(s, w.pmin, w.pmax);
-      const int p = w.lowest(t) + r, q = w.q0 + UM_TILE * t + r;
+    for (int round = 0, item; (item = item_at(round, items)) >= 0; ++round) {
+      const PromptItem<FEW> w(a, item);
+      KeyTiles tiles(s, w.pmin, w.pmax);
+      if (FEW) tiles.cut(w.part, a.by_parts);
+      const int q = w.query(a, UM_TILE * t + r), p = q + s.keys - s.queries, head = w.h + w.head(a, UM_TILE * t + r);
       const int hi = min(p, w.n - 1), lo = s.window ? p - s.window + 1 : 0;
       float ref = -INFINITY;
       uint64_t sum = 0;                                    // two partial sums
       bool first = true;
       for (int i = 0; i < tiles.count && ok; ++i) {
         const int base = tiles.base(i);
-        if (!tile_seen(s, base, w.lowest(t), w.highest(t))) continue;
+        if (!tile_seen(s, base, w.lowest(a, t), w.highest(a, t))) continue;
         ok = bar_wait_warp(s_full(t), taken & 1, &s_gone, status);
         if (!ok) break;
         fence_after();
-        const bool whole = tile_whole(s, base, w.lowest(t), w.highest(t), w.n);
+        const bool whole = tile_whole(s, base, w.lowest(a, t), w.highest(a, t), w.n);
         // Exponentials with the reference as it is, the maximum on the way: where it shows that the reference has to rise (or a
         // first guess of 0 was too high), the tile is taken again, once.  P leaves the registers when that is known.
         uint32_t pr[64];
@@ -470,11 +512,14 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
       }
       const float2 parts = apart(sum);
       const float total = parts.x + parts.y;
-      const bool row = q < s.queries, empty = first || p >= w.n || (ref == -INFINITY && total == 0.f);
+      const bool row = q < s.queries && head < w.h + w.heads, empty = first || p >= w.n || (ref == -INFINITY && total == 0.f);
       if (ok && !first) ok = bar_wait_warp(o_done(t), (taken - 1) & 1, &s_gone, status);
       fence_after();
       const float inv = empty ? 0.f : 1.f / total;
-      __half* to = out + (((size_t)w.b * s.queries + q) * s.n_heads + w.h) * D;
+      const size_t at_row = ((size_t)w.b * s.queries + q) * s.n_heads + head, rows = (size_t)s.sequences * s.queries * s.n_heads;
+      const bool cut = FEW && a.by_parts.d > 1;            // a part of the row: fp32, and its sum
+      float* to32 = partial + (w.part * rows + at_row) * D;
+      __half* to = out + at_row * D;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t y[32];
@@ -483,6 +528,16 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
           wait_load<32>(y);
         }
         if (!row) continue;
+        if (cut) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = empty ? 0.f : __uint_as_float(y[e + k]) * inv;
+            *reinterpret_cast<float4*>(to32 + c + e) = make_float4(v[0], v[1], v[2], v[3]);
+          }
+          continue;
+        }
         uint64_t all[2] = {};
 #pragma unroll
         for (int e = 0; e < 16; ++e) all[e & 1] = add2(all[e & 1], two(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1])));
@@ -496,7 +551,9 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
           *reinterpret_cast<uint4*>(to + c + e) = !ok ? make_uint4(~0u, ~0u, ~0u, ~0u) : (empty ? make_uint4(0, 0, 0, 0) : make_uint4(v[0], v[1], v[2], v[3]));
         }
       }
-      if (row) lse[((size_t)w.b * s.n_heads + w.h) * s.queries + q] = !ok ? NAN : (empty ? -INFINITY : ((ref == -INFINITY ? 0.f : ref) - LIFT + log2f(total)) * LN2);
+      const float total2 = !ok ? NAN : (empty ? -INFINITY : (ref == -INFINITY ? 0.f : ref) - LIFT + log2f(total));
+      if (row && cut) partial[a.by_parts.d * rows * D + w.part * rows + at_row] = total2;
+      else if (row) lse[((size_t)w.b * s.n_heads + head) * s.queries + q] = total2 * LN2;
     }
   }
   fence_before();
@@ -505,7 +562,110 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
     fence_after();
     dealloc(tmem, 512);
   }
-  if (warp < W_LOAD && s_nan[warp]) rows_again<D>(a, items, out, lse);
+  if (warp < W_LOAD && s_nan[warp]) rows_again<D, FEW>(a, items, out, lse);
+}
+
+// a row's parts: out = sum 2^(l_p - l) out_p, l = log2 of the sum of 2^(l_p); a warp a row
+template <int D>
+__global__ void __launch_bounds__(256) prompt_sum_kernel(const __grid_constant__ PromptArgs a, const float* __restrict__ partial, __half* out, float* lse) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  constexpr int C = D / 32;
+  const cq_prompt& s = a.s;
+  const int lane = threadIdx.x & 31, parts = (int)a.by_parts.d;
+  const size_t rows = (size_t)s.sequences * s.queries * s.n_heads, row = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const float l = lane < parts ? partial[parts * rows * D + lane * rows + row] : -INFINITY;
+  float top = l;
+#pragma unroll
+  for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  const float f = l == -INFINITY ? 0.f : exp2f(l - (top == -INFINITY ? 0.f : top));
+  float sum = f;
+#pragma unroll
+  for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  float y[C] = {};
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float w = __shfl_sync(0xffffffffu, f, p);
+    const float* from = partial + (p * rows + row) * D + C * lane;
+#pragma unroll
+    for (int i = 0; i < C; ++i) y[i] = fmaf(w, from[i], y[i]);
+  }
+  const bool empty = sum == 0.f;
+  const float inv = empty ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int i = 0; i < C; i += 2) *reinterpret_cast<uint32_t*>(out + row * D + C * lane + i) = half_pair(y[i] * inv, y[i + 1] * inv);
+  const int h = (int)(row % s.n_heads), q = (int)(row / s.n_heads % s.queries), b = (int)(row / s.n_heads / s.queries);
+  if (lane == 0) lse[((size_t)b * s.n_heads + h) * s.queries + q] = empty ? -INFINITY : (top + log2f(sum)) * LN2;
+  __syncwarp();
+  bool broken = false;
+#pragma unroll
+  for (int i = 0; i < C; ++i) broken |= y[i] != y[i];
+  if (__any_sync(0xffffffffu, broken)) row_again<D>(a, b, h, q, out, lse);
+}
+
+// The form of a call: queries of a head side by side (`rows`), heads in an item (`pack`), parts of its keys.
+struct PromptForm {
+  int rows = 256, pack = 1, parts = 1;
+  int units(const cq_prompt* s) const { return (s->n_heads / s->n_kv_heads + pack - 1) / pack; }      // items of a KV head, a block of queries, a part
+  long long items(const cq_prompt* s) const {
+    return (long long)((s->queries + rows - 1) / rows) * s->n_kv_heads * units(s) * s->sequences * parts;
+  }
+};
+// key tiles that the block's queries see
+int tiles_of(const cq_prompt* s, int block, int rows) {
+  const int off = s->keys - s->queries, pmin = block * rows + off, pmax = std::min((block + 1) * rows, s->queries) + off - 1;
+  const int key = s->window ? std::max(0, pmin - s->window + 1) : 0, ns = (std::min(s->window ? s->sinks : 0, key) + UM_TILE - 1) / UM_TILE;
+  const int wt0 = key / UM_TILE;
+  return pmax / UM_TILE + 1 - (ns >= wt0 ? 0 : wt0 - ns);
+}
+// What the first and the last CTA have to do, the longer of the two, in tiles of 256 x 128 x 128 (about 1.9 us): 0.7 where one tile of
+// 128 queries is all there is or heads are 64 wide, 2 for an item; and for joining the parts 2, and 0.5 for a million of numbers.  On 36 shapes of 1
+// to 5000 queries its choice is 0.4 % slower than the best, 8 % at most.  (16 queries of 64 / 8 heads over 4000 keys: 60 us as whole heads, 18 so;
+// 512 of 32 heads over 4096 72 and 55; 100 of 8 / 1 over 20000 273 and 34; 2048 over their own keys stay whole, 36 us, 40 in two.)
+double prompt_cost(const cq_prompt* s, const PromptForm& f) {
+  const int blocks = (s->queries + f.rows - 1) / f.rows, sms = cq_sm_count();
+  const long long items = f.items(s), row = items / blocks;
+  const bool one = s->queries <= UM_TILE && f.pack * f.rows <= 256 && (f.rows == 256 || f.pack * f.rows <= UM_TILE);
+  const double tile = (one ? 0.7 : 1.0) * (s->head_dim == 128 ? 1.0 : 0.7);
+  double most = 0;
+  for (int last = 0; last < 2; ++last) {
+    double t = 0;
+    for (long long j = 0;; ++j) {
+      const long long i = j * sms + ((j & 1) != last ? sms - 1 : 0);
+      if (i >= items) break;
+      t += (tiles_of(s, blocks - 1 - (int)(i / row), f.rows) + f.parts - 1) / f.parts * tile + 2;
+    }
+    most = std::max(most, t);
+  }
+  return most + (f.parts > 1 ? 2 + 0.5e-6 * f.parts * s->sequences * s->queries * s->n_heads * s->head_dim : 0);
+}
+PromptForm prompt_form(const cq_prompt* s) {
+  static thread_local cq_prompt last = {};
+  static thread_local PromptForm kept;                     // (of the last call's shape)
+  if (!memcmp(&last, s, offsetof(cq_prompt, q_strides))) return kept;
+  const int G = s->n_heads / s->n_kv_heads, sms = cq_sm_count();
+  PromptForm best, f;
+  if (best.items(s) < 4ll * sms) {                         // (more items fill the SMs as they are)
+    double least = prompt_cost(s, best);
+    for (int packed = 0; packed < 2; ++packed) {
+      if (packed) {
+        if (s->queries > UM_TILE || G == 1) break;
+        for (f.rows = 8; f.rows < s->queries;) f.rows *= 2;
+        f.pack = std::min(G, 256 / f.rows);
+      }
+      const int most = tiles_of(s, (s->queries + f.rows - 1) / f.rows - 1, f.rows);
+      for (f.parts = 1; f.parts <= std::min(16, most) && (f.parts == 1 || f.items(s) <= 3ll * sms); ++f.parts) {
+        const double t = prompt_cost(s, f);
+        if (t < least) {
+          least = t;
+          best = f;
+        }
+      }
+    }
+  }
+  last = *s;
+  return kept = best;
 }
 
 // ------------------------------------------------------------------ weights of the keys
@@ -613,7 +773,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
     if (lane == 0) {
       uint32_t loaded = 0, sent = 0;                       // key tiles, query tiles
       bool ok = true;
-      for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
+      for (int round = 0, item; ok && (item = item_at(round, items)) >= 0; ++round) {
         const KeysItem w(a, item, observe);
         if (!w.tiles) continue;
         const uint32_t kb = loaded & 1;
@@ -647,7 +807,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
     constexpr uint32_t SHAPE = shape_of(128, 128, false);
     uint32_t loaded = 0, sent = 0;
     bool ok = true;
-    for (int round = 0, item; ok && (item = PromptItem::at(round, items)) >= 0; ++round) {
+    for (int round = 0, item; ok && (item = item_at(round, items)) >= 0; ++round) {
       const KeysItem w(a, item, observe);
       if (!w.tiles) continue;
       const uint32_t kb = loaded & 1;
@@ -683,7 +843,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
     const uint64_t scale22 = two(scale2, scale2);
     uint32_t seen = 0, before = 0;                         // tiles, and items with any, before this one
     bool ok = true;
-    for (int round = 0, item; (item = PromptItem::at(round, items)) >= 0; ++round) {
+    for (int round = 0, item; (item = item_at(round, items)) >= 0; ++round) {
       const KeysItem w(a, item, observe);
       const int key = w.k0 + r;
       if (!w.tiles) {
@@ -783,10 +943,10 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const float* __restric
   for (int p = 0; p < parts; ++p) sum += part[p * n + i];
   weights[i] = sum;
 }
-// Into how many parts an item's queries are cut, by a model in tiles of 128 x 128 (about 1 us each): an SM's share of all of
-// them, 2 for every item that it takes, more than half of the longest item where the work runs out, 2.5 for joining the parts.  (70B
-// heads, 8192 tokens, a window of 2048 with sinks, whose tile all queries see: 1 part 843 us, 8 484, 16 531; 512 tokens of 8 KV
-// heads 38 and 14; 2048 tokens of 40 heads stay whole, 45 us, 58 in two.)
+// Into how many parts an item's queries are cut, by a model in tiles of 128 x 128 (about 0.7 us each): an SM's share of all of
+// them, 2 for every item that it takes, more than half of the longest item where the work runs out, 2.5 for joining the parts.  On 28
+// shapes its choice is 0.4 % slower than the best, 7 % at most.  (70B heads, 8192 tokens, a window of 2048 with sinks, whose tile all
+// queries see: 1 part 592 us, 6 374, 16 404; 2048 tokens of 40 heads stay whole, 35 us, 39 in two.)
 int parts_of(const cq_prompt* s, int observe) {
   const int tiles = (s->keys + UM_TILE - 1) / UM_TILE, G = s->n_heads / s->n_kv_heads, step = (tiles + 255) / 256;
   double sum = 0, longest = 0;
@@ -837,12 +997,17 @@ bool map_of(CUtensorMap* map, const void* at, const int64_t (&strides)[3], int s
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int check(const cq_prompt* s, const void* q, const void* k, const void* v) {
-  if (!s || !q || !k || (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) || s->window < 0 || s->sinks < 0 || !(s->scale > 0.f)) return CQ_ERR_BAD_ARG;
+int check_shape(const cq_prompt* s) {
+  if (!s) return CQ_ERR_BAD_ARG;
   if (s->sequences < 1 || s->sequences > 65535 || s->queries < 1 || s->keys < s->queries || s->keys > (1 << 24) || s->n_kv_heads < 1 ||
       s->n_heads < 1 || s->n_heads > 65535 || s->n_heads % s->n_kv_heads)
     return CQ_ERR_BAD_SHAPE;
   if (s->head_dim != 64 && s->head_dim != 128) return CQ_ERR_UNSUPPORTED;
+  return s->window < 0 || s->sinks < 0 ? CQ_ERR_BAD_ARG : CQ_OK;
+}
+int check(const cq_prompt* s, const void* q, const void* k, const void* v) {
+  if (!s || !q || !k || (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) || s->window < 0 || s->sinks < 0 || !(s->scale > 0.f)) return CQ_ERR_BAD_ARG;
+  if (const int rc = check_shape(s)) return rc;
   for (int i = 0; i < 3; ++i)
     if ((s->q_strides[i] | s->k_strides[i] | (v ? s->v_strides[i] : 0)) & 7) return CQ_ERR_BAD_ARG;
   if ((s->queries > 1 && s->q_strides[1] < 8) || (s->keys > 1 && (s->k_strides[1] < 8 || (v && s->v_strides[1] < 8)))) return CQ_ERR_BAD_ARG;
@@ -851,28 +1016,46 @@ int check(const cq_prompt* s, const void* q, const void* k, const void* v) {
 
 }  // namespace
 
+extern "C" size_t cq_attn_prefill_workspace_bytes(const cq_prompt* s) {
+  if (check_shape(s) != CQ_OK) return 0;
+  const int parts = prompt_form(s).parts;
+  return parts > 1 ? (size_t)parts * s->sequences * s->queries * s->n_heads * (s->head_dim + 1) * sizeof(float) : 0;
+}
+
 extern "C" int cq_attn_prefill(const cq_prompt* shape, const void* q, const void* k, const void* v, const long long* lengths, void* out,
-                               float* lse, uint32_t* status_word, cq_stream_t stream) {
+                               float* lse, void* workspace, uint32_t* status_word, cq_stream_t stream) {
   const int rc = check(shape, q, k, v);
   if (rc != CQ_OK) return rc;
   if (!v || !out || !lse || ((uintptr_t)out & 15)) return CQ_ERR_BAD_ARG;
-  PromptArgs a = {*shape, (const __half*)q, (const __half*)k, (const __half*)v, lengths, shape->n_heads / shape->n_kv_heads};
-  const int D = shape->head_dim, B = shape->sequences;
-  a.by_group = Divisor(a.group);
-  a.by_heads = Divisor(shape->n_heads);
-  a.by_row = Divisor((uint32_t)shape->n_heads * B);
+  const int D = shape->head_dim, B = shape->sequences, G = shape->n_heads / shape->n_kv_heads;
+  PromptArgs a = {*shape, (const __half*)q, (const __half*)k, (const __half*)v, lengths, G};
+  const PromptForm form = prompt_form(shape);
+  const int parts = form.parts, units = form.units(shape);
+  a.rows = form.rows;
+  a.pack = form.pack;
+  if (parts > 1 && (!workspace || ((uintptr_t)workspace & 15))) return CQ_ERR_BAD_ARG;
+  const bool few = a.rows < 256 || parts > 1;
+  while (1 << a.shift > a.rows) --a.shift;
+  a.by_group = Divisor(units);
+  a.by_heads = Divisor((uint32_t)shape->n_kv_heads * units);
+  a.by_row = Divisor((uint32_t)shape->n_kv_heads * units * B);
+  a.by_parts = Divisor(parts);
   PromptMaps maps;
-  if (!map_of(&maps.q, q, shape->q_strides, B, shape->queries, shape->n_heads, D, UM_TILE, maps.one[0]) ||
+  if (!map_of(&maps.q, q, shape->q_strides, B, shape->queries, shape->n_heads, D, std::min(a.rows, UM_TILE), maps.one[0]) ||
       !map_of(&maps.k, k, shape->k_strides, B, shape->keys, shape->n_kv_heads, D, UM_TILE, maps.one[1]) ||
       !map_of(&maps.v, v, shape->v_strides, B, shape->keys, shape->n_kv_heads, D, UM_TILE, maps.one[2]))
     return CQ_ERR_UNSUPPORTED;
-  auto fn = D == 128 ? prompt_kernel<128> : prompt_kernel<64>;
+  auto fn = D == 128 ? (few ? prompt_kernel<128, true> : prompt_kernel<128, false>) : (few ? prompt_kernel<64, true> : prompt_kernel<64, false>);
   const int smem = (2 + UM_STAGES) * (D / 64) * UM_CHUNK + 1024;
   CQ_CUDA_TRY(cq_grant_smem((const void*)fn, smem));
-  const long long items = (long long)((shape->queries + 2 * UM_TILE - 1) / (2 * UM_TILE)) * shape->n_heads * B;
-  if (items > INT32_MAX / 2) return CQ_ERR_BAD_SHAPE;
+  const long long items = form.items(shape);
+  const size_t rows = (size_t)B * shape->queries * shape->n_heads;
+  if (items > INT32_MAX / 2 || (rows + 7) / 8 > INT32_MAX) return CQ_ERR_BAD_SHAPE;
   CQ_CUDA_TRY(kv4_launch(fn, dim3((unsigned)std::min<long long>(items, cq_sm_count())), dim3(UM_THREADS), smem, (cudaStream_t)stream, a, maps,
-                         (__half*)out, lse, (int)items, status_word));
+                         (__half*)out, lse, (float*)workspace, (int)items, status_word));
+  if (parts > 1)
+    CQ_CUDA_TRY(kv4_launch(D == 128 ? prompt_sum_kernel<128> : prompt_sum_kernel<64>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0,
+                           (cudaStream_t)stream, a, (const float*)workspace, (__half*)out, lse));
   return CQ_OK;
 }
 

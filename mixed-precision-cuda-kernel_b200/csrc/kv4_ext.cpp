@@ -293,8 +293,11 @@ std::pair<torch::Tensor, torch::Tensor> attn_prefill(torch::Tensor q, torch::Ten
   TORCH_CHECK(v.sizes() == k.sizes(), "v must have the shape of k");
   auto out = torch::empty(q.sizes(), q.options());
   auto lse = torch::empty({s.sequences, s.n_heads, s.queries}, q.options().dtype(torch::kFloat32));
+  torch::Tensor ws;
+  if (const size_t bytes = cq_attn_prefill_workspace_bytes(&s)) ws = torch::empty({(int64_t)bytes}, q.options().dtype(torch::kUInt8));
   check_status(cq_attn_prefill(&s, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), n, out.data_ptr(), lse.data_ptr<float>(),
-                               device_status(q.device()), (cq_stream_t)c10::cuda::getCurrentCUDAStream().stream()),
+                               ws.defined() ? ws.data_ptr() : nullptr, device_status(q.device()),
+                               (cq_stream_t)c10::cuda::getCurrentCUDAStream().stream()),
                "attn_prefill");
   return {out, lse};
 }

@@ -261,3 +261,33 @@ def test_masked_infinities_in_a_long_prompt(qc):
     assert torch.equal(l, lse) and (out[0, 1499] == math.inf).all()
     assert ((out[0, :1499].double() - want[0, :1499].double()).abs() <= 6 * 2.0 ** -11 * float(v[0, :1499].abs().max())).all()
     assert torch.equal(out[0, :1408], want[0, :1408])
+
+
+@pytest.mark.parametrize("Tq,Tk", [(1, 1), (1, 2500), (3, 1000), (8, 8), (9, 700), (33, 33), (50, 3001), (128, 1500), (129, 1500), (300, 2000)])
+@pytest.mark.parametrize("H,KV,D", [(8, 1, 128), (6, 2, 64), (40, 1, 64), (4, 4, 128), (64, 8, 128)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (600, 70)])
+def test_few_queries(qc, Tq, Tk, H, KV, D, window, sinks):
+    """Heads side by side in a tile, keys in parts."""
+    check(qc, *make(1, Tq, Tk, H, KV, D, Tq), None, window, sinks, observe=20)
+
+
+@pytest.mark.parametrize("Tq", [5, 64, 200])
+def test_few_queries_ragged(qc, Tq):
+    q, k, v = make(5, Tq, 1100, 8, 2, 128, Tq)
+    lengths = [1100, 0, 1100 - Tq, 1100 - Tq + 1, 1098]
+    want = check(qc, q, k, v, lengths, 500, 3, observe=20)
+    for b, n in enumerate(lengths):
+        k[b, n:], v[b, n:] = math.nan, math.inf
+        q[b, max(0, n - 1100 + Tq):] = math.nan
+    out, _ = qc.attn_prefill(q, k, v, window=500, sinks=3, lengths=long(lengths))
+    assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("Tq,H,KV", [(20, 4, 1), (150, 2, 2)])
+def test_few_queries_masked_infinities(qc, Tq, H, KV):
+    q, k, v = make(1, Tq, 2000, H, KV, 128, 13)
+    want, lse = qc.attn_prefill(q, k, v, window=700)
+    v[0, 1999], v[0, 1100, 0, 7] = math.inf, math.nan
+    out, l = qc.attn_prefill(q, k, v, window=700)
+    assert torch.equal(l, lse) and (out[0, -1] == math.inf).all()
+    assert ((out[0, :-1].double() - want[0, :-1].double()).abs() <= 6 * 2.0 ** -11 * float(v[0, :1100].abs().max())).all()

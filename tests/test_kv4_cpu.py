@@ -87,7 +87,7 @@ def prompt(**o):
 ])
 def test_prompt_fields(lib, change, code):
     s, at = prompt(**change), C.c_void_p(1 << 24)
-    assert lib.cq_attn_prefill(C.byref(s), at, at, at, None, at, at, None, None) == code
+    assert lib.cq_attn_prefill(C.byref(s), at, at, at, None, at, at, at, None, None) == code
     assert lib.cq_attn_prefill_weights(C.byref(s), at, at, at, None, 4, at, at, None, None) == code
 
 
@@ -95,6 +95,6 @@ def test_prompt_calls(lib):
     s, at, odd = prompt(), C.c_void_p(1 << 24), C.c_void_p((1 << 24) + 2)
     for a in ((None, at, at, None, at, at), (at, None, at, None, at, at), (at, at, None, None, at, at), (odd, at, at, None, at, at),
               (at, at, odd, None, at, at), (at, at, at, None, None, at), (at, at, at, None, at, None)):
-        assert lib.cq_attn_prefill(C.byref(s), *a, None, None) == BAD_ARG
+        assert lib.cq_attn_prefill(C.byref(s), *a, at, None, None) == BAD_ARG
     for a in ((None, at, at, None, 4, at), (at, at, None, None, 4, at), (at, at, at, None, 0, at), (at, at, at, None, 4, None)):
         assert lib.cq_attn_prefill_weights(C.byref(s), *a, at, None, None) == BAD_ARG
