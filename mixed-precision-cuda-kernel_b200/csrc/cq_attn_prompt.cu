@@ -124,17 +124,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 // 2^x of two numbers up to 2^7 on the multiply-add pipe: x = n + f with a whole n and |f| <= 1/2, by adding and taking away
-// 1.5 * 2^23, then 2^f by the polynomial of degree 4 whose largest relative error is the least (2.6e-6; coefficients by
-// Remez's exchange) and 2^n as a bit pattern.  Below 2^-126: 2^-126.  NaN stays NaN.
+// 1.5 * 2^23, then 2^f by the polynomial of degree 5 whose largest relative error is the least (2.1e-7 in fp32; coefficients by
+// Remez's exchange; degree 4 is 2.6e-6, which the weights of keys show, and no faster) and 2^n as a bit pattern.  Below 2^-126:
+// 2^-126.  NaN stays NaN.
 __device__ __forceinline__ uint64_t power2(float2 x) {
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
   const uint64_t v = two(x.x, x.y), big = two(12582912.f, 12582912.f), less = two(-12582912.f, -12582912.f);
   const uint64_t t = add2(v, big), f = fma2(add2(t, less), two(-1.f, -1.f), v);
-  uint64_t p = fma2(f, two(0.009570102207362652f, 0.009570102207362652f), two(0.05591785907745361f, 0.05591785907745361f));
-  p = fma2(p, f, two(0.240247443318367f, 0.240247443318367f));
-  p = fma2(p, f, two(0.6931217908859253f, 0.6931217908859253f));
-  p = fma2(p, f, two(0.9999992847442627f, 0.9999992847442627f));
+  uint64_t p = fma2(f, two(0.0013276472454890609f, 0.0013276472454890609f), two(0.009675540961325169f, 0.009675540961325169f));
+  p = fma2(p, f, two(0.05550713092088699f, 0.05550713092088699f));
+  p = fma2(p, f, two(0.24022120237350464f, 0.24022120237350464f));
+  p = fma2(p, f, two(0.6931469440460205f, 0.6931469440460205f));
+  p = fma2(p, f, two(1.0000001192092896f, 1.0000001192092896f));
   const float2 n = apart(t);
   return mul2(p, two(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3F800000u), __uint_as_float((__float_as_uint(n.y) << 23) + 0x3F800000u)));
 }

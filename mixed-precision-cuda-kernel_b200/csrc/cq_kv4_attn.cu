@@ -5,8 +5,10 @@
 //   out = sum_j p_j v_j,  p = softmax over the visible slots j of scale * q . k_j,
 //   visible: j < n and (no window, or j < sinks, or j >= n - window)
 //
-// The bound is the cache, read once: 160 bytes a slot and KV head (D = 128, groups of 32) in 111 cycles of an SM's share of
-// HBM for 16 slots, against about 275 warp instructions (69 issue cycles) that take the codes apart.  So:
+// The bound is the cache, read once: 160 bytes a slot and KV head (D = 128, groups of 32), 222 cycles of an SM's share of HBM for 32
+// slots of a head.  Taking the codes apart is what it costs beyond: 690 warp instructions for them (8 query heads), 172 cycles of
+// the four schedulers if none ever waited; 60 % of their cycles issue one, tensor pipe 34 %.  4 sequences of 65536 slots with 8 KV
+// heads: 81 us for 336 MB, a kernel that only copies them into shared memory 58.  So:
 //   * slots are the M side of mma.sync.m16n8k16 and the (up to eight) query heads of a KV head its N side, in both products:
 //     S^T = K Q^T and O^T = V^T P^T.  (With the heads on the M side half of every MMA and of its accumulators were empty.)
 //     P^T is the accumulator of the first product, packed to fp16 and transposed by two movmatrix;
@@ -15,7 +17,8 @@
 //     group's scale in fp32.  The minima's part, sum over groups of minimum * (sum of the group's query columns), is one
 //     MMA more, the query sums split into three fp16 numbers.  Nothing is rounded before the softmax but the sums;
 //   * values: scale * code + minimum rounded to fp16 (three instructions for two), so that any column can ride with any
-//     group; weights are rounded to fp16.  Either costs an output about as much as its own rounding to fp16 does;
+//     group, which costs an output about as much as its own rounding to fp16 does; weights are two fp16 numbers of 11 bits each and two
+//     MMAs (rounded to one of them: error against 64 bits 3.5e-4 of the outputs' norm instead of 2.8e-4, 4 to 7 % less time);
 //   * queries are scaled by a power of two, a head's largest to 16 .. 32, so that neither codes * 2^-24 nor a sixteenth of a
 //     query (for the codes in the upper half of a byte) leaves fp16;
 //   * a warp takes 32 slots a turn from a ring of its own in shared memory that cp.async fills (two turns), and keeps its own
