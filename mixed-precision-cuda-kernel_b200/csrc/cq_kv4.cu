@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(WR_THREADS) kv4_write_kernel(
   const int end = min(tokens, ((int)blockIdx.x + 1) * WR_TOKENS);
   // every lane stays to the end: a row's lanes exchange their minima
   for (int t0 = blockIdx.x * WR_TOKENS; t0 < end; t0 += FLIGHT * ROWS) {
-    float x[FLIGHT][16];
+    uint32_t x[FLIGHT][8];
     long long pos[FLIGHT];
 #pragma unroll
     for (int f = 0; f < FLIGHT; ++f) {
@@ -47,8 +47,8 @@ __global__ void __launch_bounds__(WR_THREADS) kv4_write_kernel(
       if (is_q) {
         if (t >= end) continue;
         __half* to = q_out + ((size_t)(b * (size_t)tokens + t) * H + head) * D + c;
-        *reinterpret_cast<uint4*>(to) = kv4_halves(x[f]);
-        *reinterpret_cast<uint4*>(to + D / 2) = kv4_halves(x[f] + 8);
+        *reinterpret_cast<uint4*>(to) = make_uint4(x[f][0], x[f][1], x[f][2], x[f][3]);
+        *reinterpret_cast<uint4*>(to + D / 2) = make_uint4(x[f][4], x[f][5], x[f][6], x[f][7]);
         continue;
       }
       uint32_t words[2], pairs[2];
@@ -99,11 +99,17 @@ __global__ void __launch_bounds__(WR_THREADS) kv4_read_kernel(cq_kv4 cache, cons
   for (int f = 0; f < FLIGHT; ++f) {
     const int t = blockIdx.x * WR_TOKENS + f * ROWS + threadIdx.x / LANES;
     if (t >= count) break;
-    const float2 sm = __half22float2(pair[f]);
-    float x[8];
+    // scale * code + minimum, rounded once: 1024 + code is what a code in the lowest bits of an fp16 1024 makes
+    const __half2 s2 = __low2half2(pair[f]), m2 = __high2half2(pair[f]), less = __float2half2_rn(-1024.f);
+    uint32_t x[4];                                         // columns (0, 4), (1, 5), (2, 6), (3, 7)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __fmaf_rn((float)((word[f] >> (4 * e)) & 15u), sm.x, sm.y);
-    *reinterpret_cast<uint4*>(to + (((size_t)b * count + t) * KV + head) * D + 8 * w) = kv4_halves(x);
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t u = (word[f] >> (4 * e) & 0x000F000Fu) | 0x64006400u;
+      const __half2 y = __hfma2(__hadd2(*reinterpret_cast<const __half2*>(&u), less), s2, m2);
+      x[e] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+    *reinterpret_cast<uint4*>(to + (((size_t)b * count + t) * KV + head) * D + 8 * w) =
+        make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410), __byte_perm(x[0], x[1], 0x7632), __byte_perm(x[2], x[3], 0x7632));
   }
 }
 

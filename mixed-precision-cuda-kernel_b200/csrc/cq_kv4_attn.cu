@@ -211,11 +211,18 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
   const bool turn = STEP && fresh.cos_t && pos >= 0 && pos < fresh.table_rows;
   for (int i = tid; i < AT_HEADS * LANES; i += THREADS) {
     const int g = i / LANES, c = 8 * (i % LANES);
-    float x[16] = {};
+    uint32_t row[8] = {};
     if (g < heads) {
       const __half* src = q + (head0 + g) * D + c;
-      kv4_load16(src, src + D / 2, x);
-      if (turn) kv4_rotate(x, fresh.cos_t + pos * (D / 2) + c, fresh.sin_t + pos * (D / 2) + c);
+      kv4_load16(src, src + D / 2, row);
+      if (turn) kv4_rotate(row, fresh.cos_t + pos * (D / 2) + c, fresh.sin_t + pos * (D / 2) + c);
+    }
+    float x[16];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 f = apart(kv4_two(row[e]));
+      x[2 * e] = f.x;
+      x[2 * e + 1] = f.y;
     }
     float top = 0.f;
 #pragma unroll
@@ -239,7 +246,7 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
   if (STEP && owner && warp == WARPS - 1) {
     const int which = lane / LANES & 1, c = 8 * (lane % LANES);
     const __half* src = (which ? fresh.v : fresh.k) + ((size_t)b * cache.n_kv_heads + kvh) * D + c;
-    float x[16];
+    uint32_t x[8];
     kv4_load16(src, src + D / 2, x);
     if (!which && turn) kv4_rotate(x, fresh.cos_t + pos * (D / 2) + c, fresh.sin_t + pos * (D / 2) + c);
     uint32_t words[2], pairs[2];
