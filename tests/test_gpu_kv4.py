@@ -399,7 +399,7 @@ def test_evict_more_than_keep_to_stay(qc, n, keep, sinks, recent, want):
         assert kept[0, h].tolist() == want + [-1] * (keep - len(want)) and torch.equal(left[0, h, :len(want)], w[0, h, want])
 
 
-@pytest.mark.parametrize("n,keep", [(70000, 1000), (70001, 69990), (131072, 65536)])
+@pytest.mark.parametrize("n,keep", [(70000, 1000), (70001, 69990), (131072, 65536), (512, 200), (513, 200), (4000, 1000)])
 def test_evict_long(qc, n, keep):
     g = gen(n)
     S = (n + 31) // 32 * 32
