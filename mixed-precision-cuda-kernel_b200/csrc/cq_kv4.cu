@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(SEL_THREADS) kv4_select_kernel(const float* __
   __shared__ uint32_t hist[256];
   __shared__ uint32_t s_prefix, s_need;
   __shared__ uint32_t s_warp[2][32];
-  const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int threads = blockDim.x, head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const long long len = length[b];
   const int n = (int)(len < 0 ? 0 : (len > slots ? slots : len));
   const size_t row = (size_t)b * KV + head;
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(SEL_THREADS) kv4_select_kernel(const float* __
   float* wto = weights_out + row * keep;
   if (head == 0 && tid == 0) length_out[b] = n < keep ? n : keep;
   if (n <= keep) {
-    for (int j = tid; j < keep; j += SEL_THREADS) {
+    for (int j = tid; j < keep; j += threads) {
       to[j] = j < n ? j : -1;
       wto[j] = j < n ? w[j] : 0.f;
     }
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(SEL_THREADS) kv4_select_kernel(const float* __
     if (tid < 256) hist[tid] = 0;
     __syncthreads();
     const uint32_t prefix = s_prefix;
-    for (int j = beg + tid; j < end; j += SEL_THREADS) {
+    for (int j = beg + tid; j < end; j += threads) {
       const uint32_t key = weight_key(w[j]);
       if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
     }
@@ -206,11 +206,13 @@ __global__ void __launch_bounds__(SEL_THREADS) kv4_select_kernel(const float* __
     mask |= 255u << shift;
     if (s_need == 0) break;
   }
+  if (tid < 64) s_warp[tid >> 5][tid & 31] = 0;              // (of warps that a smaller block has not)
+  __syncthreads();
   const uint32_t limit = s_prefix, ties = s_need;           // keys above `limit` stay, and the first `ties` equal to it
   const bool none = ties == 0;
-  // in order: slots of a block of SEL_THREADS at a time, ranks by ballots
+  // in order: as many slots as threads at a time, ranks by ballots
   uint32_t above = 0, equal = 0;                            // before this block: kept because above or outside, equal
-  for (int base = 0; base < n; base += SEL_THREADS) {
+  for (int base = 0; base < n; base += threads) {
     const int j = base + tid;
     bool up = false, eq = false;
     if (j < n) {
@@ -358,7 +360,11 @@ extern "C" int cq_kv4_evict(const cq_kv4* from, const cq_kv4* to, const float* w
     if ((fp[i] == tp[i]) != in_place) return CQ_ERR_BAD_ARG;
   if (in_place && (from->slots != to->slots || !workspace || ((uintptr_t)workspace & 15))) return CQ_ERR_BAD_ARG;
   const int B = from->sequences, KV = from->n_kv_heads, D = from->head_dim;
-  CQ_CUDA_TRY(kv4_launch(kv4_select_kernel, dim3(KV, B), dim3(SEL_THREADS), 0, (cudaStream_t)stream, weights, length, length_out, kept,
+  // The passes of a head are a chain: many threads for many slots, fewer for short ones or where heads fill the SMs anyway.  (With the
+  // move, 256 / 512 / 1024 threads: 32 heads of 200 slots 5.9 / 6.1 / 6.7 us, 1000 9.3 / 7.4 / 7.5, 4000 24 / 20 / 13; 1080 heads of 200
+  // 9.6 / 13.7 / 23.7, of 1000 36 / 38 / 45, of 4000 119 / 121 / 130.)
+  const int threads = from->slots <= 512 || (from->slots <= 4096 && (long long)B * KV > 2 * cq_sm_count()) ? 256 : (from->slots <= 1024 ? 512 : SEL_THREADS);
+  CQ_CUDA_TRY(kv4_launch(kv4_select_kernel, dim3(KV, B), dim3(threads), 0, (cudaStream_t)stream, weights, length, length_out, kept,
                          weights_out, KV, from->slots, keep, sinks, recent));
   const size_t rows = (size_t)B * KV * keep;
   const int code = D / 2, scale = 4 * (D / from->group);
