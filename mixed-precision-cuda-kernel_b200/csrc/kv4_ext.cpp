@@ -43,6 +43,13 @@ const long long* whole_numbers(const torch::Tensor& t, const char* name, int64_t
   return (const long long*)t.const_data_ptr();
 }
 
+// An output or workspace, straight from the allocator: short calls are bound by the host, and a trip through the dispatcher for
+// each of them costs more than the rest of a call.  (Not where a dispatch mode watches.)
+torch::Tensor fresh_on(const c10::Device& device, c10::IntArrayRef shape, c10::ScalarType type) {
+  if (c10::impl::TorchDispatchModeTLS::any_modes_set()) return torch::empty(shape, torch::TensorOptions().device(device).dtype(type));
+  return at::detail::empty_cuda(shape, type, device, c10::nullopt);
+}
+
 // KV cache of `sequences` sequences in 4 bits; keeps its four tensors alive.
 struct KVCache4 {
   torch::Tensor k_codes, k_scales, v_codes, v_scales;
@@ -99,12 +106,7 @@ struct KVCache4 {
     return (cq_stream_t)s.stream();
   }
 
-  // An output or workspace, straight from the allocator: single tokens are bound by the host, and a trip through the
-  // dispatcher for each of them costs more than the rest of a call.  (Not where a dispatch mode watches.)
-  torch::Tensor fresh(c10::IntArrayRef shape, c10::ScalarType type) const {
-    if (c10::impl::TorchDispatchModeTLS::any_modes_set()) return torch::empty(shape, torch::TensorOptions().device(device).dtype(type));
-    return at::detail::empty_cuda(shape, type, device, c10::nullopt);
-  }
+  torch::Tensor fresh(c10::IntArrayRef shape, c10::ScalarType type) const { return fresh_on(device, shape, type); }
 
   // rows (rows, heads, D) fp16; returns the number of heads
   int check_rows(const torch::Tensor& t, const char* name, int64_t rows, int64_t heads) const {
@@ -227,11 +229,9 @@ struct KVCache4 {
                     to.c.group == c.group, "the caches must agree in all but their slots");
     TORCH_CHECK(keep > 0 && keep <= to.c.slots, "keep must be 1 to ", to.c.slots);
     TORCH_CHECK(sinks >= 0 && sinks <= INT32_MAX && recent >= 0 && recent <= INT32_MAX, "sinks and recent must be 0 or more");
-    auto kept = torch::empty({c.sequences, c.n_kv_heads, keep}, length.options().dtype(torch::kInt32));
-    auto left = torch::empty({c.sequences, c.n_kv_heads, keep}, weights.options());
-    auto now = torch::empty_like(length);
+    auto kept = fresh({c.sequences, c.n_kv_heads, keep}, torch::kInt32), left = fresh(kept.sizes(), torch::kFloat32), now = fresh(length.sizes(), torch::kInt64);
     torch::Tensor ws;
-    if (to.c.k_codes == c.k_codes) ws = torch::empty({(int64_t)cq_kv4_evict_workspace_bytes(&c, (int)keep)}, k_codes.options());
+    if (to.c.k_codes == c.k_codes) ws = fresh({(int64_t)cq_kv4_evict_workspace_bytes(&c, (int)keep)}, torch::kUInt8);
     to.use();
     check_status(cq_kv4_evict(&c, &to.c, w.first, left.data_ptr<float>(), n, (long long*)now.data_ptr(), (int)keep, (int)sinks, (int)recent,
                               kept.data_ptr<int>(), ws.defined() ? ws.data_ptr() : nullptr, use()),
@@ -291,10 +291,9 @@ std::pair<torch::Tensor, torch::Tensor> attn_prefill(torch::Tensor q, torch::Ten
   cq_prompt s = prompt_of(q, k, window, sinks, lengths, scale, &n);
   strides_of(v, "v", q.device(), s.v_strides);
   TORCH_CHECK(v.sizes() == k.sizes(), "v must have the shape of k");
-  auto out = torch::empty(q.sizes(), q.options());
-  auto lse = torch::empty({s.sequences, s.n_heads, s.queries}, q.options().dtype(torch::kFloat32));
+  auto out = fresh_on(q.device(), q.sizes(), torch::kFloat16), lse = fresh_on(q.device(), {s.sequences, s.n_heads, s.queries}, torch::kFloat32);
   torch::Tensor ws;
-  if (const size_t bytes = cq_attn_prefill_workspace_bytes(&s)) ws = torch::empty({(int64_t)bytes}, q.options().dtype(torch::kUInt8));
+  if (const size_t bytes = cq_attn_prefill_workspace_bytes(&s)) ws = fresh_on(q.device(), {(int64_t)bytes}, torch::kUInt8);
   check_status(cq_attn_prefill(&s, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), n, out.data_ptr(), lse.data_ptr<float>(),
                                ws.defined() ? ws.data_ptr() : nullptr, device_status(q.device()),
                                (cq_stream_t)c10::cuda::getCurrentCUDAStream().stream()),
@@ -313,8 +312,8 @@ torch::Tensor attn_prefill_weights(torch::Tensor q, torch::Tensor k, const torch
               "lse must be (sequences, heads, queries)");
   const int64_t last = observe.value_or(s.keys);
   TORCH_CHECK(last > 0, "observe must be positive");
-  auto out = torch::empty({s.sequences, s.n_kv_heads, s.keys}, lse.options());
-  auto ws = torch::empty({(int64_t)cq_attn_prefill_weights_workspace_bytes(&s, (int)std::min<int64_t>(last, s.keys))}, lse.options().dtype(torch::kUInt8));
+  auto out = fresh_on(q.device(), {s.sequences, s.n_kv_heads, s.keys}, torch::kFloat32);
+  auto ws = fresh_on(q.device(), {(int64_t)cq_attn_prefill_weights_workspace_bytes(&s, (int)std::min<int64_t>(last, s.keys))}, torch::kUInt8);
   check_status(cq_attn_prefill_weights(&s, q.const_data_ptr(), k.const_data_ptr(), lse.const_data_ptr<float>(), n,
                                        (int)std::min<int64_t>(last, s.keys), out.data_ptr<float>(), ws.data_ptr(),
                                        device_status(q.device()), (cq_stream_t)c10::cuda::getCurrentCUDAStream().stream()),
