@@ -761,6 +761,13 @@ def run_model(args):
     leave(torch, dist, world)
 
 
+def cache_options(args):
+    """The harness's options of the 4-bit cache; none with the fp16 cache."""
+    if args.kv_bits == 16:
+        return {}
+    return {"kv_bits": args.kv_bits, "window": args.window, "sinks": args.sinks, "kv_budget": args.kv_budget}
+
+
 def model_measure(args, torch, dist, dev, world, rank, local, name, gen=256, prompt_len=128, batch=1, max_seq=512):
     """Builds the model, decodes `gen` tokens greedily after a `prompt_len`-token random prompt (one CUDA graph
     per decode step, as benchmark_perplexity.py:92-113 of the reference times its per-token loop) and returns
@@ -770,7 +777,7 @@ def model_measure(args, torch, dist, dev, world, rank, local, name, gen=256, pro
     cfg = D.DecoderConfig(**{**base.__dict__, "max_seq": max_seq})
     t_build = time.time()
     model = D.CherryDecoder(cfg, device=dev, seed=1234, tp_group=dist.group.WORLD if world > 1 else None,
-                            tp_gather=args.gather, release_reference_buffers=True, batch=batch)
+                            tp_gather=args.gather, release_reference_buffers=True, batch=batch, **cache_options(args))
     torch.cuda.synchronize()
     t_build = time.time() - t_build
     prompt = torch.randint(0, cfg.vocab, (batch, prompt_len), device=dev, generator=torch.Generator(device=dev).manual_seed(0))
@@ -851,7 +858,7 @@ def model_measure(args, torch, dist, dev, world, rank, local, name, gen=256, pro
         "vs_baseline": None, "dtype": "f16",
         "data": "synthetic",
         "config": {"workload": f"llama2_{name}_arch_{cfg.bits}bit_g128_cherry1/256_prompt{prompt_len}_greedy{gen}_batch{batch}",
-                   "batch": batch, "max_seq": max_seq,
+                   "batch": batch, "max_seq": max_seq, **cache_options(args),
                    "layers": cfg.n_layers, "kv_heads": cfg.n_kv_heads,
                    "hidden": cfg.hidden, "ffn": cfg.ffn, "vocab": cfg.vocab, "bits": cfg.bits,
                    "l2_defeat": f"{qbytes / 1e9:.1f} GB of quantized weights + {hbytes / 1e6:.0f} MB lm_head per token, "
@@ -1004,6 +1011,10 @@ def main():
     ap.add_argument("--max-seq", type=int, default=512, help="model workload: positions of the KV cache")
     ap.add_argument("--prompt", type=int, default=128, help="model workload: prompt tokens per sequence")
     ap.add_argument("--gen", type=int, default=256, help="model workload: tokens generated per sequence")
+    ap.add_argument("--kv-bits", type=int, default=16, choices=[16, 4], help="model workload: bits of the KV cache")
+    ap.add_argument("--window", type=int, default=0, help="model workload, 4-bit cache: positions a query sees (0: all)")
+    ap.add_argument("--sinks", type=int, default=0, help="model workload, 4-bit cache: first positions that stay visible")
+    ap.add_argument("--kv-budget", type=int, default=None, help="model workload, 4-bit cache: slots that stay where it is bounded")
     ap.add_argument("--gather", default="peer", choices=["peer", "nccl"],
                     help="exchange step at N > 1: this library's peer-memory kernel (default) or NCCL")
     ap.add_argument("--repeats", type=int, default=50,
