@@ -104,11 +104,11 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // 2^x of two numbers up to 2^7 on the multiply-add pipe: x = n + f with a whole n and |f| <= 1/2, by adding and taking away
 // 1.5 * 2^23, then 2^f by the polynomial of degree 5 whose largest relative error is the least (2.1e-7 in fp32; coefficients by
-// Remez's exchange; degree 4 is 2.6e-6, which the weights of keys show, and takes 1 % off a prompt) and 2^n as a bit pattern.  Below 2^-126:
-// 2^-126.  NaN stays NaN.
+// Remez's exchange; degree 4 is 2.6e-6, which the weights of keys show, and takes 1 % off a prompt) and 2^n as a bit pattern.  x is held at -127, whose bit pattern is that of 0: below 2^-126.5 the
+// result is exactly 0, a masked score's of -infinity too (a row or key that sees nothing is known by a sum of 0).  NaN stays NaN.
 __device__ __forceinline__ uint64_t power2(float2 x) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
   const uint64_t v = two(x.x, x.y), big = two(12582912.f, 12582912.f), less = two(-12582912.f, -12582912.f);
   const uint64_t t = add2(v, big), f = fma2(add2(t, less), two(-1.f, -1.f), v);
   uint64_t p = fma2(f, two(0.0013276472454890609f, 0.0013276472454890609f), two(0.009675540961325169f, 0.009675540961325169f));

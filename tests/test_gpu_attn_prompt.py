@@ -291,3 +291,42 @@ def test_few_queries_masked_infinities(qc, Tq, H, KV):
     out, l = qc.attn_prefill(q, k, v, window=700)
     assert torch.equal(l, lse) and (out[0, -1] == math.inf).all()
     assert ((out[0, :-1].double() - want[0, :-1].double()).abs() <= 6 * 2.0 ** -11 * float(v[0, :1100].abs().max())).all()
+
+
+@pytest.mark.parametrize("Tq,Tk,H,KV,D", [(100, 1100, 8, 1, 128), (300, 2000, 4, 4, 128), (128, 1500, 8, 1, 64), (33, 700, 6, 2, 64), (200, 200, 2, 2, 128)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (600, 70)])
+@pytest.mark.parametrize("q0,k0", [(32.0, -35.375), (64.0, -53.0)])
+def test_scores_that_are_all_very_low(qc, Tq, Tk, H, KV, D, window, sinks, q0, k0):
+    """Scaled scores around q0 * k0 / sqrt(D), -100 and below: a row keeps its sum also where its keys are cut into parts and it sees
+    nothing of one.  The outputs' tolerance holds the scores' error too, twice that of lse, as the weights' relative error."""
+    q, k, v = make(1, Tq, Tk, H, KV, D, Tq)
+    q[..., 0], k[..., 0] = q0, k0
+    v += 3
+    out, lse = qc.attn_prefill(q, k, v, window=window, sinks=sinks)
+    want, l, _, big = reference(q, k, v, None, window, sinks)
+    e = (D + 8) * 2.0 ** -23 * big + 2.0 ** -20
+    assert ((lse.double() - l).abs() <= e + 2.0 ** -21 * l.abs()).all(), float((lse.double() - l).abs().max())
+    assert ((out.double() - want).abs() <= (3 * 2.0 ** -11 + 2 * e) * float(v.abs().max())).all()
+
+
+@pytest.mark.parametrize("D,H,KV", [(128, 4, 2), (64, 3, 3)])
+@pytest.mark.parametrize("window,sinks,observe", [(70, 0, 40), (130, 3, 9), (1, 1, 64), (0, 0, 30)])
+@pytest.mark.parametrize("Tq", [400, 150])
+def test_keys_that_nobody_sees_have_no_weight(qc, D, H, KV, window, sinks, observe, Tq):
+    """Exactly 0, whichever tile they lie in, so that of them an eviction keeps the lowest slots."""
+    lengths = [400, 300, 129]
+    q, k, v = make(3, Tq, 400, H, KV, D, 14)
+    out, lse = qc.attn_prefill(q, k, v, window=window, sinks=sinks, lengths=long(lengths))
+    w = qc.attn_prefill_weights(q, k, lse, window=window, sinks=sinks, lengths=long(lengths), observe=observe)
+    cache = qc.KVCache4.empty(3, KV, 416, D)
+    cache.write(None, k.reshape(-1, KV, D), v.reshape(-1, KV, D), torch.zeros(3, dtype=torch.long, device="cuda"))
+    keep = 200
+    kept, _, _ = cache.evict(torch.nn.functional.pad(w, (0, 16)), long(lengths), keep)
+    for b, n in enumerate(lengths):
+        m = seen(Tq, 400, n, window, sinks)
+        pos = torch.arange(Tq, device="cuda") + 400 - Tq
+        some = m[(pos >= n - observe) & (pos < n)].any(0)
+        assert (w[b][:, ~some] == 0).all() and (w[b][:, some] > 0).all()
+        if n > keep and int(some.sum()) <= keep:
+            slots = torch.cat([some.nonzero().flatten(), (~some).nonzero().flatten()])[:keep].sort().values
+            assert (kept[b].long() == slots).all()
