@@ -12,6 +12,7 @@
 #include <cmath>
 #include <cstddef>
 #include <cstring>
+#include <type_traits>
 
 #include "cq_kv4.cuh"
 #include "cq_umma.cuh"
@@ -869,20 +870,25 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
           wait_load<32>(x);
           const int p0 = place[c0 / 64] + c0 % 64;
           const bool whole = w.k0 + UM_TILE - 1 <= p0 && p0 + 32 <= w.last && (!s.window || w.k0 + UM_TILE - 1 < s.sinks || p0 + 31 - w.k0 < s.window);
-          if (!whole) {
-            const uint32_t vis = below32(hi + 1 - p0) & ~below32(lo - p0);
-#pragma unroll
-            for (int c = 0; c < 32; ++c) x[c] = vis >> c & 1u ? x[c] : 0xFF800000u;
-          }
           const ulonglong2* less = reinterpret_cast<const ulonglong2*>(mine + c0);
+          const uint32_t vis = below32(hi + 1 - p0) & ~below32(lo - p0);
+          // What is hidden is left out behind the subtraction of the lse: that of a query which does not see the key may be NaN.
+          auto add = [&](auto all) {
+            auto of = [&](int c, uint64_t x2, uint64_t m) {
+              const float2 f = apart(fma2(x2, scale22, m));
+              return decltype(all)::value ? f : make_float2(vis >> c & 1u ? f.x : -INFINITY, vis >> (c + 1) & 1u ? f.y : -INFINITY);
+            };
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            const ulonglong2 m = less[e / 2];
-            const float2 f = apart(fma2(two(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale22, m.x));
-            const float2 g = apart(fma2(two(__uint_as_float(x[2 * e + 2]), __uint_as_float(x[2 * e + 3])), scale22, m.y));
-            sum[0] = add2(sum[0], e % 8 < KW_POLY_OF_8 ? power2(f) : two(ex2(f.x), ex2(f.y)));
-            sum[1] = add2(sum[1], two(ex2(g.x), ex2(g.y)));
-          }
+            for (int e = 0; e < 16; e += 2) {
+              const ulonglong2 m = less[e / 2];
+              const float2 f = of(2 * e, two(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), m.x);
+              const float2 g = of(2 * e + 2, two(__uint_as_float(x[2 * e + 2]), __uint_as_float(x[2 * e + 3])), m.y);
+              sum[0] = add2(sum[0], e % 8 < KW_POLY_OF_8 ? power2(f) : two(ex2(f.x), ex2(f.y)));
+              sum[1] = add2(sum[1], two(ex2(g.x), ex2(g.y)));
+            }
+          };
+          if (whole) add(std::true_type());
+          else add(std::false_type());
         }
         fence_before();
         bar_arrive(s_free(st));

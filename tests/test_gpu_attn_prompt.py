@@ -330,3 +330,31 @@ def test_keys_that_nobody_sees_have_no_weight(qc, D, H, KV, window, sinks, obser
         if n > keep and int(some.sum()) <= keep:
             slots = torch.cat([some.nonzero().flatten(), (~some).nonzero().flatten()])[:keep].sort().values
             assert (kept[b].long() == slots).all()
+
+
+@pytest.mark.parametrize("D,H,KV", [(128, 4, 2), (64, 3, 3)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3), (150, 0)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_bad_lse_stays_with_the_keys_that_its_query_sees(qc, D, H, KV, window, sinks, bad):
+    q, k, v = make(2, 300, 340, H, KV, D, 15)
+    _, lse = qc.attn_prefill(q, k, v, window=window, sinks=sinks)
+    want = qc.attn_prefill_weights(q, k, lse, window=window, sinks=sinks)
+    lse[1, H - 1, 100] = bad
+    w = qc.attn_prefill_weights(q, k, lse, window=window, sinks=sinks)
+    m = seen(300, 340, 340, window, sinks)[100]
+    hit = torch.zeros_like(w, dtype=torch.bool)
+    hit[1, KV - 1] = m
+    assert torch.equal(w[~hit], want[~hit])
+    assert w[hit].isnan().all() if bad != bad else (w[hit] <= want[hit]).all()
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (50, 3)])
+def test_a_query_that_is_no_number_reaches_the_weights_of_its_keys(qc, window, sinks):
+    q, k, v = make(1, 300, 300, 4, 2, 128, 16)
+    _, lse = qc.attn_prefill(q, k, v, window=window, sinks=sinks)
+    want = qc.attn_prefill_weights(q, k, lse, window=window, sinks=sinks)
+    q[0, 130, 1] = math.nan
+    _, lse = qc.attn_prefill(q, k, v, window=window, sinks=sinks)
+    w = qc.attn_prefill_weights(q, k, lse, window=window, sinks=sinks)
+    m = seen(300, 300, 300, window, sinks)[130]
+    assert w[0, 0, m].isnan().all() and torch.equal(w[0, 0, ~m], want[0, 0, ~m]) and torch.equal(w[0, 1], want[0, 1])
