@@ -103,13 +103,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x of two numbers up to 2^7 on the multiply-add pipe: x = n + f with a whole n and |f| <= 1/2, by adding and taking away
+// 2^x of two numbers up to 2^7 (ANY: of any, infinity from 2^7 on) on the multiply-add pipe: x = n + f with a whole n and |f| <= 1/2, by adding and taking away
 // 1.5 * 2^23, then 2^f by the polynomial of degree 5 whose largest relative error is the least (2.1e-7 in fp32; coefficients by
 // Remez's exchange; degree 4 is 2.6e-6, which the weights of keys show, and takes 1 % off a prompt) and 2^n as a bit pattern.  x is held at -127, whose bit pattern is that of 0: below 2^-126.5 the
 // result is exactly 0, a masked score's of -infinity too (a row or key that sees nothing is known by a sum of 0).  NaN stays NaN.
-__device__ __forceinline__ uint64_t power2(float2 x) {
+template <bool ANY> __device__ __forceinline__ uint64_t power2(float2 x) {
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.f));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.f));
+  if (ANY) {
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(128.f));
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(128.f));
+  }
   const uint64_t v = two(x.x, x.y), big = two(12582912.f, 12582912.f), less = two(-12582912.f, -12582912.f);
   const uint64_t t = add2(v, big), f = fma2(add2(t, less), two(-1.f, -1.f), v);
   uint64_t p = fma2(f, two(0.0013276472454890609f, 0.0013276472454890609f), two(0.009675540961325169f, 0.009675540961325169f));
@@ -451,7 +455,7 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
               const float2 f = apart(fma2(two(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), scale22, minus2));
-              const uint64_t z = e % 8 < POLY_OF_8 ? power2(f) : two(ex2(f.x), ex2(f.y));
+              const uint64_t z = e % 8 < POLY_OF_8 ? power2<false>(f) : two(ex2(f.x), ex2(f.y));
               here = add2(here, z);
               const float2 g = apart(z);
               pr[c0 / 2 + e] = half_pair(g.x, g.y);
@@ -883,7 +887,7 @@ __global__ void __launch_bounds__(KW_THREADS, 1) prompt_keys_kernel(const __grid
               const ulonglong2 m = less[e / 2];
               const float2 f = of(2 * e, two(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), m.x);
               const float2 g = of(2 * e + 2, two(__uint_as_float(x[2 * e + 2]), __uint_as_float(x[2 * e + 3])), m.y);
-              sum[0] = add2(sum[0], e % 8 < KW_POLY_OF_8 ? power2(f) : two(ex2(f.x), ex2(f.y)));
+              sum[0] = add2(sum[0], e % 8 < KW_POLY_OF_8 ? power2<true>(f) : two(ex2(f.x), ex2(f.y)));
               sum[1] = add2(sum[1], two(ex2(g.x), ex2(g.y)));
             }
           };

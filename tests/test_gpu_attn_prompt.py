@@ -358,3 +358,24 @@ def test_a_query_that_is_no_number_reaches_the_weights_of_its_keys(qc, window, s
     w = qc.attn_prefill_weights(q, k, lse, window=window, sinks=sinks)
     m = seen(300, 300, 300, window, sinks)[130]
     assert w[0, 0, m].isnan().all() and torch.equal(w[0, 0, ~m], want[0, 0, ~m]) and torch.equal(w[0, 1], want[0, 1])
+
+
+@pytest.mark.parametrize("less,want", [(-math.inf, math.inf), (500.0, math.inf), (60.0, None)])
+def test_weights_beyond_one(qc, less, want):
+    """An lse that is not that of these scores: exp(score - lse) as it is, infinite beyond fp32."""
+    q, k, v = make(1, 300, 300, 4, 2, 128, 17)
+    _, lse = qc.attn_prefill(q, k, v, window=50)
+    clean = qc.attn_prefill_weights(q, k, lse, window=50)
+    low = lse.clone()
+    low[0, 1] = low[0, 1] - less if less > 0 else less
+    w = qc.attn_prefill_weights(q, k, low, window=50)
+    assert torch.equal(w[0, 1], clean[0, 1])
+    if want:
+        assert (w[0, 0] == want).all()
+        return
+    _, l, mass, big = reference(q, k, None, None, 50, 0)
+    other = reference(q[:, :, :1], k[:, :, :1], None, None, 50, 0)[2][0, 0]
+    full = other + (mass[0, 0] - other) * math.exp(less)
+    # the error of a score as in the other tests, and that of lse - 60, rounded to fp32
+    e = (128 + 8) * 2.0 ** -23 * big + 2.0 ** -20 + 2.0 ** -24 * (less + float(l.abs().max()))
+    assert ((w[0, 0].double() - full).abs() <= 3 * e * full).all()
