@@ -12,8 +12,9 @@ constexpr int WR_THREADS = 256, WR_TOKENS = 64;      // a block's rows of one he
 // D / 16 lanes a row of q, k or v: rotated (q and k), q to q_out, k and v quantised into their slots.  A block takes one head's
 // rows of as many tokens as it has rows of lanes, so that nothing is divided but block indices.  Bound by memory: 63 MB of rows of 40
 // heads and 34 MB of results, with reading them back 36 us.  (Two tokens a lane: 39, and 6.4 instead of 4.9 for 5 x 77 tokens; four
-// heads one after another, the angles kept in registers: 38 and 7.2.)
-template <int D, int GROUP>
+// heads one after another, the angles kept in registers: 38 and 7.2.  Tables that start off 8 bytes (PAIRS false) have an instance of their
+// own: a choice at run time costs the usual ones 24 -> 28 us of the rows' part.)
+template <int D, int GROUP, bool PAIRS>
 __global__ void __launch_bounds__(WR_THREADS, 6) kv4_write_kernel(
     const __half* __restrict__ q, __half* __restrict__ q_out, const __half* __restrict__ k, const __half* __restrict__ v,
     const float* __restrict__ cos_t, const float* __restrict__ sin_t, const long long* __restrict__ positions, int table_rows,
@@ -30,7 +31,7 @@ __global__ void __launch_bounds__(WR_THREADS, 6) kv4_write_kernel(
   kv4_load16(src, src + D / 2, x);
   const long long pos = cos_t ? positions[row] : 0, slot = is_q ? 0 : first[b] + t;
   const bool turn = cos_t && pos >= 0 && pos < table_rows;
-  if (turn && (is_q || is_k)) kv4_rotate(x, cos_t + pos * (D / 2) + c, sin_t + pos * (D / 2) + c);
+  if (turn && (is_q || is_k)) kv4_rotate<PAIRS>(x, cos_t + pos * (D / 2) + c, sin_t + pos * (D / 2) + c);
   if (is_q) {
     if (t >= tokens) return;
     __half* to = q_out + (row * H + head) * D + c;
@@ -295,9 +296,9 @@ __global__ void __launch_bounds__(WR_THREADS) kv4_gather_kernel(const MoveArgs a
 }
 
 // the instance for a cache's head width and group
-#define KV4_PICK(kernel, c)                                                                \
-  ((c)->head_dim == 128 ? ((c)->group == 32 ? kernel<128, 32> : kernel<128, 64>)           \
-                        : ((c)->group == 32 ? kernel<64, 32> : kernel<64, 64>))
+#define KV4_PICK(kernel, c, ...)                                                                                     \
+  ((c)->head_dim == 128 ? ((c)->group == 32 ? kernel<128, 32 __VA_ARGS__> : kernel<128, 64 __VA_ARGS__>)           \
+                        : ((c)->group == 32 ? kernel<64, 32 __VA_ARGS__> : kernel<64, 64 __VA_ARGS__>))
 
 }  // namespace
 
@@ -321,7 +322,9 @@ extern "C" int cq_kv4_write(const cq_kv4* cache, const void* q, void* q_out, con
   const long long kinds = n_heads + 2ll * cache->n_kv_heads;
   if (kinds > 65535) return CQ_ERR_BAD_SHAPE;
   const int rows = WR_THREADS / (cache->head_dim / 16);
-  CQ_CUDA_TRY(kv4_launch(KV4_PICK(kv4_write_kernel, cache), dim3((tokens + rows - 1) / rows, (unsigned)kinds, cache->sequences), dim3(WR_THREADS), 0,
+  const bool pairs = (((uintptr_t)cos_table | (uintptr_t)sin_table) & 7) == 0;
+  auto fn = pairs ? KV4_PICK(kv4_write_kernel, cache, , true) : KV4_PICK(kv4_write_kernel, cache, , false);
+  CQ_CUDA_TRY(kv4_launch(fn, dim3((tokens + rows - 1) / rows, (unsigned)kinds, cache->sequences), dim3(WR_THREADS), 0,
                          (cudaStream_t)stream, (const __half*)q, (__half*)q_out, (const __half*)k, (const __half*)v, cos_table, sin_table, positions,
                          table_rows, first, *cache, tokens, n_heads));
   return CQ_OK;

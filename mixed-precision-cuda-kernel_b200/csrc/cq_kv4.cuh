@@ -111,13 +111,17 @@ __device__ __forceinline__ void kv4_quantise(const uint32_t (&x)[8], uint32_t (&
 }
 
 // sixteen fp16 columns as kv4_quantise takes them, rotated by the angles of cos_p / sin_p (8 columns of the lower half):
-// products and sums rounded one by one, then to fp16, as rope_cache leaves a row
+// products and sums rounded one by one, then to fp16, as rope_cache leaves a row.  PAIRS: the tables start on 8 bytes (any 4 will do
+// without; rows of a prompt 24 us with, the single tokens' kernel is the same either way and reads them one by one)
+template <bool PAIRS>
 __device__ __forceinline__ void kv4_rotate(uint32_t (&x)[8], const float* __restrict__ cos_p, const float* __restrict__ sin_p) {
   const uint64_t minus = two(-1.f, -1.f);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint64_t a = kv4_two(x[i]), b = kv4_two(x[4 + i]);
-    const float2 cf = reinterpret_cast<const float2*>(cos_p)[i], sf = reinterpret_cast<const float2*>(sin_p)[i];
+    float2 cf, sf;
+    if (PAIRS) cf = reinterpret_cast<const float2*>(cos_p)[i], sf = reinterpret_cast<const float2*>(sin_p)[i];
+    else cf = make_float2(cos_p[2 * i], cos_p[2 * i + 1]), sf = make_float2(sin_p[2 * i], sin_p[2 * i + 1]);
     const uint64_t c = two(cf.x, cf.y), s = two(sf.x, sf.y);
     x[i] = kv4_pair(fma2(mul2(b, s), minus, mul2(a, c)));
     x[4 + i] = kv4_pair(add2(mul2(b, c), mul2(a, s)));

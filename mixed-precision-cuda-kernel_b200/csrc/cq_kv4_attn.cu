@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
     if (g < heads) {
       const __half* src = q + (head0 + g) * D + c;
       kv4_load16(src, src + D / 2, row);
-      if (turn) kv4_rotate(row, fresh.cos_t + pos * (D / 2) + c, fresh.sin_t + pos * (D / 2) + c);
+      if (turn) kv4_rotate<false>(row, fresh.cos_t + pos * (D / 2) + c, fresh.sin_t + pos * (D / 2) + c);
     }
     float x[16];
 #pragma unroll
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(WARPS * 32, AT_SM_WARPS / WARPS) kv4_attend_ke
     const __half* src = (which ? fresh.v : fresh.k) + ((size_t)b * cache.n_kv_heads + kvh) * D + c;
     uint32_t x[8];
     kv4_load16(src, src + D / 2, x);
-    if (!which && turn) kv4_rotate(x, fresh.cos_t + pos * (D / 2) + c, fresh.sin_t + pos * (D / 2) + c);
+    if (!which && turn) kv4_rotate<false>(x, fresh.cos_t + pos * (D / 2) + c, fresh.sin_t + pos * (D / 2) + c);
     uint32_t words[2], pairs[2];
     kv4_quantise<D, GROUP>(x, words, pairs);
     if (lane < 2 * LANES) {

@@ -480,3 +480,28 @@ def test_refusals(qc):
             call()
             pytest.fail(f"call {i} was taken")
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cos_off,sin_off", [(1, 1), (3, 2), (2, 2), (0, 1), (4, 0)])
+def test_tables_that_start_anywhere(qc, D, cos_off, sin_off):
+    """Views whose first number lies on any 4 bytes: the same rows, queries and outputs as with tables of their own."""
+    g = gen(20)
+    B, T, H, KV, S, P = 2, 19, 4, 2, 64, 50
+    cos, sin = randn(g, P, D // 2), randn(g, P, D // 2)
+
+    def view(x, off):
+        y = torch.empty(P * (D // 2) + off, device="cuda")[off:].view(P, D // 2)
+        return y.copy_(x)
+    a, b = qc.KVCache4.empty(B, KV, S, D), qc.KVCache4.empty(B, KV, S, D)
+    q, k, v = randn(g, B * T, H, D).half(), randn(g, B * T, KV, D).half(), randn(g, B * T, KV, D).half()
+    pos = torch.randint(0, P, (B * T,), device="cuda", generator=g)
+    qa = a.write(q, k, v, long([0, 3]), cos, sin, pos)
+    qb = b.write(q, k, v, long([0, 3]), view(cos, cos_off), view(sin, sin_off), pos)
+    assert torch.equal(qa, qb)
+    q, k, pos = randn(g, B, H, D).half(), randn(g, B, KV, D).half(), long([11, P - 1])
+    oa = a.step(q, k, k, cos, sin, pos, long([T, T + 3]))
+    ob = b.step(q, k, k, view(cos, cos_off), view(sin, sin_off), pos, long([T, T + 3]))
+    assert torch.equal(oa, ob)
+    for x, y in ((a.k_codes, b.k_codes), (a.k_scales, b.k_scales), (a.v_codes, b.v_codes), (a.v_scales, b.v_scales)):
+        assert torch.equal(x, y)
