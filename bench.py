@@ -1014,7 +1014,7 @@ def main():
     ap.add_argument("--kv-bits", type=int, default=16, choices=[16, 4], help="model workload: bits of the KV cache")
     ap.add_argument("--window", type=int, default=0, help="model workload, 4-bit cache: positions a query sees (0: all)")
     ap.add_argument("--sinks", type=int, default=0, help="model workload, 4-bit cache: first positions that stay visible")
-    ap.add_argument("--kv-budget", type=int, default=None, help="model workload, 4-bit cache: slots that stay where it is bounded")
+    ap.add_argument("--kv-budget", type=int, default=None, help="model workload, 4-bit cache: slots that stay where it is bounded (without --window)")
     ap.add_argument("--gather", default="peer", choices=["peer", "nccl"],
                     help="exchange step at N > 1: this library's peer-memory kernel (default) or NCCL")
     ap.add_argument("--repeats", type=int, default=50,

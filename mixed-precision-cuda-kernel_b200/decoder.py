@@ -28,7 +28,8 @@ draw the full random weight and pack only their rows.
 `KVCache4.step`, both with a sliding `window` and the first `sinks` positions visible if asked for.  `kv_budget` bounds the cache: a
 prompt's positions are weighed by its last `kv_observe` queries (`attn_prefill_weights`), every step adds what each slot
 received, and whenever the `kv_budget + kv_slack` slots of a layer are full the heaviest `kv_budget` stay (`KVCache4.evict`; the
-first `sinks` and the last `kv_recent` always do).  Keys keep the rotation of their own positions.
+first `sinks` and the last `kv_recent` always do).  Keys keep the rotation of their own positions.  Slots are not positions any more then,
+so that a `window` that hides any and `kv_budget` exclude one another.
 
 `dense=True` builds the parity twin: the same packed buffers, every projection computed as
 F.linear(x, unpack()) the way the reference's dense mode does (llama/qlinear.py:183-195).
@@ -112,6 +113,9 @@ class CherryDecoder:
             self.kv_recent = kv_budget // 4 if kv_recent is None else kv_recent
             if not (kv_budget > 0 and kv_slack > 0 and kv_observe > 0 and self.kv_recent >= 0 and sinks + self.kv_recent <= kv_budget):
                 raise ValueError("kv_budget must hold the sinks and the recent positions, and kv_slack and kv_observe be positive")
+            if 0 < window < cfg.max_seq:
+                # a step's window counts slots, which are positions only until the first eviction
+                raise ValueError("a window cannot be kept over a bounded cache (kv_budget), whose slots are not positions")
         self._flash = None
         grouped = cfg.n_heads // cfg.n_kv_heads
         if attention == "flash" or (attention == "auto" and kv_bits == 16 and cfg.max_seq > 1024 and

@@ -172,3 +172,17 @@ def test_refusals(dec):
     a.prefill(torch.zeros(100, dtype=torch.long, device="cuda"))
     with pytest.raises(ValueError):
         a.generate(200)
+
+
+def test_a_window_over_a_bounded_cache(dec):
+    """Slots of a bounded cache are not positions once some are evicted: a window that could hide any is refused there, one that spans
+    all positions changes nothing."""
+    cfg = tiny(dec)
+    for window in (1, 100, cfg.max_seq - 1):
+        with pytest.raises(ValueError, match="window"):
+            dec.CherryDecoder(cfg, kv_bits=4, kv_budget=32, kv_slack=16, window=window, sinks=2)
+    prompt = torch.randint(0, cfg.vocab, (60,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(4))
+    a = dec.CherryDecoder(cfg, seed=11, kv_bits=4, kv_budget=32, kv_slack=16, sinks=2)
+    b = dec.CherryDecoder(cfg, seed=11, kv_bits=4, kv_budget=32, kv_slack=16, sinks=2, window=cfg.max_seq)
+    assert torch.equal(a.prefill(prompt), b.prefill(prompt))
+    assert torch.equal(a.generate(50), b.generate(50))
