@@ -1024,6 +1024,8 @@ def main():
                     help="decode workload on another layer than the headline one, e.g. 28672x8192x3 (the 70B down "
                          "projection); for profiling: the line then names that layer as its workload")
     args = ap.parse_args()
+    if args.kv_bits == 16 and (args.window or args.sinks or args.kv_budget is not None):
+        ap.error("--window, --sinks and --kv-budget belong to the 4-bit cache: give --kv-bits 4")
     if args.shape:
         global K_IN, N_OUT, BITS, WORKLOAD
         K_IN, N_OUT, BITS = (int(v) for v in args.shape.lower().split("x"))

@@ -55,3 +55,18 @@ def test_region_partition_covers_exactly_the_requested_steps(bench):
 def test_median_and_thread_count(bench):
     assert bench.median([3.0, 1.0, 2.0]) == 2.0
     assert 1 <= bench.host_threads() <= 32
+
+
+@pytest.mark.parametrize("options", [["--window", "64"], ["--sinks", "4"], ["--kv-budget", "1024"], ["--kv-bits", "16", "--kv-budget", "0"]])
+def test_options_of_the_4_bit_cache_are_not_dropped(bench, options, monkeypatch, capsys):
+    """Without --kv-bits 4 they would measure the fp16 cache under another name."""
+    ran = []
+    for name in ("run_model", "run_ours", "run_prefill", "run_sweep"):
+        monkeypatch.setattr(bench, name, ran.append)
+    monkeypatch.setattr("sys.argv", ["bench.py", "--workload", "model", *options])
+    with pytest.raises(SystemExit) as stop:
+        bench.main()
+    assert stop.value.code == 2 and not ran and "--kv-bits 4" in capsys.readouterr().err
+    monkeypatch.setattr("sys.argv", ["bench.py", "--workload", "model", "--kv-bits", "4", *options[-2:]])
+    bench.main()
+    assert len(ran) == 1 and bench.cache_options(ran[0])["kv_bits"] == 4
