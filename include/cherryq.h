@@ -327,7 +327,7 @@ int cq_kv4_step(const cq_kv4* cache, const void* q_f16, const void* k_f16, const
  * in their order; all of them where n <= keep, and where sinks + recent > keep the first min(sinks, keep) and the last of those.
  * Their rows go to the first slots of `to` (zeros up to `keep`), which has the same shape up to its slots, and is `from` itself
  * or shares no memory with it; their numbers to kept (sequences, KV, keep) int32 (-1 behind them), their weights to weights_out
- * (sequences, KV, keep) (0 behind them), min(n, keep) to length_out.
+ * (sequences, KV, keep) (0 behind them), min(n, keep) to length_out; these three share no memory with weights and length.
  * workspace: only where to is from, cq_kv4_evict_workspace_bytes(from, keep) bytes, 16-byte aligned. */
 size_t cq_kv4_evict_workspace_bytes(const cq_kv4* cache, int keep);
 int cq_kv4_evict(const cq_kv4* from, const cq_kv4* to, const float* weights, float* weights_out, const long long* length,

@@ -2,6 +2,7 @@
 // reference the cache is the fp16 key and value tensors of its vendored LLaMA (llama/modeling_llama_quant.py:371-419 of the
 // reference project).
 #include <algorithm>
+#include <utility>
 
 #include "cq_kv4.cuh"
 
@@ -363,6 +364,15 @@ extern "C" int cq_kv4_evict(const cq_kv4* from, const cq_kv4* to, const float* w
     if ((fp[i] == tp[i]) != in_place) return CQ_ERR_BAD_ARG;
   if (in_place && (from->slots != to->slots || !workspace || ((uintptr_t)workspace & 15))) return CQ_ERR_BAD_ARG;
   const int B = from->sequences, KV = from->n_kv_heads, D = from->head_dim;
+  const size_t heads = (size_t)B * KV, row_bytes[2] = {(size_t)D / 2, 4 * (size_t)(D / from->group)};
+  for (int i = 0; i < 4 && !in_place; ++i)
+    for (int j = 0; j < 4; ++j)
+      if (!kv4_apart(tp[i], heads * to->slots * row_bytes[i & 1], fp[j], heads * from->slots * row_bytes[j & 1])) return CQ_ERR_BAD_ARG;
+  const std::pair<const void*, size_t> in[2] = {{weights, heads * from->slots * 4}, {length, (size_t)B * 8}},
+                                       res[3] = {{weights_out, heads * keep * 4}, {length_out, (size_t)B * 8}, {kept, heads * keep * 4}};
+  for (const auto& r : res)
+    for (const auto& i : in)
+      if (!kv4_apart(r.first, r.second, i.first, i.second)) return CQ_ERR_BAD_ARG;
   // The passes of a head are a chain: many threads for many slots, fewer for short ones or where heads fill the SMs anyway.  (With the
   // move, 256 / 512 / 1024 threads: 32 heads of 200 slots 5.9 / 6.1 / 6.7 us, 1000 9.3 / 7.4 / 7.5, 4000 24 / 20 / 13; 1080 heads of 200
   // 9.6 / 13.7 / 23.7, of 1000 36 / 38 / 45, of 4000 119 / 121 / 130.)

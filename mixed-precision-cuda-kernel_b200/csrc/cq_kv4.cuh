@@ -144,6 +144,11 @@ __device__ __forceinline__ uint4 kv4_halves(const float* x) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// whether a and b, that many bytes each, share none
+inline bool kv4_apart(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+  return (uintptr_t)a + a_bytes <= (uintptr_t)b || (uintptr_t)b + b_bytes <= (uintptr_t)a;
+}
+
 template <typename... KArgs, typename... Args>
 cudaError_t kv4_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
   cudaLaunchConfig_t cfg = {};

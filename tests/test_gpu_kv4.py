@@ -505,3 +505,17 @@ def test_tables_that_start_anywhere(qc, D, cos_off, sin_off):
     assert torch.equal(oa, ob)
     for x, y in ((a.k_codes, b.k_codes), (a.k_scales, b.k_scales), (a.v_codes, b.v_codes), (a.v_scales, b.v_scales)):
         assert torch.equal(x, y)
+
+
+def test_evict_into_a_cache_that_overlaps(qc):
+    """A handle over the same storage, one sequence on: refused, where the rows would be moved over rows still to be read."""
+    make = lambda *s, **o: torch.zeros(*s, device="cuda", **o)
+    codes, scales = dict(dtype=torch.uint8), dict(dtype=torch.float16)
+    t = make(3, 2, 64, 64, **codes), make(3, 2, 64, 4, 2, **scales), make(3, 2, 64, 64, **codes), make(3, 2, 64, 4, 2, **scales)
+    a, b, c = qc.KVCache4(*(x[:2] for x in t)), qc.KVCache4(*(x[1:] for x in t)), qc.KVCache4(*(x[:2] for x in t))
+    w, n = torch.ones(2, 2, 64, device="cuda"), long([64, 64])
+    with pytest.raises(RuntimeError):
+        a.evict(w, n, 16, out=b)
+    with pytest.raises(RuntimeError):
+        a.evict(w, n, 16, out=qc.KVCache4(t[0][:2], *(x.clone() for x in (t[1][:2], t[2][:2], t[3][:2]))))
+    assert a.evict(w, n, 16, out=c)[2].tolist() == [16, 16]            # the same cache by another handle: in place

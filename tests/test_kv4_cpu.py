@@ -98,3 +98,22 @@ def test_prompt_calls(lib):
         assert lib.cq_attn_prefill(C.byref(s), *a, at, None, None) == BAD_ARG
     for a in ((None, at, at, None, 4, at), (at, at, None, None, 4, at), (at, at, at, None, 0, at), (at, at, at, None, 4, None)):
         assert lib.cq_attn_prefill_weights(C.byref(s), *a, at, None, None) == BAD_ARG
+
+
+def test_evict_into_memory_of_its_own(lib):
+    """Another cache, and the results, must share no memory with what is read: codes of 16384 bytes, scales of 4096, weights of 1024."""
+    c, at = cache(), lambda n: C.c_void_p((1 << 28) + n)
+
+    def evict(to, w=at(0), left=at(1 << 16), n=at(2 << 16), now=at(3 << 16), kept=at(4 << 16)):
+        return lib.cq_kv4_evict(C.byref(c), C.byref(to), w, left, n, now, 8, 0, 0, kept, at(5 << 16), None)
+    apart = dict(k_codes=5 << 20, k_scales=6 << 20, v_codes=7 << 20, v_scales=9 << 20)
+    for field, address in (("k_codes", (1 << 20) + 16384 - 16), ("k_codes", (1 << 20) - 16384 + 16), ("v_codes", (1 << 20) + 64), ("k_scales", (1 << 22) + 16),
+                           ("v_scales", (1 << 23) + 4096 - 16), ("v_scales", (1 << 21) - 4096 + 16)):
+        assert evict(cache(**{**apart, field: address})) == BAD_ARG, (field, hex(address))
+    to = cache(**apart)
+    for bad in (dict(left=at(0)), dict(left=at(1020)), dict(left=at(-124)), dict(now=at(2 << 16)), dict(now=at((2 << 16) + 8)), dict(now=at((2 << 16) - 8)),
+                dict(kept=at(0)), dict(kept=at(2 << 16))):
+        assert evict(to, **bad) == BAD_ARG, bad
+    # side by side is apart, and in place is in place
+    for fine in (cache(**{**apart, "k_codes": (1 << 20) + 16384}), cache(**{**apart, "v_scales": (1 << 21) - 4096}), c):
+        assert evict(fine, left=at(1024)) not in (0, BAD_ARG, BAD_SHAPE, UNSUPPORTED)      # (no device to launch on)
