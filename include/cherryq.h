@@ -309,7 +309,7 @@ int cq_kv4_write(const cq_kv4* cache, const void* q_f16, void* q_out_f16, const 
 int cq_kv4_read(const cq_kv4* cache, const long long* first, int count, void* k_f16, void* v_f16, cq_stream_t stream);
 /* Attention of one query per sequence: out (sequences, n_heads, D) = softmax(scale * q . k_j) . v_j over the visible slots
  * j < n = length[s] (device int64, bounded by the cache): all of them (window 0), or those with j < sinks or j >= n - window.
- * Nothing visible: zeros.  weights, weights_out (sequences, KV, slots) fp32, both or neither, possibly the same:
+ * Nothing visible: zeros.  weights, weights_out (sequences, KV, slots) fp32, both or neither, the same or apart:
  * weights_out = weights + the sum over the head's queries of their softmax weights for j < n, and 0 from n on.
  * workspace: device memory of cq_kv4_attend_workspace_bytes(...) bytes (may be NULL where that is 0), 16-byte aligned, not
  * shared by calls that can overlap. */

@@ -723,6 +723,8 @@ int check(const cq_kv4* cache, const void* q, const long long* length, const voi
   if (!q || !length || !out || window < 0 || sinks < 0 || (!weights != !weights_out)) return CQ_ERR_BAD_ARG;
   if (n_heads < 1 || n_heads % cache->n_kv_heads || (n_heads + 7ll * cache->n_kv_heads) / 8 > 65535) return CQ_ERR_BAD_SHAPE;
   if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)weights | (uintptr_t)weights_out | (uintptr_t)workspace) & 15) return CQ_ERR_BAD_ARG;
+  const size_t bytes = (size_t)cache->sequences * cache->n_kv_heads * cache->slots * 4;
+  if (weights != weights_out && !kv4_apart(weights, bytes, weights_out, bytes)) return CQ_ERR_BAD_ARG;
   if (!workspace && cq_kv4_attend_workspace_bytes(cache, n_heads, window, sinks, weights != nullptr)) return CQ_ERR_BAD_ARG;
   return CQ_OK;
 }

@@ -519,3 +519,13 @@ def test_evict_into_a_cache_that_overlaps(qc):
     with pytest.raises(RuntimeError):
         a.evict(w, n, 16, out=qc.KVCache4(t[0][:2], *(x.clone() for x in (t[1][:2], t[2][:2], t[3][:2]))))
     assert a.evict(w, n, 16, out=c)[2].tolist() == [16, 16]            # the same cache by another handle: in place
+
+
+def test_weights_over_themselves_or_apart(qc):
+    g = gen(21)
+    cache = filled(qc, g, 1, 2, 64, 64, 32)
+    q, n, w = randn(g, 1, 4, 64).half(), long([50]), torch.zeros(3, 2, 64, device="cuda")
+    with pytest.raises(RuntimeError):
+        cache.attend(q, n, weights=w.flatten()[:128].view(1, 2, 64), weights_out=w.flatten()[64:192].view(1, 2, 64))
+    out = cache.attend(q, n, weights=w[:1], weights_out=w[1:2])
+    assert torch.equal(out, cache.attend(q, n, weights=w[:1])) and torch.equal(w[0], w[1]) and (w[2] == 0).all()

@@ -117,3 +117,15 @@ def test_evict_into_memory_of_its_own(lib):
     # side by side is apart, and in place is in place
     for fine in (cache(**{**apart, "k_codes": (1 << 20) + 16384}), cache(**{**apart, "v_scales": (1 << 21) - 4096}), c):
         assert evict(fine, left=at(1024)) not in (0, BAD_ARG, BAD_SHAPE, UNSUPPORTED)      # (no device to launch on)
+
+
+def test_weights_over_themselves_or_apart(lib):
+    """weights_out is weights or shares no memory with it (1024 bytes each)."""
+    c, at = cache(), C.c_void_p(1 << 24)
+    for off in (16, -16, 1008, -1008):
+        wo = C.c_void_p((1 << 25) + off)
+        assert lib.cq_kv4_attend(C.byref(c), at, at, at, 4, 0, 0, C.c_float(1.0), C.c_void_p(1 << 25), wo, at, None) == BAD_ARG
+        assert lib.cq_kv4_step(C.byref(c), at, at, at, None, None, None, 0, at, at, 4, 0, 0, C.c_float(1.0), C.c_void_p(1 << 25), wo, at, None) == BAD_ARG
+    for off in (0, 1024, -1024):
+        rc = lib.cq_kv4_attend(C.byref(c), at, at, at, 4, 0, 0, C.c_float(1.0), C.c_void_p(1 << 25), C.c_void_p((1 << 25) + off), at, None)
+        assert rc not in (0, BAD_ARG, BAD_SHAPE, UNSUPPORTED)          # (no device to launch on)
