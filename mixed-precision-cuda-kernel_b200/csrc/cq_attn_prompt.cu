@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
 #pragma unroll
         for (int e = 0; e < 16; ++e) all[e & 1] = add2(all[e & 1], two(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1])));
         const float2 any = apart(add2(all[0], all[1]));
-        if (any.x != any.x || any.y != any.y) s_nan[warp] = 1;
+        if (!empty && (any.x != any.x || any.y != any.y)) s_nan[warp] = 1;      // (an empty row's sums may be anything)
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
           uint32_t v[4];

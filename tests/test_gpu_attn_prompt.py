@@ -379,3 +379,30 @@ def test_weights_beyond_one(qc, less, want):
     # the error of a score as in the other tests, and that of lse - 60, rounded to fp32
     e = (128 + 8) * 2.0 ** -23 * big + 2.0 ** -20 + 2.0 ** -24 * (less + float(l.abs().max()))
     assert ((w[0, 0].double() - full).abs() <= 3 * e * full).all()
+
+
+def test_padding_that_is_no_number_takes_no_time(qc):
+    """Rows behind a prompt's end are zeros whatever they hold; that theirs are NaN is no reason to look at rows again (twice the time)."""
+    q, k, v = make(4, 1000, 1000, 64, 8, 128, 18)
+    ends = [1000, 700, 300, 77]
+
+    def median():
+        for _ in range(3):
+            qc.attn_prefill(q, k, v, lengths=long(ends))
+        took = []
+        for _ in range(15):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            n = long(ends)
+            a.record()
+            for _ in range(5):
+                out, _ = qc.attn_prefill(q, k, v, lengths=n)
+            b.record()
+            torch.cuda.synchronize()
+            took.append(a.elapsed_time(b))
+        return sorted(took)[7], out
+    finite, want = median()
+    for b, n in enumerate(ends):
+        q[b, n:] = k[b, n:] = v[b, n:] = math.nan
+    padded, out = median()
+    assert torch.equal(out, want)
+    assert padded <= 1.4 * finite, (finite, padded)
