@@ -186,3 +186,58 @@ def test_a_window_over_a_bounded_cache(dec):
     b = dec.CherryDecoder(cfg, seed=11, kv_bits=4, kv_budget=32, kv_slack=16, sinks=2, window=cfg.max_seq)
     assert torch.equal(a.prefill(prompt), b.prefill(prompt))
     assert torch.equal(a.generate(50), b.generate(50))
+
+
+@pytest.mark.parametrize("options", [dict(), dict(window=20, sinks=2), dict(kv_budget=32, kv_slack=16, sinks=2, kv_recent=8, kv_observe=16)])
+def test_two_ranks_of_a_group(dec, options, monkeypatch):
+    """Each rank keeps the cache of its own heads.  Both ranks run on one device, a thread each, one behind the other on its stream; their
+    slices meet on the host's side.  One layer, so that all sides quantise the same rows (see above)."""
+    import threading
+    cfg = tiny(dec, layers=1)
+    prompt = torch.randint(0, cfg.vocab, (2, 45), device="cuda", generator=torch.Generator(device="cuda").manual_seed(6))
+
+    def run(model, tokens):
+        logits = [model.prefill(prompt).clone()]
+        for i in range(40):
+            if i < len(tokens):
+                model.tok.copy_(tokens[i])
+            else:
+                tokens.append(model.tok.clone())
+            model._kv4_room()
+            logits.append(model._step().clone())
+        return logits
+
+    tokens = []
+    want = run(dec.CherryDecoder(cfg, seed=5, batch=2, kv_bits=4, **options), tokens)
+    monkeypatch.setattr("torch.distributed.get_world_size", lambda group: 2)
+    monkeypatch.setattr("torch.distributed.get_rank", lambda group: group)
+    ranks = [dec.CherryDecoder(cfg, seed=5, batch=2, kv_bits=4, tp_group=r, tp_gather="nccl", **options) for r in (0, 1)]
+    slices, meet, got = [None, None], threading.Barrier(2, timeout=60), [None, None]
+
+    def gather(r):
+        def call(x):
+            slices[r] = x
+            meet.wait()
+            both = torch.cat(slices, 1)
+            meet.wait()
+            return both
+        return call
+
+    def work(r):
+        try:
+            got[r] = run(ranks[r], list(tokens))
+        except BaseException:
+            meet.abort()
+            raise
+    for r in (0, 1):
+        ranks[r]._gather = gather(r)
+        assert ranks[r].caches[0].n_kv_heads == cfg.n_kv_heads // 2
+    threads = [threading.Thread(target=work, args=(r,)) for r in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for r in (0, 1):
+        assert len(got[r]) == len(want)
+        for x, y in zip(got[r], want):
+            assert float((x.float() - y.float()).abs().max()) <= 2e-2 * float(y.float().abs().max())
