@@ -317,7 +317,8 @@ size_t cq_kv4_attend_workspace_bytes(const cq_kv4* cache, int n_heads, int windo
 int cq_kv4_attend(const cq_kv4* cache, const void* q_f16, const long long* length, void* out_f16, int n_heads, int window,
                   int sinks, float scale, const float* weights, float* weights_out, void* workspace, cq_stream_t stream);
 /* One decode step: cq_kv4_write of one token per sequence at slot length[s], then cq_kv4_attend over n = length[s] + 1 slots
- * (q is not changed; the new slot's weight starts at 0; the caller counts length up). */
+ * (q is not changed; the new slot's weight starts at 0; the caller counts length up).  n counts the new slot also where its row is left out
+ * for its position: what the slot held is attended then. */
 int cq_kv4_step(const cq_kv4* cache, const void* q_f16, const void* k_f16, const void* v_f16, const float* cos_table,
                 const float* sin_table, const long long* positions, int table_rows, const long long* length, void* out_f16,
                 int n_heads, int window, int sinks, float scale, const float* weights, float* weights_out, void* workspace,
@@ -350,8 +351,8 @@ size_t cq_attn_prefill_workspace_bytes(const cq_prompt* shape);
 int cq_attn_prefill(const cq_prompt* shape, const void* q_f16, const void* k_f16, const void* v_f16, const long long* lengths,
                     void* out_f16, float* lse, void* workspace, uint32_t* status_word, cq_stream_t stream);
 /* The weight that each key received from the last `observe` positions of its sequence (of those that are among the queries):
- * weights (sequences, n_kv_heads, keys) fp32 = sum over them and the head's queries of exp(scale * q . k_j - lse); 0 where no
- * such query sees the key.  workspace: device memory of cq_attn_prefill_weights_workspace_bytes(...) bytes, not shared by
+ * weights (sequences, n_kv_heads, keys) fp32 = sum over them and the head's queries of exp(scale * q . k_j - lse); exactly 0 where
+ * no such query sees the key.  An lse that is no number reaches the keys that its query sees.  workspace: device memory of cq_attn_prefill_weights_workspace_bytes(...) bytes, not shared by
  * calls that can overlap. */
 size_t cq_attn_prefill_weights_workspace_bytes(const cq_prompt* shape, int observe);
 int cq_attn_prefill_weights(const cq_prompt* shape, const void* q_f16, const void* k_f16, const float* lse,

@@ -64,8 +64,9 @@ __device__ __forceinline__ int length_of(const PromptArgs& a, int b) {
 // fp16 (2^-11 of each weight; the row sum is of the unrounded ones, in fp32).
 // Bound by the softmax phases: 2000 cycles for a tile with a warp a scheduler, and a tile's next scores wait for its weights, in whose
 // place they go; two tiles by 128 keys take 3900 cycles, their MMAs alone 2160.  8192 tokens of 32 heads 1.03 PFLOP/s, 2048 of 40 heads
-// 65 us, 8192 of 64 / 8 heads with a window of 2048 518 us (603 once the power cap holds the clock at 1.69 GHz).  Sixteen softmax warps
-// of half a row spill (0.69 to 0.92), two MMA warps 0.83, two score buffers of 64 keys 0.50 to 0.61.
+// 65 us, 8192 of 64 / 8 heads with a window of 2048 527 us in a burst, 610 once the power cap holds the clock at 1.69 GHz (normal
+// random inputs).  Keys with a few columns four times as large, whose scores make rows raise their reference and take tiles twice: 75, 654 and
+// 690 us.  Sixteen softmax warps of half a row spill (0.69 to 0.92 PFLOP/s), two MMA warps 0.83, two score buffers of 64 keys 0.50 to 0.61.
 constexpr int UM_THREADS = 320, UM_TILE = 128, UM_STAGES = 4, UM_CHUNK = 64 * 128 * 2;      // bytes of 64 columns of a tile
 constexpr int W_LOAD = 8, W_MMA = 9;
 constexpr int POLY_OF_8 = 1;                      // of eight pairs of exponentials, how many are polynomials
@@ -662,11 +663,11 @@ PromptForm prompt_form(const cq_prompt* s) {
 //   warps 0-15  four groups, every fourth tile each: sums of exponentials, joined by the group with an item's last tile
 //   warp 16     TMA of K, Q;  warp 17  MMAs, up to four score buffers ahead
 // (Two groups that met at every item's end were 47.6 us for 2048 tokens of 40 heads of 128 and 490 for 8192 of 64 / 8 heads with
-// window and sinks, four are 37.2 and 366: two warps a scheduler leave most of their instructions' latency open.)
+// window and sinks, four are 36 and 363: two warps a scheduler leave most of their instructions' latency open.)
 constexpr int KW_GROUPS = 4, KW_THREADS = 128 * KW_GROUPS + 64, KW_Q = 64, KW_BUFFERS = 4;
 constexpr int KW_LOAD = 4 * KW_GROUPS, KW_MMA = KW_LOAD + 1, KW_SLOTS = 12;
 static_assert(KW_GROUPS == KW_BUFFERS, "a group's tiles come in one buffer");
-constexpr int KW_POLY_OF_8 = 2;
+constexpr int KW_POLY_OF_8 = 1;                   // as POLY_OF_8
 
 // An item: 128 keys of a KV head, the queries [first, last) of its heads in blocks of 64, and of those one of `parts` parts
 struct KeysItem {

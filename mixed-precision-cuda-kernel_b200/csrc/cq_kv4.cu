@@ -11,8 +11,9 @@ namespace {
 constexpr int WR_THREADS = 256, WR_TOKENS = 64;      // a block's rows of one head (reads, moves)
 
 // D / 16 lanes a row of q, k or v: rotated (q and k), q to q_out, k and v quantised into their slots.  A block takes one head's
-// rows of as many tokens as it has rows of lanes, so that nothing is divided but block indices.  Bound by memory: 63 MB of rows of 40
-// heads and 34 MB of results, with reading them back 36 us.  (Two tokens a lane: 39, and 6.4 instead of 4.9 for 5 x 77 tokens; four
+// rows of as many tokens as it has rows of lanes, so that nothing is divided but block indices.  63 MB of rows of 40 heads and
+// 34 MB of results take 24 us, 4.0 TB/s, with reading them back 36: neither memory (DRAM 30 % busy under ncu, much of the results still in
+// L2) nor instructions (62 % of the cycles issue one) are full, and warps wait for their loads (6.6 of 16 cycles an issue).  (Two tokens a lane: 39, and 6.4 instead of 4.9 for 5 x 77 tokens; four
 // heads one after another, the angles kept in registers: 38 and 7.2.  Tables that start off 8 bytes (PAIRS false) have an instance of their
 // own: a choice at run time costs the usual ones 24 -> 28 us of the rows' part.)
 template <int D, int GROUP, bool PAIRS>

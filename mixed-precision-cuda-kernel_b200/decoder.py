@@ -21,7 +21,8 @@ scaled_dot_product_attention.  Both are plumbing here, not the measured path.
 (column parallel: heads for q / k / v, output features for o / gate / up / down) and gathers the
 slices with an NCCL all-gather where the next op needs the whole vector (attention output, o,
 SwiGLU output, down): four collectives per layer.  Every output element is still computed by
-exactly the single-GPU arithmetic, so the tokens are identical for every group size; all ranks
+exactly the single-GPU arithmetic, so the tokens are identical for every group size (with the 4-bit
+cache up to the rounding of attention's sums, whose split goes by the heads of a rank); all ranks
 draw the full random weight and pack only their rows.
 
 `kv_bits=4` keeps keys and values in 4 bits (`quant_cuda.KVCache4`): prompts go through `attn_prefill`, steps through
