@@ -285,7 +285,8 @@ int cq_silu_mul_full(const void* gate_f16, const void* up_f16, void* out_f16, lo
  * A row is one slot of one KV head: D codes of 4 bits (the even column of a byte in its low half) and
  * for every `group` columns a pair (scale, minimum) fp16; a column stands for scale * code + minimum.
  *   minimum = min x, scale = fp16((max x - minimum) / 15), code = rint((x - minimum) / scale) in 0..15
- * (0 where the scale is 0; a group with an infinite or NaN column is NaN as a whole).
+ * (0 where the scale is 0; a group with an infinite or NaN column is NaN as a whole; the scale is the fp16 number below that
+ * where minimum + 15 scale would round beyond fp16, so that finite rows stay finite).
  * Codes are (sequences, n_kv_heads, slots, D / 2) bytes, scales (sequences, n_kv_heads, slots,
  * D / group, 2) fp16, all 16-byte aligned and contiguous.  head_dim 64 or 128, group 32 or 64, slots a
  * multiple of 32.  Calls that write the cache or its workspace must not overlap other calls on it.

@@ -55,7 +55,8 @@ __device__ __forceinline__ uint32_t kv4_max2(uint32_t a, uint32_t b) {
 
 // Quantises one row that LANES = D / 16 neighbouring lanes hold, 8 columns of the lower half of the head and the same 8 of the
 // upper half each (x[0..3] at 8 * lane, x[4..7] at D / 2 + 8 * lane, two fp16 numbers a word).  minimum = min x, scale =
-// fp16((max x - minimum) / 15), code = rint((x - minimum) / scale) within 0..15, and 0 where the scale is 0.  A group with an
+// fp16((max x - minimum) / 15) (the fp16 number below it where 15 of them would leave fp16), code = rint((x - minimum) / scale)
+// within 0..15, and 0 where the scale is 0.  A group with an
 // infinite or NaN column cannot be kept in 4 bits: it is NaN as a whole (scale 0, minimum NaN), so that nothing finite comes
 // of it.  words: the two words of codes; pairs: scale | minimum << 16 of the groups of the two halves.
 template <int D, int GROUP>
@@ -82,7 +83,10 @@ __device__ __forceinline__ void kv4_quantise(const uint32_t (&x)[8], uint32_t (&
     const float2 e = __half22float2(*reinterpret_cast<const __half2*>(&ends[h]));      // (-min, max)
     // Quotients as the division rounds them, by one residual step after the product with the reciprocal (Markstein).
     const float range = __fadd_rn(e.y, e.x), q15 = __fmul_rn(range, 1.f / 15.f);
-    const __half s16 = bad ? __ushort_as_half(0) : __float2half_rn(__fmaf_rn(__fmaf_rn(-q15, 15.f, range), 1.f / 15.f, q15));
+    const __half near16 = __float2half_rn(__fmaf_rn(__fmaf_rn(-q15, 15.f, range), 1.f / 15.f, q15));
+    // code 15 would stand for 65520 or more, which fp16 rounds to infinity: the next lower scale is below range / 15
+    const bool beyond = __fmaf_rn(15.f, __half2float(near16), -e.x) >= 65520.f;
+    const __half s16 = __ushort_as_half(bad ? 0 : (unsigned short)(__half_as_ushort(near16) - beyond));
     const float s = __half2float(s16);
     pairs[h] = (uint32_t)__half_as_ushort(s16) | (bad ? 0x7FFF0000u : (ends[h] ^ 0x8000u) << 16);
     uint32_t w = 0;

@@ -529,3 +529,29 @@ def test_weights_over_themselves_or_apart(qc):
         cache.attend(q, n, weights=w.flatten()[:128].view(1, 2, 64), weights_out=w.flatten()[64:192].view(1, 2, 64))
     out = cache.attend(q, n, weights=w[:1], weights_out=w[1:2])
     assert torch.equal(out, cache.attend(q, n, weights=w[:1])) and torch.equal(w[0], w[1]) and (w[2] == 0).all()
+
+
+@pytest.mark.parametrize("low", [-65504.0, -8000.0, 0.0, 4000.0])
+@pytest.mark.parametrize("D,group", [(128, 32), (64, 64)])
+def test_the_largest_values_stay_finite(qc, low, D, group):
+    """Groups that reach to fp16's end: code 15 stands for no infinity, a column is at most half a step off, and attention over such
+    values is what it is over the values that were kept."""
+    g = gen(22)
+    KV, n = 2, 40
+    cache = qc.KVCache4.empty(1, KV, 64, D, group)
+    v = (low + (65504.0 - low) * torch.rand(n, KV, D, device="cuda", generator=g)).half()
+    v[..., ::group], v[..., 1::group] = 65504.0, low
+    k = randn(g, n, KV, D).half()
+    cache.write(None, k, v, long([0]))
+    _, rv = cache.read(long([0]), n)
+    assert rv.isfinite().all()
+    step = (65504.0 - low) / 15
+    # the scale may be 2^-11 of itself off, upwards or downwards, fifteen times, or one step of fp16 where it was lowered; then one rounding
+    assert ((rv[0].double() - v.double()).abs() <= 0.5 * step * (1 + 2.0 ** -10) + 15 * step * 2.0 ** -10 + 16).all()
+    q = randn(g, 1, 4, D).half()
+    out = cache.attend(q, long([n]))
+    want, _, _ = attend_ref(cache, q, [n], 0, 0)
+    assert out.isfinite().all() and ((out.double() - want).abs() <= value_bound(cache, [n], 0, 0)).all()
+    other = qc.KVCache4.empty(1, KV, 64, D, group)
+    other.step(q, k[:1], v[:1], None, None, None, long([0]))
+    assert torch.equal(other.v_codes[:, :, 0], cache.v_codes[:, :, 0]) and torch.equal(other.v_scales[:, :, 0], cache.v_scales[:, :, 0])
