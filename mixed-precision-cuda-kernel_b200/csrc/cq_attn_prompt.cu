@@ -131,6 +131,10 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// A mean of finite values is none of fp16's infinities, but where they are near its largest number the weights' roundings can carry it there.
+constexpr float LARGEST = 65504.f;
+__device__ __forceinline__ float within(float x, float most) { return fabsf(x) < INFINITY ? fminf(fmaxf(x, -most), most) : x; }
+
 // which of the 32 keys from `first` on a query sees that sees lo .. hi and those below `sinks`: a bit each
 __device__ __forceinline__ uint32_t below32(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u); }
 __device__ __forceinline__ uint32_t visible32(int first, int lo, int hi, int sinks) {
@@ -530,6 +534,12 @@ __global__ void __launch_bounds__(UM_THREADS, 1) prompt_kernel(const __grid_cons
         for (int e = 0; e < 16; ++e) all[e & 1] = add2(all[e & 1], two(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1])));
         const float2 any = apart(add2(all[0], all[1]));
         if (!empty && (any.x != any.x || any.y != any.y)) s_nan[warp] = 1;      // (an empty row's sums may be anything)
+        float most = 0.f;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) most = fmaxf(most, fabsf(__uint_as_float(y[e])));
+        if (most * inv > LARGEST)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(within(__uint_as_float(y[e]), LARGEST * total));
 #pragma unroll
         for (int e = 0; e < 32; e += 8) {
           uint32_t v[4];
@@ -581,7 +591,8 @@ __global__ void __launch_bounds__(256) prompt_sum_kernel(const __grid_constant__
   const bool empty = sum == 0.f;
   const float inv = empty ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int i = 0; i < C; i += 2) *reinterpret_cast<uint32_t*>(out + row * D + C * lane + i) = half_pair(y[i] * inv, y[i + 1] * inv);
+  for (int i = 0; i < C; i += 2)
+    *reinterpret_cast<uint32_t*>(out + row * D + C * lane + i) = half_pair(within(y[i] * inv, LARGEST), within(y[i + 1] * inv, LARGEST));
   const int h = (int)(row % s.n_heads), q = (int)(row / s.n_heads % s.queries), b = (int)(row / s.n_heads / s.queries);
   if (lane == 0) lse[((size_t)b * s.n_heads + h) * s.queries + q] = empty ? -INFINITY : (top + log2f(sum)) * LN2;
   __syncwarp();

@@ -406,3 +406,18 @@ def test_padding_that_is_no_number_takes_no_time(qc):
     padded, out = median()
     assert torch.equal(out, want)
     assert padded <= 1.4 * finite, (finite, padded)
+
+
+@pytest.mark.parametrize("Tq,Tk,H,KV,D", [(200, 200, 8, 2, 128), (1, 1, 8, 8, 64), (60, 1500, 4, 1, 128), (300, 300, 4, 4, 64)])
+@pytest.mark.parametrize("window", [0, 1, 3])
+def test_the_largest_values_stay_finite(qc, Tq, Tk, H, KV, D, window):
+    """An output lies between the values of its row: where all of them are fp16's largest, the weights' roundings make no infinity of it."""
+    q, k, v = make(1, Tq, Tk, H, KV, D, 19, scale=2.0)
+    v[:] = 65504.0
+    v[..., 1::2] = -65504.0
+    out, _ = qc.attn_prefill(q, k, v, window=window)
+    assert out.isfinite().all()
+    assert ((out.double() - v[0, 0, 0].double()).abs() <= 3 * 2.0 ** -11 * 65504).all()
+    v[0, Tk - 1, :, 5] = math.inf                         # an infinite value is one
+    out, _ = qc.attn_prefill(q, k, v, window=window)
+    assert (out[0, -1, :, 5] == math.inf).all() and out[..., :5].isfinite().all() and out[..., 6:].isfinite().all() and out[0, :-1].isfinite().all()
