@@ -65,8 +65,8 @@ __device__ __forceinline__ int length_of(const PromptArgs& a, int b) {
 // Bound by the softmax phases: 2000 cycles for a tile with a warp a scheduler, and a tile's next scores wait for its weights, in whose
 // place they go; two tiles by 128 keys take 3900 cycles, their MMAs alone 2160.  8192 tokens of 32 heads 1.03 PFLOP/s, 2048 of 40 heads
 // 65 us, 8192 of 64 / 8 heads with a window of 2048 527 us in a burst, 610 once the power cap holds the clock at 1.69 GHz (normal
-// random inputs).  Keys with a few columns four times as large, whose scores make rows raise their reference and take tiles twice: 75, 654 and
-// 690 us.  Sixteen softmax warps of half a row spill (0.69 to 0.92 PFLOP/s), two MMA warps 0.83, two score buffers of 64 keys 0.50 to 0.61.
+// random inputs).  Keys with a few columns four times as large, whose scores make rows raise their reference and take tiles twice: 77, 654 and
+// 691 us.  Sixteen softmax warps of half a row spill (0.69 to 0.92 PFLOP/s), two MMA warps 0.83, two score buffers of 64 keys 0.50 to 0.61.
 constexpr int UM_THREADS = 320, UM_TILE = 128, UM_STAGES = 4, UM_CHUNK = 64 * 128 * 2;      // bytes of 64 columns of a tile
 constexpr int W_LOAD = 8, W_MMA = 9;
 constexpr int POLY_OF_8 = 1;                      // of eight pairs of exponentials, how many are polynomials
@@ -132,6 +132,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 // A mean of finite values is none of fp16's infinities, but where they are near its largest number the weights' roundings can carry it there.
+// (Looking at a row's largest sum and holding it is 1 % of a prompt.)
 constexpr float LARGEST = 65504.f;
 __device__ __forceinline__ float within(float x, float most) { return fabsf(x) < INFINITY ? fminf(fmaxf(x, -most), most) : x; }
 
