@@ -335,6 +335,85 @@ size_t cq_kv4_evict_workspace_bytes(const cq_kv4* cache, int keep);
 int cq_kv4_evict(const cq_kv4* from, const cq_kv4* to, const float* weights, float* weights_out, const long long* length,
                  long long* length_out, int keep, int sinks, int recent, int* kept, void* workspace, cq_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Paged KV cache (the reference keeps one contiguous cache, llama/modeling_llama_quant.py:371-419).
+ * A pool of pages holds page_size slots of every KV head each: k and v (pages, n_kv_heads, page_size, D), contiguous, 16-byte
+ * aligned, not overlapping; dtype 0 = fp16, 2 = bf16; page_size 16, 32, 64, 128 or 256; head_dim 64 or 128.  A table
+ * (sequences, width) int32 on the device, rows `stride` entries apart, names the page of every page_size slots of a sequence; an
+ * entry outside the pool stands for no page: its slots are not written, not seen and read as zeros.  Sequences may share
+ * pages; a page that a call writes to is in its tables once.  All rows have contiguous columns, 16-byte aligned addresses
+ * and strides (in elements) that are multiples of 8.
+ * ---------------------------------------------------------------------- */
+typedef struct cq_pages {
+  int32_t pages, n_kv_heads, page_size, head_dim, dtype;
+  void *k, *v;
+} cq_pages;
+typedef struct cq_table {
+  const int32_t* entries;
+  int32_t sequences, width;
+  int64_t stride;
+} cq_table;
+typedef struct cq_rows {               /* (tokens, heads, D) of the pool's type */
+  const void* at;
+  int64_t token_stride, head_stride;
+} cq_rows;
+/* Whether the fields describe a pool that the calls below take. */
+int cq_pages_check(const cq_pages* pages);
+/* New rows: row t of k and v goes to slot first[s] + t - starts[s] of the sequence s with starts[s] <= t < starts[s + 1] (starts: sequences
+ * + 1 numbers in order; NULL: the same number of rows each).  Rows in front of starts[0] or from starts[sequences] on, and rows
+ * whose slot has no page, are left out.  With tables (table_rows, D / 2) q (rows, n_heads, D) and k are rotated at positions[t]
+ * first, as by cq_rope_cache, each product and sum rounded, then to the type; q goes to q_out (rows, n_heads, D) contiguous, whether or not
+ * its row is in a sequence (n_heads 0: no queries).  A row whose position lies outside the tables is not rotated and not written.  cos_table
+ * NULL: nothing is rotated.  first, starts, positions: device int64. */
+int cq_pages_write(const cq_pages* pages, const cq_table* table, const cq_rows* q, void* q_out, const cq_rows* k, const cq_rows* v,
+                   const float* cos_table, const float* sin_table, const long long* positions, int table_rows, const long long* first,
+                   const long long* starts, int rows, int n_heads, cq_stream_t stream);
+/* The slots first[s] .. first[s] + count - 1: k, v (sequences, count, KV, D); zeros where there is no page. */
+int cq_pages_read(const cq_pages* pages, const cq_table* table, const long long* first, int count, void* k, void* v, cq_stream_t stream);
+/* Attention of one query per sequence: out (sequences, n_heads, D) contiguous = softmax(scale * q . k_j) . v_j over the visible slots
+ * j < n = length[s] (device int64, bounded by the table): all of them (window 0), or those with j < sinks or j >= n - window, and of these
+ * those that have a page.  Nothing visible: zeros.  scale positive.  workspace: device memory of cq_pages_attend_workspace_bytes(...)
+ * bytes (may be NULL where that is 0), 16-byte aligned, not shared by calls that can overlap. */
+size_t cq_pages_attend_workspace_bytes(const cq_pages* pages, const cq_table* table, int n_heads, int window, int sinks);
+int cq_pages_attend(const cq_pages* pages, const cq_table* table, const cq_rows* q, const long long* length, void* out, int n_heads,
+                    int window, int sinks, float scale, void* workspace, cq_stream_t stream);
+/* One decode step: cq_pages_write of one row per sequence at slot length[s], then cq_pages_attend over n = length[s] + 1 slots (q is not
+ * changed; the caller counts length up).  n counts the new slot also where its row is left out for its position: what the slot held
+ * is attended then.  A negative length: nothing is written or seen. */
+int cq_pages_step(const cq_pages* pages, const cq_table* table, const cq_rows* q, const cq_rows* k, const cq_rows* v,
+                  const float* cos_table, const float* sin_table, const long long* positions, int table_rows, const long long* length,
+                  void* out, int n_heads, int window, int sinks, float scale, void* workspace, cq_stream_t stream);
+
+/* Adjusted logits and the token that they pick.  Of row b and token v, with c = how often v stands among tokens[b][prompt[b] ..
+ * length[b] - 1], in fp32, each operation rounded:
+ *   x = logits[b][v]
+ *   v among tokens[b][0 .. length[b] - 1]:  x = x > 0 ? x / repetition[b] : x * repetition[b]
+ *   c > 0:  x = x - frequency[b] * c, then x = x - presence[b]
+ *   v in bias_ids[b]:  x = x + bias[b][i], i its last place there
+ *   bit v % 32 of word v / 32 of mask row mask_rows[b] is 0:  x = -infinity
+ * out[b][v] = x, rounded to the type; next[b] = the lowest v of the largest x (before rounding; NaN counts as the largest).
+ * Every pointer but logits, out and next may be NULL: without tokens no penalties, without length all `width` tokens, without prompt from the
+ * first.  Numbers outside the vocabulary among tokens and bias_ids stand for nothing, a mask row outside the masks for no
+ * mask (mask_rows NULL: row b of at least as many masks).  length and prompt are bounded by the row.  Strides in elements between rows,
+ * whose columns are contiguous; those of what is only read may be 0.  out is logits (with the same stride) or shares no memory with it.
+ * tokens, length, prompt, bias_ids, mask_rows, next: device int64; repetition (positive), presence, frequency, bias: device fp32. */
+typedef struct cq_adjust {
+  int32_t dtype;                       /* of logits and out: 0 = fp16, 1 = fp32, 2 = bf16 */
+  int32_t biases, masks;
+  int64_t width;
+  const void* logits;
+  void* out;
+  long long* next;
+  int64_t logits_stride, out_stride, tokens_stride, bias_ids_stride, bias_stride, mask_stride;
+  const long long *tokens, *length, *prompt;
+  const float *repetition, *presence, *frequency;
+  const long long* bias_ids;
+  const float* bias;
+  const uint32_t* mask;
+  const long long* mask_rows;
+} cq_adjust;
+int cq_adjust_logits(const cq_adjust* args, int rows, int vocab, cq_stream_t stream);
+
 /* Attention of prompts: q (sequences, queries, n_heads, D), k and v (sequences, keys, n_kv_heads, D) fp16 with the given
  * strides in elements (the columns of a head are contiguous; addresses and strides multiples of 16 bytes; tokens do not share a row).  Query i stands at
  * position p = i + keys - queries and sees the keys j <= p with j < lengths[s] (device int64; NULL: keys), with a window only

@@ -29,6 +29,7 @@
 
 #include "cherryq.h"
 #include "kv4_ext.h"
+#include "pages_ext.h"
 
 namespace {
 
@@ -906,6 +907,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_decode_step", &attn_decode_step, "rotary embedding, KV cache write and attention of a decode step");
   m.def("attn_decode", &attn_decode, "single-query attention over the KV cache");
   register_kv4(m);
+  register_pages(m);
   m.def("poll", []() { check_status(cq_poll(current_stream()), "poll"); });
   m.def("device_timed_out", &device_timed_out);
   m.def("row_layers_matvec", &row_layers_matvec, "one launch for row-tile layers sharing an activation row");
