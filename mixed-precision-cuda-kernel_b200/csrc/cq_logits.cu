@@ -1,36 +1,76 @@
 // Logits on their way to a token: penalties for tokens that occurred, biases of single tokens, a grammar's bit mask, and the largest.
 //
-// A cluster of CTAs takes a row, a CTA a part of the vocabulary.  How often its tokens occurred is counted in shared memory from the
-// row's history (integer additions: their order changes nothing), where a part is larger than that memory one slice after
-// another; then every logit is read once and written once.  The largest travels as one 64-bit key, its value in the order of
-// unsigned numbers above the complement of its token: the maximum of keys is the lowest token of the largest value.
+// The bound is the logits' traffic, each read once and written once; penalties are the business of few tokens and are settled token by
+// token, beside it.  The tokens that occurred or have a bias are marked in a bit map; a token's rank among the marked ones is its
+// place in arrays of as many entries, where occurrences are counted (integer additions: their order changes nothing).  The pass over the
+// logits leaves the marked ones out of the maximum; their values are written over its results.  (Penalties in that pass took 57
+// instructions a logit, 256 rows of 131071 138 us; counters for all tokens, a slice of the vocabulary after the other, 87.)
+// Every thread has four pieces of 16 bytes on the way, copied asynchronously to places of its own, and waits for no other
+// thread.  Of eight logits only the largest meets the thread's best.  The largest travels as one 64-bit key, its value in the
+// order of unsigned numbers above the complement of its token: the maximum of keys is the lowest token of the largest value.
 #include <algorithm>
-
-#include <cooperative_groups.h>
+#include <type_traits>
 
 #include "cq_pages.cuh"
 
 namespace {
 
-namespace cg = cooperative_groups;
-
-constexpr int THREADS = 512;
-constexpr int SLICE = 16384;                 // tokens counted at a time
-constexpr uint32_t OCCURRED = 0x80000000u;   // anywhere in the history; the bits below count the generated part
+constexpr int THREADS = 512, WARPS = THREADS / 32;
+constexpr int STAGES = 4;                    // pieces of 16 bytes of a thread on their way
+constexpr int PARTS = 8;                     // CTAs of a row, at most
+constexpr int TOKENS = 4 * THREADS;          // of the history, loads in flight
+constexpr int SLICE = 129 * 1024;            // tokens that the bit map holds
+constexpr int PLACES = STAGES * THREADS * 16 / 12;          // marked tokens at a time, in the pieces' memory
+// what is known of a token: whether it occurred in the prompt, whether it has a bias, and below how often it was generated
+constexpr uint32_t PROMPT = 0x80000000u, BIAS = 0x40000000u, TIMES = 0x3FFFFFFFu;
 
 struct Adjust {
   cq_adjust a;
-  int rows, vocab;
+  int vocab, part, slice;                    // logits of a row, of a CTA, and of the bit map
+  int keep;                                  // tokens of the history in shared memory
 };
 
-template <typename T> __device__ __forceinline__ float value_of(T x);
-template <> __device__ __forceinline__ float value_of(__half x) { return __half2float(x); }
-template <> __device__ __forceinline__ float value_of(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ float value_of(T x) { return cq_paged::Type<T>::one(x); }
 template <> __device__ __forceinline__ float value_of(float x) { return x; }
 template <typename T> __device__ __forceinline__ T rounded(float x);
 template <> __device__ __forceinline__ __half rounded(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 rounded(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ float rounded(float x) { return x; }
+
+// 16 bytes of logits.  largest(): NaN where one is; hide(): -infinity in the places whose bits are set, `lut` the 16-bit lanes of four bits
+template <typename T> struct Piece {
+  uint4 w;
+  using Two = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  __device__ __forceinline__ float largest() const {
+    const Two* t = reinterpret_cast<const Two*>(&w);
+    const Two m = __hmax2_nan(__hmax2_nan(t[0], t[1]), __hmax2_nan(t[2], t[3]));
+    const float2 f = cq_paged::Type<T>::apart(*reinterpret_cast<const uint32_t*>(&m));
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(f.x), "f"(f.y));
+    return d;
+  }
+  __device__ __forceinline__ void hide(uint32_t bits, const uint2* lut) {
+    constexpr uint32_t NONE = std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+    const uint2 a = lut[bits & 15u], b = lut[bits >> 4];
+    w.x = (w.x & ~a.x) | (NONE & a.x), w.y = (w.y & ~a.y) | (NONE & a.y);
+    w.z = (w.z & ~b.x) | (NONE & b.x), w.w = (w.w & ~b.y) | (NONE & b.y);
+  }
+  __device__ __forceinline__ T at(int e) const { return reinterpret_cast<const T*>(&w)[e]; }
+};
+template <> struct Piece<float> {
+  uint4 w;
+  __device__ __forceinline__ float largest() const {
+    float d;
+    asm("{\n\t.reg .f32 a, b;\n\tmax.NaN.f32 a, %1, %2;\n\tmax.NaN.f32 b, %3, %4;\n\tmax.NaN.f32 %0, a, b;\n\t}"
+        : "=f"(d) : "f"(__uint_as_float(w.x)), "f"(__uint_as_float(w.y)), "f"(__uint_as_float(w.z)), "f"(__uint_as_float(w.w)));
+    return d;
+  }
+  __device__ __forceinline__ void hide(uint32_t bits, const uint2*) {
+    constexpr uint32_t NONE = 0xFF800000u;
+    w.x = bits & 1u ? NONE : w.x, w.y = bits & 2u ? NONE : w.y, w.z = bits & 4u ? NONE : w.z, w.w = bits & 8u ? NONE : w.w;
+  }
+  __device__ __forceinline__ float at(int e) const { return reinterpret_cast<const float*>(&w)[e]; }
+};
 
 // fp32 numbers in the order of unsigned ones: NaN above all, both zeros alike
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -40,93 +80,313 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 __device__ __forceinline__ unsigned long long larger(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS) adjust_logits_kernel(const Adjust p) {
-  extern __shared__ __align__(16) uint32_t s_count[];      // [slice], and where there are biases [slice] 1 + the entry that counts
+// until every CTA of the cluster has arrived once, or for two seconds
+__device__ __forceinline__ void wait_for_all(uint32_t bar) {
+  unsigned long long t0 = 0;
+  for (uint32_t it = 0; it < (1u << 26); ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0, %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(20000u) : "memory");
+    if (ok) return;
+    unsigned long long t1;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
+    if (t0 == 0) t0 = t1;
+    else if (t1 - t0 > 2000000000ull) return;
+  }
+}
+
+template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(BYTES) : "memory");
+}
+
+template <typename T, bool ALIKE>
+__global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust p) {
+  constexpr int VEC = 16 / sizeof(T);
+  extern __shared__ __align__(16) uint8_t smem[];
   __shared__ unsigned long long s_key[THREADS / 32];
-  __shared__ unsigned long long s_best;
+  __shared__ unsigned long long s_part[PARTS], s_arrived;
+  __shared__ int s_sum[WARPS];
+  __shared__ uint2 s_lut[16];                // what four bits are in 16-bit lanes
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const cq_adjust& a = p.a;
-  cg::cluster_group cluster = cg::this_cluster();
   const int parts = gridDim.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int part = (p.vocab + parts - 1) / parts, begin = min(p.vocab, (int)blockIdx.x * part), end = min(p.vocab, begin + part);
+  if (parts > 1) {
+    if (tid == 0) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(&s_arrived)), "r"(parts) : "memory");
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (tid < 16) s_lut[tid] = make_uint2((tid & 1 ? 0xFFFFu : 0u) | (tid & 2 ? 0xFFFF0000u : 0u), (tid & 4 ? 0xFFFFu : 0u) | (tid & 8 ? 0xFFFF0000u : 0u));
+  const bool counts = a.tokens != nullptr, known = counts || a.biases;
+  uint4* s_piece = reinterpret_cast<uint4*>(smem) + tid;                     // [stage][thread]
+  uint32_t* s_known = reinterpret_cast<uint32_t*>(smem);                     // [place], after the pieces
+  uint32_t* s_token = s_known + PLACES;
+  uint32_t* s_bias = s_token + PLACES;                                       // 1 + the entry that counts
+  uint64_t* s_bits = reinterpret_cast<uint64_t*>(smem + 16 * STAGES * THREADS);
+  int* s_rank = reinterpret_cast<int*>(s_bits + (known ? p.slice / 64 : 0));  // of a word's first marked token
+  int* s_history = s_rank + (known ? p.slice / 64 : 0);                      // -1 outside the vocabulary
+  uint32_t* s_mask = reinterpret_cast<uint32_t*>(s_history + (counts ? p.keep : 0));      // numbered as the marks
   const T* in = (const T*)a.logits + (int64_t)row * a.logits_stride;
   T* out = (T*)a.out + (int64_t)row * a.out_stride;
-  uint32_t* s_bias = s_count + (a.tokens ? min(part, SLICE) : 0);
+  // Logits are numbered from the 16-byte boundary in front of the row's first, so that pieces are aligned.  (Where results lie otherwise,
+  // they are written one by one.)
+  const int skip = (int)(((uintptr_t)in / sizeof(T)) % VEC);
+  in -= skip;
+  out -= skip;
+  const int total = p.vocab + skip, begin = min(total, (int)blockIdx.x * p.part), end = min(total, begin + p.part);
+  auto whole = [&](int i) { return (unsigned)(i - skip) <= (unsigned)(p.vocab - VEC) && p.vocab >= VEC; };
+  auto fetch = [&](int i, int stage) {
+    if (whole(i)) {
+      copy_async<16>(s_piece + stage * THREADS, in + i);
+    } else {
+      T* w = reinterpret_cast<T*>(s_piece + stage * THREADS);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) w[e] = i + e >= skip && i + e < total ? in[i + e] : T(-INFINITY);
+    }
+  };
+  constexpr int STEP = THREADS * VEC;
+  auto first_pieces = [&](int base, int stop) {
+#pragma unroll
+    for (int k = 0; k < STAGES; ++k) {
+      if (base + k * STEP + tid * VEC < stop) fetch(base + k * STEP + tid * VEC, k);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  first_pieces(begin, min(end, begin + p.slice));
 
-  long long n = 0, prompt = 0;
+  const long long* tokens = counts ? a.tokens + (int64_t)row * a.tokens_stride : nullptr;
+  const long long* ids = a.biases ? a.bias_ids + (int64_t)row * a.bias_ids_stride : nullptr;
+  auto token_of = [&](long long v) { return (unsigned long long)v < (unsigned)p.vocab ? (int)v : -1; };
+  // all that the row says in one round of loads
+  long long v0[TOKENS / THREADS], n64 = a.width, prompt64 = 0, mask_row = row;
   float rep = 1.f, pres = 0.f, freq = 0.f;
-  if (a.tokens) {
-    n = a.length ? a.length[row] : a.width;
-    n = n < 0 ? 0 : (n > a.width ? a.width : n);
-    prompt = a.prompt ? a.prompt[row] : 0;
+  if (counts) {
+#pragma unroll
+    for (int k = 0; k < TOKENS / THREADS; ++k) v0[k] = tid + k * THREADS < a.width ? tokens[tid + k * THREADS] : -1;
+    if (a.length) n64 = a.length[row];
+    if (a.prompt) prompt64 = a.prompt[row];
     if (a.repetition) rep = a.repetition[row];
     if (a.presence) pres = a.presence[row];
     if (a.frequency) freq = a.frequency[row];
   }
-  const long long* tokens = a.tokens ? a.tokens + (int64_t)row * a.tokens_stride : nullptr;
-  const uint32_t* mask = nullptr;
-  if (a.mask) {
-    const long long m = a.mask_rows ? a.mask_rows[row] : row;
-    if (m >= 0 && m < a.masks) mask = a.mask + m * a.mask_stride;
-  }
+  if (a.mask && a.mask_rows) mask_row = a.mask_rows[row];
+  const uint32_t* mask = a.mask && mask_row >= 0 && mask_row < a.masks ? a.mask + mask_row * a.mask_stride : nullptr;
+  const int n = !counts || n64 < 0 ? 0 : (int)(n64 > a.width ? a.width : n64), prompt = (int)(prompt64 < 0 ? 0 : (prompt64 > n ? n : prompt64));
 
+  float top = -INFINITY;                     // the thread's largest, the piece that has it and where that begins
+  Piece<T> of_top = {};
+  int at_top = -1;
   unsigned long long best = 0;
-  for (int base = begin; base < end; base += SLICE) {
-    const int size = min(SLICE, end - base);
-    if (a.tokens)
-      for (int i = tid; i < size; i += THREADS) s_count[i] = 0u;
-    if (a.biases)
-      for (int i = tid; i < size; i += THREADS) s_bias[i] = 0u;
-    __syncthreads();
-    for (long long i = tid; i < n; i += THREADS) {
-      const long long v = tokens[i] - base;
-      if (v < 0 || v >= size) continue;
-      if (i < prompt) atomicOr(&s_count[v], OCCURRED);
-      else {
-        atomicOr(&s_count[v], OCCURRED);
-        atomicAdd(&s_count[v], 1u);
+  auto key_of = [&](float x, int v) { return (unsigned long long)order_of(x) << 32 | (0xFFFFFFFFu - (uint32_t)v); };
+#pragma unroll 1
+  for (int base = begin; base < end; base += p.slice) {
+    const int stop = min(end, base + p.slice), size = stop - base, words = (size + 63) / 64;
+    if (base != begin) first_pieces(base, stop);
+    // The mask's words, moved to where the marks of the same tokens are
+    if (mask)
+#pragma unroll 4
+      for (int i = tid; i < (size + 31) / 32; i += THREADS) {
+        const int v = base + 32 * i - skip, w = v >> 5;
+        const uint32_t low = w >= 0 ? __ldg(mask + w) : 0u, high = 32 * (w + 1) < p.vocab ? __ldg(mask + w + 1) : 0u;
+        s_mask[i] = __funnelshift_r(low, high, v & 31);
       }
+    // the place of a token in the slice, -1 outside
+    auto place = [&](int v) {
+      const int j = v < 0 ? -1 : v + skip - base;
+      return j < size ? j : -1;
+    };
+    // what(place, number) of the history's tokens, and of those with a bias
+    auto each_token = [&](auto find, auto what) {
+#pragma unroll 1
+      for (int j0 = tid; j0 < n; j0 += 4 * THREADS) {
+        int at[4], i[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = j0 + k * THREADS;
+          at[k] = j < n ? place(j < p.keep ? s_history[j] : token_of(tokens[j])) : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) i[k] = find(at[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i[k] >= 0) what(i[k], at[k], j0 + k * THREADS);
+      }
+    };
+    auto each_bias = [&](auto find, auto what) {
+#pragma unroll 1
+      for (int j = tid; j < a.biases; j += THREADS) {
+        const int at = place(token_of(ids[j])), i = find(at);
+        if (i >= 0) what(i, at, j);
+      }
+    };
+    if (known) {
+      for (int i = tid; i < words; i += THREADS) s_bits[i] = 0u;
+      __syncthreads();
+      // -1 of a token that is outside, or marked already
+      auto unmarked = [&](int at) {
+        const uint32_t word = reinterpret_cast<volatile uint32_t*>(s_bits)[max(at, 0) >> 5];
+        return at >= 0 && !(word >> (at & 31) & 1u) ? at : -1;
+      };
+      auto mark = [&](int at, int, int) { atomicOr(reinterpret_cast<uint32_t*>(s_bits) + (at >> 5), 1u << (at & 31)); };
+      if (counts && base == begin) {
+        int at[TOKENS / THREADS];
+#pragma unroll
+        for (int k = 0; k < TOKENS / THREADS; ++k) {
+          const int j = tid + k * THREADS, v = token_of(v0[k]);
+          if (j < p.keep) s_history[j] = v;
+          at[k] = unmarked(j < n ? place(v) : -1);
+        }
+#pragma unroll
+        for (int k = 0; k < TOKENS / THREADS; ++k)
+          if (at[k] >= 0) mark(at[k], 0, 0);
+#pragma unroll 4
+        for (int j = TOKENS + tid; j < n; j += THREADS) {
+          const int v = token_of(tokens[j]);
+          if (j < p.keep) s_history[j] = v;
+          if (const int i = unmarked(place(v)); i >= 0) mark(i, 0, 0);
+        }
+      } else if (counts) {
+        each_token(unmarked, mark);
+      }
+      each_bias(unmarked, mark);
     }
-    for (int i = tid; i < a.biases; i += THREADS) {        // of the same token's entries the last one counts
-      const long long v = a.bias_ids[(int64_t)row * a.bias_ids_stride + i] - base;
-      if (v >= 0 && v < size) atomicMax(&s_bias[v], (uint32_t)i + 1u);
-    }
-    __syncthreads();
-    for (int i = tid; i < size; i += THREADS) {
-      const int v = base + i;
-      float x = value_of<T>(in[v]);
-      const uint32_t c = a.tokens ? s_count[i] : 0u;
-      if (c) {
-        if (a.repetition) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-        if (c & ~OCCURRED) {
-          if (a.frequency) x = __fsub_rn(x, __fmul_rn(freq, (float)(c & ~OCCURRED)));
-          if (a.presence) x = __fsub_rn(x, pres);
+    if (mask || known) __syncthreads();      // (the mask's words and the marks are there)
+    // what is known of the marked tokens with ranks from rank0 on
+    auto count = [&](int rank0, int here) {
+      for (int i = tid; i < here; i += THREADS) {
+        s_known[i] = 0u;
+        if (a.biases) s_bias[i] = 0u;
+      }
+      __syncthreads();
+      auto index = [&](int at) {             // -1: outside, or has its turn earlier or later
+        const int w = max(at, 0) >> 6, i = s_rank[w] + __popcll(s_bits[w] & ((1ull << (at & 63)) - 1ull)) - rank0;
+        return at >= 0 && i >= 0 && i < here ? i : -1;
+      };
+      if (counts)
+        each_token(index, [&](int i, int at, int j) {
+          s_token[i] = at;
+          if (j < prompt) atomicOr(&s_known[i], PROMPT);
+          else atomicAdd(&s_known[i], 1u);
+        });
+      each_bias(index, [&](int i, int at, int j) {         // of the same token's entries the last one counts
+        s_token[i] = at;
+        atomicOr(&s_known[i], BIAS);
+        atomicMax(&s_bias[i], (uint32_t)j + 1u);
+      });
+      __syncthreads();
+    };
+    // (of a masked token the pass over the logits may have left -infinity in place of the logit, which changes nothing)
+    auto put = [&](int i) {
+      const uint32_t c = s_known[i];
+      const int at = base + s_token[i];
+      float x = value_of<T>(in[at]);
+      if (a.repetition && (c & (PROMPT | TIMES))) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+      if (c & TIMES) {
+        if (a.frequency) x = __fsub_rn(x, __fmul_rn(freq, (float)(c & TIMES)));
+        if (a.presence) x = __fsub_rn(x, pres);
+      }
+      if (c & BIAS) x = __fadd_rn(x, a.bias[(int64_t)row * a.bias_stride + s_bias[i] - 1u]);
+      if (mask && !(s_mask[s_token[i] >> 5] >> (s_token[i] & 31) & 1u)) x = -INFINITY;
+      out[at] = rounded<T>(x);
+      best = larger(best, key_of(x, at - skip));
+    };
+
+    for (int i0 = base + tid * VEC; i0 < stop; i0 += STAGES * STEP) {
+#pragma unroll
+      for (int k = 0; k < STAGES; ++k) {
+        const int i = i0 + k * STEP, j = i - base;
+        if (i >= stop) break;
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        Piece<T> piece;
+        piece.w = s_piece[k * THREADS];
+        if (i + STAGES * STEP < stop) fetch(i + STAGES * STEP, k);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (mask) {
+          const uint32_t hidden = ~(s_mask[j >> 5] >> (j & 31)) & ((1u << VEC) - 1u);
+          if (hidden) piece.hide(hidden, s_lut);
+        }
+        if (ALIKE && whole(i)) *reinterpret_cast<uint4*>(out + i) = piece.w;
+        else
+          for (int e = 0; e < VEC; ++e)
+            if (i + e >= skip && i + e < total) out[i + e] = piece.at(e);
+        if (known) {
+          const uint32_t own = reinterpret_cast<const uint32_t*>(s_bits)[j >> 5] >> (j & 31) & ((1u << VEC) - 1u);
+          if (own) piece.hide(own, s_lut);
+        }
+        const float m = piece.largest();
+        if (at_top < 0 || (!(m <= top) && top == top)) {
+          top = m;
+          at_top = i;
+          of_top = piece;
         }
       }
-      if (a.biases && s_bias[i]) x = __fadd_rn(x, a.bias[(int64_t)row * a.bias_stride + s_bias[i] - 1u]);
-      if (mask && !(mask[v >> 5] >> (v & 31) & 1u)) x = -INFINITY;
-      out[v] = rounded<T>(x);
-      best = larger(best, (unsigned long long)order_of(x) << 32 | (0xFFFFFFFFu - (uint32_t)v));
     }
-    __syncthreads();
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (known) {
+      // ranks: a thread takes consecutive words
+      const int each = (words + THREADS - 1) / THREADS, w0 = min(words, tid * each), w1 = min(words, w0 + each);
+      int mine = 0;
+      for (int w = w0; w < w1; ++w) mine += __popcll(s_bits[w]);
+      int before = mine;
+      for (int d = 1; d < 32; d *= 2) {
+        const int o = __shfl_up_sync(0xffffffffu, before, d);
+        if (lane >= d) before += o;
+      }
+      if (lane == 31) s_sum[warp] = before;
+      __syncthreads();
+      int all = lane < WARPS ? s_sum[lane] : 0;
+      for (int d = 1; d < WARPS; d *= 2) {
+        const int o = __shfl_up_sync(0xffffffffu, all, d);
+        if (lane >= d) all += o;
+      }
+      const int marked = __shfl_sync(0xffffffffu, all, WARPS - 1);
+      const int in_front = __shfl_sync(0xffffffffu, all, max(0, warp - 1));
+      before += (warp ? in_front : 0) - mine;
+      for (int w = w0; w < w1; ++w) {
+        s_rank[w] = before;
+        before += __popcll(s_bits[w]);
+      }
+      __syncthreads();                       // (results of the pass lie under those of the marked tokens; the pieces' memory is free)
+      for (int rank0 = 0; rank0 < marked; rank0 += PLACES) {
+        const int here = min(PLACES, marked - rank0);
+        if (rank0) __syncthreads();
+        count(rank0, here);
+        for (int i = tid; i < here; i += THREADS) put(i);
+      }
+    }
+    if (stop < end) __syncthreads();         // (the next slice takes the same memory)
   }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e)
+    if (at_top >= 0 && at_top + e >= skip && at_top + e < total) best = larger(best, key_of(value_of<T>(of_top.at(e)), at_top + e - skip));
   for (int d = 16; d; d /= 2) best = larger(best, __shfl_xor_sync(0xffffffffu, best, d));
   if (lane == 0) s_key[warp] = best;
   __syncthreads();
   if (warp == 0) {
     best = lane < THREADS / 32 ? s_key[lane] : 0ull;
     for (int d = 16; d; d /= 2) best = larger(best, __shfl_xor_sync(0xffffffffu, best, d));
-    if (lane == 0) s_best = best;
   }
-  if (parts > 1) cluster.sync();
-  if (blockIdx.x == 0 && warp == 0) {
-    if (parts > 1) best = lane < parts ? *cluster.map_shared_rank(&s_best, lane) : 0ull;
-    for (int d = 16; d; d /= 2) best = larger(best, __shfl_xor_sync(0xffffffffu, best, d));
-    if (lane == 0) a.next[row] = (long long)(0xFFFFFFFFu - (uint32_t)best);
+  if (parts > 1) {
+    // To the cluster's first CTA, the only one that waits for the others.
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (tid == 0) {
+      uint32_t at, bar;
+      asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(&s_part[blockIdx.x])));
+      asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(bar) : "r"((uint32_t)__cvta_generic_to_shared(&s_arrived)));
+      asm volatile("st.relaxed.cluster.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(best) : "memory");
+      asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    }
+    if (blockIdx.x || tid) return;
+    wait_for_all((uint32_t)__cvta_generic_to_shared(&s_arrived));
+    for (int i = 1; i < parts; ++i) best = larger(best, *(volatile unsigned long long*)&s_part[i]);
   }
-  if (parts > 1) cluster.sync();                           // (nobody leaves while its key may be read)
+  if (tid == 0) a.next[row] = (long long)(0xFFFFFFFFu - (uint32_t)best);
 }
 
 // bytes from the first to behind the last element of `rows` rows of `cols`
@@ -136,7 +396,7 @@ size_t span(int64_t rows, int64_t cols, int64_t stride, size_t item) { return (s
 
 extern "C" int cq_adjust_logits(const cq_adjust* a, int rows, int vocab, cq_stream_t stream) {
   if (!a || !a->logits || !a->out || !a->next) return CQ_ERR_BAD_ARG;
-  if (rows < 1 || rows > 65535 || vocab < 1 || vocab > (1 << 30) || a->width > INT32_MAX) return CQ_ERR_BAD_SHAPE;
+  if (rows < 1 || rows > 65535 || vocab < 1 || vocab > (1 << 30) || a->width >= (1 << 30)) return CQ_ERR_BAD_SHAPE;
   if (a->dtype < 0 || a->dtype > 2) return CQ_ERR_UNSUPPORTED;
   const size_t item = a->dtype == 1 ? 4 : 2;
   if (((uintptr_t)a->logits | (uintptr_t)a->out) & (item - 1)) return CQ_ERR_BAD_ARG;
@@ -147,11 +407,18 @@ extern "C" int cq_adjust_logits(const cq_adjust* a, int rows, int vocab, cq_stre
   // in place, or apart
   const bool in_place = a->logits == a->out && (rows == 1 || a->logits_stride == a->out_stride);
   if (!in_place && !kv4_apart(a->logits, span(rows, vocab, a->logits_stride, item), a->out, span(rows, vocab, a->out_stride, item))) return CQ_ERR_BAD_ARG;
-  const int sms = cq_sm_count();
+  const int sms = cq_sm_count(), vec = 16 / (int)item;
   int parts = 1;
-  while (parts < 8 && (vocab > parts * SLICE || rows * parts < sms) && vocab > parts * 1024) parts *= 2;
-  const int part = (vocab + parts - 1) / parts, slice = std::min(part, SLICE), smem = 4 * slice * ((a->tokens ? 1 : 0) + (a->biases ? 1 : 0));
-  auto fn = a->dtype == 0 ? adjust_logits_kernel<__half> : (a->dtype == 1 ? adjust_logits_kernel<float> : adjust_logits_kernel<__nv_bfloat16>);
+  while (parts < PARTS && rows * parts < sms && vocab > parts * 1024) parts *= 2;
+  const int part = ((vocab + vec - 1 + parts - 1) / parts + vec - 1) / vec * vec, slice = std::min((part + 63) / 64 * 64, SLICE);
+  // (two CTAs on an SM)
+  const int base_smem = STAGES * THREADS * 16 + (a->tokens || a->biases ? slice / 64 * 12 : 0) + (a->mask ? slice / 8 + 16 : 0);
+  const int keep = a->tokens ? (int)std::min<int64_t>(a->width, (112 * 1024 - base_smem) / 4) : 0, smem = base_smem + 4 * keep;
+  // 16 bytes at a time where a row's logits and results lie alike
+  const bool alike = (((uintptr_t)a->logits ^ (uintptr_t)a->out) & 15) == 0 && (rows == 1 || (a->logits_stride - a->out_stride) % vec == 0);
+  auto fn = a->dtype == 0   ? (alike ? adjust_logits_kernel<__half, true> : adjust_logits_kernel<__half, false>)
+            : a->dtype == 1 ? (alike ? adjust_logits_kernel<float, true> : adjust_logits_kernel<float, false>)
+                            : (alike ? adjust_logits_kernel<__nv_bfloat16, true> : adjust_logits_kernel<__nv_bfloat16, false>);
   CQ_CUDA_TRY(cq_grant_smem((const void*)fn, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(parts, rows);
@@ -166,6 +433,6 @@ extern "C" int cq_adjust_logits(const cq_adjust* a, int rows, int vocab, cq_stre
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  CQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, Adjust{*a, rows, vocab}));
+  CQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, Adjust{*a, vocab, part, slice, keep}));
   return CQ_OK;
 }

@@ -212,7 +212,7 @@ std::pair<torch::Tensor, torch::Tensor> adjust_logits(const torch::Tensor& logit
               "length, prompt and penalties need tokens");
   if (tokens.has_value()) {
     a.tokens_stride = matrix(*tokens, "tokens", torch::kInt64, device, rows);
-    TORCH_CHECK(tokens->size(1) <= INT32_MAX, "at most 2^31 - 1 tokens a row");
+    TORCH_CHECK(tokens->size(1) < (1 << 30), "less than 2^30 tokens a row");
     a.tokens = (const long long*)tokens->const_data_ptr();
     a.width = tokens->size(1);
     if (length.has_value()) a.length = whole_numbers(*length, "length", rows, device);
