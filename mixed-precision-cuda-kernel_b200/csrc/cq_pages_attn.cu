@@ -6,10 +6,15 @@
 // operands agree), then the weights as the A operand of P . V.  A weight is two numbers of the cache's type, its upper bits in rows
 // 0-7 and what is left in rows 8-15, which the heads leave empty.  An MMA cuts its sums off instead of rounding them: each one
 // sums its 16 products alone, fp32 additions do the rest.  A warp takes 16 slots a turn (they lie in one page) and keeps its own
-// running maximum, a whole number of powers of two, sum and weighted values; warps meet in shared memory, ranges of slots in the
-// workspace.
+// running maximum, a whole number of powers of two, sum and weighted values; warps meet in shared memory, CTAs that share a head
+// in a cluster, or, where a head's slots are cut wherever the equal shares of all CTAs end, in a second kernel.
+//
+// Tried and not taken: rings of tiles copied asynchronously, each warp its own (three tiles of 8 KB a warp, eight warps an SM; 70B heads, 16
+// sequences up to 4001 slots 42 us against 41, 13B heads with a window 38 against 33, four of 65531 slots 172 against 172), the next
+// tile's loads between the sums (registers spill: 53 against 41), two tiles a warp in rings on three CTAs an SM (249 against 172).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "cq_pages.cuh"
 
@@ -20,14 +25,19 @@ using namespace cq_paged;
 constexpr int AT_HEADS = 8;                  // query heads of a CTA
 constexpr int AT_SLOTS = 16;                 // slots of a turn
 constexpr int AT_WARPS = 4;
+constexpr int MAX_CLUSTER = 8;
+constexpr int per_sm(int head_dim) { return head_dim == 64 ? 4 : 3; }      // CTAs that an SM holds
 
-__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, __half) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, __nv_bfloat16) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+// sums of 16 products without an addend, rows 0-7 and rows 8-15 in pairs
+template <typename T> __device__ __forceinline__ void mma(uint64_t (&d)[2], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  float x[4];
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  d[0] = two(x[0], x[1]), d[1] = two(x[2], x[3]);
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -80,252 +90,431 @@ template <typename T> struct NewRow {
   int table_rows;
 };
 
-template <typename T, int D, bool STEP>
-__global__ void __launch_bounds__(AT_WARPS * 32, 3) pages_attend_kernel(const Rows<T> q, const Pool<T> pool, const Table table, const NewRow<T> fresh,
-                                                                        const long long* __restrict__ length, T* __restrict__ out,
-                                                                        float* __restrict__ part, int H, int chunks, int window, int sinks, float scale) {
+// What the kernels get besides their tensors
+struct Shape {
+  int sequences, H, chunks, window, sinks, ctas;
+  float scale;
+};
+constexpr int PART = 4;                      // in front of a head's D partial sums: maximum, sum of weights
+// The partial results of a CTA: of a head whose slots begin with an earlier CTA, of a head that a later CTA goes on with; and how many CTAs
+// that head has, its first one's sequence and head.
+struct Span {
+  int parts, seq, head, heads;
+};
+template <int D> __device__ __forceinline__ float* part_of(void* ws, int ctas, int cta, int which) {
+  return reinterpret_cast<float*>(reinterpret_cast<Span*>(ws) + ctas) + (size_t)(2 * cta + which) * AT_HEADS * (D + PART);
+}
+
+// (most quotients fit 32 bits, whose division takes a quarter of the time)
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+// CLUSTER: a cluster of CTAs for the heads of a KV head and sequence, each with the same share of its tiles.  Otherwise all tiles of all
+// sequences and KV heads in a row, cut into equal ranges for the CTAs that the device holds at once.
+template <typename T, int D, bool STEP, bool CLUSTER>
+__global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(const Rows<T> q, const Pool<T> pool, const Table table, const NewRow<T> fresh,
+                                                                        const long long* __restrict__ length, T* __restrict__ out, void* ws, const Shape shape) {
   constexpr int THREADS = AT_WARPS * 32;
   constexpr int KP = D / 32;                 // 16-byte pieces of a key per lane (four lanes a slot)
   constexpr int VS = D / 64;                 // of a value (eight lanes a slot)
+  // Weights times a power of two: fp16's halves of their split then reach down to 2^-38 of the largest; in bf16, whose halves reach anywhere,
+  // sums of 2^24 of the largest values stay finite.
+  constexpr float LIFT = std::is_same<T, __half>::value ? 32768.f : 5.9604644775390625e-8f;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ __align__(16) float s_sum[AT_WARPS][AT_HEADS][D];
+  __shared__ __align__(16) float s_part[CLUSTER ? AT_HEADS : 1][D + PART];
   __shared__ __align__(16) T s_q[AT_HEADS][D + 32];
   __shared__ float s_m[AT_WARPS][AT_HEADS], s_l[AT_WARPS][AT_HEADS];
-  const int split = blockIdx.x, nsplit = gridDim.x, kvh = blockIdx.y / chunks, seq = blockIdx.z, KV = pool.heads;
-  const int G = H / KV, h0 = (blockIdx.y - kvh * chunks) * AT_HEADS, heads = min(AT_HEADS, G - h0);
+  const int KV = pool.heads, H = shape.H, G = H / KV, chunks = shape.chunks, heads_each = KV * chunks, slots = table.width << pool.log_page;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g8 = lane >> 2, t4 = lane & 3;
+  const float scale2 = shape.scale * 1.4426950408889634f;  // scores in powers of two
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int slots = table.width << pool.log_page;
-  const Visible<AT_SLOTS> vis(held(length, seq, STEP, slots), window, sinks);
-  const int each = (vis.tiles + nsplit - 1) / nsplit, tile0 = split * each, tile1 = min(vis.tiles, tile0 + each);
-  const int head0 = kvh * G + h0;            // the CTA's first head, of a sequence's
 
-  long long at = -1;                         // the new row's slot, where it is written
-  bool turn = false;
-  long long pos = 0;
-  if (STEP) {
-    pos = fresh.cos_t ? fresh.positions[seq] : 0;
-    turn = fresh.cos_t && pos >= 0 && pos < fresh.table_rows;
-    at = !fresh.cos_t || turn ? length[seq] : -1;
-    if (at < 0 || at >= slots) at = -1;
-  }
-  // queries in shared memory, rotated: a lane's pieces 8 t4 + 32 i of head g8
-  constexpr int PIECES = D / 16;
-  for (int i = tid; i < AT_HEADS * PIECES; i += THREADS) {
-    const int g = i / PIECES, c = 8 * (i - g * PIECES);
-    uint4 x1 = make_uint4(0, 0, 0, 0), x2 = x1;
-    if (g < heads) {
-      const T* src = q.row(seq, head0 + g) + c;
-      x1 = *reinterpret_cast<const uint4*>(src);
-      x2 = *reinterpret_cast<const uint4*>(src + D / 2);
-      if (turn) rotate8<T>(x1, x2, fresh.cos_t + pos * (D / 2) + c, fresh.sin_t + pos * (D / 2) + c);
+  // Tiles tile0 .. tile1 - 1 of one sequence and task (a KV head and eight of its query heads at most): to `out`, or partial results to `part`.
+  auto segment = [&](int seq, int task, const Visible<AT_SLOTS>& vis, int tile0, int tile1, float* part) {
+    const int kvh = task / chunks, h0 = (task - kvh * chunks) * AT_HEADS, heads = min(AT_HEADS, G - h0), head0 = kvh * G + h0;
+    long long at = -1;                       // the new row's slot, where it is written
+    bool turn = false;
+    long long pos = 0;
+    if (STEP) {
+      pos = fresh.cos_t ? fresh.positions[seq] : 0;
+      turn = fresh.cos_t && pos >= 0 && pos < fresh.table_rows;
+      at = !fresh.cos_t || turn ? length[seq] : -1;
+      if (at < 0 || at >= slots) at = -1;
     }
-    *reinterpret_cast<uint4*>(&s_q[g][c]) = x1;
-    *reinterpret_cast<uint4*>(&s_q[g][c + D / 2]) = x2;
-  }
-  // The new row, by the CTA that will read it (those of other query heads write the same).
-  if (STEP && at >= 0 && tile1 == vis.tiles && tile0 < tile1 && tid < 2 * PIECES) {
-    const int page = table.page_of(pool, seq, at), c = 8 * (tid % PIECES);
-    if (page >= 0) {
-      const bool value = tid >= PIECES;
-      const T* src = (value ? fresh.v : fresh.k).row(seq, kvh) + c;
-      T* dst = (value ? pool.v : pool.k) + (pool.rows(page, kvh) + (at & ((1 << pool.log_page) - 1))) * D + c;
-      uint4 x1 = *reinterpret_cast<const uint4*>(src), x2 = *reinterpret_cast<const uint4*>(src + D / 2);
-      if (turn && !value) rotate8<T>(x1, x2, fresh.cos_t + pos * (D / 2) + c, fresh.sin_t + pos * (D / 2) + c);
-      *reinterpret_cast<uint4*>(dst) = x1;
-      *reinterpret_cast<uint4*>(dst + D / 2) = x2;
+    // queries in shared memory, rotated: a lane's pieces 8 t4 + 32 i of head g8
+    constexpr int PIECES = D / 16;
+    for (int i = tid; i < AT_HEADS * PIECES; i += THREADS) {
+      const int g = i / PIECES, c = 8 * (i - g * PIECES);
+      uint4 x1 = make_uint4(0, 0, 0, 0), x2 = x1;
+      if (g < heads) {
+        const T* src = q.row(seq, head0 + g) + c;
+        x1 = *reinterpret_cast<const uint4*>(src);
+        x2 = *reinterpret_cast<const uint4*>(src + D / 2);
+        if (turn) rotate8<T>(x1, x2, fresh.cos_t + pos * (D / 2) + c, fresh.sin_t + pos * (D / 2) + c);
+      }
+      *reinterpret_cast<uint4*>(&s_q[g][c]) = x1;
+      *reinterpret_cast<uint4*>(&s_q[g][c + D / 2]) = x2;
     }
-  }
-  __syncthreads();
-  const T* mine_q = &s_q[g8][8 * t4];
+    // The new row, by the CTA that will read it (those of other query heads write the same).
+    if (STEP && at >= 0 && tile0 < tile1 && tile1 == vis.tiles && tid < 2 * PIECES) {
+      const int page = table.page_of(pool, seq, at), c = 8 * (tid % PIECES);
+      if (page >= 0) {
+        const bool value = tid >= PIECES;
+        const T* src = (value ? fresh.v : fresh.k).row(seq, kvh) + c;
+        T* dst = (value ? pool.v : pool.k) + (pool.rows(page, kvh) + (at & ((1 << pool.log_page) - 1))) * D + c;
+        uint4 x1 = *reinterpret_cast<const uint4*>(src), x2 = *reinterpret_cast<const uint4*>(src + D / 2);
+        if (turn && !value) rotate8<T>(x1, x2, fresh.cos_t + pos * (D / 2) + c, fresh.sin_t + pos * (D / 2) + c);
+        *reinterpret_cast<uint4*>(dst) = x1;
+        *reinterpret_cast<uint4*>(dst + D / 2) = x2;
+      }
+    }
+    __syncthreads();
+    const T* mine_q = &s_q[g8][8 * t4];
 
-  const float scale2 = scale * 1.4426950408889634f;        // scores in powers of two
-  float m = -INFINITY, l = 0.f;
-  float o[8 * VS][2];                        // MMA j + 8 s: its column n is column 64 s + 8 n + j of the head
+    float m = -INFINITY, l = 0.f;
+    uint64_t o2[8 * VS];                     // MMA j + 8 s: its column n is column 64 s + 8 n + j of the head; n = 2 t4 and 2 t4 + 1
 #pragma unroll
-  for (int i = 0; i < 8 * VS; ++i) o[i][0] = o[i][1] = 0.f;
+    for (int i = 0; i < 8 * VS; ++i) o2[i] = 0;
 
 #pragma unroll 1
-  for (int i = tile0 + warp; i < tile1; i += AT_WARPS) {
-    const int base = vis.tile(i) * AT_SLOTS, page = table.page_of(pool, seq, base);
-    if (page < 0) continue;
-    const size_t row0 = pool.rows(page, kvh) + (base & ((1 << pool.log_page) - 1));
-    uint4 kk[2][KP], vv[4][VS];
+    for (int i = tile0 + warp; i < tile1; i += AT_WARPS) {
+      const int base = vis.tile(i) * AT_SLOTS, page = table.page_of(pool, seq, base);
+      if (page < 0) continue;
+      const size_t row0 = pool.rows(page, kvh) + (base & ((1 << pool.log_page) - 1));
+      uint4 kk[2][KP], vv[4][VS];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int e = 0; e < KP; ++e) kk[h][e] = ld16(pool.k + (row0 + 8 * h + g8) * D + 8 * t4 + 32 * e);
+        for (int e = 0; e < KP; ++e) kk[h][e] = ld16(pool.k + (row0 + 8 * h + g8) * D + 8 * t4 + 32 * e);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int p = 8 * (u >> 1) + 2 * t4 + (u & 1);
+      for (int u = 0; u < 4; ++u) {
+        const int p = 8 * (u >> 1) + 2 * t4 + (u & 1);
 #pragma unroll
-      for (int e = 0; e < VS; ++e) vv[u][e] = vis.sees(base + p) ? ld16(pool.v + (row0 + p) * D + 8 * g8 + 64 * e) : make_uint4(0, 0, 0, 0);
-    }
-    float s[2][2] = {};
+        for (int e = 0; e < VS; ++e) vv[u][e] = vis.sees(base + p) ? ld16(pool.v + (row0 + p) * D + 8 * g8 + 64 * e) : make_uint4(0, 0, 0, 0);
+      }
+      uint64_t pairs[2] = {0, 0};
 #pragma unroll
-    for (int e = 0; e < KP; ++e) {
-      const uint4 qa = *reinterpret_cast<const uint4*>(mine_q + 32 * e);
+      for (int e = 0; e < KP; ++e) {
+        const uint4 qa = *reinterpret_cast<const uint4*>(mine_q + 32 * e);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint64_t d0[2], d1[2];
+          mma<T>(d0, qa.x, 0u, qa.y, 0u, kk[h][e].x, kk[h][e].y);
+          mma<T>(d1, qa.z, 0u, qa.w, 0u, kk[h][e].z, kk[h][e].w);
+          pairs[h] = add2(pairs[h], add2(d0[0], d1[0]));
+        }
+      }
+      float s[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float d0[4], d1[4];
-        mma(d0, qa.x, 0u, qa.y, 0u, kk[h][e].x, kk[h][e].y, T());
-        mma(d1, qa.z, 0u, qa.w, 0u, kk[h][e].z, kk[h][e].w, T());
-        s[h][0] += d0[0] + d1[0];
-        s[h][1] += d0[1] + d1[1];
+        const float2 f = apart(pairs[h]);
+        s[h][0] = f.x, s[h][1] = f.y;
       }
-    }
-    // this lane: head g8, slots base + 8 h + 2 t4 + e
-    bool sees[2][2];
-    float top = m;
+      // this lane: head g8, slots base + 8 h + 2 t4 + e
+      bool sees[2][2];
+      float top = m;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        sees[h][e] = vis.sees(base + 8 * h + 2 * t4 + e);
-        top = fmaxf(top, sees[h][e] ? s[h][e] * scale2 : -INFINITY);
-      }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // A whole number at or above the maximum, so that rescaling sums is exact.  (No finite score so far: weights 0, or NaN
-    // where a score is NaN, which no maximum shows.)
-    top = ceilf(top);
-    const float ref = top == -INFINITY ? 0.f : top;
-    const float keep = whole_pow2(m - ref);
-    m = top;
-    // weights times 2^15: fp16's halves of their split then reach down to 2^-38 of the largest
-    float w[2][2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) w[h][e] = sees[h][e] ? 32768.f * ex2(__fmaf_rn(s[h][e], scale2, -ref)) : 0.f;
-    l = l * keep + ((w[0][0] + w[0][1]) + (w[1][0] + w[1][1]));
-    const uint2 w0 = split_weights<T>(w[0][0], w[0][1]), w1 = split_weights<T>(w[1][0], w[1][1]);
-#pragma unroll
-    for (int e = 0; e < VS; ++e) {
-      const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vv[0][e]);
-      const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vv[1][e]);
-      const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vv[2][e]);
-      const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vv[3][e]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-        float d[4];
-        mma(d, w0.x, w0.y, w1.x, w1.y, __byte_perm(v0[j >> 1], v1[j >> 1], sel), __byte_perm(v2[j >> 1], v3[j >> 1], sel), T());
-        o[8 * e + j][0] = o[8 * e + j][0] * keep + (d[0] + d[2]);
-        o[8 * e + j][1] = o[8 * e + j][1] * keep + (d[1] + d[3]);
-      }
-    }
-  }
-  l += __shfl_xor_sync(0xffffffffu, l, 1);
-  l += __shfl_xor_sync(0xffffffffu, l, 2);
-  if (t4 == 0) {
-    s_m[warp][g8] = m;
-    s_l[warp][g8] = l;
-  }
-#pragma unroll
-  for (int e = 0; e < VS; ++e)
-#pragma unroll
-    for (int c = 0; c < 2; ++c)              // columns n = 2 t4 + c
-#pragma unroll
-      for (int j = 0; j < 8; j += 4)
-        *reinterpret_cast<float4*>(&s_sum[warp][g8][64 * e + 8 * (2 * t4 + c) + j]) =
-            make_float4(o[8 * e + j][c], o[8 * e + j + 1][c], o[8 * e + j + 2][c], o[8 * e + j + 3][c]);
-  __syncthreads();
-  for (int i = tid; i < heads * D / 4; i += THREADS) {
-    const int g = i / (D / 4), d = 4 * (i - g * (D / 4));
-    float top = s_m[0][g];
-#pragma unroll
-    for (int w = 1; w < AT_WARPS; ++w) top = fmaxf(top, s_m[w][g]);
-    float tot = 0.f, sum[4] = {};
-#pragma unroll
-    for (int w = 0; w < AT_WARPS; ++w) {
-      const float f = share_of(s_m[w][g], s_l[w][g], top);
-      const float4 x = *reinterpret_cast<const float4*>(&s_sum[w][g][d]);
-      tot += f * s_l[w][g];
-      sum[0] += f * x.x, sum[1] += f * x.y, sum[2] += f * x.z, sum[3] += f * x.w;
-    }
-    if (!(fabsf(sum[0]) + fabsf(sum[1]) + fabsf(sum[2]) + fabsf(sum[3]) <= 3.0e38f) && tot == tot) {
-      // An infinite or NaN value takes part.  The two halves of a weight turn infinity into NaN where the product does
-      // not: these columns are added again, weight by weight.
-      sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
-      for (int t = tile0; t < tile1; ++t)
-        for (int j = vis.tile(t) * AT_SLOTS, end = j + AT_SLOTS; j < end; ++j) {
-          const int page = vis.sees(j) ? table.page_of(pool, seq, j) : -1;
-          if (page < 0) continue;
-          const size_t row = pool.rows(page, kvh) + (j & ((1 << pool.log_page) - 1));
-          float dot = 0.f;
-          for (int c = 0; c < D; ++c) dot += Type<T>::one(s_q[g][c]) * Type<T>::one(pool.k[row * D + c]);
-          const float w = 32768.f * ex2(__fmaf_rn(dot, scale2, top == -INFINITY ? 0.f : -top));
-#pragma unroll
-          for (int c = 0; c < 4; ++c) sum[c] += w * Type<T>::one(pool.v[row * D + d + c]);
+        for (int e = 0; e < 2; ++e) {
+          sees[h][e] = vis.sees(base + 8 * h + 2 * t4 + e);
+          top = fmaxf(top, sees[h][e] ? s[h][e] * scale2 : -INFINITY);
         }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // A whole number at or above the maximum, so that rescaling sums is exact.  (No finite score so far: weights 0, or NaN
+      // where a score is NaN, which no maximum shows.)
+      top = ceilf(top);
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float keep = whole_pow2(m - ref);
+      const uint64_t keep2 = two(keep, keep);
+      m = top;
+      float w[2][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) w[h][e] = sees[h][e] ? LIFT * ex2(__fmaf_rn(s[h][e], scale2, -ref)) : 0.f;
+      l = l * keep + ((w[0][0] + w[0][1]) + (w[1][0] + w[1][1]));
+      const uint2 w0 = split_weights<T>(w[0][0], w[0][1]), w1 = split_weights<T>(w[1][0], w[1][1]);
+#pragma unroll
+      for (int e = 0; e < VS; ++e) {
+        const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vv[0][e]);
+        const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vv[1][e]);
+        const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vv[2][e]);
+        const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vv[3][e]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+          uint64_t d[2];
+          mma<T>(d, w0.x, w0.y, w1.x, w1.y, __byte_perm(v0[j >> 1], v1[j >> 1], sel), __byte_perm(v2[j >> 1], v3[j >> 1], sel));
+          o2[8 * e + j] = fma2(o2[8 * e + j], keep2, add2(d[0], d[1]));
+        }
+      }
     }
-    const size_t head = (size_t)seq * H + head0 + g;
-    if (nsplit == 1) {
-      const bool none = tot == 0.f;          // no slot is visible (a visible one's weight is not 0)
-      *reinterpret_cast<uint2*>(out + head * D + d) =
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    if (t4 == 0) {
+      s_m[warp][g8] = m;
+      s_l[warp][g8] = l;
+    }
+#pragma unroll
+    for (int e = 0; e < VS; ++e)
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {       // columns n = 2 t4 and 2 t4 + 1
+        const float2 x0 = apart(o2[8 * e + j]), x1 = apart(o2[8 * e + j + 1]), x2 = apart(o2[8 * e + j + 2]), x3 = apart(o2[8 * e + j + 3]);
+        *reinterpret_cast<float4*>(&s_sum[warp][g8][64 * e + 16 * t4 + j]) = make_float4(x0.x, x1.x, x2.x, x3.x);
+        *reinterpret_cast<float4*>(&s_sum[warp][g8][64 * e + 16 * t4 + 8 + j]) = make_float4(x0.y, x1.y, x2.y, x3.y);
+      }
+    __syncthreads();
+    for (int i = tid; i < heads * D / 4; i += THREADS) {
+      const int g = i / (D / 4), d = 4 * (i - g * (D / 4));
+      float top = s_m[0][g];
+#pragma unroll
+      for (int w = 1; w < AT_WARPS; ++w) top = fmaxf(top, s_m[w][g]);
+      float tot = 0.f, sum[4] = {};
+#pragma unroll
+      for (int w = 0; w < AT_WARPS; ++w) {
+        const float f = share_of(s_m[w][g], s_l[w][g], top);
+        const float4 x = *reinterpret_cast<const float4*>(&s_sum[w][g][d]);
+        tot += f * s_l[w][g];
+        sum[0] += f * x.x, sum[1] += f * x.y, sum[2] += f * x.z, sum[3] += f * x.w;
+      }
+      if (!(fabsf(sum[0]) + fabsf(sum[1]) + fabsf(sum[2]) + fabsf(sum[3]) <= 3.0e38f) && tot == tot) {
+        // An infinite or NaN value takes part.  The two halves of a weight turn infinity into NaN where the product does
+        // not: these columns are added again, weight by weight.
+        sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+        for (int t = tile0; t < tile1; ++t)
+          for (int j = vis.tile(t) * AT_SLOTS, end = j + AT_SLOTS; j < end; ++j) {
+            const int page = vis.sees(j) ? table.page_of(pool, seq, j) : -1;
+            if (page < 0) continue;
+            const size_t row = pool.rows(page, kvh) + (j & ((1 << pool.log_page) - 1));
+            float dot = 0.f;
+            for (int c = 0; c < D; ++c) dot += Type<T>::one(s_q[g][c]) * Type<T>::one(pool.k[row * D + c]);
+            const float w = LIFT * ex2(__fmaf_rn(dot, scale2, top == -INFINITY ? 0.f : -top));
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum[c] += w * Type<T>::one(pool.v[row * D + d + c]);
+          }
+      }
+      if (part) {
+        float* mine = part + g * (D + PART);
+        *reinterpret_cast<float4*>(mine + PART + d) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        if (d == 0) *reinterpret_cast<float2*>(mine) = make_float2(top, tot);
+      } else {
+        const bool none = tot == 0.f;        // no slot is visible (a visible one's weight is not 0)
+        *reinterpret_cast<uint2*>(out + ((size_t)seq * H + head0 + g) * D + d) =
+            none ? make_uint2(0u, 0u) : make_uint2(Type<T>::pair(sum[0] / tot, sum[1] / tot), Type<T>::pair(sum[2] / tot, sum[3] / tot));
+      }
+    }
+  };
+
+  if constexpr (CLUSTER) {
+    const int rank = blockIdx.x, n = gridDim.x, task = blockIdx.y, seq = blockIdx.z;
+    const Visible<AT_SLOTS> vis(held(length, seq, STEP, slots), shape.window, shape.sinks);
+    const int each = (vis.tiles + n - 1) / n, tile0 = min(vis.tiles, rank * each), tile1 = min(vis.tiles, tile0 + each);
+    segment(seq, task, vis, tile0, tile1, n > 1 ? &s_part[0][0] : nullptr);
+    if (n == 1) return;
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    const int kvh = task / chunks, h0 = (task - kvh * chunks) * AT_HEADS, heads = min(AT_HEADS, G - h0), head0 = kvh * G + h0;
+    // an equal share of the columns for every CTA
+    for (int i = rank * THREADS + tid; i < heads * D / 4; i += n * THREADS) {
+      const int g = i / (D / 4), d = 4 * (i - g * (D / 4));
+      auto from = [&](int r, int c) {
+        uint32_t to;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"((uint32_t)__cvta_generic_to_shared(&s_part[g][c])), "r"(r));
+        return to;
+      };
+      float m[MAX_CLUSTER], l[MAX_CLUSTER], top = -INFINITY, tot = 0.f, sum[4] = {};
+      float4 x[MAX_CLUSTER];
+#pragma unroll
+      for (int r = 0; r < MAX_CLUSTER; ++r) {
+        m[r] = -INFINITY, l[r] = 0.f, x[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < n) {
+          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(m[r]), "=f"(l[r]) : "r"(from(r, 0)) : "memory");
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[r].x), "=f"(x[r].y), "=f"(x[r].z), "=f"(x[r].w) : "r"(from(r, PART + d)) : "memory");
+        }
+        top = fmaxf(top, m[r]);
+      }
+#pragma unroll
+      for (int r = 0; r < MAX_CLUSTER; ++r)
+        if (r < n) {
+          const float f = share_of(m[r], l[r], top);
+          tot += f * l[r];
+          sum[0] += f * x[r].x, sum[1] += f * x[r].y, sum[2] += f * x[r].z, sum[3] += f * x[r].w;
+        }
+      const bool none = tot == 0.f;
+      *reinterpret_cast<uint2*>(out + ((size_t)seq * H + head0 + g) * D + d) =
           none ? make_uint2(0u, 0u) : make_uint2(Type<T>::pair(sum[0] / tot, sum[1] / tot), Type<T>::pair(sum[2] / tot, sum[3] / tot));
-    } else {
-      float* mine = part + (head * nsplit + split) * (size_t)(D + 4);
-      *reinterpret_cast<float4*>(mine + 4 + d) = make_float4(sum[0], sum[1], sum[2], sum[3]);
-      if (d == 0) *reinterpret_cast<float2*>(mine) = make_float2(top, tot);
     }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    const int cta = blockIdx.x, ctas = gridDim.x, B = shape.sequences;
+    auto visible = [&](int s) { return Visible<AT_SLOTS>(held(length, s, STEP, slots), shape.window, shape.sinks); };
+    // Lengths of 32 sequences at a time: all tiles, then those in front of the CTA's.
+    long long all = 0, before = 0;
+    int mine = 0, upto = 0;                  // of the lane's sequence in the last 32, and of those in front of it and its own
+    auto scan = [&](int s) {
+      mine = upto = s + lane < B ? visible(s + lane).tiles : 0;
+      for (int d = 1; d < 32; d *= 2) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += y;
+      }
+      return (long long)__shfl_sync(0xffffffffu, upto, 31);
+    };
+    for (int s = 0; s < B; s += 32) all += scan(s);
+    all *= heads_each;
+    // tiles of a CTA: for each warp one at least
+    const long long each = max((long long)AT_WARPS, quotient(all + ctas - 1, ctas));
+    const long long begin = min(all, each * cta), end = min(all, begin + each);
+    int seq = 0;
+    long long from = 0;                      // where the sequence's tiles begin
+    if (begin < end)
+      for (int s = 0;; s += 32) {
+        const long long these = B <= 32 ? all / heads_each : scan(s);
+        if (begin < (before + these) * heads_each) {
+          const int k = __ffs(__ballot_sync(0xffffffffu, begin < (before + upto) * heads_each)) - 1;
+          seq = s + k;
+          from = (before + __shfl_sync(0xffffffffu, upto - mine, k)) * heads_each;
+          break;
+        }
+        before += these;
+      }
+    Span mark = {0, 0, 0, 0};
+    if (begin < end) {
+      long long x = begin;
+      Visible<AT_SLOTS> vis = visible(seq);
+#pragma unroll 1
+      while (true) {
+        const int task = (int)quotient(x - from, vis.tiles);
+        const long long begins = from + (long long)task * vis.tiles, ends = begins + vis.tiles;
+        const int tile0 = (int)(x - begins), tile1 = (int)(min(end, ends) - begins);
+        float* part = tile0 > 0 ? part_of<D>(ws, ctas, cta, 0) : (tile1 < vis.tiles ? part_of<D>(ws, ctas, cta, 1) : nullptr);
+        segment(seq, task, vis, tile0, tile1, part);
+        if (tile0 == 0 && tile1 < vis.tiles) {
+          const int kvh = task / chunks, h0 = (task - kvh * chunks) * AT_HEADS;
+          mark = {(int)quotient(ends - 1, each) - cta + 1, seq, kvh * G + h0, min(AT_HEADS, G - h0)};
+        }
+        x = begins + tile1;
+        if (x >= end) break;
+        if (x == from + (long long)vis.tiles * heads_each) {
+          from = x;
+          do vis = visible(++seq);
+          while (vis.tiles == 0);
+        }
+        __syncthreads();
+      }
+    }
+    if (tid == 0) reinterpret_cast<Span*>(ws)[cta] = mark;
+    // (sequences that see nothing)
+    for (int s = cta; s < B; s += ctas)
+      if (visible(s).tiles == 0)
+        for (int i = tid; i < H * D / 8; i += THREADS) reinterpret_cast<uint4*>(out + (size_t)s * H * D)[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
-// joins a head's ranges: a warp a head, D / 32 columns a lane
+// joins the partial results of heads that several CTAs share: a block for the first of these; a warp a head, more where there are few
 template <typename T, int D>
-__global__ void __launch_bounds__(256) pages_join_kernel(const float* __restrict__ part, int nsplit, long long heads, T* __restrict__ out) {
+__global__ void __launch_bounds__(32 * AT_HEADS) pages_join_kernel(void* ws, int H, T* __restrict__ out) {
   constexpr int CPL = D / 32;
+  __shared__ float s_sum[AT_HEADS][D], s_top[AT_HEADS], s_tot[AT_HEADS];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const long long head = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (head >= heads) return;
-  const float* mine = part + (size_t)head * nsplit * (D + 4);
-  const float2 ml = lane < nsplit ? *reinterpret_cast<const float2*>(mine + (size_t)lane * (D + 4)) : make_float2(-INFINITY, 0.f);
-  float top = ml.x;
-  for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  const float f = share_of(ml.x, ml.y, top);
-  float tot = f * ml.y, sum[CPL] = {};
-  for (int d = 16; d; d /= 2) tot += __shfl_xor_sync(0xffffffffu, tot, d);
+  const int cta = blockIdx.x, ctas = gridDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Span span = reinterpret_cast<const Span*>(ws)[cta];
+  if (span.parts == 0) return;
+  const int groups = AT_HEADS / span.heads, g = warp / groups, group = warp - g * groups;
+  auto part = [&](int r) { return part_of<D>(ws, ctas, cta + r, r == 0) + g * (D + PART); };
+  float top = -INFINITY, tot = 0.f, sum[CPL] = {};
+  if (g < span.heads) {
+    for (int r = group + lane * groups; r < span.parts; r += 32 * groups) top = fmaxf(top, part(r)[0]);
+    for (int d = 16; d; d /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
 #pragma unroll 8
-  for (int r = 0; r < nsplit; ++r) {
-    const float fr = __shfl_sync(0xffffffffu, f, r);
+    for (int r = group; r < span.parts; r += groups) {
+      const float* p = part(r);
+      const float2 ml = *reinterpret_cast<const float2*>(p);
+      const float f = share_of(ml.x, ml.y, top);
+      tot += f * ml.y;
 #pragma unroll
-    for (int i = 0; i < CPL; i += 2) {
-      const float2 x = *reinterpret_cast<const float2*>(mine + r * (D + 4) + 4 + CPL * lane + i);
-      sum[i] = __fmaf_rn(fr, x.x, sum[i]);
-      sum[i + 1] = __fmaf_rn(fr, x.y, sum[i + 1]);
+      for (int i = 0; i < CPL; i += 2) {
+        const float2 x = *reinterpret_cast<const float2*>(p + PART + CPL * lane + i);
+        sum[i] = __fmaf_rn(f, x.x, sum[i]);
+        sum[i + 1] = __fmaf_rn(f, x.y, sum[i + 1]);
+      }
     }
   }
-  const bool none = tot == 0.f;
 #pragma unroll
-  for (int i = 0; i < CPL; i += 2)
-    *reinterpret_cast<uint32_t*>(out + head * D + CPL * lane + i) = none ? 0u : Type<T>::pair(sum[i] / tot, sum[i + 1] / tot);
+  for (int i = 0; i < CPL; ++i) s_sum[warp][CPL * lane + i] = sum[i];
+  if (lane == 0) s_top[warp] = top, s_tot[warp] = tot;
+  __syncthreads();
+  if (g >= span.heads || group) return;
+  float best = -INFINITY;
+  for (int k = 0; k < groups; ++k) best = fmaxf(best, s_top[warp + k]);
+  tot = 0.f;
+#pragma unroll
+  for (int i = 0; i < CPL; ++i) sum[i] = 0.f;
+  for (int k = 0; k < groups; ++k) {
+    if (s_top[warp + k] == -INFINITY && s_tot[warp + k] == 0.f) continue;
+    const float f = share_of(s_top[warp + k], s_tot[warp + k], best);
+    tot += f * s_tot[warp + k];
+#pragma unroll
+    for (int i = 0; i < CPL; ++i) sum[i] = __fmaf_rn(f, s_sum[warp + k][CPL * lane + i], sum[i]);
+  }
+  const bool none = tot == 0.f;
+  T* to = out + ((size_t)span.seq * H + span.head + g) * D + CPL * lane;
+#pragma unroll
+  for (int i = 0; i < CPL; i += 2) *reinterpret_cast<uint32_t*>(to + i) = none ? 0u : Type<T>::pair(sum[i] / tot, sum[i + 1] / tot);
 }
 
-// ranges that a head's slots are cut into: what fills the SMs with three CTAs, four turns a warp at least
-int splits_of(const cq_pages* pages, const cq_table* table, int n_heads, int window, int sinks) {
-  const int KV = pages->n_kv_heads, chunks = (n_heads / KV + AT_HEADS - 1) / AT_HEADS;
-  const long long tasks = (long long)table->sequences * KV * chunks, all = (long long)table->width * pages->page_size;
-  const long long most = window ? std::min<long long>(all, (long long)window + sinks + AT_SLOTS) : all;
-  return (int)std::max<long long>(1, std::min<long long>({32, 3 * cq_sm_count() / tasks, most / (4 * AT_WARPS * AT_SLOTS)}));
+// CTAs of a cluster for each sequence and task, 0: equal ranges.  The least time by a model (us): waves of CTAs, each its start and the
+// turns of a warp, which take longer the fuller the SMs are; joins; for ranges what all warps need together, a start for every task and
+// the second kernel.  It goes by the table's width: lengths are known to the device alone.  (16 sequences of 64 / 8 heads up to
+// 4001 slots: 1 CTA 81 us, 2 54, 3 41, 4 51, 8 50, ranges 49; 8 of 40 heads, window 1021: 1 34, 2 39, ranges 40; 4 of 64 / 8 heads,
+// 65531 slots: 8 208, ranges 174; 1 of 32 heads, 256 slots: 1 8.0, 6 6.0, ranges 12.6; 55 of 16 / 4 heads, 2 slots: 1 4.5, ranges 14.7.)
+int plan_of(const cq_pages* pages, const cq_table* table, int n_heads, int window, int sinks) {
+  const int KV = pages->n_kv_heads, chunks = (n_heads / KV + AT_HEADS - 1) / AT_HEADS, sms = cq_sm_count(), slots = per_sm(pages->head_dim) * sms;
+  const bool narrow = pages->head_dim == 64;
+  const double tasks = (double)table->sequences * KV * chunks;
+  const long long all = (long long)table->width * pages->page_size;
+  const long long most = window ? std::min<long long>(all, (long long)window + sinks + AT_SLOTS) : all, tiles = (most + AT_SLOTS - 1) / AT_SLOTS;
+  const double full = narrow ? 1.48 : 2.2;                 // a turn of all warps that the SMs hold
+  double least = 9 + 2.5 * (1 + tasks / slots) + std::max(1.0, tasks * tiles / (slots * AT_WARPS)) * full;
+  int best = 0;
+  for (int n = 1; n <= MAX_CLUSTER; ++n) {
+    if (n > 1 && (n - 1) * AT_WARPS >= tiles) break;
+    const double ctas = tasks * n, each = std::min((double)per_sm(pages->head_dim), std::max(1.0, ctas / sms));
+    const double turn = narrow ? std::max(0.85 + 0.1 * each, 0.37 * each) : std::max(1.0 + 0.3 * each, 0.74 * each);
+    const double t = 1.2 + std::ceil(ctas / slots) * (((tiles + n * AT_WARPS - 1) / (n * AT_WARPS)) * turn + 2.1) + (n > 1 ? 0.9 + 0.05 * n : 0.0);
+    if (t < least) {
+      least = t;
+      best = n;
+    }
+  }
+  return best;
 }
 
 template <typename T, int D>
 int attend(const cq_pages* pages, const cq_table* table, const cq_rows* q, const cq_rows* k, const cq_rows* v, const float* cos_t, const float* sin_t,
            const long long* positions, int table_rows, const long long* length, void* out, int H, int window, int sinks, float scale, void* workspace,
            cudaStream_t stream) {
-  const int KV = pages->n_kv_heads, chunks = (H / KV + AT_HEADS - 1) / AT_HEADS, nsplit = splits_of(pages, table, H, window, sinks);
+  const int KV = pages->n_kv_heads, chunks = (H / KV + AT_HEADS - 1) / AT_HEADS, cluster = plan_of(pages, table, H, window, sinks), ctas = per_sm(D) * cq_sm_count();
   const NewRow<T> fresh = {rows_of<T>(k), rows_of<T>(v), cos_t, sin_t, positions, table_rows};
-  CQ_CUDA_TRY(kv4_launch(k ? pages_attend_kernel<T, D, true> : pages_attend_kernel<T, D, false>, dim3(nsplit, KV * chunks, table->sequences),
-                         dim3(AT_WARPS * 32), 0, stream, rows_of<T>(q), pool_of<T>(pages), table_of(table), fresh, length, (T*)out, (float*)workspace, H,
-                         chunks, window, sinks, scale));
-  if (nsplit > 1) {
-    const long long heads = (long long)table->sequences * H;
-    CQ_CUDA_TRY(kv4_launch(pages_join_kernel<T, D>, dim3((unsigned)((heads + 7) / 8)), dim3(256), 0, stream, (const float*)workspace, nsplit, heads, (T*)out));
-  }
+  const Shape shape = {table->sequences, H, chunks, window, sinks, ctas, scale};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = cluster ? dim3(cluster, KV * chunks, table->sequences) : dim3(ctas);
+  cfg.blockDim = dim3(AT_WARPS * 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster ? 2 : 1;
+  auto fn = cluster ? (k ? pages_attend_kernel<T, D, true, true> : pages_attend_kernel<T, D, false, true>)
+                    : (k ? pages_attend_kernel<T, D, true, false> : pages_attend_kernel<T, D, false, false>);
+  CQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, rows_of<T>(q), pool_of<T>(pages), table_of(table), fresh, length, (T*)out, workspace, shape));
+  if (!cluster) CQ_CUDA_TRY(kv4_launch(pages_join_kernel<T, D>, dim3(ctas), dim3(32 * AT_HEADS), 0, stream, workspace, H, (T*)out));
   return CQ_OK;
 }
 
@@ -346,8 +535,8 @@ int call(const cq_pages* pages, const cq_table* table, const cq_rows* q, const c
 
 extern "C" size_t cq_pages_attend_workspace_bytes(const cq_pages* pages, const cq_table* table, int n_heads, int window, int sinks) {
   if (check(pages, table) != CQ_OK || n_heads < 1 || n_heads % pages->n_kv_heads || window < 0 || sinks < 0) return 0;
-  const int nsplit = splits_of(pages, table, n_heads, window, sinks);
-  return nsplit > 1 ? (size_t)table->sequences * n_heads * nsplit * (pages->head_dim + 4) * 4 : 0;
+  if (plan_of(pages, table, n_heads, window, sinks)) return 0;
+  return (size_t)per_sm(pages->head_dim) * cq_sm_count() * (sizeof(Span) + 2 * AT_HEADS * (pages->head_dim + PART) * sizeof(float));
 }
 
 extern "C" int cq_pages_attend(const cq_pages* pages, const cq_table* table, const cq_rows* q, const long long* length, void* out, int n_heads,
