@@ -19,7 +19,7 @@ namespace {
 
 using namespace cq_paged;
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, TOKENS = 2, SLOTS = 2;
 
 // The sequence of packed row t: the last one that starts at or before it, -1 in front of the first and behind the last.
 __device__ __forceinline__ int sequence_of(const long long* __restrict__ starts, int sequences, long long t) {
@@ -34,74 +34,83 @@ __device__ __forceinline__ int sequence_of(const long long* __restrict__ starts,
 }
 
 // D / 16 lanes a row of q, k or v, eight columns of each half of the head a lane: q and k rotated, q to q_out, k and v to their
-// slots.  A block takes as many rows of one head as it has rows of lanes.
+// slots.  The bound is memory: a block takes 16 or 32 heads of two tokens, whose angles, positions and slots it reads once, and writes
+// beside one another what lies so (2048 tokens of 40 heads 21 us, 5.9 TB/s; with a block for the rows of one head, which reads
+// 512 bytes of angles for 256 of a row, 32; one token 21, four 22, sixteen 25).
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS) pages_write_kernel(const Rows<T> q, T* __restrict__ q_out, const Rows<T> k, const Rows<T> v,
                                                               const float* __restrict__ cos_t, const float* __restrict__ sin_t,
                                                               const long long* __restrict__ positions, int table_rows,
                                                               const long long* __restrict__ first, const long long* __restrict__ starts, const Pool<T> pool,
                                                               const Table table, int sequences, int rows, int H) {
-  constexpr int LANES = D / 16, ROWS = THREADS / LANES;
+  constexpr int LANES = D / 16, HEADS = THREADS / LANES / TOKENS;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int j = blockIdx.y, KV = pool.heads, c = 8 * (threadIdx.x % LANES);
-  const long long t = (long long)blockIdx.x * ROWS + threadIdx.x / LANES;
-  if (t >= rows) return;
+  const int r = threadIdx.x / LANES, j = blockIdx.y * HEADS + r % HEADS, KV = pool.heads, c = 8 * (threadIdx.x % LANES);
+  const long long t = (long long)blockIdx.x * TOKENS + r / HEADS;
+  if (t >= rows || j >= H + 2 * KV) return;
   const bool is_q = j < H, is_k = !is_q && j < H + KV;
   const int head = is_q ? j : (is_k ? j - H : j - H - KV);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const T* src = (is_q ? q : (is_k ? k : v)).row(t, head) + c;
   uint4 x1 = *reinterpret_cast<const uint4*>(src), x2 = *reinterpret_cast<const uint4*>(src + D / 2);
   const long long pos = cos_t ? positions[t] : 0;
   const bool turn = cos_t && pos >= 0 && pos < table_rows;
-  if (turn && (is_q || is_k)) rotate8<T>(x1, x2, cos_t + pos * (D / 2) + c, sin_t + pos * (D / 2) + c);
-  T* to;
+  T* to = nullptr;
   if (is_q) {
     to = q_out + (t * H + head) * D + c;
-  } else {
-    // a key without a position in the tables is left out, and its value with it
-    if (cos_t && !turn) return;
+  } else if (!cos_t || turn) {               // (a key without a position in the tables is left out, and its value with it)
     const int each = rows / sequences, s = starts ? sequence_of(starts, sequences, t) : (int)(t / each);
-    if (s < 0) return;
-    const long long slot = first[s] + t - (starts ? starts[s] : (long long)s * each);
-    const int page = slot < 0 ? -1 : table.page_of(pool, s, slot);
-    if (page < 0) return;
-    to = (is_k ? pool.k : pool.v) + (pool.rows(page, head) + (slot & ((1 << pool.log_page) - 1))) * D + c;
+    if (s >= 0) {
+      const long long slot = first[s] + t - (starts ? starts[s] : (long long)s * each);
+      const int page = slot < 0 ? -1 : table.page_of(pool, s, slot);
+      if (page >= 0) to = (is_k ? pool.k : pool.v) + (pool.rows(page, head) + (slot & ((1 << pool.log_page) - 1))) * D + c;
+    }
   }
+  if (turn && (is_q || is_k)) rotate8<T>(x1, x2, cos_t + pos * (D / 2) + c, sin_t + pos * (D / 2) + c);
+  if (!to) return;
   *reinterpret_cast<uint4*>(to) = x1;
   *reinterpret_cast<uint4*>(to + D / 2) = x2;
 }
 
-// D / 8 lanes a row, 16 bytes each: k and v (sequence, count, KV, D).  Slots without a page read as zeros.
+// D / 8 lanes a row, 16 bytes of its key and of its value each: k and v (sequence, count, KV, D).  Slots without a page read as zeros.
+// A block takes the heads of two slots, whose rows lie one behind the other where they are written (5 x 2001 slots of 40 heads 64 us,
+// 6.4 TB/s; a head's slots, one behind the other where they are read, 70).
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS) pages_read_kernel(const Pool<T> pool, const Table table, const long long* __restrict__ first, int count,
                                                              T* __restrict__ k, T* __restrict__ v) {
-  constexpr int LANES = D / 8, ROWS = THREADS / LANES;
+  constexpr int LANES = D / 8, HEADS = THREADS / LANES / SLOTS;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int s = blockIdx.z, r = threadIdx.x / LANES, head = blockIdx.y * HEADS + r % HEADS, c = 8 * (threadIdx.x % LANES);
+  const int i = blockIdx.x * SLOTS + r / HEADS;
+  if (i >= count || head >= pool.heads) return;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int s = blockIdx.z, head = blockIdx.y >> 1, c = 8 * (threadIdx.x % LANES), i = blockIdx.x * ROWS + threadIdx.x / LANES;
-  if (i >= count) return;
-  const bool value = blockIdx.y & 1;
   const long long slot = first[s] + i;
   const int page = slot < 0 ? -1 : table.page_of(pool, s, slot);
-  uint4 x = make_uint4(0, 0, 0, 0);
-  if (page >= 0) x = *reinterpret_cast<const uint4*>((value ? pool.v : pool.k) + (pool.rows(page, head) + (slot & ((1 << pool.log_page) - 1))) * D + c);
-  *reinterpret_cast<uint4*>((value ? v : k) + (((size_t)s * count + i) * pool.heads + head) * D + c) = x;
+  uint4 x = make_uint4(0, 0, 0, 0), y = x;
+  if (page >= 0) {
+    const size_t at = (pool.rows(page, head) + (slot & ((1 << pool.log_page) - 1))) * D + c;
+    x = *reinterpret_cast<const uint4*>(pool.k + at);
+    y = *reinterpret_cast<const uint4*>(pool.v + at);
+  }
+  const size_t to = (((size_t)s * count + i) * pool.heads + head) * D + c;
+  *reinterpret_cast<uint4*>(k + to) = x;
+  *reinterpret_cast<uint4*>(v + to) = y;
 }
 
 template <typename T, int D>
 int write(const cq_pages* pages, const cq_table* table, const cq_rows* q, void* q_out, const cq_rows* k, const cq_rows* v, const float* cos_t,
           const float* sin_t, const long long* positions, int table_rows, const long long* first, const long long* starts, int rows, int H,
           cudaStream_t stream) {
-  constexpr int ROWS = THREADS / (D / 16);
-  CQ_CUDA_TRY(kv4_launch(pages_write_kernel<T, D>, dim3((rows + ROWS - 1) / ROWS, H + 2 * pages->n_kv_heads), dim3(THREADS), 0, stream,
+  constexpr int HEADS = THREADS / (D / 16) / TOKENS;
+  CQ_CUDA_TRY(kv4_launch(pages_write_kernel<T, D>, dim3((rows + TOKENS - 1) / TOKENS, (H + 2 * pages->n_kv_heads + HEADS - 1) / HEADS), dim3(THREADS), 0, stream,
                          rows_of<T>(H ? q : nullptr), (T*)q_out, rows_of<T>(k), rows_of<T>(v), cos_t, sin_t, positions, table_rows, first, starts,
                          pool_of<T>(pages), table_of(table), table->sequences, rows, H));
   return CQ_OK;
 }
 template <typename T, int D>
 int read(const cq_pages* pages, const cq_table* table, const long long* first, int count, void* k, void* v, cudaStream_t stream) {
-  constexpr int ROWS = THREADS / (D / 8);
-  CQ_CUDA_TRY(kv4_launch(pages_read_kernel<T, D>, dim3((count + ROWS - 1) / ROWS, 2 * pages->n_kv_heads, table->sequences), dim3(THREADS), 0, stream,
+  constexpr int HEADS = THREADS / (D / 8) / SLOTS;
+  CQ_CUDA_TRY(kv4_launch(pages_read_kernel<T, D>, dim3((count + SLOTS - 1) / SLOTS, (pages->n_kv_heads + HEADS - 1) / HEADS, table->sequences), dim3(THREADS), 0, stream,
                          pool_of<T>(pages), table_of(table), first, count, (T*)k, (T*)v));
   return CQ_OK;
 }
