@@ -1,13 +1,15 @@
 // Logits on their way to a token: penalties for tokens that occurred, biases of single tokens, a grammar's bit mask, and the largest.
 //
 // The bound is the logits' traffic, each read once and written once; penalties are the business of few tokens and are settled token by
-// token, beside it.  The tokens that occurred or have a bias are marked in a bit map; a token's rank among the marked ones is its
-// place in arrays of as many entries, where occurrences are counted (integer additions: their order changes nothing).  The pass over the
-// logits leaves the marked ones out of the maximum; their values are written over its results.  (Penalties in that pass took 57
-// instructions a logit, 256 rows of 131071 138 us; counters for all tokens, a slice of the vocabulary after the other, 87.)
-// Every thread has four pieces of 16 bytes on the way, copied asynchronously to places of its own, and waits for no other
-// thread.  Of eight logits only the largest meets the thread's best.  The largest travels as one 64-bit key, its value in the
-// order of unsigned numbers above the complement of its token: the maximum of keys is the lowest token of the largest value.
+// token, beside it.  The tokens that occurred or have a bias are marked in a bit map, occurrences are counted in shared memory (integer
+// additions: their order changes nothing): in a place for every token where a CTA's part of the vocabulary is small, else in
+// the marked tokens' places, a token's rank among them.  The pass over the logits leaves the marked ones out of the maximum;
+// their values are written over its results.  (256 rows of 131071 bf16 logits, histories of 1500 and masks: 31 us; penalties in the pass take 57
+// instructions a logit, 138 us; counters for all tokens, a slice of the vocabulary after the other, 87.  A row of 32000
+// with a history of 300 4.8 us, without 3.4.)  Every thread has four pieces of 16 bytes on the way, copied asynchronously to places of its
+// own, and waits for no other thread; what no mask changes is neither converted nor rounded.  Of eight logits only the largest
+// meets the thread's best.  The largest travels as one 64-bit key, its value in the order of unsigned numbers above the
+// complement of its token: the maximum of keys is the lowest token of the largest value.
 #include <algorithm>
 #include <type_traits>
 
@@ -19,6 +21,7 @@ constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int STAGES = 4;                    // pieces of 16 bytes of a thread on their way
 constexpr int PARTS = 8;                     // CTAs of a row, at most
 constexpr int TOKENS = 4 * THREADS;          // of the history, loads in flight
+constexpr int FEW = 8192;                    // tokens of a slice with a place each, at most
 constexpr int SLICE = 129 * 1024;            // tokens that the bit map holds
 constexpr int PLACES = STAGES * THREADS * 16 / 12;          // marked tokens at a time, in the pieces' memory
 // what is known of a token: whether it occurred in the prompt, whether it has a bias, and below how often it was generated
@@ -28,6 +31,7 @@ struct Adjust {
   cq_adjust a;
   int vocab, part, slice;                    // logits of a row, of a CTA, and of the bit map
   int keep;                                  // tokens of the history in shared memory
+  bool alike;                                // results lie as the logits do, by 16 bytes
 };
 
 template <typename T> __device__ __forceinline__ float value_of(T x) { return cq_paged::Type<T>::one(x); }
@@ -102,13 +106,13 @@ template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const 
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(BYTES) : "memory");
 }
 
-template <typename T, bool ALIKE>
+template <typename T, bool DIRECT>
 __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust p) {
   constexpr int VEC = 16 / sizeof(T);
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ unsigned long long s_key[THREADS / 32];
   __shared__ unsigned long long s_part[PARTS], s_arrived;
-  __shared__ int s_sum[WARPS];
+  __shared__ int s_sum[WARPS], s_count;
   __shared__ uint2 s_lut[16];                // what four bits are in 16-bit lanes
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const cq_adjust& a = p.a;
@@ -125,13 +129,15 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
   if (tid < 16) s_lut[tid] = make_uint2((tid & 1 ? 0xFFFFu : 0u) | (tid & 2 ? 0xFFFF0000u : 0u), (tid & 4 ? 0xFFFFu : 0u) | (tid & 8 ? 0xFFFF0000u : 0u));
   const bool counts = a.tokens != nullptr, known = counts || a.biases;
   uint4* s_piece = reinterpret_cast<uint4*>(smem) + tid;                     // [stage][thread]
-  uint32_t* s_known = reinterpret_cast<uint32_t*>(smem);                     // [place], after the pieces
-  uint32_t* s_token = s_known + PLACES;
-  uint32_t* s_bias = s_token + PLACES;                                       // 1 + the entry that counts
-  uint64_t* s_bits = reinterpret_cast<uint64_t*>(smem + 16 * STAGES * THREADS);
-  int* s_rank = reinterpret_cast<int*>(s_bits + (known ? p.slice / 64 : 0));  // of a word's first marked token
-  int* s_history = s_rank + (known ? p.slice / 64 : 0);                      // -1 outside the vocabulary
-  uint32_t* s_mask = reinterpret_cast<uint32_t*>(s_history + (counts ? p.keep : 0));      // numbered as the marks
+  uint32_t* s_mask = reinterpret_cast<uint32_t*>(smem + 16 * STAGES * THREADS);             // numbered as the marks
+  uint64_t* s_bits = reinterpret_cast<uint64_t*>(smem + 16 * STAGES * THREADS + (a.mask ? p.slice / 8 + 16 : 0));
+  int* s_rank = reinterpret_cast<int*>(s_bits + p.slice / 64);               // of a word's first marked token
+  int* s_history = s_rank + p.slice / 64;                                    // -1 outside the vocabulary
+  // [place], DIRECT: a place for every token, otherwise after the pieces and in their memory
+  uint32_t* s_known = DIRECT ? reinterpret_cast<uint32_t*>(s_rank) : reinterpret_cast<uint32_t*>(smem);
+  uint32_t* s_token = s_known + PLACES;                                      // (not DIRECT)
+  uint32_t* s_bias = DIRECT ? s_known + p.slice : s_token + PLACES;          // 1 + the entry that counts
+  uint16_t* s_list = reinterpret_cast<uint16_t*>(s_known + (a.biases ? 2 : 1) * p.slice);   // DIRECT: the marked tokens, in any order
   const T* in = (const T*)a.logits + (int64_t)row * a.logits_stride;
   T* out = (T*)a.out + (int64_t)row * a.out_stride;
   // Logits are numbered from the 16-byte boundary in front of the row's first, so that pieces are aligned.  (Where results lie otherwise,
@@ -225,36 +231,74 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
         if (i >= 0) what(i, at, j);
       }
     };
+    // what is known of the token in place i
+    auto occurred = [&](int i, int j) {
+      if (j < prompt) atomicOr(&s_known[i], PROMPT);
+      else atomicAdd(&s_known[i], 1u);
+    };
+    auto biased = [&](int i, int j) {        // of the same token's entries the last one counts
+      atomicOr(&s_known[i], BIAS);
+      atomicMax(&s_bias[i], (uint32_t)j + 1u);
+    };
     if (known) {
       for (int i = tid; i < words; i += THREADS) s_bits[i] = 0u;
+      if (DIRECT)
+        for (int i = tid; i < size; i += THREADS) {
+          s_known[i] = 0u;
+          if (a.biases) s_bias[i] = 0u;
+        }
+      if (DIRECT && tid == 0) s_count = 0;
       __syncthreads();
       // -1 of a token that is outside, or marked already
       auto unmarked = [&](int at) {
         const uint32_t word = reinterpret_cast<volatile uint32_t*>(s_bits)[max(at, 0) >> 5];
         return at >= 0 && !(word >> (at & 31) & 1u) ? at : -1;
       };
-      auto mark = [&](int at, int, int) { atomicOr(reinterpret_cast<uint32_t*>(s_bits) + (at >> 5), 1u << (at & 31)); };
-      if (counts && base == begin) {
-        int at[TOKENS / THREADS];
+      // marks a token, -1: none; DIRECT: by all lanes of a warp, which take the list's next places together
+      auto mark = [&](int at) {
+        const uint32_t bit = 1u << (at & 31);
+        const uint32_t old = at >= 0 ? atomicOr(reinterpret_cast<uint32_t*>(s_bits) + (at >> 5), bit) : bit;
+        if constexpr (DIRECT) {
+          const uint32_t fresh = __ballot_sync(0xffffffffu, !(old & bit));
+          if (!fresh) return;
+          int to = 0;
+          if (lane == 0) to = atomicAdd(&s_count, __popc(fresh));
+          to = __shfl_sync(0xffffffffu, to, 0) + __popc(fresh & ((1u << lane) - 1u));
+          if (!(old & bit)) s_list[to] = (uint16_t)at;
+        }
+      };
+      if (counts && (DIRECT || base == begin)) {
+        int at[TOKENS / THREADS], fresh[TOKENS / THREADS];
 #pragma unroll
         for (int k = 0; k < TOKENS / THREADS; ++k) {
+          at[k] = fresh[k] = -1;
+          if (k * THREADS >= n) continue;
           const int j = tid + k * THREADS, v = token_of(v0[k]);
-          if (j < p.keep) s_history[j] = v;
-          at[k] = unmarked(j < n ? place(v) : -1);
+          at[k] = j < n ? place(v) : -1;
+          if (!DIRECT && j < p.keep) s_history[j] = v;
+          fresh[k] = unmarked(at[k]);
         }
 #pragma unroll
-        for (int k = 0; k < TOKENS / THREADS; ++k)
-          if (at[k] >= 0) mark(at[k], 0, 0);
+        for (int k = 0; k < TOKENS / THREADS; ++k) {
+          if (k * THREADS >= n) break;
+          mark(fresh[k]);
+          if (DIRECT && at[k] >= 0) occurred(at[k], tid + k * THREADS);
+        }
 #pragma unroll 4
-        for (int j = TOKENS + tid; j < n; j += THREADS) {
-          const int v = token_of(tokens[j]);
-          if (j < p.keep) s_history[j] = v;
-          if (const int i = unmarked(place(v)); i >= 0) mark(i, 0, 0);
+        for (int j0 = TOKENS; j0 < n; j0 += THREADS) {
+          const int j = j0 + tid, v = j < n ? token_of(tokens[j]) : -1, to = place(v);
+          if (!DIRECT && j < p.keep) s_history[j] = v;
+          mark(unmarked(to));
+          if (DIRECT && to >= 0) occurred(to, j);
         }
       } else if (counts) {
-        each_token(unmarked, mark);
+        each_token(unmarked, [&](int i, int, int) { mark(i); });
       }
-      each_bias(unmarked, mark);
+      for (int j0 = 0; j0 < a.biases; j0 += THREADS) {
+        const int j = j0 + tid, at = j < a.biases ? place(token_of(ids[j])) : -1;
+        mark(unmarked(at));
+        if (DIRECT && at >= 0) biased(at, j);
+      }
     }
     if (mask || known) __syncthreads();      // (the mask's words and the marks are there)
     // what is known of the marked tokens with ranks from rank0 on
@@ -271,28 +315,26 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
       if (counts)
         each_token(index, [&](int i, int at, int j) {
           s_token[i] = at;
-          if (j < prompt) atomicOr(&s_known[i], PROMPT);
-          else atomicAdd(&s_known[i], 1u);
+          occurred(i, j);
         });
-      each_bias(index, [&](int i, int at, int j) {         // of the same token's entries the last one counts
+      each_bias(index, [&](int i, int at, int j) {
         s_token[i] = at;
-        atomicOr(&s_known[i], BIAS);
-        atomicMax(&s_bias[i], (uint32_t)j + 1u);
+        biased(i, j);
       });
       __syncthreads();
     };
     // (of a masked token the pass over the logits may have left -infinity in place of the logit, which changes nothing)
-    auto put = [&](int i) {
+    auto put = [&](int i, int j) {
       const uint32_t c = s_known[i];
-      const int at = base + s_token[i];
-      float x = value_of<T>(in[at]);
+      const int at = base + j;
+      float x = value_of<T>(DIRECT ? reinterpret_cast<const T*>(smem)[j] : in[at]);         // (a small slice's pieces are all there yet)
       if (a.repetition && (c & (PROMPT | TIMES))) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
       if (c & TIMES) {
         if (a.frequency) x = __fsub_rn(x, __fmul_rn(freq, (float)(c & TIMES)));
         if (a.presence) x = __fsub_rn(x, pres);
       }
       if (c & BIAS) x = __fadd_rn(x, a.bias[(int64_t)row * a.bias_stride + s_bias[i] - 1u]);
-      if (mask && !(s_mask[s_token[i] >> 5] >> (s_token[i] & 31) & 1u)) x = -INFINITY;
+      if (mask && !(s_mask[j >> 5] >> (j & 31) & 1u)) x = -INFINITY;
       out[at] = rounded<T>(x);
       best = larger(best, key_of(x, at - skip));
     };
@@ -311,7 +353,7 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
           const uint32_t hidden = ~(s_mask[j >> 5] >> (j & 31)) & ((1u << VEC) - 1u);
           if (hidden) piece.hide(hidden, s_lut);
         }
-        if (ALIKE && whole(i)) *reinterpret_cast<uint4*>(out + i) = piece.w;
+        if (p.alike && whole(i)) *reinterpret_cast<uint4*>(out + i) = piece.w;
         else
           for (int e = 0; e < VEC; ++e)
             if (i + e >= skip && i + e < total) out[i + e] = piece.at(e);
@@ -328,7 +370,10 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (known) {
+    if (known && DIRECT) {
+      __syncthreads();                       // (results of the pass lie under those of the marked tokens)
+      for (int i = tid; i < s_count; i += THREADS) put(s_list[i], s_list[i]);
+    } else if (known) {
       // ranks: a thread takes consecutive words
       const int each = (words + THREADS - 1) / THREADS, w0 = min(words, tid * each), w1 = min(words, w0 + each);
       int mine = 0;
@@ -357,7 +402,7 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
         const int here = min(PLACES, marked - rank0);
         if (rank0) __syncthreads();
         count(rank0, here);
-        for (int i = tid; i < here; i += THREADS) put(i);
+        for (int i = tid; i < here; i += THREADS) put(i, s_token[i]);
       }
     }
     if (stop < end) __syncthreads();         // (the next slice takes the same memory)
@@ -411,14 +456,17 @@ extern "C" int cq_adjust_logits(const cq_adjust* a, int rows, int vocab, cq_stre
   int parts = 1;
   while (parts < PARTS && rows * parts < sms && vocab > parts * 1024) parts *= 2;
   const int part = ((vocab + vec - 1 + parts - 1) / parts + vec - 1) / vec * vec, slice = std::min((part + 63) / 64 * 64, SLICE);
-  // (two CTAs on an SM)
-  const int base_smem = STAGES * THREADS * 16 + (a->tokens || a->biases ? slice / 64 * 12 : 0) + (a->mask ? slice / 8 + 16 : 0);
-  const int keep = a->tokens ? (int)std::min<int64_t>(a->width, (112 * 1024 - base_smem) / 4) : 0, smem = base_smem + 4 * keep;
-  // 16 bytes at a time where a row's logits and results lie alike
+  // Two CTAs on an SM; small slices with a place for every token
+  const bool known = a->tokens || a->biases;
+  constexpr int HALF = 112 * 1024 + 256;
+  const int ring = STAGES * THREADS * 16 + (a->mask ? slice / 8 + 16 : 0), few = ring + slice / 8 + slice * (a->biases ? 10 : 6);
+  const bool direct = known && slice <= FEW && few <= HALF;
+  const int fixed = !known ? ring : (direct ? few : ring + slice / 64 * 12);
+  const int keep = a->tokens && !direct ? (int)std::min<int64_t>(a->width, (112 * 1024 - fixed) / 4) : 0, smem = fixed + 4 * keep;
   const bool alike = (((uintptr_t)a->logits ^ (uintptr_t)a->out) & 15) == 0 && (rows == 1 || (a->logits_stride - a->out_stride) % vec == 0);
-  auto fn = a->dtype == 0   ? (alike ? adjust_logits_kernel<__half, true> : adjust_logits_kernel<__half, false>)
-            : a->dtype == 1 ? (alike ? adjust_logits_kernel<float, true> : adjust_logits_kernel<float, false>)
-                            : (alike ? adjust_logits_kernel<__nv_bfloat16, true> : adjust_logits_kernel<__nv_bfloat16, false>);
+  auto fn = a->dtype == 0   ? (direct ? adjust_logits_kernel<__half, true> : adjust_logits_kernel<__half, false>)
+            : a->dtype == 1 ? (direct ? adjust_logits_kernel<float, true> : adjust_logits_kernel<float, false>)
+                            : (direct ? adjust_logits_kernel<__nv_bfloat16, true> : adjust_logits_kernel<__nv_bfloat16, false>);
   CQ_CUDA_TRY(cq_grant_smem((const void*)fn, smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(parts, rows);
@@ -433,6 +481,6 @@ extern "C" int cq_adjust_logits(const cq_adjust* a, int rows, int vocab, cq_stre
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  CQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, Adjust{*a, vocab, part, slice, keep}));
+  CQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, Adjust{*a, vocab, part, slice, keep, alike}));
   return CQ_OK;
 }
