@@ -84,24 +84,6 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 __device__ __forceinline__ unsigned long long larger(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
 
-// until every CTA of the cluster has arrived once, or for two seconds
-__device__ __forceinline__ void wait_for_all(uint32_t bar) {
-  unsigned long long t0 = 0;
-  for (uint32_t it = 0; it < (1u << 26); ++it) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0, %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(bar), "r"(20000u) : "memory");
-    if (ok) return;
-    unsigned long long t1;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t1));
-    if (t0 == 0) t0 = t1;
-    else if (t1 - t0 > 2000000000ull) return;
-  }
-}
-
 template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(BYTES) : "memory");
 }
@@ -111,20 +93,13 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
   constexpr int VEC = 16 / sizeof(T);
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ unsigned long long s_key[THREADS / 32];
-  __shared__ unsigned long long s_part[PARTS], s_arrived;
+  __shared__ unsigned long long s_part[PARTS];
   __shared__ int s_sum[WARPS], s_count;
   __shared__ uint2 s_lut[16];                // what four bits are in 16-bit lanes
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const cq_adjust& a = p.a;
   const int parts = gridDim.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (parts > 1) {
-    if (tid == 0) {
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"((uint32_t)__cvta_generic_to_shared(&s_arrived)), "r"(parts) : "memory");
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  }
+  if (parts > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");      // (this CTA runs: its memory may be written)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (tid < 16) s_lut[tid] = make_uint2((tid & 1 ? 0xFFFFu : 0u) | (tid & 2 ? 0xFFFF0000u : 0u), (tid & 4 ? 0xFFFFu : 0u) | (tid & 8 ? 0xFFFF0000u : 0u));
   const bool counts = a.tokens != nullptr, known = counts || a.biases;
@@ -417,19 +392,18 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
     best = lane < THREADS / 32 ? s_key[lane] : 0ull;
     for (int d = 16; d; d /= 2) best = larger(best, __shfl_xor_sync(0xffffffffu, best, d));
   }
-  if (parts > 1) {
-    // To the cluster's first CTA, the only one that waits for the others.
+  if (parts > 1) {                           // to the cluster's first CTA
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (tid == 0) {
-      uint32_t at, bar;
+      uint32_t at;
       asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(&s_part[blockIdx.x])));
-      asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(bar) : "r"((uint32_t)__cvta_generic_to_shared(&s_arrived)));
-      asm volatile("st.relaxed.cluster.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(best) : "memory");
-      asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+      asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(best) : "memory");
     }
-    if (blockIdx.x || tid) return;
-    wait_for_all((uint32_t)__cvta_generic_to_shared(&s_arrived));
-    for (int i = 1; i < parts; ++i) best = larger(best, *(volatile unsigned long long*)&s_part[i]);
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (blockIdx.x) return;
+    if (tid == 0)
+      for (int i = 1; i < parts; ++i) best = larger(best, s_part[i]);
   }
   if (tid == 0) a.next[row] = (long long)(0xFFFFFFFFu - (uint32_t)best);
 }
