@@ -32,6 +32,13 @@ received, and whenever the `kv_budget + kv_slack` slots of a layer are full the 
 first `sinks` and the last `kv_recent` always do).  Keys keep the rotation of their own positions.  Slots are not positions any more then,
 so that a `window` that hides any and `kv_budget` exclude one another.
 
+`kv_page=64` keeps the fp16 cache in pages of so many slots (`quant_cuda.KVPages`), `kv_pages` of them for all sequences of a layer:
+prompts may have different lengths (`prefill(tokens, lengths)`), single sequences get a new one while the others go on
+(`prefill(tokens, lengths, rows)`) or give their pages back (`release`), and a `window` with `sinks` can be asked for.
+
+`control(...)` puts `quant_cuda.adjust_logits` behind the logits of every step: penalties for tokens that occurred in a sequence, biases
+of single tokens, and a grammar as bit masks with a table of the states that follow.
+
 `dense=True` builds the parity twin: the same packed buffers, every projection computed as
 F.linear(x, unpack()) the way the reference's dense mode does (llama/qlinear.py:183-195).
 """
@@ -86,7 +93,8 @@ class CherryDecoder:
     def __init__(self, cfg: DecoderConfig, device="cuda", seed: int = 0, dense: bool = False,
                  release_reference_buffers: bool = False, tp_group=None, tp_gather: str = "peer", batch: int = 1,
                  attention: str = "auto", kv_bits: int = 16, kv_group: int = 32, window: int = 0, sinks: int = 0,
-                 kv_budget: int = None, kv_slack: int = 256, kv_recent: int = None, kv_observe: int = 64):
+                 kv_budget: int = None, kv_slack: int = 256, kv_recent: int = None, kv_observe: int = 64, kv_page: int = 0,
+                 kv_pages: int = None):
         if not torch.cuda.is_available():
             raise RuntimeError("CherryDecoder needs a CUDA device (there is no CPU path)")
         if batch < 1:
@@ -105,11 +113,16 @@ class CherryDecoder:
             raise ValueError("kv_bits is 16 or 4")
         if window < 0 or sinks < 0:
             raise ValueError("window and sinks must not be negative")
-        if kv_bits == 16 and (window or sinks or kv_budget is not None):
-            raise ValueError("window, sinks and kv_budget need the 4-bit cache (kv_bits=4)")
+        if kv_bits == 16 and (((window or sinks) and not kv_page) or kv_budget is not None):
+            raise ValueError("window, sinks and kv_budget need the 4-bit cache (kv_bits=4); window and sinks a paged one (kv_page)")
+        if kv_page < 0 or (kv_pages is not None and (not kv_page or kv_pages < 1)):
+            raise ValueError("kv_page and kv_pages must be positive, and come together")
+        if kv_page and (kv_bits != 16 or attention == "flash" or cfg.head_dim not in (64, 128)):
+            raise ValueError("the paged cache is fp16 and has its own attention, for heads 64 or 128 wide")
         if kv_bits == 4 and (attention == "flash" or cfg.head_dim not in (64, 128)):
             raise ValueError("the 4-bit cache has its own attention, for heads 64 or 128 wide")
         self.kv_bits, self.window, self.sinks, self.kv_budget, self.kv_observe = kv_bits, window, sinks, kv_budget, kv_observe
+        self.kv_page = kv_page
         if kv_budget is not None:
             self.kv_recent = kv_budget // 4 if kv_recent is None else kv_recent
             if not (kv_budget > 0 and kv_slack > 0 and kv_observe > 0 and self.kv_recent >= 0 and sinks + self.kv_recent <= kv_budget):
@@ -119,7 +132,7 @@ class CherryDecoder:
                 raise ValueError("a window cannot be kept over a bounded cache (kv_budget), whose slots are not positions")
         self._flash = None
         grouped = cfg.n_heads // cfg.n_kv_heads
-        if attention == "flash" or (attention == "auto" and kv_bits == 16 and cfg.max_seq > 1024 and
+        if attention == "flash" or (attention == "auto" and kv_bits == 16 and not kv_page and cfg.max_seq > 1024 and
                                     grouped > (8 if cfg.head_dim in (64, 128) else 1)):
             try:
                 from flash_attn import flash_attn_with_kvcache
@@ -182,14 +195,24 @@ class CherryDecoder:
                 self.kv_weights = torch.zeros(cfg.n_layers, batch, self.kv_local, self.caches[0].slots, device=self.dev)
                 # slots that hold a position, on the device and on the host
                 self.length, self.length_host = torch.zeros(batch, dtype=torch.long, device=self.dev), 0
+        elif kv_page:
+            from .pages import PageTable
+            each = -(-cfg.max_seq // kv_page)
+            self.page_table = PageTable(batch, cfg.max_seq, batch * each if kv_pages is None else kv_pages, kv_page)
+            self.table = self.page_table.host.to(self.dev)           # the same for all layers
+            self.pages = [self.qc.KVPages.empty(self.page_table.pages, self.kv_local, kv_page, hd, torch.float16, self.dev)
+                          for _ in range(cfg.n_layers)]
+            self.zero = torch.zeros(batch, dtype=torch.long, device=self.dev)
         else:
             self.k_cache = torch.zeros(cfg.n_layers, batch, cfg.max_seq, self.kv_local, hd, dtype=torch.float16, device=self.dev)
             self.v_cache = torch.zeros_like(self.k_cache)
         # state of the decode loop, all on the device: next token and position of every sequence
         self.tok = torch.zeros(batch, dtype=torch.long, device=self.dev)
         self.pos = torch.zeros(batch, dtype=torch.long, device=self.dev)
-        self.pos_host = 0           # the host's copy of `pos`: every step is checked against max_seq before it is launched
+        self.pos_host = 0           # the host's copy of `pos` (the largest): every step is checked against max_seq before it is launched
+        self.held = [0] * batch     # positions of each sequence, with pages
         self.graph = None
+        self.controls = None
 
     # ------------------------------------------------------------------ construction
     def _make_linear(self, k: int, n: int, g: torch.Generator) -> QuantLinear:
@@ -273,6 +296,8 @@ class CherryDecoder:
         q, k, v = q.view(t, nh, hd), k.view(t, kv, hd), v.view(t, kv, hd)
         if self.kv_bits == 4:
             a = (self._kv4_step if decode else self._kv4_prompt)(li, q, k, v, pos).view(t, nh * hd)
+        elif self.kv_page:
+            a = (self._pages_step if decode else self._pages_prompt)(li, q, k, v, pos).view(t, nh * hd)
         elif decode and self._flash is None:
             a = self.qc.attn_decode_step(q, k, v, self.cos, self.sin, pos, self.k_cache[li], self.v_cache[li]).view(t, nh * hd)
         else:
@@ -334,43 +359,161 @@ class CherryDecoder:
         rows = [x[:, :, :3] for c in self.caches for x in (c.k_codes, c.k_scales, c.v_codes, c.v_scales)]
         return rows if self.kv_budget is None else rows + [self.kv_weights, self.length]
 
+    # ------------------------------------------------------------------ paged cache
+    def _pages_step(self, li: int, q, k, v, pos):
+        return self.pages[li].step(q, k, v, self.cos, self.sin, pos, self.table, pos, window=self.window, sinks=self.sinks)
+
+    def _pages_prompt(self, li: int, q, k, v, pos):
+        """Attention of the prompts on their own keys and values, which go into their sequences' pages (rows behind a prompt's end
+        have no position and go nowhere)."""
+        table, lengths = self.prompts
+        nb, (t, nh, hd), kv = len(lengths), q.shape, k.shape[1]
+        turned = self.pages[li].write(torch.cat([q, k], 1), k, v, table, self.zero[:nb], self.cos, self.sin, pos).view(nb, t // nb, nh + kv, hd)
+        return self.qc.attn_prefill(turned[:, :, :nh], turned[:, :, nh:], v.view(nb, t // nb, kv, hd), window=self.window, sinks=self.sinks,
+                                    lengths=lengths)[0]
+
+    def _pages_reserve(self, slots):
+        """Pages for the first slots[s] positions of the sequences named."""
+        if self.page_table.reserve(slots):
+            self.table.copy_(self.page_table.host)
+
+    def release(self, rows):
+        """These sequences' pages are free for others; their steps are computed, on nothing, until they get a prompt."""
+        if not self.kv_page:
+            raise ValueError("only a paged cache (kv_page) has pages to give back")
+        for s in rows:
+            self.page_table.release(s)
+            self.held[s] = 0
+        self.table.copy_(self.page_table.host)
+        self.pos_host = max(self.held)
+
+    # ------------------------------------------------------------------ control over what is picked
+    def control(self, repetition=None, presence=None, frequency=None, bias=None, grammar=None):
+        """From here on tokens are picked from adjusted logits.  repetition, presence, frequency: a number for all sequences or
+        one for each; presence and frequency count what was generated, repetition the prompt too.  bias: {token: number}.  grammar: (masks
+        (states, words) int32 with a bit for each token, follow (states, vocab) integers: the state behind a token, -1 for none);
+        sequences start in state 0 with their prompt.  Without arguments: the bare logits again."""
+        self.graph = None
+        if all(x is None for x in (repetition, presence, frequency, bias, grammar)):
+            self.controls = None
+            return
+        each = lambda x: None if x is None else torch.broadcast_to(torch.as_tensor(x, dtype=torch.float32), (self.batch,)).contiguous().to(self.dev)
+        c = {"repetition": each(repetition), "presence": each(presence), "frequency": each(frequency)}
+        if bias is not None:
+            ids, numbers = list(bias.keys()), list(bias.values())
+            c["bias_ids"] = torch.tensor(ids, dtype=torch.long, device=self.dev).expand(self.batch, -1)
+            c["bias"] = torch.tensor(numbers, dtype=torch.float32, device=self.dev).expand(self.batch, -1)
+        self.follow = None
+        if grammar is not None:
+            masks, follow = grammar
+            if masks.dtype != torch.int32 or masks.dim() != 2 or masks.shape[1] < -(-self.cfg.vocab // 32) or \
+                    tuple(follow.shape) != (masks.shape[0], self.cfg.vocab) or int(follow.max()) >= masks.shape[0]:
+                raise ValueError("grammar is (masks (states, words) int32, follow (states, vocab) of states or -1)")
+            c["mask"], self.follow = masks.to(self.dev), follow.to(self.dev, torch.long)
+            c["mask_rows"] = torch.zeros(self.batch, dtype=torch.long, device=self.dev)
+        if any(c[n] is not None for n in ("repetition", "presence", "frequency")):
+            # a sequence's tokens by position, up to the one that is read next
+            c["tokens"] = torch.zeros(self.batch, self.cfg.max_seq, dtype=torch.long, device=self.dev)
+            c["length"], c["prompt"] = (torch.zeros(self.batch, dtype=torch.long, device=self.dev) for _ in range(2))
+        self.controls = c
+
+    def _pick(self, logits: torch.Tensor, rows=None) -> torch.Tensor:
+        """The next token of every sequence (of `rows`); logits are adjusted in place."""
+        c = self.controls
+        if c is None:
+            return logits.argmax(-1)
+        mine = c if rows is None else {n: x if x is None or n == "mask" else x[rows] for n, x in c.items()}
+        _, picked = self.qc.adjust_logits(logits, **mine, out=logits)
+        if self.follow is not None:
+            state = mine["mask_rows"]
+            behind = torch.where(state >= 0, self.follow[state.clamp(min=0), picked], state)
+            if rows is None:
+                state.copy_(behind)
+            else:
+                c["mask_rows"][rows] = behind
+        return picked
+
+    def _remember(self):
+        """The token that a step reads, in the history."""
+        c = self.controls
+        if c is not None and c.get("tokens") is not None:
+            c["tokens"].scatter_(1, self.pos.clamp(max=self.cfg.max_seq - 1)[:, None], self.tok[:, None])
+            c["length"].copy_(self.pos + 1)
+
     def _logits(self, h: torch.Tensor, delta) -> torch.Tensor:
         return F.linear(self._norm(h, delta, self.final_norm)[0], self.lm_head)
 
     # ------------------------------------------------------------------ prefill / decode
     @torch.inference_mode()
-    def prefill(self, tokens: torch.Tensor) -> torch.Tensor:
+    def prefill(self, tokens: torch.Tensor, lengths=None, rows=None) -> torch.Tensor:
         """Runs the prompts (T,) or (batch, T) through the model, fills the caches, returns the last
-        position's logits (batch, vocab)."""
+        position's logits (batch, vocab).  With a paged cache: lengths[i] of the T tokens are prompt i's, and prompt i is that of
+        sequence rows[i] while the others keep what they have."""
         if tokens.dim() == 1:
             tokens = tokens[None]
-        if tokens.shape[0] != self.batch:
-            raise ValueError(f"{tokens.shape[0]} prompts for a decoder of batch {self.batch}")
-        t = tokens.shape[1]
-        if not 0 < t < self.cfg.max_seq:
+        if not self.kv_page and (lengths is not None or rows is not None):
+            raise ValueError("prompts of different lengths, and of some sequences alone, need a paged cache (kv_page)")
+        some = rows is not None
+        rows = list(range(self.batch)) if rows is None else [int(r) for r in rows]
+        if tokens.shape[0] != len(rows):
+            raise ValueError(f"{tokens.shape[0]} prompts for a decoder of batch {self.batch}" if not some else f"{tokens.shape[0]} prompts for {len(rows)} sequences")
+        if len(set(rows)) != len(rows) or any(not 0 <= r < self.batch for r in rows):
+            raise ValueError(f"rows must be different sequences of the {self.batch}")
+        n, t = tokens.shape
+        ends = [t] * n if lengths is None else [int(x) for x in lengths]
+        if len(ends) != n or t == 0 or any(not 0 < x <= t for x in ends) or max(ends) >= self.cfg.max_seq:
+            if lengths is not None:
+                raise ValueError(f"lengths must be 1 to {min(t, self.cfg.max_seq - 1)}, one for each prompt")
             raise ValueError(f"a prompt of {t} tokens does not fit max_seq = {self.cfg.max_seq} (one position must stay free)")
-        pos = torch.arange(t, device=self.dev).repeat(self.batch)
+        t = min(t, max(ends))
+        tokens = tokens[:, :t]
+        place = torch.arange(t, device=self.dev)
+        if self.kv_page:
+            old = [self.page_table.held[r] for r in rows]
+            need = sum(-(-x // self.kv_page) for x in ends)
+            if need > len(self.page_table.free) + sum(old):
+                raise ValueError(f"{need} pages are needed, {len(self.page_table.free) + sum(old)} of {self.page_table.pages} are free")
+            for r in rows:
+                self.page_table.release(r)
+            self.page_table.reserve(dict(zip(rows, ends)))
+            self.table.copy_(self.page_table.host)
+            end = torch.tensor(ends, dtype=torch.long, device=self.dev)
+            self.prompts = self.table[rows] if some else self.table, end
+            pos = torch.where(place < end[:, None], place, -1).reshape(-1)
+        else:
+            pos = place.repeat(n)
         h, delta = self.embed[tokens.reshape(-1)], None
         for li in range(self.cfg.n_layers):
             h, delta = self._layer(li, h, delta, pos, decode=False)
-        last = torch.arange(self.batch, device=self.dev) * t + (t - 1)
+        last = torch.tensor([i * t + x - 1 for i, x in enumerate(ends)], device=self.dev)
         logits = self._logits(h[last].contiguous(), delta[last].contiguous())
         self._check_exchange()
-        self.pos.fill_(t)
-        self.pos_host = t
+        for r, x in zip(rows, ends):
+            self.held[r] = x
+        self.pos_host = max(self.held)
         if self.kv_budget is not None:
             self.length_host = min(t, self.kv_budget)
-        self.tok.copy_(logits.argmax(-1))
+        at = torch.tensor(rows, device=self.dev)
+        filled = torch.tensor(ends, dtype=torch.long, device=self.dev)
+        self.pos[at] = filled
+        c = self.controls
+        if c is not None and c.get("tokens") is not None:
+            c["tokens"][at, :t] = tokens
+            c["length"][at], c["prompt"][at] = filled, filled
+        if c is not None and c.get("mask_rows") is not None:
+            c["mask_rows"][at] = 0
+        self.tok[at] = self._pick(logits, at if some else None)
         return logits
 
     @torch.inference_mode()
     def _step(self) -> torch.Tensor:
         """One greedy decode step on the device-side state; returns the logits (1, vocab)."""
+        self._remember()
         h, delta = self.embed[self.tok], None
         for li in range(self.cfg.n_layers):
             h, delta = self._layer(li, h, delta, self.pos, decode=True)
         logits = self._logits(h, delta)
-        self.tok.copy_(logits.argmax(-1))
+        self.tok.copy_(self._pick(logits))
         self.pos.add_(1)
         if self.kv_budget is not None:
             self.length.add_(1)
@@ -383,9 +526,14 @@ class CherryDecoder:
             raise ValueError("max_seq must be at least 4")
         # the warm-up and the captured step run at positions 0, 1, 2: always inside the cache, whatever
         # the current position is (state and those cache rows are restored below)
-        rows = self._kv4_rows() if self.kv_bits == 4 else [self.k_cache[:, :, :3], self.v_cache[:, :, :3]]
+        # (with pages no sequence has any meanwhile)
+        rows = self._kv4_rows() if self.kv_bits == 4 else [self.table] if self.kv_page else [self.k_cache[:, :, :3], self.v_cache[:, :, :3]]
+        if self.controls is not None:
+            rows = rows + [x[:, :3] if n == "tokens" else x for n, x in self.controls.items() if n in ("tokens", "length", "mask_rows") and x is not None]
         saved = [x.clone() for x in (self.tok, self.pos, *rows)]
         self.pos.zero_()
+        if self.kv_page:
+            self.table.fill_(-1)
         if self.kv_budget is not None:
             self.length.zero_()
         s = torch.cuda.Stream(device=self.dev)
@@ -409,6 +557,8 @@ class CherryDecoder:
         if n_tokens < 0 or self.pos_host + n_tokens > self.cfg.max_seq:
             raise ValueError(f"{n_tokens} more tokens after position {self.pos_host} do not fit max_seq = "
                              f"{self.cfg.max_seq}: the KV cache holds max_seq positions")
+        if self.kv_page:
+            self._pages_reserve({r: x + n_tokens for r, x in enumerate(self.held) if x})
         out = torch.empty(n_tokens, self.batch, dtype=torch.long, device=self.dev)
         if use_graph and self.graph is None:
             self.capture()
@@ -420,6 +570,7 @@ class CherryDecoder:
                 self.graph.replay()
             else:
                 self._step()
+        self.held = [x + n_tokens if x else 0 for x in self.held]
         self.pos_host += n_tokens
         self._check_exchange()
         return out[:, 0] if self.batch == 1 else out
