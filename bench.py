@@ -762,7 +762,9 @@ def run_model(args):
 
 
 def cache_options(args):
-    """The harness's options of the 4-bit cache; none with the fp16 cache."""
+    """The harness's options of the 4-bit and of the paged cache; none with the contiguous fp16 cache."""
+    if args.kv_page:
+        return {"kv_page": args.kv_page, "window": args.window, "sinks": args.sinks}
     if args.kv_bits == 16:
         return {}
     return {"kv_bits": args.kv_bits, "window": args.window, "sinks": args.sinks, "kv_budget": args.kv_budget}
@@ -780,6 +782,8 @@ def model_measure(args, torch, dist, dev, world, rank, local, name, gen=256, pro
                             tp_gather=args.gather, release_reference_buffers=True, batch=batch, **cache_options(args))
     torch.cuda.synchronize()
     t_build = time.time() - t_build
+    if args.repetition is not None:
+        model.control(repetition=args.repetition)
     prompt = torch.randint(0, cfg.vocab, (batch, prompt_len), device=dev, generator=torch.Generator(device=dev).manual_seed(0))
 
     def timed(fn):
@@ -858,7 +862,7 @@ def model_measure(args, torch, dist, dev, world, rank, local, name, gen=256, pro
         "vs_baseline": None, "dtype": "f16",
         "data": "synthetic",
         "config": {"workload": f"llama2_{name}_arch_{cfg.bits}bit_g128_cherry1/256_prompt{prompt_len}_greedy{gen}_batch{batch}",
-                   "batch": batch, "max_seq": max_seq, **cache_options(args),
+                   "batch": batch, "max_seq": max_seq, **cache_options(args), **({} if args.repetition is None else {"repetition": args.repetition}),
                    "layers": cfg.n_layers, "kv_heads": cfg.n_kv_heads,
                    "hidden": cfg.hidden, "ffn": cfg.ffn, "vocab": cfg.vocab, "bits": cfg.bits,
                    "l2_defeat": f"{qbytes / 1e9:.1f} GB of quantized weights + {hbytes / 1e6:.0f} MB lm_head per token, "
@@ -1012,8 +1016,10 @@ def main():
     ap.add_argument("--prompt", type=int, default=128, help="model workload: prompt tokens per sequence")
     ap.add_argument("--gen", type=int, default=256, help="model workload: tokens generated per sequence")
     ap.add_argument("--kv-bits", type=int, default=16, choices=[16, 4], help="model workload: bits of the KV cache")
-    ap.add_argument("--window", type=int, default=0, help="model workload, 4-bit cache: positions a query sees (0: all)")
-    ap.add_argument("--sinks", type=int, default=0, help="model workload, 4-bit cache: first positions that stay visible")
+    ap.add_argument("--kv-page", type=int, default=0, help="model workload: slots of a page of the fp16 cache (0: one block a sequence)")
+    ap.add_argument("--repetition", type=float, default=None, help="model workload: penalty on the logits of tokens that occurred")
+    ap.add_argument("--window", type=int, default=0, help="model workload, 4-bit or paged cache: positions a query sees (0: all)")
+    ap.add_argument("--sinks", type=int, default=0, help="model workload, 4-bit or paged cache: first positions that stay visible")
     ap.add_argument("--kv-budget", type=int, default=None, help="model workload, 4-bit cache: slots that stay where it is bounded (without --window)")
     ap.add_argument("--gather", default="peer", choices=["peer", "nccl"],
                     help="exchange step at N > 1: this library's peer-memory kernel (default) or NCCL")
@@ -1024,8 +1030,12 @@ def main():
                     help="decode workload on another layer than the headline one, e.g. 28672x8192x3 (the 70B down "
                          "projection); for profiling: the line then names that layer as its workload")
     args = ap.parse_args()
-    if args.kv_bits == 16 and (args.window or args.sinks or args.kv_budget is not None):
-        ap.error("--window, --sinks and --kv-budget belong to the 4-bit cache: give --kv-bits 4")
+    if args.kv_page and (args.kv_bits != 16 or args.kv_budget is not None):
+        ap.error("--kv-page is a form of the fp16 cache: without --kv-bits 4 and --kv-budget")
+    if args.kv_bits == 16 and not args.kv_page and (args.window or args.sinks or args.kv_budget is not None):
+        ap.error("--window, --sinks and --kv-budget belong to the 4-bit cache: give --kv-bits 4 (--window and --sinks to a paged one, too: --kv-page)")
+    if args.repetition is not None and args.repetition <= 0:
+        ap.error("--repetition must be positive")
     if args.shape:
         global K_IN, N_OUT, BITS, WORKLOAD
         K_IN, N_OUT, BITS = (int(v) for v in args.shape.lower().split("x"))
