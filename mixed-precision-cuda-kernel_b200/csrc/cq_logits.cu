@@ -423,6 +423,9 @@ extern "C" int cq_adjust_logits(const cq_adjust* a, int rows, int vocab, cq_stre
   if (a->tokens ? a->width < 0 || a->tokens_stride < 0 : (a->length || a->prompt || a->repetition || a->presence || a->frequency)) return CQ_ERR_BAD_ARG;
   if (a->biases < 0 || (a->biases > 0 && (!a->bias_ids || !a->bias || a->bias_ids_stride < 0 || a->bias_stride < 0))) return CQ_ERR_BAD_ARG;
   if (a->mask ? a->masks < 1 || a->mask_stride < 0 || (!a->mask_rows && a->masks < rows) : a->mask_rows != nullptr) return CQ_ERR_BAD_ARG;
+  if (((uintptr_t)a->tokens | (uintptr_t)a->length | (uintptr_t)a->prompt | (uintptr_t)a->bias_ids | (uintptr_t)a->mask_rows | (uintptr_t)a->next) & 7)
+    return CQ_ERR_BAD_ARG;
+  if (((uintptr_t)a->repetition | (uintptr_t)a->presence | (uintptr_t)a->frequency | (uintptr_t)a->bias | (uintptr_t)a->mask) & 3) return CQ_ERR_BAD_ARG;
   // in place, or apart
   const bool in_place = a->logits == a->out && (rows == 1 || a->logits_stride == a->out_stride);
   if (!in_place && !kv4_apart(a->logits, span(rows, vocab, a->logits_stride, item), a->out, span(rows, vocab, a->out_stride, item))) return CQ_ERR_BAD_ARG;

@@ -133,7 +133,7 @@ extern "C" int cq_pages_write(const cq_pages* pages, const cq_table* table, cons
   if (rc != CQ_OK) return rc;
   if (!rows_fit(k) || !rows_fit(v) || !first || rows < 1 || n_heads < 0 || (n_heads > 0 && (!rows_fit(q) || !q_out || ((uintptr_t)q_out & 15))))
     return CQ_ERR_BAD_ARG;
-  if (cos_table && (!sin_table || !positions || table_rows < 1)) return CQ_ERR_BAD_ARG;
+  if (!tables_fit(cos_table, sin_table, positions, table_rows) || (((uintptr_t)first | (uintptr_t)starts) & 7)) return CQ_ERR_BAD_ARG;
   if (n_heads + 2ll * pages->n_kv_heads > 65535 || (!starts && rows % table->sequences)) return CQ_ERR_BAD_SHAPE;
   auto fn = pages->dtype == 0 ? (pages->head_dim == 128 ? write<__half, 128> : write<__half, 64>)
                               : (pages->head_dim == 128 ? write<__nv_bfloat16, 128> : write<__nv_bfloat16, 64>);
@@ -143,7 +143,7 @@ extern "C" int cq_pages_write(const cq_pages* pages, const cq_table* table, cons
 extern "C" int cq_pages_read(const cq_pages* pages, const cq_table* table, const long long* first, int count, void* k, void* v, cq_stream_t stream) {
   const int rc = check(pages, table);
   if (rc != CQ_OK) return rc;
-  if (!first || !k || !v || count < 1 || (((uintptr_t)k | (uintptr_t)v) & 15)) return CQ_ERR_BAD_ARG;
+  if (!first || ((uintptr_t)first & 7) || !k || !v || count < 1 || (((uintptr_t)k | (uintptr_t)v) & 15)) return CQ_ERR_BAD_ARG;
   auto fn = pages->dtype == 0 ? (pages->head_dim == 128 ? read<__half, 128> : read<__half, 64>)
                               : (pages->head_dim == 128 ? read<__nv_bfloat16, 128> : read<__nv_bfloat16, 64>);
   return fn(pages, table, first, count, k, v, (cudaStream_t)stream);

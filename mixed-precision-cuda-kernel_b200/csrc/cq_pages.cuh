@@ -79,6 +79,10 @@ template <typename T> Rows<T> rows_of(const cq_rows* r) { return r ? Rows<T>{(co
 inline bool rows_fit(const cq_rows* r) {
   return r && r->at && ((uintptr_t)r->at & 15) == 0 && r->token_stride >= 0 && r->head_stride >= 0 && r->token_stride % 8 == 0 && r->head_stride % 8 == 0;
 }
+// no tables, or all of them
+inline bool tables_fit(const float* cos_t, const float* sin_t, const long long* positions, int rows) {
+  return !cos_t || (sin_t && positions && rows > 0 && (((uintptr_t)cos_t | (uintptr_t)sin_t) & 3) == 0 && ((uintptr_t)positions & 7) == 0);
+}
 int check(const cq_pages* pages, const cq_table* table);
 
 }  // namespace cq_paged

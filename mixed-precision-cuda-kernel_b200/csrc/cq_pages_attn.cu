@@ -523,7 +523,7 @@ int call(const cq_pages* pages, const cq_table* table, const cq_rows* q, const c
          cudaStream_t stream) {
   const int rc = check(pages, table);
   if (rc != CQ_OK) return rc;
-  if (!rows_fit(q) || !length || !out || window < 0 || sinks < 0 || !(scale > 0.f) || (((uintptr_t)out | (uintptr_t)workspace) & 15)) return CQ_ERR_BAD_ARG;
+  if (!rows_fit(q) || !length || ((uintptr_t)length & 7) || !out || window < 0 || sinks < 0 || !(scale > 0.f) || (((uintptr_t)out | (uintptr_t)workspace) & 15)) return CQ_ERR_BAD_ARG;
   if (H < 1 || H % pages->n_kv_heads || (H + 7ll * pages->n_kv_heads) / 8 > 65535) return CQ_ERR_BAD_SHAPE;
   if (!workspace && cq_pages_attend_workspace_bytes(pages, table, H, window, sinks)) return CQ_ERR_BAD_ARG;
   auto fn = pages->dtype == 0 ? (pages->head_dim == 128 ? attend<__half, 128> : attend<__half, 64>)
@@ -549,7 +549,7 @@ extern "C" int cq_pages_step(const cq_pages* pages, const cq_table* table, const
                              const float* cos_table, const float* sin_table, const long long* positions, int table_rows, const long long* length,
                              void* out, int n_heads, int window, int sinks, float scale, void* workspace, cq_stream_t stream) {
   if (!rows_fit(k) || !rows_fit(v)) return CQ_ERR_BAD_ARG;
-  if (cos_table && (!sin_table || !positions || table_rows < 1)) return CQ_ERR_BAD_ARG;
+  if (!tables_fit(cos_table, sin_table, positions, table_rows)) return CQ_ERR_BAD_ARG;
   return call(pages, table, q, k, v, cos_table, sin_table, positions, table_rows, length, out, n_heads, window, sinks, scale, workspace,
               (cudaStream_t)stream);
 }

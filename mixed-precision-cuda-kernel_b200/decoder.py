@@ -390,9 +390,9 @@ class CherryDecoder:
     # ------------------------------------------------------------------ control over what is picked
     def control(self, repetition=None, presence=None, frequency=None, bias=None, grammar=None):
         """From here on tokens are picked from adjusted logits.  repetition, presence, frequency: a number for all sequences or
-        one for each; presence and frequency count what was generated, repetition the prompt too.  bias: {token: number}.  grammar: (masks
-        (states, words) int32 with a bit for each token, follow (states, vocab) integers: the state behind a token, -1 for none);
-        sequences start in state 0 with their prompt.  Without arguments: the bare logits again."""
+        one for each, from a sequence's next prompt on; presence and frequency count what was generated, repetition the prompt too.  bias:
+        {token: number}.  grammar: (masks (states, words) int32 with a bit for each token, follow (states, vocab) integers: the state
+        behind a token, -1 for none); sequences start in state 0, here and with every prompt.  Without arguments: the bare logits again."""
         self.graph = None
         if all(x is None for x in (repetition, presence, frequency, bias, grammar)):
             self.controls = None
@@ -438,7 +438,7 @@ class CherryDecoder:
         c = self.controls
         if c is not None and c.get("tokens") is not None:
             c["tokens"].scatter_(1, self.pos.clamp(max=self.cfg.max_seq - 1)[:, None], self.tok[:, None])
-            c["length"].copy_(self.pos + 1)
+            c["length"].copy_(torch.where(c["prompt"] > 0, self.pos + 1, 0))       # (0: its prompt was not noted)
 
     def _logits(self, h: torch.Tensor, delta) -> torch.Tensor:
         return F.linear(self._norm(h, delta, self.final_norm)[0], self.lm_head)

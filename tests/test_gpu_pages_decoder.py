@@ -192,6 +192,21 @@ def test_penalties_and_biases(dec, options, control):
     assert torch.equal(a.generate(20), b.generate(20))
 
 
+def test_control_in_the_middle(dec):
+    """Penalties begin with a sequence's next prompt: what was not noted does not count"""
+    cfg = tiny(dec)
+    prompt = tokens(cfg, 2, 20, seed=8)
+    a, b = (dec.CherryDecoder(cfg, seed=12, batch=2, kv_page=16) for _ in range(2))
+    a.prefill(prompt), b.prefill(prompt)
+    a.generate(5), b.generate(5)
+    a.control(repetition=3.0, presence=2.0)
+    assert torch.equal(a.generate(20), b.generate(20))
+    a.prefill(prompt[:1], rows=[0]), b.prefill(prompt[:1], rows=[0])
+    x, y = a.generate(20), b.generate(20)
+    assert torch.equal(x[:, 1], y[:, 1]) and not torch.equal(x[:, 0], y[:, 0])
+    assert len(set(x[:, 0].tolist())) > len(set(y[:, 0].tolist())) or len(set(y[:, 0].tolist())) == 20
+
+
 def test_grammar(dec):
     """Sequences follow an automaton; behind a token without a next state everything is allowed; the mask of an empty state gives token 0"""
     cfg = tiny(dec, vocab=1003)

@@ -107,16 +107,17 @@ def test_calls(lib):
     assert lib.cq_pages_check(C.byref(pages(v=(1 << 26) + 7 * 2 * 16 * 256))) == 0         # side by side is apart
     for call in (attend, step):
         for bad in (dict(q=None), dict(length=None), dict(out=None), dict(out=AT + 8), dict(ws=AT + 8), dict(window=-1), dict(sinks=-1), dict(scale=0.0),
-                    dict(scale=-1.0), dict(scale=float("nan"))):
+                    dict(scale=-1.0), dict(scale=float("nan")), dict(length=AT + 4)):
             assert call(lib, **bad) == BAD_ARG, bad
         assert call(lib, heads=0) == call(lib, heads=3) == BAD_SHAPE
         assert call(lib) not in (0, BAD_ARG, BAD_SHAPE, UNSUPPORTED)                      # (no device to launch on)
-    for bad in (dict(k=None), dict(v=None), dict(cos=AT), dict(cos=AT, sin=AT, pos=AT, table_rows=0), dict(cos=AT, pos=AT, table_rows=4)):
+    for bad in (dict(k=None), dict(v=None), dict(cos=AT), dict(cos=AT, sin=AT, pos=AT, table_rows=0), dict(cos=AT, pos=AT, table_rows=4),
+                dict(cos=AT, sin=AT, pos=AT + 4, table_rows=4), dict(cos=AT + 2, sin=AT, pos=AT, table_rows=4)):
         assert step(lib, **bad) == BAD_ARG and write(lib, **bad) == BAD_ARG, bad
-    for bad in (dict(first=None), dict(n=0), dict(heads=-1), dict(q=None), dict(q_out=None), dict(q_out=AT + 8)):
+    for bad in (dict(first=None), dict(first=AT + 4), dict(starts=AT + 4), dict(n=0), dict(heads=-1), dict(q=None), dict(q_out=None), dict(q_out=AT + 8)):
         assert write(lib, **bad) == BAD_ARG, bad
     assert write(lib, n=7) == BAD_SHAPE                                                    # not the same for three sequences
-    for bad in (dict(first=None), dict(count=0), dict(k=None), dict(v=AT + 8)):
+    for bad in (dict(first=None), dict(first=AT + 4), dict(count=0), dict(k=None), dict(v=AT + 8)):
         assert read(lib, **bad) == BAD_ARG, bad
     assert write(lib, q=None, q_out=None, heads=0) not in (0, BAD_ARG, BAD_SHAPE, UNSUPPORTED)
     # a long table is cut into ranges, whose sums need room
@@ -135,6 +136,7 @@ def adjust(**o):
     (dict(logits=AT + 1), BAD_ARG), (dict(dtype=1, out=AT + (1 << 20) + 2), BAD_ARG), (dict(logits_stride=-1), BAD_ARG), (dict(out_stride=999), BAD_ARG),
     (dict(width=-1), BAD_ARG), (dict(width=1 << 31), BAD_SHAPE), (dict(tokens=None, length=AT), BAD_ARG), (dict(tokens=None, repetition=AT), BAD_ARG),
     (dict(tokens_stride=-1), BAD_ARG), (dict(biases=-1), BAD_ARG), (dict(bias=None), BAD_ARG), (dict(bias_ids=None), BAD_ARG), (dict(bias_stride=-1), BAD_ARG),
+    (dict(tokens=AT + 4), BAD_ARG), (dict(prompt=AT + 4), BAD_ARG), (dict(next=AT + 4), BAD_ARG), (dict(mask=AT + 2), BAD_ARG), (dict(presence=AT + 1), BAD_ARG),
     (dict(masks=1), BAD_ARG), (dict(masks=0, mask_rows=AT), BAD_ARG), (dict(mask=None, mask_rows=AT), BAD_ARG), (dict(mask_stride=-1), BAD_ARG),
     # out over logits in part, one row further, and with another stride
     (dict(out=AT + 2), BAD_ARG), (dict(out=AT + 2000), BAD_ARG), (dict(out=AT - 3998), BAD_ARG), (dict(out=AT, out_stride=1001), BAD_ARG),
