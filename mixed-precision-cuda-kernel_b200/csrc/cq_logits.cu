@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
   int* s_rank = reinterpret_cast<int*>(s_bits + p.slice / 64);               // of a word's first marked token
   int* s_history = s_rank + p.slice / 64;                                    // -1 outside the vocabulary
   // [place], DIRECT: a place for every token, otherwise after the pieces and in their memory
-  uint32_t* s_known = DIRECT ? reinterpret_cast<uint32_t*>(s_rank) : reinterpret_cast<uint32_t*>(smem);
+  uint32_t* s_known = DIRECT ? reinterpret_cast<uint32_t*>(s_bits) + p.slice / 32 : reinterpret_cast<uint32_t*>(smem);
   uint32_t* s_token = s_known + PLACES;                                      // (not DIRECT)
   uint32_t* s_bias = DIRECT ? s_known + p.slice : s_token + PLACES;          // 1 + the entry that counts
   uint16_t* s_list = reinterpret_cast<uint16_t*>(s_known + (a.biases ? 2 : 1) * p.slice);   // DIRECT: the marked tokens, in any order
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
   const long long* ids = a.biases ? a.bias_ids + (int64_t)row * a.bias_ids_stride : nullptr;
   auto token_of = [&](long long v) { return (unsigned long long)v < (unsigned)p.vocab ? (int)v : -1; };
   // all that the row says in one round of loads
-  long long v0[TOKENS / THREADS], n64 = a.width, prompt64 = 0, mask_row = row;
+  long long v0[TOKENS / THREADS] = {}, n64 = a.width, prompt64 = 0, mask_row = row;
   float rep = 1.f, pres = 0.f, freq = 0.f;
   if (counts) {
 #pragma unroll
@@ -216,7 +216,8 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
       atomicMax(&s_bias[i], (uint32_t)j + 1u);
     };
     if (known) {
-      for (int i = tid; i < words; i += THREADS) s_bits[i] = 0u;
+      for (int i = tid; i < (size + 31) / 32; i += THREADS) reinterpret_cast<uint32_t*>(s_bits)[i] = 0u;
+      if (!DIRECT && tid == 0 && (size + 31) / 32 % 2) reinterpret_cast<uint32_t*>(s_bits)[(size + 31) / 32] = 0u;      // (the last word's other half)
       if (DIRECT)
         for (int i = tid; i < size; i += THREADS) {
           s_known[i] = 0u;
@@ -224,55 +225,77 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
         }
       if (DIRECT && tid == 0) s_count = 0;
       __syncthreads();
-      // -1 of a token that is outside, or marked already
-      auto unmarked = [&](int at) {
-        const uint32_t word = reinterpret_cast<volatile uint32_t*>(s_bits)[max(at, 0) >> 5];
-        return at >= 0 && !(word >> (at & 31) & 1u) ? at : -1;
-      };
-      // marks a token, -1: none; DIRECT: by all lanes of a warp, which take the list's next places together
-      auto mark = [&](int at) {
-        const uint32_t bit = 1u << (at & 31);
-        const uint32_t old = at >= 0 ? atomicOr(reinterpret_cast<uint32_t*>(s_bits) + (at >> 5), bit) : bit;
+      uint32_t* bits = reinterpret_cast<uint32_t*>(s_bits);
+      // Tokens at `at` (-1: none) of a lane, K at a time.  DIRECT: first(k) is whether that is the first that is known of the token, which then
+      // goes on the list; a warp takes the list's next places for all of its lanes.
+      auto note = [&](auto size, const int* at, auto first) {
+        constexpr int K = decltype(size)::value;
         if constexpr (DIRECT) {
-          const uint32_t fresh = __ballot_sync(0xffffffffu, !(old & bit));
-          if (!fresh) return;
+          uint32_t fresh[K];
+          int all = 0;
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            fresh[k] = __ballot_sync(0xffffffffu, first(k));
+            all += __popc(fresh[k]);
+          }
+          if (!all) return;
           int to = 0;
-          if (lane == 0) to = atomicAdd(&s_count, __popc(fresh));
-          to = __shfl_sync(0xffffffffu, to, 0) + __popc(fresh & ((1u << lane) - 1u));
-          if (!(old & bit)) s_list[to] = (uint16_t)at;
+          if (lane == 0) to = atomicAdd(&s_count, all);
+          to = __shfl_sync(0xffffffffu, to, 0);
+#pragma unroll
+          for (int k = 0; k < K; ++k) {
+            if (fresh[k] >> lane & 1u) {
+              s_list[to + __popc(fresh[k] & ((1u << lane) - 1u))] = (uint16_t)at[k];
+              atomicOr(&bits[at[k] >> 5], 1u << (at[k] & 31));
+            }
+            to += __popc(fresh[k]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+            if (at[k] >= 0 && !(*(volatile uint32_t*)&bits[at[k] >> 5] >> (at[k] & 31) & 1u)) atomicOr(&bits[at[k] >> 5], 1u << (at[k] & 31));
         }
       };
+      using std::integral_constant;
+      constexpr int K = TOKENS / THREADS;
       if (counts && (DIRECT || base == begin)) {
-        int at[TOKENS / THREADS], fresh[TOKENS / THREADS];
+#pragma unroll 1
+        for (int j0 = tid; j0 - tid < n; j0 += TOKENS) {
+          int at[K];
+          uint32_t old[K];
 #pragma unroll
-        for (int k = 0; k < TOKENS / THREADS; ++k) {
-          at[k] = fresh[k] = -1;
-          if (k * THREADS >= n) continue;
-          const int j = tid + k * THREADS, v = token_of(v0[k]);
-          at[k] = j < n ? place(v) : -1;
-          if (!DIRECT && j < p.keep) s_history[j] = v;
-          fresh[k] = unmarked(at[k]);
-        }
+          for (int k = 0; k < K; ++k) {
+            const int j = j0 + k * THREADS, v = token_of(v0[k]);
+            at[k] = j < n ? place(v) : -1;
+            if (!DIRECT && j < p.keep) s_history[j] = v;
+          }
+          // (the next ones are on their way meanwhile)
 #pragma unroll
-        for (int k = 0; k < TOKENS / THREADS; ++k) {
-          if (k * THREADS >= n) break;
-          mark(fresh[k]);
-          if (DIRECT && at[k] >= 0) occurred(at[k], tid + k * THREADS);
-        }
-#pragma unroll 4
-        for (int j0 = TOKENS; j0 < n; j0 += THREADS) {
-          const int j = j0 + tid, v = j < n ? token_of(tokens[j]) : -1, to = place(v);
-          if (!DIRECT && j < p.keep) s_history[j] = v;
-          mark(unmarked(to));
-          if (DIRECT && to >= 0) occurred(to, j);
+          for (int k = 0; k < K; ++k) v0[k] = j0 + TOKENS + k * THREADS < n ? tokens[j0 + TOKENS + k * THREADS] : -1;
+          if (DIRECT)
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+              old[k] = 1u;
+              if (at[k] >= 0) old[k] = j0 + k * THREADS < prompt ? atomicOr(&s_known[at[k]], PROMPT) : atomicAdd(&s_known[at[k]], 1u);
+            }
+          note(integral_constant<int, K>(), at, [&](int k) { return old[k] == 0u; });
         }
       } else if (counts) {
-        each_token(unmarked, [&](int i, int, int) { mark(i); });
+#pragma unroll 1
+        for (int j = tid; j < n; j += THREADS) {
+          const int at = place(j < p.keep ? s_history[j] : token_of(tokens[j]));
+          note(integral_constant<int, 1>(), &at, [](int) { return false; });
+        }
       }
-      for (int j0 = 0; j0 < a.biases; j0 += THREADS) {
+#pragma unroll 1
+      for (int j0 = 0; j0 < a.biases; j0 += THREADS) {     // of the same token's entries the last one counts
         const int j = j0 + tid, at = j < a.biases ? place(token_of(ids[j])) : -1;
-        mark(unmarked(at));
-        if (DIRECT && at >= 0) biased(at, j);
+        uint32_t old = 1u;
+        if (DIRECT && at >= 0) {
+          old = atomicOr(&s_known[at], BIAS);
+          atomicMax(&s_bias[at], (uint32_t)j + 1u);
+        }
+        note(integral_constant<int, 1>(), &at, [&](int) { return old == 0u; });
       }
     }
     if (mask || known) __syncthreads();      // (the mask's words and the marks are there)
@@ -432,13 +455,15 @@ extern "C" int cq_adjust_logits(const cq_adjust* a, int rows, int vocab, cq_stre
   const int sms = cq_sm_count(), vec = 16 / (int)item;
   int parts = 1;
   while (parts < PARTS && rows * parts < sms && vocab > parts * 1024) parts *= 2;
-  const int part = ((vocab + vec - 1 + parts - 1) / parts + vec - 1) / vec * vec, slice = std::min((part + 63) / 64 * 64, SLICE);
-  // Two CTAs on an SM; small slices with a place for every token
+  const int part = ((vocab + vec - 1 + parts - 1) / parts + vec - 1) / vec * vec;
+  // Two CTAs on an SM; small parts with a place for every token
+  constexpr int HALF = 112 * 1024 + 512;
   const bool known = a->tokens || a->biases;
-  constexpr int HALF = 112 * 1024 + 256;
-  const int ring = STAGES * THREADS * 16 + (a->mask ? slice / 8 + 16 : 0), few = ring + slice / 8 + slice * (a->biases ? 10 : 6);
+  int slice = (part + 31) / 32 * 32;
+  const int few = STAGES * THREADS * 16 + (a->mask ? slice / 8 + 16 : 0) + slice / 8 + slice * (a->biases ? 10 : 6);
   const bool direct = known && slice <= FEW && few <= HALF;
-  const int fixed = !known ? ring : (direct ? few : ring + slice / 64 * 12);
+  if (!direct) slice = std::min((part + 63) / 64 * 64, SLICE);
+  const int ring = STAGES * THREADS * 16 + (a->mask ? slice / 8 + 16 : 0), fixed = !known ? ring : (direct ? few : ring + slice / 64 * 12);
   const int keep = a->tokens && !direct ? (int)std::min<int64_t>(a->width, (112 * 1024 - fixed) / 4) : 0, smem = fixed + 4 * keep;
   const bool alike = (((uintptr_t)a->logits ^ (uintptr_t)a->out) & 15) == 0 && (rows == 1 || (a->logits_stride - a->out_stride) % vec == 0);
   auto fn = a->dtype == 0   ? (direct ? adjust_logits_kernel<__half, true> : adjust_logits_kernel<__half, false>)
