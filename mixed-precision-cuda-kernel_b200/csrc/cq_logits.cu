@@ -482,7 +482,7 @@ extern "C" int cq_adjust_logits(const cq_adjust* a, int rows, int vocab, cq_stre
   attr[1].val.clusterDim.x = parts;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = parts > 1 ? 2 : 1;
   CQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, Adjust{*a, vocab, part, slice, keep, alike}));
   return CQ_OK;
 }

@@ -519,7 +519,7 @@ int attend(const cq_pages* pages, const cq_table* table, const cq_rows* q, const
   attr[1].val.clusterDim.x = cluster;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = cluster ? 2 : 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   auto fn = cluster ? (k ? pages_attend_kernel<T, D, true, true> : pages_attend_kernel<T, D, false, true>)
                     : (k ? pages_attend_kernel<T, D, true, false> : pages_attend_kernel<T, D, false, false>);
   CQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, rows_of<T>(q), pool_of<T>(pages), table_of(table), fresh, length, (T*)out, workspace, shape));
