@@ -92,7 +92,7 @@ template <typename T> struct NewRow {
 
 // What the kernels get besides their tensors
 struct Shape {
-  int sequences, H, chunks, window, sinks, ctas;
+  int sequences, H, chunks, window, sinks;
   float scale;
 };
 constexpr int PART = 4;                      // in front of a head's D partial sums: maximum, sum of weights
@@ -352,11 +352,11 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
     auto visible = [&](int s) { return Visible<AT_SLOTS>(held(length, s, STEP, slots), shape.window, shape.sinks); };
     // Lengths of 32 sequences at a time: all tiles, then those in front of the CTA's.
     long long all = 0, before = 0;
-    int mine = 0, upto = 0;                  // of the lane's sequence in the last 32, and of those in front of it and its own
+    uint32_t mine = 0, upto = 0;             // of the lane's sequence in the last 32, and of those in front of it and its own
     auto scan = [&](int s) {
-      mine = upto = s + lane < B ? visible(s + lane).tiles : 0;
+      mine = upto = s + lane < B ? visible(s + lane).tiles : 0;      // (2^26 at most)
       for (int d = 1; d < 32; d *= 2) {
-        const int y = __shfl_up_sync(0xffffffffu, upto, d);
+        const uint32_t y = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += y;
       }
       return (long long)__shfl_sync(0xffffffffu, upto, 31);
@@ -507,7 +507,7 @@ int attend(const cq_pages* pages, const cq_table* table, const cq_rows* q, const
            cudaStream_t stream) {
   const int KV = pages->n_kv_heads, chunks = (H / KV + AT_HEADS - 1) / AT_HEADS, cluster = plan_of(pages, table, H, window, sinks), ctas = per_sm(D) * cq_sm_count();
   const NewRow<T> fresh = {rows_of<T>(k), rows_of<T>(v), cos_t, sin_t, positions, table_rows};
-  const Shape shape = {table->sequences, H, chunks, window, sinks, ctas, scale};
+  const Shape shape = {table->sequences, H, chunks, window, sinks, scale};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = cluster ? dim3(cluster, KV * chunks, table->sequences) : dim3(ctas);
   cfg.blockDim = dim3(AT_WARPS * 32);
