@@ -381,10 +381,16 @@ class CherryDecoder:
         """These sequences' pages are free for others; their steps are computed, on nothing, until they get a prompt."""
         if not self.kv_page:
             raise ValueError("only a paged cache (kv_page) has pages to give back")
-        for s in rows:
-            self.page_table.release(s)
-            self.held[s] = 0
+        rows = [int(r) for r in rows]
+        if any(not 0 <= r < self.batch for r in rows):
+            raise ValueError(f"rows must be sequences of the {self.batch}")
+        if not rows:
+            return
+        for r in rows:
+            self.page_table.release(r)
+            self.held[r] = 0
         self.table.copy_(self.page_table.host)
+        self.pos[torch.tensor(rows, device=self.dev)] = 0            # (nothing is looked for in pages that it no longer has)
         self.pos_host = max(self.held)
 
     # ------------------------------------------------------------------ control over what is picked
@@ -479,7 +485,8 @@ class CherryDecoder:
             self.table.copy_(self.page_table.host)
             end = torch.tensor(ends, dtype=torch.long, device=self.dev)
             self.prompts = self.table[rows] if some else self.table, end
-            pos = torch.where(place < end[:, None], place, -1).reshape(-1)
+            inside = place < end[:, None]
+            tokens, pos = torch.where(inside, tokens.to(self.dev), 0), torch.where(inside, place, -1).reshape(-1)
         else:
             pos = place.repeat(n)
         h, delta = self.embed[tokens.reshape(-1)], None
@@ -571,7 +578,7 @@ class CherryDecoder:
             else:
                 self._step()
         self.held = [x + n_tokens if x else 0 for x in self.held]
-        self.pos_host += n_tokens
+        self.pos_host = max(self.held) if self.kv_page else self.pos_host + n_tokens
         self._check_exchange()
         return out[:, 0] if self.batch == 1 else out
 

@@ -116,6 +116,46 @@ def test_sequences_come_and_go(dec):
     a.generate(5)
 
 
+@pytest.mark.parametrize("pad", [-1, 1000, 1 << 40])
+def test_what_stands_behind_a_prompt(dec, pad):
+    """Any number pads a batch, on the host too"""
+    cfg = tiny(dec)
+    lengths = [9, 30, 1]
+    prompt = tokens(cfg, 3, 30)
+    a = dec.CherryDecoder(cfg, seed=6, batch=3, kv_page=16)
+    a.control(repetition=1.5)
+    want = a.prefill(prompt, lengths)
+    told = a.generate(5)
+    for r, n in enumerate(lengths):
+        prompt[r, n:] = pad
+    assert torch.equal(a.prefill(prompt, lengths), want) and torch.equal(a.generate(5), told)
+    assert torch.equal(a.prefill(prompt.cpu(), lengths), want)
+
+
+def test_released_sequences_start_anew(dec):
+    """Their positions, which go on meanwhile, are none of their next prompt's"""
+    cfg = tiny(dec)
+    a = dec.CherryDecoder(cfg, seed=6, batch=2, kv_page=16)
+    a.prefill(tokens(cfg, 2, 20))
+    a.generate(100)
+    a.release([0, 0])
+    a.release([])
+    assert a.pos.tolist() == [0, 120] and a.held == [0, 120] and a.pos_host == 120
+    a.generate(100)
+    assert a.held == [0, 220] and a.page_table.held == [0, 14]
+    a.release([1])
+    for _ in range(2):
+        a.generate(200)                      # nobody is left
+    assert a.held == [0, 0] and len(a.page_table.free) == a.page_table.pages
+    one = a.prefill(tokens(cfg, 1, 20, seed=3), rows=[0])
+    b = dec.CherryDecoder(cfg, seed=6, batch=1, kv_page=16)
+    near(one, b.prefill(tokens(cfg, 1, 20, seed=3)))
+    for rows in ([-1], [2], [0, 2]):
+        with pytest.raises(ValueError):
+            a.release(rows)
+    assert a.held == [20, 0]
+
+
 def test_refusals(dec):
     cfg = tiny(dec)
     for bad in (dict(kv_page=-16), dict(kv_pages=4), dict(kv_page=16, kv_pages=0), dict(kv_page=16, kv_bits=4), dict(kv_page=16, attention="flash"),
