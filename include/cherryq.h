@@ -346,7 +346,7 @@ int cq_kv4_evict(const cq_kv4* from, const cq_kv4* to, const float* weights, flo
  * ---------------------------------------------------------------------- */
 typedef struct cq_pages {
   int32_t pages, n_kv_heads, page_size, head_dim, dtype;
-  void *k, *v;
+  void *k, *v;                          /* 32-byte aligned */
 } cq_pages;
 typedef struct cq_table {
   const int32_t* entries;

@@ -118,7 +118,7 @@ int read(const cq_pages* pages, const cq_table* table, const long long* first, i
 }  // namespace
 
 extern "C" int cq_pages_check(const cq_pages* p) {
-  if (!p || !p->k || !p->v || (((uintptr_t)p->k | (uintptr_t)p->v) & 15)) return CQ_ERR_BAD_ARG;
+  if (!p || !p->k || !p->v || (((uintptr_t)p->k | (uintptr_t)p->v) & 31)) return CQ_ERR_BAD_ARG;
   if (p->pages < 1 || p->n_kv_heads < 1 || p->n_kv_heads > 16383 || p->page_size < 16 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
     return CQ_ERR_BAD_SHAPE;
   if ((p->head_dim != 64 && p->head_dim != 128) || (p->dtype != 0 && p->dtype != 2)) return CQ_ERR_UNSUPPORTED;

@@ -13,6 +13,7 @@
 // sequences up to 4001 slots 42 us against 41, 13B heads with a window 38 against 33, four of 65531 slots 172 against 172), the next
 // tile's loads between the sums (registers spill: 53 against 41), two tiles a warp in rings on three CTAs an SM (249 against 172).
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -61,6 +62,10 @@ __device__ __forceinline__ uint4 ld16(const void* p) {
   asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
   return v;
 }
+__device__ __forceinline__ void ld32(uint4& a, uint4& b, const void* p) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w) : "l"(p) : "memory");
+}
 
 // What a query sees of n slots: j < first or from <= j < n, in tiles of TILE slots
 template <int TILE> struct Visible {
@@ -77,8 +82,7 @@ template <int TILE> struct Visible {
 };
 
 // slots that hold a row, a step's new one among them (more 1)
-__device__ __forceinline__ int held(const long long* length, int s, int more, int slots) {
-  const long long n = length[s];
+__device__ __forceinline__ int held(long long n, int more, int slots) {
   return n < 0 ? 0 : (n >= slots ? slots : (int)n + more);
 }
 
@@ -96,19 +100,69 @@ struct Shape {
   float scale;
 };
 constexpr int PART = 4;                      // in front of a head's D partial sums: maximum, sum of weights
-// The partial results of a CTA: of a head whose slots begin with an earlier CTA, of a head that a later CTA goes on with; and how many CTAs
-// that head has, its first one's sequence and head.
-struct Span {
-  int parts, seq, head, heads;
-};
-template <int D> __device__ __forceinline__ float* part_of(void* ws, int ctas, int cta, int which) {
-  return reinterpret_cast<float*>(reinterpret_cast<Span*>(ws) + ctas) + (size_t)(2 * cta + which) * AT_HEADS * (D + PART);
+// The partial results of a CTA: 0 of a head whose slots begin with an earlier CTA, 1 of a head that a later CTA goes on with
+template <int D> __device__ __forceinline__ float* part_of(void* ws, int cta, int which) {
+  return reinterpret_cast<float*>(ws) + (size_t)(2 * cta + which) * AT_HEADS * (D + PART);
 }
 
 // (most quotients fit 32 bits, whose division takes a quarter of the time)
 __device__ __forceinline__ long long quotient(long long a, long long b) {
   return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
 }
+// All tiles of all sequences and tasks in a row, cut into equal ranges for `ctas` CTAs.  (By whole warps, 32 sequences at a time.)
+// FAR: lengths past the first-level cache.
+template <bool FAR> struct Tiles {
+  const long long* length;
+  const Shape& shape;
+  const int slots, more, heads_each, lane;
+  long long total, each;
+  int n;                                     // slots of the lane's sequence in the last 32
+  uint32_t mine, upto;                       // its tiles, and those of the ones in front of it too (2^26 each at most)
+  __device__ __forceinline__ Tiles(const long long* length, const Shape& shape, int slots, int more, int heads_each, int ctas)
+      : length(length), shape(shape), slots(slots), more(more), heads_each(heads_each), lane(threadIdx.x & 31), total(0) {
+    for (int s = 0; s < shape.sequences; s += 32) total += scan(s);
+    total *= heads_each;
+    each = max((long long)AT_WARPS, quotient(total + ctas - 1, ctas));       // for each warp one at least
+  }
+  __device__ __forceinline__ Visible<AT_SLOTS> sees(int n) const { return Visible<AT_SLOTS>(n, shape.window, shape.sinks); }
+  __device__ __forceinline__ int slots_of(int s) const { return held(FAR ? __ldcg(length + s) : length[s], more, slots); }
+  __device__ __forceinline__ Visible<AT_SLOTS> visible(int s) const { return sees(slots_of(s)); }
+  __device__ __forceinline__ long long scan(int s) {
+    n = s + lane < shape.sequences ? slots_of(s + lane) : 0;
+    mine = upto = s + lane < shape.sequences ? sees(n).tiles : 0;
+    for (int d = 1; d < 32; d *= 2) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += y;
+    }
+    return (long long)__shfl_sync(0xffffffffu, upto, 31);
+  }
+  // the sequence with tile x < total; from: its first one; all: how many slots it has
+  __device__ __forceinline__ int find(long long x, long long& from, int& all) {
+    long long before = 0;
+    for (int s = 0;; s += 32) {
+      if (shape.sequences > 32) scan(s);
+      const uint32_t found = __ballot_sync(0xffffffffu, x < (before + upto) * heads_each);
+      if (found) {
+        const int k = __ffs(found) - 1;
+        from = (before + __shfl_sync(0xffffffffu, upto - mine, k)) * heads_each;
+        all = __shfl_sync(0xffffffffu, n, k);
+        return s + k;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  // a sequence's first tile; all: as above
+  __device__ __forceinline__ long long front(int seq, int& all) {
+    long long before = 0;
+    for (int s = 0; s < seq - seq % 32; s += 32) before += scan(s);
+    if (shape.sequences > 32) scan(seq - seq % 32);
+    all = __shfl_sync(0xffffffffu, n, seq % 32);
+    return (before + __shfl_sync(0xffffffffu, upto - mine, seq % 32)) * heads_each;
+  }
+};
+// Where the four columns 4 f .. of a head's sums are in shared memory: eight lanes with what one MMA gave them, and eight lanes
+// with consecutive columns, meet different banks (one sequence of 32 heads, 256 slots: 5.4 us; in order 5.8).
+__device__ __forceinline__ int place_of(int f) { return 4 * (f ^ (f >> 3 & 3)); }
 // CLUSTER: a cluster of CTAs for the heads of a KV head and sequence, each with the same share of its tiles.  Otherwise all tiles of all
 // sequences and KV heads in a row, cut into equal ranges for the CTAs that the device holds at once.
 template <typename T, int D, bool STEP, bool CLUSTER>
@@ -116,19 +170,24 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
                                                                         const long long* __restrict__ length, T* __restrict__ out, void* ws, const Shape shape) {
   constexpr int THREADS = AT_WARPS * 32;
   constexpr int KP = D / 32;                 // 16-byte pieces of a key per lane (four lanes a slot)
+  // Narrow heads' keys come two pieces at a time, whole lines for four lanes (64 sequences of 16 / 4 heads up to 5000 slots 54.3 us, so 55.8;
+  // wide ones 42.6 that way, also values 43.1, against 40.9).
+  constexpr bool PAIRS = D == 64;
+  auto piece = [](int i) { return PAIRS ? 64 * (i >> 1) + 8 * (i & 1) : 32 * i; };          // its columns, behind the lane's first
   constexpr int VS = D / 64;                 // of a value (eight lanes a slot)
   // Weights times a power of two: fp16's halves of their split then reach down to 2^-38 of the largest; in bf16, whose halves reach anywhere,
   // sums of 2^24 of the largest values stay finite.
   constexpr float LIFT = std::is_same<T, __half>::value ? 32768.f : 5.9604644775390625e-8f;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  __shared__ __align__(16) float s_sum[AT_WARPS][AT_HEADS][D];
+  if (CLUSTER) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ __align__(16) float s_sum[AT_WARPS][AT_HEADS][D + 8];
   __shared__ __align__(16) float s_part[CLUSTER ? AT_HEADS : 1][D + PART];
-  __shared__ __align__(16) T s_q[AT_HEADS][D + 32];
+  __shared__ __align__(16) T s_q[AT_HEADS][D + (PAIRS ? 8 : 32)];
   __shared__ float s_m[AT_WARPS][AT_HEADS], s_l[AT_WARPS][AT_HEADS];
   const int KV = pool.heads, H = shape.H, G = H / KV, chunks = shape.chunks, heads_each = KV * chunks, slots = table.width << pool.log_page;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g8 = lane >> 2, t4 = lane & 3;
   const float scale2 = shape.scale * 1.4426950408889634f;  // scores in powers of two
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!CLUSTER) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");          // (the second kernel reads lengths before it waits)
 
   // Tiles tile0 .. tile1 - 1 of one sequence and task (a KV head and eight of its query heads at most): to `out`, or partial results to `part`.
   auto segment = [&](int seq, int task, const Visible<AT_SLOTS>& vis, int tile0, int tile1, float* part) {
@@ -142,7 +201,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
       at = !fresh.cos_t || turn ? length[seq] : -1;
       if (at < 0 || at >= slots) at = -1;
     }
-    // queries in shared memory, rotated: a lane's pieces 8 t4 + 32 i of head g8
+    // queries in shared memory, rotated
     constexpr int PIECES = D / 16;
     for (int i = tid; i < AT_HEADS * PIECES; i += THREADS) {
       const int g = i / PIECES, c = 8 * (i - g * PIECES);
@@ -170,7 +229,8 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
       }
     }
     __syncthreads();
-    const T* mine_q = &s_q[g8][8 * t4];
+    const int first = (PAIRS ? 16 : 8) * t4; // of the lane's columns in queries and keys
+    const T* mine_q = &s_q[g8][first];
 
     float m = -INFINITY, l = 0.f;
     uint64_t o2[8 * VS];                     // MMA j + 8 s: its column n is column 64 s + 8 n + j of the head; n = 2 t4 and 2 t4 + 1
@@ -186,7 +246,11 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < KP; ++e) kk[h][e] = ld16(pool.k + (row0 + 8 * h + g8) * D + 8 * t4 + 32 * e);
+        for (int e = 0; e < KP; e += PAIRS ? 2 : 1) {
+          const T* from = pool.k + (row0 + 8 * h + g8) * D + first + piece(e);
+          if constexpr (PAIRS) ld32(kk[h][e], kk[h][e + 1], from);
+          else kk[h][e] = ld16(from);
+        }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int p = 8 * (u >> 1) + 2 * t4 + (u & 1);
@@ -196,7 +260,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
       uint64_t pairs[2] = {0, 0};
 #pragma unroll
       for (int e = 0; e < KP; ++e) {
-        const uint4 qa = *reinterpret_cast<const uint4*>(mine_q + 32 * e);
+        const uint4 qa = *reinterpret_cast<const uint4*>(mine_q + piece(e));
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint64_t d0[2], d1[2];
@@ -263,8 +327,8 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
 #pragma unroll
       for (int j = 0; j < 8; j += 4) {       // columns n = 2 t4 and 2 t4 + 1
         const float2 x0 = apart(o2[8 * e + j]), x1 = apart(o2[8 * e + j + 1]), x2 = apart(o2[8 * e + j + 2]), x3 = apart(o2[8 * e + j + 3]);
-        *reinterpret_cast<float4*>(&s_sum[warp][g8][64 * e + 16 * t4 + j]) = make_float4(x0.x, x1.x, x2.x, x3.x);
-        *reinterpret_cast<float4*>(&s_sum[warp][g8][64 * e + 16 * t4 + 8 + j]) = make_float4(x0.y, x1.y, x2.y, x3.y);
+        *reinterpret_cast<float4*>(&s_sum[warp][g8][place_of(16 * e + 4 * t4 + j / 4)]) = make_float4(x0.x, x1.x, x2.x, x3.x);
+        *reinterpret_cast<float4*>(&s_sum[warp][g8][place_of(16 * e + 4 * t4 + 2 + j / 4)]) = make_float4(x0.y, x1.y, x2.y, x3.y);
       }
     __syncthreads();
     for (int i = tid; i < heads * D / 4; i += THREADS) {
@@ -276,7 +340,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
 #pragma unroll
       for (int w = 0; w < AT_WARPS; ++w) {
         const float f = share_of(s_m[w][g], s_l[w][g], top);
-        const float4 x = *reinterpret_cast<const float4*>(&s_sum[w][g][d]);
+        const float4 x = *reinterpret_cast<const float4*>(&s_sum[w][g][place_of(d / 4)]);
         tot += f * s_l[w][g];
         sum[0] += f * x.x, sum[1] += f * x.y, sum[2] += f * x.z, sum[3] += f * x.w;
       }
@@ -310,7 +374,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
 
   if constexpr (CLUSTER) {
     const int rank = blockIdx.x, n = gridDim.x, task = blockIdx.y, seq = blockIdx.z;
-    const Visible<AT_SLOTS> vis(held(length, seq, STEP, slots), shape.window, shape.sinks);
+    const Visible<AT_SLOTS> vis(held(length[seq], STEP, slots), shape.window, shape.sinks);
     const int each = (vis.tiles + n - 1) / n, tile0 = min(vis.tiles, rank * each), tile1 = min(vis.tiles, tile0 + each);
     segment(seq, task, vis, tile0, tile1, n > 1 ? &s_part[0][0] : nullptr);
     if (n == 1) return;
@@ -349,91 +413,91 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   } else {
     const int cta = blockIdx.x, ctas = gridDim.x, B = shape.sequences;
-    auto visible = [&](int s) { return Visible<AT_SLOTS>(held(length, s, STEP, slots), shape.window, shape.sinks); };
-    // Lengths of 32 sequences at a time: all tiles, then those in front of the CTA's.
-    long long all = 0, before = 0;
-    uint32_t mine = 0, upto = 0;             // of the lane's sequence in the last 32, and of those in front of it and its own
-    auto scan = [&](int s) {
-      mine = upto = s + lane < B ? visible(s + lane).tiles : 0;      // (2^26 at most)
-      for (int d = 1; d < 32; d *= 2) {
-        const uint32_t y = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += y;
-      }
-      return (long long)__shfl_sync(0xffffffffu, upto, 31);
-    };
-    for (int s = 0; s < B; s += 32) all += scan(s);
-    all *= heads_each;
-    // tiles of a CTA: for each warp one at least
-    const long long each = max((long long)AT_WARPS, quotient(all + ctas - 1, ctas));
-    const long long begin = min(all, each * cta), end = min(all, begin + each);
-    int seq = 0;
-    long long from = 0;                      // where the sequence's tiles begin
-    if (begin < end)
-      for (int s = 0;; s += 32) {
-        const long long these = B <= 32 ? all / heads_each : scan(s);
-        if (begin < (before + these) * heads_each) {
-          const int k = __ffs(__ballot_sync(0xffffffffu, begin < (before + upto) * heads_each)) - 1;
-          seq = s + k;
-          from = (before + __shfl_sync(0xffffffffu, upto - mine, k)) * heads_each;
-          break;
-        }
-        before += these;
-      }
-    Span mark = {0, 0, 0, 0};
+    Tiles<false> all(length, shape, slots, STEP, heads_each, ctas);
+    const long long begin = min(all.total, all.each * cta), end = min(all.total, begin + all.each);
     if (begin < end) {
-      long long x = begin;
-      Visible<AT_SLOTS> vis = visible(seq);
+      long long x = begin, from;
+      int held_by, seq = all.find(x, from, held_by);
+      Visible<AT_SLOTS> vis = all.sees(held_by);
 #pragma unroll 1
       while (true) {
         const int task = (int)quotient(x - from, vis.tiles);
         const long long begins = from + (long long)task * vis.tiles, ends = begins + vis.tiles;
         const int tile0 = (int)(x - begins), tile1 = (int)(min(end, ends) - begins);
-        float* part = tile0 > 0 ? part_of<D>(ws, ctas, cta, 0) : (tile1 < vis.tiles ? part_of<D>(ws, ctas, cta, 1) : nullptr);
-        segment(seq, task, vis, tile0, tile1, part);
-        if (tile0 == 0 && tile1 < vis.tiles) {
-          const int kvh = task / chunks, h0 = (task - kvh * chunks) * AT_HEADS;
-          mark = {(int)quotient(ends - 1, each) - cta + 1, seq, kvh * G + h0, min(AT_HEADS, G - h0)};
-        }
+        segment(seq, task, vis, tile0, tile1, tile0 > 0 ? part_of<D>(ws, cta, 0) : (tile1 < vis.tiles ? part_of<D>(ws, cta, 1) : nullptr));
         x = begins + tile1;
         if (x >= end) break;
         if (x == from + (long long)vis.tiles * heads_each) {
           from = x;
-          do vis = visible(++seq);
+          do vis = all.visible(++seq);
           while (vis.tiles == 0);
         }
         __syncthreads();
       }
     }
-    if (tid == 0) reinterpret_cast<Span*>(ws)[cta] = mark;
     // (sequences that see nothing)
     for (int s = cta; s < B; s += ctas)
-      if (visible(s).tiles == 0)
+      if (all.visible(s).tiles == 0)
         for (int i = tid; i < H * D / 8; i += THREADS) reinterpret_cast<uint4*>(out + (size_t)s * H * D)[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
-// Joins the partial results of heads that several CTAs share: a block for the first of these; two warps a head, more where there are few.  A
-// warp has the shares of 32 parts in its lanes before it fetches their sums (fetched one by one with them, 8 x 8 heads of 55 parts on
-// cold caches take 23 us, so 17).
-constexpr int JOIN_WARPS = 2 * AT_HEADS;
+// Joins the partial results of heads that several CTAs share: a row of blocks for each task where there are few of them, otherwise for the one
+// that begins in a CTA and goes on behind it; `heads` of the task's heads for a block, the more warps a head the fewer tasks there are.
+// Which parts they are follows from the lengths alone, and is known before the first kernel ends: that one lets this one begin when its own
+// wait is over, so that lengths may be read (past the first-level cache).  A warp has the shares of 32 parts in its
+// lanes, and the first four parts' sums on their way, before it adds.  (One sequence of 64 / 8 heads, 32000 slots: 34.6 us with
+// the attention, 29.2 without this kernel; as one block for a task's heads, which looked up the parts in memory, 42.3.)
+constexpr int JOIN_WARPS = AT_HEADS;
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * JOIN_WARPS) pages_join_kernel(const void* ws, int H, T* __restrict__ out) {
-  constexpr int CPL = D / 32;
+__global__ void __launch_bounds__(32 * JOIN_WARPS) pages_join_kernel(const void* ws, const long long* __restrict__ length, const Shape shape, int slots, int more,
+                                                                     int KV, int ctas, int heads, T* __restrict__ out) {
+  constexpr int CPL = D / 32, EARLY = 4;
   using Columns = typename std::conditional<CPL == 4, float4, float2>::type;
   __shared__ __align__(16) float s_sum[JOIN_WARPS][D];
   __shared__ float s_top[JOIN_WARPS], s_tot[JOIN_WARPS];
+  __shared__ int4 s_job;                     // sequence, task, first CTA, parts
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, H = shape.H, G = H / KV, heads_each = KV * shape.chunks;
+  if (warp == 0) {
+    const bool few = gridDim.x == (long long)shape.sequences * heads_each;        // a row of blocks for each task
+    Tiles<true> all(length, shape, slots, more, heads_each, ctas);
+    int seq = -1, task = 0, n = 0, parts = 0, cta = 0;
+    long long from = 0;
+    if (few) {
+      seq = blockIdx.x / heads_each;
+      task = blockIdx.x - seq * heads_each;
+      from = all.front(seq, n);
+    } else if (all.each * (blockIdx.x + 1ll) < all.total) {
+      const long long x = all.each * (blockIdx.x + 1ll) - 1;
+      seq = all.find(x, from, n);
+      task = (int)quotient(x - from, all.sees(n).tiles);
+    }
+    if (const int tiles = seq < 0 ? 0 : all.sees(n).tiles) {
+      const long long begins = from + (long long)task * tiles;
+      cta = (int)quotient(begins, all.each);
+      if (few || cta == blockIdx.x) parts = (int)quotient(begins + tiles - 1, all.each) - cta + 1;
+    }
+    if (lane == 0) s_job = make_int4(seq, task, cta, parts);
+  }
+  __syncthreads();
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int cta = blockIdx.x, ctas = gridDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Span span = reinterpret_cast<const Span*>(ws)[cta];
-  if (span.parts == 0) return;
-  const int groups = JOIN_WARPS / span.heads, g = warp / groups, group = warp - g * groups;
-  auto part = [&](int r) { return part_of<D>(const_cast<void*>(ws), ctas, cta + r, r == 0) + g * (D + PART); };
+  const int seq = s_job.x, task = s_job.y, cta = s_job.z, parts = s_job.w;
+  const int kvh = task / shape.chunks, h0 = (task - kvh * shape.chunks) * AT_HEADS, first = blockIdx.y * heads;
+  heads = min(heads, min(AT_HEADS, G - h0) - first);
+  if (parts < 2 || heads <= 0) return;
+  const int groups = JOIN_WARPS / heads, g = warp / groups, group = warp - g * groups;
+  auto part = [&](int r) { return part_of<D>(const_cast<void*>(ws), cta + r, r == 0) + (first + g) * (D + PART); };
+  auto columns = [&](int r) { return *reinterpret_cast<const Columns*>(part(r) + PART + CPL * lane); };
   float top = -INFINITY, tot = 0.f, sum[CPL] = {};
-  if (g < span.heads)
-    for (int r0 = group; r0 < span.parts; r0 += 32 * groups) {
-      const int r = r0 + lane * groups, n = min(32, (span.parts - r0 + groups - 1) / groups);
-      const float2 ml = r < span.parts ? *reinterpret_cast<const float2*>(part(r)) : make_float2(-INFINITY, 0.f);
+  if (g < heads)
+    for (int r0 = group; r0 < parts; r0 += 32 * groups) {
+      const int r = r0 + lane * groups, n = min(32, (parts - r0 + groups - 1) / groups);
+      const float2 ml = r < parts ? *reinterpret_cast<const float2*>(part(r)) : make_float2(-INFINITY, 0.f);
+      Columns x[EARLY];
+#pragma unroll
+      for (int k = 0; k < EARLY; ++k)
+        if (k < n) x[k] = columns(r0 + k * groups);
       float next = fmaxf(top, ml.x);
       for (int d = 16; d; d /= 2) next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, d));
       const float keep = share_of(top, tot, next), f = share_of(ml.x, ml.y, next);
@@ -443,19 +507,22 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) pages_join_kernel(const void*
       tot = tot * keep + add;
 #pragma unroll
       for (int i = 0; i < CPL; ++i) sum[i] *= keep;
-#pragma unroll 8
-      for (int k = 0; k < n; ++k) {
-        const Columns x = *reinterpret_cast<const Columns*>(part(r0 + k * groups) + PART + CPL * lane);
+      auto more_of = [&](const Columns& c, int k) {
         const float fk = __shfl_sync(0xffffffffu, f, k);
 #pragma unroll
-        for (int i = 0; i < CPL; ++i) sum[i] = __fmaf_rn(fk, reinterpret_cast<const float*>(&x)[i], sum[i]);
-      }
+        for (int i = 0; i < CPL; ++i) sum[i] = __fmaf_rn(fk, reinterpret_cast<const float*>(&c)[i], sum[i]);
+      };
+#pragma unroll
+      for (int k = 0; k < EARLY; ++k)
+        if (k < n) more_of(x[k], k);
+#pragma unroll 8
+      for (int k = EARLY; k < n; ++k) more_of(columns(r0 + k * groups), k);
     }
 #pragma unroll
   for (int i = 0; i < CPL; ++i) s_sum[warp][CPL * lane + i] = sum[i];
   if (lane == 0) s_top[warp] = top, s_tot[warp] = tot;
   __syncthreads();
-  if (g >= span.heads || group) return;
+  if (g >= heads || group) return;
   float best = -INFINITY;
   for (int k = 0; k < groups; ++k) best = fmaxf(best, s_top[warp + k]);
   tot = 0.f;
@@ -469,30 +536,58 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) pages_join_kernel(const void*
     for (int i = 0; i < CPL; ++i) sum[i] = __fmaf_rn(f, s_sum[warp + k][CPL * lane + i], sum[i]);
   }
   const bool none = tot == 0.f;
-  T* to = out + ((size_t)span.seq * H + span.head + g) * D + CPL * lane;
+  T* to = out + ((size_t)seq * H + kvh * G + h0 + first + g) * D + CPL * lane;
 #pragma unroll
   for (int i = 0; i < CPL; i += 2) *reinterpret_cast<uint32_t*>(to + i) = none ? 0u : Type<T>::pair(sum[i] / tot, sum[i + 1] / tot);
 }
 
-// CTAs of a cluster for each sequence and task, 0: equal ranges.  The least time by a model (us): waves of CTAs, each its start and the
+// Clusters of n CTAs that the device holds at once (fewer than its CTAs / n: a cluster lies in one part of the device)
+int clusters_of(int head_dim, int n) {
+  static std::atomic<int> known[64][2][MAX_CLUSTER + 1];
+  const int rest = per_sm(head_dim) * cq_sm_count() / n;
+  int dev = 0, clusters = 0;
+  if (n == 1 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return rest;
+  std::atomic<int>& kept = known[dev][head_dim == 64][n];
+  if ((clusters = kept.load(std::memory_order_relaxed)) > 0) return clusters;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(n);
+  cfg.blockDim = dim3(AT_WARPS * 32);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = n;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&clusters, head_dim == 64 ? pages_attend_kernel<__half, 64, false, true> : pages_attend_kernel<__half, 128, false, true>,
+                                     &cfg) != cudaSuccess || clusters < 1) {
+    (void)cudaGetLastError();
+    return rest;
+  }
+  kept.store(clusters, std::memory_order_relaxed);
+  return clusters;
+}
+
+// CTAs of a cluster for each sequence and task, 0: equal ranges.  The least time by a model (us): waves of clusters, each its start and the
 // turns of a warp, which take longer the fuller the SMs are; joins; for ranges what all warps need together, a start for every task and
-// the second kernel.  It goes by the table's width: lengths are known to the device alone.  (16 sequences of 64 / 8 heads up to
-// 4001 slots: 1 CTA 81 us, 2 54, 3 41, 4 51, 8 50, ranges 49; 8 of 40 heads, window 1021: 1 34, 2 39, ranges 40; 4 of 64 / 8 heads,
-// 65531 slots: 8 208, ranges 174; 1 of 32 heads, 256 slots: 1 8.0, 6 6.0, ranges 12.6; 55 of 16 / 4 heads, 2 slots: 1 4.5, ranges 14.7.)
+// the second kernel.  It goes by the table's width: lengths are known to the device alone.  Its numbers are those with which it lost
+// least over 937 calls (1 to 128 sequences of 32 / 32, 64 / 8 and 16 / 4 heads, 60 to 65000 slots, equal and mixed lengths): the plan taken is 0.6 %
+// behind the best on average, 12 % at most.  (16 sequences of 64 / 8 heads up to 4001 slots: 1 CTA 83 us, 2 53, 3 41, 4 50, 8 49, ranges
+// 44; 8 of 40 heads, window 1021: 1 32, 2 39, ranges 38; 2 of 64 / 8 heads up to 20000 slots: 8 53, ranges 33; 24 of 16 / 4 heads, 1500 slots: 5
+// 11.6, 6, of which the device does not hold 96, 16.8; 5 of them, 60 slots: 1 2.7, ranges 8.1.)
 int plan_of(const cq_pages* pages, const cq_table* table, int n_heads, int window, int sinks) {
   const int KV = pages->n_kv_heads, chunks = (n_heads / KV + AT_HEADS - 1) / AT_HEADS, sms = cq_sm_count(), slots = per_sm(pages->head_dim) * sms;
   const bool narrow = pages->head_dim == 64;
   const double tasks = (double)table->sequences * KV * chunks;
   const long long all = (long long)table->width * pages->page_size;
   const long long most = window ? std::min<long long>(all, (long long)window + sinks + AT_SLOTS) : all, tiles = (most + AT_SLOTS - 1) / AT_SLOTS;
-  const double full = narrow ? 1.48 : 2.2;                 // a turn of all warps that the SMs hold
-  double least = 9 + 2.5 * (1 + tasks / slots) + std::max(1.0, tasks * tiles / (slots * AT_WARPS)) * full;
+  double least = 13 + 3.4 * tasks / slots + std::max(1.0, tasks * tiles / (slots * AT_WARPS)) * (narrow ? 1.12 : 2.2);
   int best = 0;
   for (int n = 1; n <= MAX_CLUSTER; ++n) {
     if (n > 1 && (n - 1) * AT_WARPS >= tiles) break;
-    const double ctas = tasks * n, each = std::min((double)per_sm(pages->head_dim), std::max(1.0, ctas / sms));
-    const double turn = narrow ? std::max(0.85 + 0.1 * each, 0.37 * each) : std::max(1.0 + 0.3 * each, 0.74 * each);
-    const double t = 1.2 + std::ceil(ctas / slots) * (((tiles + n * AT_WARPS - 1) / (n * AT_WARPS)) * turn + 2.1) + (n > 1 ? 0.9 + 0.05 * n : 0.0);
+    const double held = clusters_of(pages->head_dim, n), each = std::min(held * n / sms, std::max(1.0, tasks * n / sms));
+    const double turn = narrow ? std::max(0.97 + 0.11 * each, 0.31 * each) : std::max(0.82 + 0.45 * each, 0.7 * each);
+    const double waves = tasks <= held ? 1.0 : 0.75 * tasks / held + 0.25 * std::ceil(tasks / held);
+    const double t = 1.3 + waves * (((tiles + n * AT_WARPS - 1) / (n * AT_WARPS)) * turn + 2.0) + (n > 1 ? 1.35 + 0.085 * n : 0.0);
     if (t < least) {
       least = t;
       best = n;
@@ -523,7 +618,14 @@ int attend(const cq_pages* pages, const cq_table* table, const cq_rows* q, const
   auto fn = cluster ? (k ? pages_attend_kernel<T, D, true, true> : pages_attend_kernel<T, D, false, true>)
                     : (k ? pages_attend_kernel<T, D, true, false> : pages_attend_kernel<T, D, false, false>);
   CQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, fn, rows_of<T>(q), pool_of<T>(pages), table_of(table), fresh, length, (T*)out, workspace, shape));
-  if (!cluster) CQ_CUDA_TRY(kv4_launch(pages_join_kernel<T, D>, dim3(ctas), dim3(32 * JOIN_WARPS), 0, stream, (const void*)workspace, H, (T*)out));
+  if (!cluster) {
+    // as many blocks as there are CTAs, or fewer
+    const int tasks = std::min(table->sequences, ctas) * std::min(KV * chunks, ctas), most = std::min(AT_HEADS, H / KV);
+    int heads = most;
+    while (heads > 1 && tasks * ((most + heads / 2 - 1) / (heads / 2)) <= ctas) heads /= 2;
+    CQ_CUDA_TRY(kv4_launch(pages_join_kernel<T, D>, dim3(std::min(tasks, ctas), (most + heads - 1) / heads), dim3(32 * JOIN_WARPS), 0, stream,
+                           (const void*)workspace, length, shape, table->width * pages->page_size, (int)(k != nullptr), KV, ctas, heads, (T*)out));
+  }
   return CQ_OK;
 }
 
@@ -545,7 +647,7 @@ int call(const cq_pages* pages, const cq_table* table, const cq_rows* q, const c
 extern "C" size_t cq_pages_attend_workspace_bytes(const cq_pages* pages, const cq_table* table, int n_heads, int window, int sinks) {
   if (check(pages, table) != CQ_OK || n_heads < 1 || n_heads % pages->n_kv_heads || window < 0 || sinks < 0) return 0;
   if (plan_of(pages, table, n_heads, window, sinks)) return 0;
-  return (size_t)per_sm(pages->head_dim) * cq_sm_count() * (sizeof(Span) + 2 * AT_HEADS * (pages->head_dim + PART) * sizeof(float));
+  return (size_t)per_sm(pages->head_dim) * cq_sm_count() * 2 * AT_HEADS * (pages->head_dim + PART) * sizeof(float);
 }
 
 extern "C" int cq_pages_attend(const cq_pages* pages, const cq_table* table, const cq_rows* q, const long long* length, void* out, int n_heads,

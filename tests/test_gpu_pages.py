@@ -383,6 +383,77 @@ def test_read(qc, dtype, D):
                 assert torch.equal(k[b, i], want[0]) and torch.equal(v[b, i], want[1]), (b, i)
 
 
+# ---------------------------------------------------------------------------------- long tables: equal ranges of all tiles, joined
+def long_table(qc, D, H, KV, B, page, width, dtype, seed):
+    """A small pool for a long table (pages in several places), a page of its own where each sequence's next row goes"""
+    g = gen(seed)
+    lengths = (torch.rand(B, device="cuda", generator=g) ** 6 * (width * page - 1)).long()
+    lengths[0] = width * page - 10
+    if B > 2:
+        lengths[B // 2], lengths[B - 1] = 0, -3
+    n = 3 * width // 4
+    cache = pool(qc, g, n + B, KV, page, D, dtype)
+    table = torch.randint(0, n, (B, width), device="cuda", generator=g).to(torch.int32)
+    at = torch.arange(B, device="cuda")
+    table[at, (lengths.clamp(min=0) // page)] = (n + at).to(torch.int32)
+    return g, cache, table, lengths, randn(g, B, H, D).to(dtype)
+
+
+LONG_TABLES = [
+    (128, 10, 2, 1, 64, 500, FP16),            # few heads, many parts of each
+    (128, 8, 8, 2, 16, 1200, BF16),
+    (64, 3, 1, 40, 64, 300, FP16),
+    (128, 24, 2, 33, 32, 300, BF16),           # two tiles of queries a head
+    (64, 2, 1, 600, 16, 400, FP16),            # more heads than ranges
+    (64, 4, 4, 260, 16, 400, BF16),
+]
+
+
+@pytest.mark.parametrize("D,H,KV,B,page,width,dtype", LONG_TABLES)
+def test_long_tables(qc, D, H, KV, B, page, width, dtype):
+    g, cache, table, lengths, q = long_table(qc, D, H, KV, B, page, width, dtype, D + B)
+    out = cache.attend(q, table, lengths)
+    close(out, *attend_ref(cache, q, table, lengths.tolist()))
+    assert not out[lengths <= 0].any()
+    k, v = (randn(g, B, KV, D).to(dtype) for _ in range(2))
+    before = cache.k.clone()
+    out = cache.step(q, k, v, None, None, None, table, lengths)
+    close(out, *attend_ref(cache, q, table, [n + 1 if n >= 0 else 0 for n in lengths.tolist()]))
+    there = lengths >= 0
+    before[table[torch.arange(B, device="cuda"), lengths.clamp(min=0) // page][there].long(), :, (lengths % page)[there]] = k[there]
+    assert torch.equal(cache.k, before)
+
+
+@pytest.mark.parametrize("case", LONG_TABLES[::2])
+def test_long_tables_whose_lengths_change(qc, case):
+    """The second kernel looks at lengths while the first one runs, not while what wrote them does"""
+    g, cache, table, lengths, q = long_table(qc, *case, 7)
+    far = torch.full((1 << 22,), 1.0, device="cuda")
+    ends = [lengths, lengths.flip(0), lengths // 3, torch.zeros_like(lengths), lengths]
+    want = [cache.attend(q, table, n) for n in ends]
+    torch.cuda.synchronize()
+    now, outs = lengths.clone(), []
+
+    def run():
+        outs.clear()
+        for n in ends:
+            far.mul_(1.0)
+            now.copy_(n)
+            outs.append(cache.attend(q, table, now))
+    run()
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        run()
+    for _ in range(10):
+        for x in outs:
+            x.fill_(float("nan"))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
 # ---------------------------------------------------------------------------------- steps
 @pytest.mark.parametrize("dtype", [FP16, BF16])
 @pytest.mark.parametrize("turn", [False, True])

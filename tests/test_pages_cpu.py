@@ -86,6 +86,15 @@ def test_pool_fields(lib, field, value, code):
     assert lib.cq_pages_attend_workspace_bytes(C.byref(p), C.byref(table()), 4, 0, 0) == 0
 
 
+def test_pools_start_on_32_bytes(lib):
+    for field in ("k", "v"):
+        p = pages()
+        setattr(p, field, getattr(p, field) + 16)
+        assert lib.cq_pages_check(C.byref(p)) == BAD_ARG
+        setattr(p, field, getattr(p, field) + 16)
+        assert lib.cq_pages_check(C.byref(p)) == 0
+
+
 @pytest.mark.parametrize("field,value,code", [
     ("entries", None, BAD_ARG), ("entries", AT + 2, BAD_ARG), ("stride", -1, BAD_ARG), ("sequences", 0, BAD_SHAPE), ("sequences", 65536, BAD_SHAPE),
     ("width", 0, BAD_SHAPE), ("width", (1 << 26) + 1, BAD_SHAPE),
