@@ -6,7 +6,7 @@
 // the marked tokens' places, a token's rank among them.  The pass over the logits leaves the marked ones out of the maximum;
 // their values are written over its results.  (256 rows of 131071 bf16 logits, histories of 1500 and masks: 31 us; penalties in the pass take 57
 // instructions a logit, 138 us; counters for all tokens, a slice of the vocabulary after the other, 87.  A row of 32000
-// with a history of 300 4.8 us, without 3.4.)  Every thread has four pieces of 16 bytes on the way, copied asynchronously to places of its
+// with a history of 300 4.7 us, without 3.4.)  Every thread has four pieces of 16 bytes on the way, copied asynchronously to places of its
 // own, and waits for no other thread; what no mask changes is neither converted nor rounded.  Of eight logits only the largest
 // meets the thread's best.  The largest travels as one 64-bit key, its value in the order of unsigned numbers above the
 // complement of its token: the maximum of keys is the lowest token of the largest value.
@@ -21,7 +21,6 @@ constexpr int THREADS = 512, WARPS = THREADS / 32;
 constexpr int STAGES = 4;                    // pieces of 16 bytes of a thread on their way
 constexpr int PARTS = 8;                     // CTAs of a row, at most
 constexpr int TOKENS = 4 * THREADS;          // of the history, loads in flight
-constexpr int FEW = 8192;                    // tokens of a slice with a place each, at most
 constexpr int SLICE = 129 * 1024;            // tokens that the bit map holds
 constexpr int PLACES = STAGES * THREADS * 16 / 12;          // marked tokens at a time, in the pieces' memory
 // what is known of a token: whether it occurred in the prompt, whether it has a bias, and below how often it was generated
@@ -88,6 +87,12 @@ template <int BYTES> __device__ __forceinline__ void copy_async(void* to, const 
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from), "n"(BYTES) : "memory");
 }
 
+// the largest key of a warp's lanes
+__device__ __forceinline__ unsigned long long largest_of_warp(unsigned long long key) {
+  const uint32_t high = (uint32_t)(key >> 32), top = __reduce_max_sync(0xffffffffu, high);
+  return (unsigned long long)top << 32 | __reduce_max_sync(0xffffffffu, high == top ? (uint32_t)key : 0u);
+}
+
 template <typename T, bool DIRECT>
 __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust p) {
   constexpr int VEC = 16 / sizeof(T);
@@ -139,8 +144,6 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
   };
-  first_pieces(begin, min(end, begin + p.slice));
-
   const long long* tokens = counts ? a.tokens + (int64_t)row * a.tokens_stride : nullptr;
   const long long* ids = a.biases ? a.bias_ids + (int64_t)row * a.bias_ids_stride : nullptr;
   auto token_of = [&](long long v) { return (unsigned long long)v < (unsigned)p.vocab ? (int)v : -1; };
@@ -157,6 +160,7 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
     if (a.frequency) freq = a.frequency[row];
   }
   if (a.mask && a.mask_rows) mask_row = a.mask_rows[row];
+  first_pieces(begin, min(end, begin + p.slice));
   const uint32_t* mask = a.mask && mask_row >= 0 && mask_row < a.masks ? a.mask + mask_row * a.mask_stride : nullptr;
   const int n = !counts || n64 < 0 ? 0 : (int)(n64 > a.width ? a.width : n64), prompt = (int)(prompt64 < 0 ? 0 : (prompt64 > n ? n : prompt64));
 
@@ -169,14 +173,17 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
   for (int base = begin; base < end; base += p.slice) {
     const int stop = min(end, base + p.slice), size = stop - base, words = (size + 63) / 64;
     if (base != begin) first_pieces(base, stop);
-    // The mask's words, moved to where the marks of the same tokens are
-    if (mask)
-#pragma unroll 4
-      for (int i = tid; i < (size + 31) / 32; i += THREADS) {
-        const int v = base + 32 * i - skip, w = v >> 5;
-        const uint32_t low = w >= 0 ? __ldg(mask + w) : 0u, high = 32 * (w + 1) < p.vocab ? __ldg(mask + w + 1) : 0u;
-        s_mask[i] = __funnelshift_r(low, high, v & 31);
-      }
+    if (known) {
+      for (int i = tid; i < (size + 31) / 32; i += THREADS) reinterpret_cast<uint32_t*>(s_bits)[i] = 0u;
+      if (!DIRECT && tid == 0 && (size + 31) / 32 % 2) reinterpret_cast<uint32_t*>(s_bits)[(size + 31) / 32] = 0u;      // (the last word's other half)
+      if (DIRECT)
+        for (int i = tid; i < size; i += THREADS) {
+          s_known[i] = 0u;
+          if (a.biases) s_bias[i] = 0u;
+        }
+      if (DIRECT && tid == 0) s_count = 0;
+      __syncthreads();
+    }
     // the place of a token in the slice, -1 outside
     auto place = [&](int v) {
       const int j = v < 0 ? -1 : v + skip - base;
@@ -216,15 +223,6 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
       atomicMax(&s_bias[i], (uint32_t)j + 1u);
     };
     if (known) {
-      for (int i = tid; i < (size + 31) / 32; i += THREADS) reinterpret_cast<uint32_t*>(s_bits)[i] = 0u;
-      if (!DIRECT && tid == 0 && (size + 31) / 32 % 2) reinterpret_cast<uint32_t*>(s_bits)[(size + 31) / 32] = 0u;      // (the last word's other half)
-      if (DIRECT)
-        for (int i = tid; i < size; i += THREADS) {
-          s_known[i] = 0u;
-          if (a.biases) s_bias[i] = 0u;
-        }
-      if (DIRECT && tid == 0) s_count = 0;
-      __syncthreads();
       uint32_t* bits = reinterpret_cast<uint32_t*>(s_bits);
       // Tokens at `at` (-1: none) of a lane, K at a time.  DIRECT: first(k) is whether that is the first that is known of the token, which then
       // goes on the list; a warp takes the list's next places for all of its lanes.
@@ -298,6 +296,14 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
         note(integral_constant<int, 1>(), &at, [&](int) { return old == 0u; });
       }
     }
+    // The mask's words, moved to where the marks of the same tokens are
+    if (mask)
+#pragma unroll 4
+      for (int i = tid; i < (size + 31) / 32; i += THREADS) {
+        const int v = base + 32 * i - skip, w = v >> 5;
+        const uint32_t low = w >= 0 ? __ldg(mask + w) : 0u, high = 32 * (w + 1) < p.vocab ? __ldg(mask + w + 1) : 0u;
+        s_mask[i] = __funnelshift_r(low, high, v & 31);
+      }
     if (mask || known) __syncthreads();      // (the mask's words and the marks are there)
     // what is known of the marked tokens with ranks from rank0 on
     auto count = [&](int rank0, int here) {
@@ -325,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
     auto put = [&](int i, int j) {
       const uint32_t c = s_known[i];
       const int at = base + j;
-      float x = value_of<T>(DIRECT ? reinterpret_cast<const T*>(smem)[j] : in[at]);         // (a small slice's pieces are all there yet)
+      float x = value_of<T>(DIRECT && size <= STAGES * STEP ? reinterpret_cast<const T*>(smem)[j] : in[at]);       // (a small slice's pieces are all there yet)
       if (a.repetition && (c & (PROMPT | TIMES))) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
       if (c & TIMES) {
         if (a.frequency) x = __fsub_rn(x, __fmul_rn(freq, (float)(c & TIMES)));
@@ -408,12 +414,11 @@ __global__ void __launch_bounds__(THREADS, 2) adjust_logits_kernel(const Adjust 
 #pragma unroll
   for (int e = 0; e < VEC; ++e)
     if (at_top >= 0 && at_top + e >= skip && at_top + e < total) best = larger(best, key_of(value_of<T>(of_top.at(e)), at_top + e - skip));
-  for (int d = 16; d; d /= 2) best = larger(best, __shfl_xor_sync(0xffffffffu, best, d));
+  best = largest_of_warp(best);
   if (lane == 0) s_key[warp] = best;
   __syncthreads();
   if (warp == 0) {
-    best = lane < THREADS / 32 ? s_key[lane] : 0ull;
-    for (int d = 16; d; d /= 2) best = larger(best, __shfl_xor_sync(0xffffffffu, best, d));
+    best = largest_of_warp(lane < THREADS / 32 ? s_key[lane] : 0ull);
   }
   if (parts > 1) {                           // to the cluster's first CTA
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -453,17 +458,24 @@ extern "C" int cq_adjust_logits(const cq_adjust* a, int rows, int vocab, cq_stre
   const bool in_place = a->logits == a->out && (rows == 1 || a->logits_stride == a->out_stride);
   if (!in_place && !kv4_apart(a->logits, span(rows, vocab, a->logits_stride, item), a->out, span(rows, vocab, a->out_stride, item))) return CQ_ERR_BAD_ARG;
   const int sms = cq_sm_count(), vec = 16 / (int)item;
+  const bool known = a->tokens || a->biases;
+  auto part_of = [&](int parts) { return ((vocab + vec - 1 + parts - 1) / parts + vec - 1) / vec * vec; };
+  // bytes of a CTA with a place for every token of its part (64 bits: a part may be the whole vocabulary)
+  auto places = [&](int parts) {
+    const int64_t slice = (part_of(parts) + 31) / 32 * 32;
+    return STAGES * THREADS * 16 + (a->mask ? slice / 8 + 16 : 0) + slice / 8 + slice * (a->biases ? 10 : 6);
+  };
+  // Two CTAs on an SM, or one where few run.  A place for every token, where there is room (a row of 128256 logits with a history of 8000 10.9 us,
+  // with ranks 13.1); for that also half the CTAs, which then see a history half as often (64 rows of 50257 logits 7.2 us, so 8.0; 100 of
+  // 25000 7.2, so 8.4).  More CTAs than fill the device lose (128 rows of 32000 14.0 against 9.9).
+  constexpr int HALF = 112 * 1024 + 512, WHOLE = 225 * 1024;
   int parts = 1;
   while (parts < PARTS && rows * parts < sms && vocab > parts * 1024) parts *= 2;
-  const int part = ((vocab + vec - 1 + parts - 1) / parts + vec - 1) / vec * vec;
-  // Two CTAs on an SM; small parts with a place for every token
-  constexpr int HALF = 112 * 1024 + 512;
-  const bool known = a->tokens || a->biases;
-  int slice = (part + 31) / 32 * 32;
-  const int few = STAGES * THREADS * 16 + (a->mask ? slice / 8 + 16 : 0) + slice / 8 + slice * (a->biases ? 10 : 6);
-  const bool direct = known && slice <= FEW && few <= HALF;
-  if (!direct) slice = std::min((part + 63) / 64 * 64, SLICE);
-  const int ring = STAGES * THREADS * 16 + (a->mask ? slice / 8 + 16 : 0), fixed = !known ? ring : (direct ? few : ring + slice / 64 * 12);
+  int room = rows * parts <= sms / 2 ? WHOLE : HALF;
+  if (known && (parts == 2 || parts == 4) && rows * parts / 2 <= sms && places(parts / 2) <= WHOLE) parts /= 2, room = WHOLE;
+  const bool direct = known && places(parts) <= room;
+  const int part = part_of(parts), slice = direct ? (part + 31) / 32 * 32 : std::min((part + 63) / 64 * 64, SLICE);
+  const int ring = STAGES * THREADS * 16 + (a->mask ? slice / 8 + 16 : 0), fixed = !known ? ring : (direct ? (int)places(parts) : ring + slice / 64 * 12);
   const int keep = a->tokens && !direct ? (int)std::min<int64_t>(a->width, (112 * 1024 - fixed) / 4) : 0, smem = fixed + 4 * keep;
   const bool alike = (((uintptr_t)a->logits ^ (uintptr_t)a->out) & 15) == 0 && (rows == 1 || (a->logits_stride - a->out_stride) % vec == 0);
   auto fn = a->dtype == 0   ? (direct ? adjust_logits_kernel<__half, true> : adjust_logits_kernel<__half, false>)

@@ -110,6 +110,24 @@ def test_adjust(qc, dtype, R, V, W, biases, masks):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,V,W,biases,masks", [
+    (64, 50257, 30, 0, 0), (100, 32000, 20, 0, 0), (140, 20001, 40, 0, 2), (40, 31999, 40, 3, 1), (74, 12345, 30, 8, 3), (8, 128256, 70, 0, 2),
+    (9, 100003, 50, 9, 0), (1, 200000, 3000, 0, 1), (37, 36001, 30, 0, 0), (149, 20000, 10, 0, 0),
+])
+def test_adjust_large_parts(qc, dtype, R, V, W, biases, masks):
+    """Parts of a row with a place for every token, on more logits than are on their way at a time; in place, from odd addresses too"""
+    g = gen(R + V)
+    host, a = (torch.randn(R, V, generator=g) * 3).to(dtype), args_of(g, R, V, W, biases, masks)
+    check(qc, host, a)
+    want, picked = qc.adjust_logits(host.cuda(), **on_gpu(a))
+    room = torch.full((R, V + 9), 5.0, dtype=dtype, device="cuda")
+    view = room[:, 3:V + 3]
+    view.copy_(host)
+    got, again = qc.adjust_logits(view, **on_gpu(a), out=view)
+    assert torch.equal(got, want) and torch.equal(again, picked) and bool((room[:, :3] == 5).all()) and bool((room[:, V + 3:] == 5).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_each_alone(qc, dtype):
     """Every argument without the others"""
     g, R, V, W = gen(1), 4, 3001, 60
