@@ -13,7 +13,6 @@
 // sequences up to 4001 slots 42 us against 41, 13B heads with a window 38 against 33, four of 65531 slots 172 against 172), the next
 // tile's loads between the sums (registers spill: 53 against 41), two tiles a warp in rings on three CTAs an SM (249 against 172).
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -541,30 +540,35 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) pages_join_kernel(const void*
   for (int i = 0; i < CPL; i += 2) *reinterpret_cast<uint32_t*>(to + i) = none ? 0u : Type<T>::pair(sum[i] / tot, sum[i + 1] / tot);
 }
 
-// Clusters of n CTAs that the device holds at once (fewer than its CTAs / n: a cluster lies in one part of the device)
-int clusters_of(int head_dim, int n) {
-  static std::atomic<int> known[64][2][MAX_CLUSTER + 1];
-  const int rest = per_sm(head_dim) * cq_sm_count() / n;
-  int dev = 0, clusters = 0;
-  if (n == 1 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return rest;
-  std::atomic<int>& kept = known[dev][head_dim == 64][n];
-  if ((clusters = kept.load(std::memory_order_relaxed)) > 0) return clusters;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(n);
-  cfg.blockDim = dim3(AT_WARPS * 32);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = n;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(&clusters, head_dim == 64 ? pages_attend_kernel<__half, 64, false, true> : pages_attend_kernel<__half, 128, false, true>,
-                                     &cfg) != cudaSuccess || clusters < 1) {
-    (void)cudaGetLastError();
-    return rest;
+// Clusters of 1 .. MAX_CLUSTER CTAs that the device holds at once (fewer than its CTAs / n: a cluster lies in one part of the device)
+struct Held {
+  int clusters[MAX_CLUSTER + 1];
+  explicit Held(int head_dim) {
+    for (int n = 1; n <= MAX_CLUSTER; ++n) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(n);
+      cfg.blockDim = dim3(AT_WARPS * 32);
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = n;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      auto fn = head_dim == 64 ? pages_attend_kernel<__half, 64, false, true> : pages_attend_kernel<__half, 128, false, true>;
+      if (cudaOccupancyMaxActiveClusters(&clusters[n], fn, &cfg) == cudaSuccess && clusters[n] > 0) continue;
+      (void)cudaGetLastError();
+      clusters[n] = per_sm(head_dim) * cq_sm_count() / n;
+    }
   }
-  kept.store(clusters, std::memory_order_relaxed);
-  return clusters;
+};
+// (of the first device: those of one machine are alike)
+const Held& held_by_device(int head_dim) {
+  if (head_dim == 64) {
+    static const Held held(64);
+    return held;
+  }
+  static const Held held(128);
+  return held;
 }
 
 // CTAs of a cluster for each sequence and task, 0: equal ranges.  The least time by a model (us): waves of clusters, each its start and the
@@ -580,11 +584,12 @@ int plan_of(const cq_pages* pages, const cq_table* table, int n_heads, int windo
   const double tasks = (double)table->sequences * KV * chunks;
   const long long all = (long long)table->width * pages->page_size;
   const long long most = window ? std::min<long long>(all, (long long)window + sinks + AT_SLOTS) : all, tiles = (most + AT_SLOTS - 1) / AT_SLOTS;
+  const Held& device = held_by_device(pages->head_dim);
   double least = 13 + 3.4 * tasks / slots + std::max(1.0, tasks * tiles / (slots * AT_WARPS)) * (narrow ? 1.12 : 2.2);
   int best = 0;
   for (int n = 1; n <= MAX_CLUSTER; ++n) {
     if (n > 1 && (n - 1) * AT_WARPS >= tiles) break;
-    const double held = clusters_of(pages->head_dim, n), each = std::min(held * n / sms, std::max(1.0, tasks * n / sms));
+    const double held = device.clusters[n], each = std::min(held * n / sms, std::max(1.0, tasks * n / sms));
     const double turn = narrow ? std::max(0.97 + 0.11 * each, 0.31 * each) : std::max(0.82 + 0.45 * each, 0.7 * each);
     const double waves = tasks <= held ? 1.0 : 0.75 * tasks / held + 0.25 * std::ceil(tasks / held);
     const double t = 1.3 + waves * (((tiles + n * AT_WARPS - 1) / (n * AT_WARPS)) * turn + 2.0) + (n > 1 ? 1.35 + 0.085 * n : 0.0);
@@ -601,6 +606,7 @@ int attend(const cq_pages* pages, const cq_table* table, const cq_rows* q, const
            const long long* positions, int table_rows, const long long* length, void* out, int H, int window, int sinks, float scale, void* workspace,
            cudaStream_t stream) {
   const int KV = pages->n_kv_heads, chunks = (H / KV + AT_HEADS - 1) / AT_HEADS, cluster = plan_of(pages, table, H, window, sinks), ctas = per_sm(D) * cq_sm_count();
+  if (!cluster && !workspace) return CQ_ERR_BAD_ARG;
   const NewRow<T> fresh = {rows_of<T>(k), rows_of<T>(v), cos_t, sin_t, positions, table_rows};
   const Shape shape = {table->sequences, H, chunks, window, sinks, scale};
   cudaLaunchConfig_t cfg = {};
@@ -636,7 +642,6 @@ int call(const cq_pages* pages, const cq_table* table, const cq_rows* q, const c
   if (rc != CQ_OK) return rc;
   if (!rows_fit(q) || !length || ((uintptr_t)length & 7) || !out || window < 0 || sinks < 0 || !(scale > 0.f) || (((uintptr_t)out | (uintptr_t)workspace) & 15)) return CQ_ERR_BAD_ARG;
   if (H < 1 || H % pages->n_kv_heads || (H + 7ll * pages->n_kv_heads) / 8 > 65535) return CQ_ERR_BAD_SHAPE;
-  if (!workspace && cq_pages_attend_workspace_bytes(pages, table, H, window, sinks)) return CQ_ERR_BAD_ARG;
   auto fn = pages->dtype == 0 ? (pages->head_dim == 128 ? attend<__half, 128> : attend<__half, 64>)
                               : (pages->head_dim == 128 ? attend<__nv_bfloat16, 128> : attend<__nv_bfloat16, 64>);
   return fn(pages, table, q, k, v, cos_t, sin_t, positions, table_rows, length, out, H, window, sinks, scale, workspace, stream);
