@@ -212,7 +212,7 @@ class CherryDecoder:
         self.pos_host = 0           # the host's copy of `pos` (the largest): every step is checked against max_seq before it is launched
         self.held = [0] * batch     # positions of each sequence, with pages
         self.graph = None
-        self.controls = None
+        self.controls = self.follow = None
 
     # ------------------------------------------------------------------ construction
     def _make_linear(self, k: int, n: int, g: torch.Generator) -> QuantLinear:
@@ -399,29 +399,28 @@ class CherryDecoder:
         one for each, from a sequence's next prompt on; presence and frequency count what was generated, repetition the prompt too.  bias:
         {token: number}.  grammar: (masks (states, words) int32 with a bit for each token, follow (states, vocab) integers: the state
         behind a token, -1 for none); sequences start in state 0, here and with every prompt.  Without arguments: the bare logits again."""
-        self.graph = None
         if all(x is None for x in (repetition, presence, frequency, bias, grammar)):
-            self.controls = None
+            self.controls = self.follow = self.graph = None
             return
         each = lambda x: None if x is None else torch.broadcast_to(torch.as_tensor(x, dtype=torch.float32), (self.batch,)).contiguous().to(self.dev)
-        c = {"repetition": each(repetition), "presence": each(presence), "frequency": each(frequency)}
+        c, states = {"repetition": each(repetition), "presence": each(presence), "frequency": each(frequency)}, None
         if bias is not None:
             ids, numbers = list(bias.keys()), list(bias.values())
             c["bias_ids"] = torch.tensor(ids, dtype=torch.long, device=self.dev).expand(self.batch, -1)
             c["bias"] = torch.tensor(numbers, dtype=torch.float32, device=self.dev).expand(self.batch, -1)
-        self.follow = None
         if grammar is not None:
             masks, follow = grammar
-            if masks.dtype != torch.int32 or masks.dim() != 2 or masks.shape[1] < -(-self.cfg.vocab // 32) or \
+            if masks.dtype != torch.int32 or masks.dim() != 2 or masks.shape[0] < 1 or masks.shape[1] < -(-self.cfg.vocab // 32) or \
                     tuple(follow.shape) != (masks.shape[0], self.cfg.vocab) or int(follow.max()) >= masks.shape[0]:
                 raise ValueError("grammar is (masks (states, words) int32, follow (states, vocab) of states or -1)")
-            c["mask"], self.follow = masks.to(self.dev), follow.to(self.dev, torch.long)
+            c["mask"], states = masks.to(self.dev), follow.to(self.dev, torch.long)
             c["mask_rows"] = torch.zeros(self.batch, dtype=torch.long, device=self.dev)
         if any(c[n] is not None for n in ("repetition", "presence", "frequency")):
             # a sequence's tokens by position, up to the one that is read next
             c["tokens"] = torch.zeros(self.batch, self.cfg.max_seq, dtype=torch.long, device=self.dev)
             c["length"], c["prompt"] = (torch.zeros(self.batch, dtype=torch.long, device=self.dev) for _ in range(2))
-        self.controls = c
+        # (nothing has changed so far: a call that is refused leaves the present control, and the graph, as they are)
+        self.controls, self.follow, self.graph = c, states, None
 
     def _pick(self, logits: torch.Tensor, rows=None) -> torch.Tensor:
         """The next token of every sequence (of `rows`); logits are adjusted in place."""

@@ -1,0 +1,65 @@
+"""Control over what is picked, where calls go wrong or come in other forms: refused calls, prompts of other types and places, sequences
+without a prompt."""
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+CACHES = [dict(), dict(kv_bits=4), dict(kv_page=16)]
+
+
+@pytest.fixture(scope="module")
+def dec():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from cherryq_b200 import decoder
+    return decoder
+
+
+def tiny(dec, max_seq=256, vocab=1003):
+    return dec.DecoderConfig(n_layers=2, hidden=256, n_heads=4, n_kv_heads=2, ffn=512, vocab=vocab, bits=4, group=128, cherry_fraction=1 / 32,
+                             max_seq=max_seq)
+
+
+def tokens(cfg, *shape, seed=1):
+    return torch.randint(0, cfg.vocab, shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
+
+
+def cycle(vocab, steps):
+    """A grammar that allows tokens 10 s .. 10 s + 9 in state s, one state after the other"""
+    masks, follow = torch.zeros(steps, -(-vocab // 32), dtype=torch.int64), torch.full((steps, vocab), -1, dtype=torch.int32)
+    for s in range(steps):
+        for t in range(10 * s, 10 * s + 10):
+            masks[s, t // 32] |= 1 << (t % 32)
+        follow[s, 10 * s:10 * s + 10] = (s + 1) % steps
+    return torch.where(masks >= 1 << 31, masks - (1 << 32), masks).to(torch.int32), follow
+
+
+@pytest.mark.parametrize("options", CACHES)
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_refused_calls_change_nothing(dec, options, use_graph):
+    """The grammar, its states and the penalties that are active stay so"""
+    cfg = tiny(dec)
+    a, b = (dec.CherryDecoder(cfg, seed=3, batch=2, **options) for _ in range(2))
+    masks, follow = cycle(cfg.vocab, 5)
+    prompt = tokens(cfg, 2, 12)
+    for m in (a, b):
+        m.control(grammar=(masks, follow), repetition=1.3)
+        m.prefill(prompt)
+        m.generate(3, use_graph)
+    graph = a.graph
+    for bad in (dict(grammar=(masks[:, :-1], follow)), dict(grammar=(masks, follow + 5)), dict(grammar=(masks, follow[:, :-1])),
+                dict(grammar=(masks.long(), follow)), dict(repetition=[1.0, 2.0, 3.0]), dict(presence="a"), dict(bias={1: "b"}),
+                dict(repetition=2.0, frequency=[0.1, 0.2, 0.3]), dict(bias={2: 1.0}, grammar=(masks[:4], follow))):
+        with pytest.raises((ValueError, RuntimeError, TypeError)):
+            a.control(**bad)
+    assert a.graph is graph
+    x, y = a.generate(20, use_graph), b.generate(20, use_graph)
+    assert torch.equal(x, y)
+    for i, row in enumerate(x.tolist()):
+        assert all(t // 10 == (3 + i) % 5 for t in row)
+    a.prefill(prompt), b.prefill(prompt)
+    assert torch.equal(a.generate(10, use_graph), b.generate(10, use_graph))
+    # and a call that is not refused takes their place
+    a.control(presence=0.5), b.control(presence=0.5)
+    a.prefill(prompt), b.prefill(prompt)
+    assert torch.equal(a.generate(10, use_graph), b.generate(10, use_graph))
