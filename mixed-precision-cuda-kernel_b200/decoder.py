@@ -451,9 +451,11 @@ class CherryDecoder:
     # ------------------------------------------------------------------ prefill / decode
     @torch.inference_mode()
     def prefill(self, tokens: torch.Tensor, lengths=None, rows=None) -> torch.Tensor:
-        """Runs the prompts (T,) or (batch, T) through the model, fills the caches, returns the last
+        """Runs the prompts (T,) or (batch, T), integers of any type on any device, through the model, fills the caches, returns the last
         position's logits (batch, vocab).  With a paged cache: lengths[i] of the T tokens are prompt i's, and prompt i is that of
         sequence rows[i] while the others keep what they have."""
+        if tokens.is_floating_point() or tokens.is_complex() or tokens.dtype == torch.bool:
+            raise ValueError(f"tokens must be whole numbers, not {tokens.dtype}")
         if tokens.dim() == 1:
             tokens = tokens[None]
         if not self.kv_page and (lengths is not None or rows is not None):
@@ -471,7 +473,7 @@ class CherryDecoder:
                 raise ValueError(f"lengths must be 1 to {min(t, self.cfg.max_seq - 1)}, one for each prompt")
             raise ValueError(f"a prompt of {t} tokens does not fit max_seq = {self.cfg.max_seq} (one position must stay free)")
         t = min(t, max(ends))
-        tokens = tokens[:, :t]
+        tokens = tokens[:, :t].to(self.dev, torch.long)
         place = torch.arange(t, device=self.dev)
         if self.kv_page:
             old = [self.page_table.held[r] for r in rows]
@@ -485,7 +487,7 @@ class CherryDecoder:
             end = torch.tensor(ends, dtype=torch.long, device=self.dev)
             self.prompts = self.table[rows] if some else self.table, end
             inside = place < end[:, None]
-            tokens, pos = torch.where(inside, tokens.to(self.dev), 0), torch.where(inside, place, -1).reshape(-1)
+            tokens, pos = torch.where(inside, tokens, 0), torch.where(inside, place, -1).reshape(-1)
         else:
             pos = place.repeat(n)
         h, delta = self.embed[tokens.reshape(-1)], None

@@ -63,3 +63,40 @@ def test_refused_calls_change_nothing(dec, options, use_graph):
     a.control(presence=0.5), b.control(presence=0.5)
     a.prefill(prompt), b.prefill(prompt)
     assert torch.equal(a.generate(10, use_graph), b.generate(10, use_graph))
+
+
+@pytest.mark.parametrize("options", CACHES)
+@pytest.mark.parametrize("form", ["int32", "int16", "host", "host int32"])
+def test_prompts_of_other_types_and_places(dec, options, form):
+    """With penalties as without them"""
+    cfg = tiny(dec)
+    a = dec.CherryDecoder(cfg, seed=4, batch=2, **options)
+    prompt = tokens(cfg, 2, 30)
+    other = prompt.to("cpu" if "host" in form else "cuda", torch.int32 if "int32" in form else torch.int16 if "int16" in form else torch.long)
+    for control in (dict(), dict(repetition=1.5, presence=0.3, frequency=[0.1, 0.4])):
+        a.control(**control)
+        want = a.prefill(prompt), a.generate(12)
+        got = a.prefill(other), a.generate(12)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    if "kv_page" in options:
+        want = a.prefill(prompt[1:], [20], rows=[1]), a.generate(5)
+        a.prefill(prompt), a.generate(12)
+        a.prefill(prompt), a.prefill(prompt[1:], [20], rows=[1])
+        want = a.generate(5)
+        a.prefill(prompt), a.prefill(other[1:], [20], rows=[1])
+        assert torch.equal(a.generate(5), want)
+
+
+@pytest.mark.parametrize("options", CACHES)
+def test_prompts_that_are_no_tokens(dec, options):
+    """Refused before anything is changed"""
+    cfg = tiny(dec)
+    a = dec.CherryDecoder(cfg, seed=4, batch=2, **options)
+    prompt = tokens(cfg, 2, 30)
+    a.prefill(prompt)
+    want = a.generate(10)
+    a.prefill(prompt)
+    for bad in (prompt.float(), prompt.half(), prompt > 5):
+        with pytest.raises(ValueError, match="whole numbers"):
+            a.prefill(bad)
+    assert a.held == [30, 30] and a.pos.tolist() == [30, 30] and torch.equal(a.generate(10), want)
