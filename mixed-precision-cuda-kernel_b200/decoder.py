@@ -396,7 +396,7 @@ class CherryDecoder:
     # ------------------------------------------------------------------ control over what is picked
     def control(self, repetition=None, presence=None, frequency=None, bias=None, grammar=None):
         """From here on tokens are picked from adjusted logits.  repetition, presence, frequency: a number for all sequences or
-        one for each, from a sequence's next prompt on; presence and frequency count what was generated, repetition the prompt too.  bias:
+        one for each (repetition positive), from a sequence's next prompt on; presence and frequency count what was generated, repetition the prompt too.  bias:
         {token: number}.  grammar: (masks (states, words) int32 with a bit for each token, follow (states, vocab) integers: the state
         behind a token, -1 for none); sequences start in state 0, here and with every prompt.  Without arguments: the bare logits again."""
         if all(x is None for x in (repetition, presence, frequency, bias, grammar)):
@@ -404,6 +404,8 @@ class CherryDecoder:
             return
         each = lambda x: None if x is None else torch.broadcast_to(torch.as_tensor(x, dtype=torch.float32), (self.batch,)).contiguous().to(self.dev)
         c, states = {"repetition": each(repetition), "presence": each(presence), "frequency": each(frequency)}, None
+        if repetition is not None and not bool((c["repetition"] > 0).all()):
+            raise ValueError("repetition must be positive")
         if bias is not None:
             ids, numbers = list(bias.keys()), list(bias.values())
             c["bias_ids"] = torch.tensor(ids, dtype=torch.long, device=self.dev).expand(self.batch, -1)

@@ -100,3 +100,13 @@ def test_prompts_that_are_no_tokens(dec, options):
         with pytest.raises(ValueError, match="whole numbers"):
             a.prefill(bad)
     assert a.held == [30, 30] and a.pos.tolist() == [30, 30] and torch.equal(a.generate(10), want)
+
+
+def test_repetition_is_positive(dec):
+    cfg = tiny(dec)
+    a = dec.CherryDecoder(cfg, seed=4, batch=2, kv_page=16)
+    for bad in (0, 0.0, -1.0, [1.2, 0.0], [-0.5, 2.0], float("nan")):
+        with pytest.raises(ValueError, match="repetition"):
+            a.control(repetition=bad)
+    assert a.controls is None
+    a.control(repetition=[1e-3, 5.0], presence=-1.0, frequency=0.0)       # the others may be any number
