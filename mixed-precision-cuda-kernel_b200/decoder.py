@@ -211,6 +211,8 @@ class CherryDecoder:
         self.pos = torch.zeros(batch, dtype=torch.long, device=self.dev)
         self.pos_host = 0           # the host's copy of `pos` (the largest): every step is checked against max_seq before it is launched
         self.held = [0] * batch     # positions of each sequence, with pages
+        # what a step adds to the positions: nothing where a sequence has no pages, which would be looked for in more and more places
+        self.moves = torch.zeros(batch, dtype=torch.long, device=self.dev) if kv_page else 1
         self.graph = None
         self.controls = self.follow = None
 
@@ -390,7 +392,8 @@ class CherryDecoder:
             self.page_table.release(r)
             self.held[r] = 0
         self.table.copy_(self.page_table.host)
-        self.pos[torch.tensor(rows, device=self.dev)] = 0            # (nothing is looked for in pages that it no longer has)
+        at = torch.tensor(rows, device=self.dev)
+        self.pos[at] = self.moves[at] = 0            # (nothing is looked for in pages that they no longer have)
         self.pos_host = max(self.held)
 
     # ------------------------------------------------------------------ control over what is picked
@@ -506,6 +509,8 @@ class CherryDecoder:
         at = torch.tensor(rows, device=self.dev)
         filled = torch.tensor(ends, dtype=torch.long, device=self.dev)
         self.pos[at] = filled
+        if self.kv_page:
+            self.moves[at] = 1
         c = self.controls
         if c is not None and c.get("tokens") is not None:
             c["tokens"][at, :t] = tokens
@@ -524,7 +529,7 @@ class CherryDecoder:
             h, delta = self._layer(li, h, delta, self.pos, decode=True)
         logits = self._logits(h, delta)
         self.tok.copy_(self._pick(logits))
-        self.pos.add_(1)
+        self.pos.add_(self.moves)
         if self.kv_budget is not None:
             self.length.add_(1)
         return logits

@@ -110,3 +110,34 @@ def test_repetition_is_positive(dec):
             a.control(repetition=bad)
     assert a.controls is None
     a.control(repetition=[1e-3, 5.0], presence=-1.0, frequency=0.0)       # the others may be any number
+
+
+@pytest.mark.parametrize("control", [dict(), dict(repetition=1.2, frequency=0.1)])
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_sequences_without_a_prompt_stay_where_they_are(dec, control, use_graph):
+    """Positions of released sequences, and of those that had no prompt yet, do not count up: steps look for nothing in pages that they
+    do not have"""
+    cfg = tiny(dec)
+    a = dec.CherryDecoder(cfg, seed=5, batch=3, kv_page=16)
+    if control:
+        a.control(**control)
+    prompt = tokens(cfg, 3, 20)
+    a.prefill(prompt[:1], rows=[0])
+    a.generate(10, use_graph)
+    assert a.pos.tolist() == [30, 0, 0]
+    a.prefill(prompt[1:], rows=[2, 1])
+    a.generate(10, use_graph)
+    assert a.pos.tolist() == [40, 30, 30]
+    a.release([1])
+    for _ in range(3):
+        a.generate(20, use_graph)
+    assert a.pos.tolist() == [100, 0, 90] and a.held == [100, 0, 90]
+    # the next prompt counts again, as one that came first
+    a.prefill(prompt[:1], rows=[1])
+    got = a.generate(15, use_graph)[:, 1]
+    assert a.pos.tolist() == [115, 35, 105]
+    b = dec.CherryDecoder(cfg, seed=5, batch=3, kv_page=16)
+    if control:
+        b.control(**control)
+    b.prefill(prompt[:1].expand(3, -1))
+    assert torch.equal(b.generate(15, use_graph)[:, 1], got)
