@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           sees[h][e] = vis.sees(base + 8 * h + 2 * t4 + e);
-          top = fmaxf(top, sees[h][e] ? s[h][e] * scale2 : -INFINITY);
+          top = fmaxf(top, sees[h][e] ? __fmul_rn(s[h][e], scale2) : -INFINITY);
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -293,11 +293,17 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
       const float keep = whole_pow2(m - ref);
       const uint64_t keep2 = two(keep, keep);
       m = top;
+      // From 2^23 on the maximum is a rounded product itself: the products that it is compared with are then rounded alike.  (Unrounded ones may
+      // lie a power of two and more above it, whose weights fp16 does not hold, or all of them far below.)
+      const bool coarse = fabsf(ref) >= 8388608.f;
       float w[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) w[h][e] = sees[h][e] ? LIFT * ex2(__fmaf_rn(s[h][e], scale2, -ref)) : 0.f;
+        for (int e = 0; e < 2; ++e) {
+          const float x = coarse ? __fsub_rn(__fmul_rn(s[h][e], scale2), ref) : __fmaf_rn(s[h][e], scale2, -ref);
+          w[h][e] = sees[h][e] ? LIFT * ex2(x) : 0.f;
+        }
       l = l * keep + ((w[0][0] + w[0][1]) + (w[1][0] + w[1][1]));
       const uint2 w0 = split_weights<T>(w[0][0], w[0][1]), w1 = split_weights<T>(w[1][0], w[1][1]);
 #pragma unroll

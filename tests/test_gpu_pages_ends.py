@@ -1,0 +1,65 @@
+"""The paged cache where scores and values are at the ends of their types or infinite, through a cluster of CTAs and through equal ranges
+whose parts a second kernel joins."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+FP16, BF16 = torch.float16, torch.bfloat16
+LONG = torch.long
+PAGE, SLOTS = 16, 300
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.fixture(scope="module")
+def qc():
+    import cherryq_b200
+    return cherryq_b200.load_quant_cuda()
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, device="cuda", generator=g)
+
+
+def cache_of(qc, g, KV, D, dtype):
+    """SLOTS slots of one sequence: a cache, and the tables and lengths with which it is read: in a table of their own length, and with their
+    pages far apart in a long one"""
+    n = -(-SLOTS // PAGE)
+    cache = qc.KVPages(randn(g, n, KV, PAGE, D).to(dtype), randn(g, n, KV, PAGE, D).to(dtype))
+    short = torch.arange(n, device="cuda", dtype=torch.int32)[None]
+    wide = torch.full((1, 40000 // PAGE), -1, dtype=torch.int32, device="cuda")
+    at = torch.arange(n, device="cuda") * (wide.shape[1] // n)
+    wide[0, at] = short[0]
+    length = lambda slots: torch.tensor([slots], dtype=LONG, device="cuda")
+    return cache, ((short, length(SLOTS)), (wide, length(int(at[-1]) * PAGE + SLOTS - (n - 1) * PAGE)))
+
+
+def slot(x, j):
+    """Slot j of all KV heads of a pool's keys or values"""
+    return x[j // PAGE, :, j % PAGE]
+
+
+def lost(dtype):
+    """A weight in its two halves, and the few sums of these tests in 32 bits"""
+    return (2.0 ** -21 if dtype == FP16 else 2.0 ** -17) + 8 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("dtype,big", [(FP16, 30000.0), (FP16, 3000.0), (BF16, 30000.0), (BF16, 1e17)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_large_scores(qc, dtype, big, D, sign):
+    """Scores of 2^24 and more, whose products are rounded to whole powers of two and coarser: one key far above the others gives its value, two
+    equal ones their mean.  (The other scores are 0, or twice as far below: their weights vanish, however scores are rounded.)"""
+    g, KV, G = torch.Generator(device="cuda").manual_seed(D), 2, 6
+    cache, ways = cache_of(qc, g, KV, D, dtype)
+    most = cache.v.abs().max().double()
+    for first, second in ((0, 0), (7, 7), (299, 299), (150, 150), (3, 298), (17, 33), (64, 65)):
+        q = (big * (1 + 0.3 * torch.rand(1, KV * G, D, device="cuda", generator=g))).to(dtype)
+        row = (sign * big * (0.5 + 0.3 * torch.rand(KV, D, device="cuda", generator=g))).to(dtype)
+        cache.k.fill_(0.0 if sign > 0 else -2 * big)
+        slot(cache.k, first).copy_(row)
+        slot(cache.k, second).copy_(row)
+        want = (slot(cache.v, first).double() + slot(cache.v, second).double()) / 2
+        want = want[:, None].expand(KV, G, D).reshape(KV * G, D)
+        for table, length in ways:
+            out = cache.attend(q, table, length)[0].double()
+            assert bool(((out - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() + lost(dtype) * most).all()), (first, second, int(length))
