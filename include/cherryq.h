@@ -372,7 +372,7 @@ int cq_pages_write(const cq_pages* pages, const cq_table* table, const cq_rows* 
 int cq_pages_read(const cq_pages* pages, const cq_table* table, const long long* first, int count, void* k, void* v, cq_stream_t stream);
 /* Attention of one query per sequence: out (sequences, n_heads, D) contiguous = softmax(scale * q . k_j) . v_j over the visible slots
  * j < n = length[s] (device int64, bounded by the table): all of them (window 0), or those with j < sinks or j >= n - window, and of these
- * those that have a page.  Nothing visible: zeros.  scale positive.  workspace: device memory of cq_pages_attend_workspace_bytes(...)
+ * those that have a page.  Nothing visible: zeros; visible scores that are all -infinity: NaN, as in the formula.  scale positive.  workspace: device memory of cq_pages_attend_workspace_bytes(...)
  * bytes (may be NULL where that is 0), 16-byte aligned, not shared by calls that can overlap. */
 size_t cq_pages_attend_workspace_bytes(const cq_pages* pages, const cq_table* table, int n_heads, int window, int sinks);
 int cq_pages_attend(const cq_pages* pages, const cq_table* table, const cq_rows* q, const long long* length, void* out, int n_heads,

@@ -46,9 +46,10 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // 2^d of a whole number d <= 0; 0 below the normal numbers (and 1 for NaN, whose sums are NaN)
 __device__ __forceinline__ float whole_pow2(float d) { return __int_as_float(max(0, 127 + __float2int_rn(d)) << 23); }
-// the share of sums (maximum m, sum of weights l) in those that reach up to `top`: 0 where they have no slot, but 1 where their
-// only scores are NaN
-__device__ __forceinline__ float share_of(float m, float l, float top) { return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : whole_pow2(m - top); }
+// The maximum of scores of which none is above -infinity (NaN does not count): below all others, above that of no slot, which is -infinity
+constexpr float LOWEST = -3.402823466e38f;
+// the share of sums with maximum m in those that reach up to `top`: 0 where they have no slot
+__device__ __forceinline__ float share_of(float m, float top) { return m == -INFINITY ? 0.f : whole_pow2(m - top); }
 // two weights: their upper bits, and what is left of them
 template <typename T> __device__ __forceinline__ uint2 split_weights(float a, float b) {
   const uint32_t hi = Type<T>::pair(a, b);
@@ -286,13 +287,11 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // A whole number at or above the maximum, so that rescaling sums is exact.  (No finite score so far: weights 0, or NaN
-      // where a score is NaN, which no maximum shows.)
-      top = ceilf(top);
-      const float ref = top == -INFINITY ? 0.f : top;
-      const float keep = whole_pow2(m - ref);
+      // A whole number at or above the maximum, so that rescaling sums is exact.  (A tile has a slot that all heads see.  No finite
+      // score so far: weights 0, or NaN where a score is NaN, which no maximum shows.)
+      const float ref = fmaxf(ceilf(top), LOWEST), keep = whole_pow2(m - ref);
       const uint64_t keep2 = two(keep, keep);
-      m = top;
+      m = ref;
       // From 2^23 on the maximum is a rounded product itself: the products that it is compared with are then rounded alike.  (Unrounded ones may
       // lie a power of two and more above it, whose weights fp16 does not hold, or all of them far below.)
       const bool coarse = fabsf(ref) >= 8388608.f;
@@ -344,7 +343,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
       float tot = 0.f, sum[4] = {};
 #pragma unroll
       for (int w = 0; w < AT_WARPS; ++w) {
-        const float f = share_of(s_m[w][g], s_l[w][g], top);
+        const float f = share_of(s_m[w][g], top);
         const float4 x = *reinterpret_cast<const float4*>(&s_sum[w][g][place_of(d / 4)]);
         tot += f * s_l[w][g];
         sum[0] += f * x.x, sum[1] += f * x.y, sum[2] += f * x.z, sum[3] += f * x.w;
@@ -360,7 +359,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
             const size_t row = pool.rows(page, kvh) + (j & ((1 << pool.log_page) - 1));
             float dot = 0.f;
             for (int c = 0; c < D; ++c) dot += Type<T>::one(s_q[g][c]) * Type<T>::one(pool.k[row * D + c]);
-            const float w = LIFT * ex2(__fmaf_rn(dot, scale2, top == -INFINITY ? 0.f : -top));
+            const float w = LIFT * ex2(__fmaf_rn(dot, scale2, -top));
 #pragma unroll
             for (int c = 0; c < 4; ++c) sum[c] += w * Type<T>::one(pool.v[row * D + d + c]);
           }
@@ -370,7 +369,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
         *reinterpret_cast<float4*>(mine + PART + d) = make_float4(sum[0], sum[1], sum[2], sum[3]);
         if (d == 0) *reinterpret_cast<float2*>(mine) = make_float2(top, tot);
       } else {
-        const bool none = tot == 0.f;        // no slot is visible (a visible one's weight is not 0)
+        const bool none = top == -INFINITY;  // no slot is visible (where all scores are -infinity 0 / 0, as in the formula)
         *reinterpret_cast<uint2*>(out + ((size_t)seq * H + head0 + g) * D + d) =
             none ? make_uint2(0u, 0u) : make_uint2(Type<T>::pair(sum[0] / tot, sum[1] / tot), Type<T>::pair(sum[2] / tot, sum[3] / tot));
       }
@@ -407,11 +406,11 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
 #pragma unroll
       for (int r = 0; r < MAX_CLUSTER; ++r)
         if (r < n) {
-          const float f = share_of(m[r], l[r], top);
+          const float f = share_of(m[r], top);
           tot += f * l[r];
           sum[0] += f * x[r].x, sum[1] += f * x[r].y, sum[2] += f * x[r].z, sum[3] += f * x[r].w;
         }
-      const bool none = tot == 0.f;
+      const bool none = top == -INFINITY;
       *reinterpret_cast<uint2*>(out + ((size_t)seq * H + head0 + g) * D + d) =
           none ? make_uint2(0u, 0u) : make_uint2(Type<T>::pair(sum[0] / tot, sum[1] / tot), Type<T>::pair(sum[2] / tot, sum[3] / tot));
     }
@@ -505,7 +504,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) pages_join_kernel(const void*
         if (k < n) x[k] = columns(r0 + k * groups);
       float next = fmaxf(top, ml.x);
       for (int d = 16; d; d /= 2) next = fmaxf(next, __shfl_xor_sync(0xffffffffu, next, d));
-      const float keep = share_of(top, tot, next), f = share_of(ml.x, ml.y, next);
+      const float keep = share_of(top, next), f = share_of(ml.x, next);
       top = next;
       float add = f * ml.y;
       for (int d = 16; d; d /= 2) add += __shfl_xor_sync(0xffffffffu, add, d);
@@ -534,13 +533,13 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS) pages_join_kernel(const void*
 #pragma unroll
   for (int i = 0; i < CPL; ++i) sum[i] = 0.f;
   for (int k = 0; k < groups; ++k) {
-    if (s_top[warp + k] == -INFINITY && s_tot[warp + k] == 0.f) continue;
-    const float f = share_of(s_top[warp + k], s_tot[warp + k], best);
+    if (s_top[warp + k] == -INFINITY) continue;
+    const float f = share_of(s_top[warp + k], best);
     tot += f * s_tot[warp + k];
 #pragma unroll
     for (int i = 0; i < CPL; ++i) sum[i] = __fmaf_rn(f, s_sum[warp + k][CPL * lane + i], sum[i]);
   }
-  const bool none = tot == 0.f;
+  const bool none = best == -INFINITY;
   T* to = out + ((size_t)seq * H + kvh * G + h0 + first + g) * D + CPL * lane;
 #pragma unroll
   for (int i = 0; i < CPL; i += 2) *reinterpret_cast<uint32_t*>(to + i) = none ? 0u : Type<T>::pair(sum[i] / tot, sum[i + 1] / tot);

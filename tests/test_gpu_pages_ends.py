@@ -63,3 +63,37 @@ def test_large_scores(qc, dtype, big, D, sign):
         for table, length in ways:
             out = cache.attend(q, table, length)[0].double()
             assert bool(((out - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() + lost(dtype) * most).all()), (first, second, int(length))
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_infinite_scores(qc, dtype, D):
+    """-infinity beside finite scores is a weight of 0; scores that are all -infinity have no softmax: NaN, as infinity; no slot at all gives zeros"""
+    g, KV, G = torch.Generator(device="cuda").manual_seed(D + 1), 2, 4
+    cache, ways = cache_of(qc, g, KV, D, dtype)
+    q = randn(g, 1, KV * G, D).to(dtype)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    q[:, 1::2, 0] *= -1                                  # every second head sees -infinity where the others see infinity
+    finite = cache.k.clone()
+    cache.k[..., 0] = -INF
+    for table, length in ways:
+        assert cache.attend(q, table, length).isnan().all()
+        one = table.clone()
+        one[0, 1:] = -1
+        for n in (1, 5, 16, int(length)):                # a single slot, or a page's, and absent pages
+            assert cache.attend(q, one, torch.tensor([n], device="cuda")).isnan().all()
+        assert not cache.attend(q, torch.full_like(table, -1), length).any() and not cache.attend(q, table, length * 0).any()
+    # a finite score in one place alone: of the heads that see -infinity elsewhere it has all of the weight
+    for j in (0, 50, 299):
+        cache.k.copy_(finite)
+        cache.k[..., 0] = -INF
+        slot(cache.k, j).copy_(slot(finite, j))
+        for table, length in ways:
+            out = cache.attend(q, table, length).view(KV, G, D)
+            assert bool(((out[:, ::2].double() - slot(cache.v, j)[:, None].double()).abs() <= lost(dtype) * cache.v.abs().max().double()).all())
+            assert out[:, 1::2].isnan().all()
+    # a step whose own row is all that there is
+    k, v = slot(cache.k, 7)[None].clone(), randn(g, 1, KV, D).to(dtype)
+    for table, _ in ways:
+        out = cache.step(q, k, v, None, None, None, table, torch.zeros(1, dtype=LONG, device="cuda"))
+        assert out.isnan().all()
