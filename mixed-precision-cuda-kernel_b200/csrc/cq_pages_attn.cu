@@ -48,8 +48,11 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float whole_pow2(float d) { return __int_as_float(max(0, 127 + __float2int_rn(d)) << 23); }
 // The maximum of scores of which none is above -infinity (NaN does not count): below all others, above that of no slot, which is -infinity
 constexpr float LOWEST = -3.402823466e38f;
-// the share of sums with maximum m in those that reach up to `top`: 0 where they have no slot
-__device__ __forceinline__ float share_of(float m, float top) { return m == -INFINITY ? 0.f : whole_pow2(m - top); }
+// The share of sums with maximum m in those that reach up to `top`: 0 where they have no slot.  Otherwise it is not 0, so that infinite sums
+// stay infinite (2^-126 of other sums is nothing beside `top`'s own weight, which is 1/2 at least).
+__device__ __forceinline__ float share_of(float m, float top) {
+  return m == -INFINITY ? 0.f : __int_as_float(max(1, 127 + __float2int_rn(m - top)) << 23);
+}
 // two weights: their upper bits, and what is left of them
 template <typename T> __device__ __forceinline__ uint2 split_weights(float a, float b) {
   const uint32_t hi = Type<T>::pair(a, b);
@@ -160,6 +163,38 @@ template <bool FAR> struct Tiles {
     return (before + __shfl_sync(0xffffffffu, upto - mine, seq % 32)) * heads_each;
   }
 };
+// The infinite and NaN values of columns d .. d + 3 that a query sees in some tiles, summed without their weights, which are not 0; NaN where
+// the score is -infinity, and 0 where there are none.  A thread's four columns wait for sixteen slots at a time (one infinite value in four sequences
+// of 65531 slots: 1.05 ms in place of 0.17; with the weights summed again 26).  Out of line: its registers are none of the kernel's (inlined
+// four sequences of 30000 slots 69.6 us, so 68.1; 64 of 16 / 4 heads 51.4, so 51.6, without either 50.6).
+template <typename T, int D>
+__device__ __noinline__ float4 infinities(const Pool<T> pool, const Table table, const Visible<AT_SLOTS> vis, int tile0, int tile1, int seq, int kvh,
+                                          const T* query, int d, float scale2) {
+  float odd[4] = {};
+  for (int t = tile0; t < tile1; ++t) {
+    const int base = vis.tile(t) * AT_SLOTS, page = table.page_of(pool, seq, base);
+    if (page < 0) continue;
+    const size_t row0 = pool.rows(page, kvh) + (base & ((1 << pool.log_page) - 1));
+    uint2 raw[AT_SLOTS];
+#pragma unroll
+    for (int j = 0; j < AT_SLOTS; ++j) raw[j] = vis.sees(base + j) ? *reinterpret_cast<const uint2*>(pool.v + (row0 + j) * D + d) : make_uint2(0u, 0u);
+#pragma unroll
+    for (int j = 0; j < AT_SLOTS; ++j) {
+      const float2 lo = Type<T>::apart(raw[j].x), hi = Type<T>::apart(raw[j].y);
+      const float v[4] = {lo.x, lo.y, hi.x, hi.y};
+      if (isfinite(v[0]) && isfinite(v[1]) && isfinite(v[2]) && isfinite(v[3])) continue;
+      float dot = 0.f;
+#pragma unroll 1
+      for (int c = 0; c < D; ++c) dot += Type<T>::one(query[c]) * Type<T>::one(pool.k[(row0 + j) * D + c]);
+      const bool none = dot * scale2 == -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (!isfinite(v[c])) odd[c] += none ? NAN : v[c];
+    }
+  }
+  return make_float4(odd[0], odd[1], odd[2], odd[3]);
+}
+
 // Where the four columns 4 f .. of a head's sums are in shared memory: eight lanes with what one MMA gave them, and eight lanes
 // with consecutive columns, meet different banks (one sequence of 32 heads, 256 slots: 5.4 us; in order 5.8).
 __device__ __forceinline__ int place_of(int f) { return 4 * (f ^ (f >> 3 & 3)); }
@@ -349,20 +384,12 @@ __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(
         sum[0] += f * x.x, sum[1] += f * x.y, sum[2] += f * x.z, sum[3] += f * x.w;
       }
       if (!(fabsf(sum[0]) + fabsf(sum[1]) + fabsf(sum[2]) + fabsf(sum[3]) <= 3.0e38f) && tot == tot) {
-        // An infinite or NaN value takes part.  The two halves of a weight turn infinity into NaN where the product does
-        // not: these columns are added again, weight by weight.
-        sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
-        for (int t = tile0; t < tile1; ++t)
-          for (int j = vis.tile(t) * AT_SLOTS, end = j + AT_SLOTS; j < end; ++j) {
-            const int page = vis.sees(j) ? table.page_of(pool, seq, j) : -1;
-            if (page < 0) continue;
-            const size_t row = pool.rows(page, kvh) + (j & ((1 << pool.log_page) - 1));
-            float dot = 0.f;
-            for (int c = 0; c < D; ++c) dot += Type<T>::one(s_q[g][c]) * Type<T>::one(pool.k[row * D + c]);
-            const float w = LIFT * ex2(__fmaf_rn(dot, scale2, -top));
-#pragma unroll
-            for (int c = 0; c < 4; ++c) sum[c] += w * Type<T>::one(pool.v[row * D + d + c]);
-          }
+        // An infinite or NaN value takes part.  What the halves of its weight and rescaled sums make of it may be NaN where the product
+        // is infinite; no weight is 0, however small, but that of a score of -infinity: such values are added again without their weights.
+        // (Columns without one are right as they are.)
+        const float4 odd = infinities<T, D>(pool, table, vis, tile0, tile1, seq, kvh, s_q[g], d, scale2);
+        sum[0] = odd.x != 0.f ? odd.x : sum[0], sum[1] = odd.y != 0.f ? odd.y : sum[1];
+        sum[2] = odd.z != 0.f ? odd.z : sum[2], sum[3] = odd.w != 0.f ? odd.w : sum[3];
       }
       if (part) {
         float* mine = part + g * (D + PART);

@@ -1,5 +1,7 @@
 """The paged cache where scores and values are at the ends of their types or infinite, through a cluster of CTAs and through equal ranges
 whose parts a second kernel joins."""
+import math
+
 import pytest
 import torch
 
@@ -97,3 +99,60 @@ def test_infinite_scores(qc, dtype, D):
     for table, _ in ways:
         out = cache.step(q, k, v, None, None, None, table, torch.zeros(1, dtype=LONG, device="cuda"))
         assert out.isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("below", [1, 30, 100, 120, 130, 140, 148, 200, 3000])
+def test_infinite_values_of_small_weights(qc, dtype, D, below):
+    """A weight is not 0 however far its score, here 2^-below of the largest, lies below the others: an infinite value is infinite in its
+    column, NaN where it meets the other infinity or a NaN, or where its score is -infinity; the other columns are what they are without it"""
+    g, KV, G = torch.Generator(device="cuda").manual_seed(below), 2, 4
+    cache, ways = cache_of(qc, g, KV, D, dtype)
+    q = torch.zeros(1, KV * G, D, device="cuda", dtype=dtype)
+    q[..., 0] = 8.0
+    scale = math.log(2.0) / 8.0                          # the key's first column is its score in powers of two
+    cache.k.zero_()
+    for j in range(SLOTS):
+        slot(cache.k, j)[:, 0] = -float(below)
+    for top in (0, 123, 299):
+        slot(cache.k, top)[:, 0] = 0.0
+        clean = [cache.attend(q, table, length, scale=scale)[0] for table, length in ways]
+        v = cache.v.clone()
+        for low in (1, 20, 63, 64, 150, 200, 298):
+            slot(cache.v, low)[:, 5] = INF
+            slot(cache.v, low)[:, D - 1] = -INF
+            slot(cache.v, low)[:, 9] = NAN
+            slot(cache.v, low)[:, 10] = INF
+            slot(cache.v, (low + 7) % 299 + (top == (low + 7) % 299))[:, 10] = -INF
+            slot(cache.k, low)[:, 1] = 0.0
+            for (table, length), whole in zip(ways, clean):
+                out = cache.attend(q, table, length, scale=scale)[0]
+                assert (out[:, 5] == INF).all() and (out[:, D - 1] == -INF).all() and out[:, 9].isnan().all() and out[:, 10].isnan().all(), (top, low)
+                rest = [c for c in range(D) if c not in (5, 9, 10, D - 1)]
+                assert torch.equal(out[:, rest], whole[:, rest]), (top, low)
+            # a score of -infinity: 0 times infinity
+            held = slot(cache.k, low).clone()
+            slot(cache.k, low)[:, 0] = -INF
+            for table, length in ways:
+                out = cache.attend(q, table, length, scale=scale)[0]
+                assert out[:, [5, 9, 10, D - 1]].isnan().all() and torch.isfinite(out[:, rest]).all()
+            slot(cache.k, low).copy_(held)
+            cache.v.copy_(v)
+        slot(cache.k, top)[:, 0] = -float(below)
+
+
+def test_infinite_values_of_long_sequences(qc):
+    """One in each of two long sequences, of many tiles a CTA"""
+    g, KV, H, D = torch.Generator(device="cuda").manual_seed(5), 1, 8, 128
+    n = 20000
+    cache = qc.KVPages(randn(g, 2 * n // 64 + 2, KV, 64, D).half(), randn(g, 2 * n // 64 + 2, KV, 64, D).half())
+    table = torch.randperm(cache.pages, device="cuda", generator=g)[:2 * (n // 64 + 1)].view(2, -1).to(torch.int32)
+    q, length = randn(g, 2, H, D).half(), torch.tensor([n, n - 7000], device="cuda")
+    clean = cache.attend(q, table, length)
+    cache.v[table[0, 100].long(), 0, 3, 17] = INF
+    cache.v[table[1, 200].long(), 0, 63, 100] = -INF
+    out = cache.attend(q, table, length)
+    assert (out[0, :, 17] == INF).all() and (out[1, :, 100] == -INF).all()
+    out[0, :, 17], out[1, :, 100] = clean[0, :, 17], clean[1, :, 100]
+    assert torch.equal(out, clean)
