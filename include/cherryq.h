@@ -337,7 +337,7 @@ int cq_kv4_evict(const cq_kv4* from, const cq_kv4* to, const float* weights, flo
 
 /* ------------------------------------------------------------------------
  * Paged KV cache (the reference keeps one contiguous cache, llama/modeling_llama_quant.py:371-419).
- * A pool of pages holds page_size slots of every KV head each: k and v (pages, n_kv_heads, page_size, D), contiguous, 16-byte
+ * A pool of pages holds page_size slots of every KV head each: k and v (pages, n_kv_heads, page_size, D), contiguous, 32-byte
  * aligned, not overlapping; dtype 0 = fp16, 2 = bf16; page_size 16, 32, 64, 128 or 256; head_dim 64 or 128.  A table
  * (sequences, width) int32 on the device, rows `stride` entries apart, names the page of every page_size slots of a sequence; an
  * entry outside the pool stands for no page: its slots are not written, not seen and read as zeros.  Sequences may share
