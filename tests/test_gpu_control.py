@@ -141,3 +141,20 @@ def test_sequences_without_a_prompt_stay_where_they_are(dec, control, use_graph)
         b.control(**control)
     b.prefill(prompt[:1].expand(3, -1))
     assert torch.equal(b.generate(15, use_graph)[:, 1], got)
+
+
+@pytest.mark.parametrize("options", CACHES)
+def test_masks_of_any_strides(dec, options):
+    """Masks whose words do not lie one behind the other"""
+    cfg = tiny(dec)
+    a, b = (dec.CherryDecoder(cfg, seed=6, batch=2, **options) for _ in range(2))
+    masks, follow = cycle(cfg.vocab, 5)
+    prompt = tokens(cfg, 2, 12)
+    b.control(grammar=(masks, follow)), b.prefill(prompt)
+    want = b.generate(10)
+    wide = torch.zeros(5, 2 * masks.shape[1], dtype=torch.int32, device="cuda")
+    wide[:, ::2] = masks.cuda()
+    for form in (masks.T.contiguous().T, masks.cuda().T.contiguous().T, wide[:, ::2], masks.cuda()):
+        a.control(grammar=(form, follow))
+        a.prefill(prompt)
+        assert torch.equal(a.generate(10), want)
