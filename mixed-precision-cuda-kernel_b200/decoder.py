@@ -401,7 +401,8 @@ class CherryDecoder:
         """From here on tokens are picked from adjusted logits.  repetition, presence, frequency: a number for all sequences or
         one for each (repetition positive), from a sequence's next prompt on; presence and frequency count what was generated, repetition the prompt too.  bias:
         {token: number}.  grammar: (masks (states, words) int32 with a bit for each token, follow (states, vocab) integers: the state
-        behind a token, -1 for none); sequences start in state 0, here and with every prompt.  Without arguments: the bare logits again."""
+        behind a token, -1 for none; kept in 32 bits, 128 KB a state for 32000 tokens); sequences start in state 0, here and with every
+        prompt.  Without arguments: the bare logits again."""
         if all(x is None for x in (repetition, presence, frequency, bias, grammar)):
             self.controls = self.follow = self.graph = None
             return
@@ -418,7 +419,7 @@ class CherryDecoder:
             if masks.dtype != torch.int32 or masks.dim() != 2 or masks.shape[0] < 1 or masks.shape[1] < -(-self.cfg.vocab // 32) or \
                     tuple(follow.shape) != (masks.shape[0], self.cfg.vocab) or int(follow.max()) >= masks.shape[0]:
                 raise ValueError("grammar is (masks (states, words) int32, follow (states, vocab) of states or -1)")
-            c["mask"], states = masks.to(self.dev).contiguous(), follow.to(self.dev, torch.long)
+            c["mask"], states = masks.to(self.dev).contiguous(), follow.to(self.dev, torch.int32)
             c["mask_rows"] = torch.zeros(self.batch, dtype=torch.long, device=self.dev)
         if any(c[n] is not None for n in ("repetition", "presence", "frequency")):
             # a sequence's tokens by position, up to the one that is read next

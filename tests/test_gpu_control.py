@@ -158,3 +158,14 @@ def test_masks_of_any_strides(dec, options):
         a.control(grammar=(form, follow))
         a.prefill(prompt)
         assert torch.equal(a.generate(10), want)
+
+
+def test_memory_of_a_grammar(dec):
+    """4 bytes a state and token for the states that follow, a bit for the masks"""
+    cfg = tiny(dec)
+    a = dec.CherryDecoder(cfg, seed=6, batch=2, kv_page=16)
+    masks, follow = torch.zeros(2000, 32, dtype=torch.int32), torch.full((2000, cfg.vocab), -1, dtype=torch.int64)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    a.control(grammar=(masks, follow))
+    assert torch.cuda.memory_allocated() - before < 2000 * (4 * cfg.vocab + 128) + 100000
