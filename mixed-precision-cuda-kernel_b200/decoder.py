@@ -419,7 +419,7 @@ class CherryDecoder:
             if masks.dtype != torch.int32 or masks.dim() != 2 or masks.shape[0] < 1 or masks.shape[1] < -(-self.cfg.vocab // 32) or \
                     tuple(follow.shape) != (masks.shape[0], self.cfg.vocab) or int(follow.max()) >= masks.shape[0]:
                 raise ValueError("grammar is (masks (states, words) int32, follow (states, vocab) of states or -1)")
-            c["mask"], states = masks.to(self.dev).contiguous(), follow.to(self.dev, torch.int32)
+            c["mask"], states = masks.to(self.dev).contiguous(), (follow.clamp(min=-1) if follow.dtype == torch.long else follow).to(self.dev, torch.int32)
             c["mask_rows"] = torch.zeros(self.batch, dtype=torch.long, device=self.dev)
         if any(c[n] is not None for n in ("repetition", "presence", "frequency")):
             # a sequence's tokens by position, up to the one that is read next

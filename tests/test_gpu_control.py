@@ -169,3 +169,18 @@ def test_memory_of_a_grammar(dec):
     before = torch.cuda.memory_allocated()
     a.control(grammar=(masks, follow))
     assert torch.cuda.memory_allocated() - before < 2000 * (4 * cfg.vocab + 128) + 100000
+
+
+@pytest.mark.parametrize("dtype,none", [(torch.int8, -100), (torch.int32, -2 ** 31), (torch.int64, -2 ** 40), (torch.int64, -2 ** 32 + 1)])
+def test_states_below_none(dec, dtype, none):
+    """Any negative state is none"""
+    cfg = tiny(dec)
+    masks, follow = cycle(cfg.vocab, 3)
+    follow[2] = -1
+    got = []
+    for f in (follow, torch.where(follow < 0, none, follow.long()).to(dtype)):
+        a = dec.CherryDecoder(cfg, seed=6, batch=2, kv_page=16)
+        a.control(grammar=(masks, f))
+        a.prefill(tokens(cfg, 2, 12))
+        got.append(a.generate(20))
+    assert torch.equal(*got)
