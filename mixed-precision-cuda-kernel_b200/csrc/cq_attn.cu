@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(WARPS * 32, AM_SM_WARPS / WARPS) attn_decode_m
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) top = fmaxf(top, base + 8 * h + 2 * t4 + e < n_pos ? s[h][e] * scale2 : -INFINITY);
+      for (int e = 0; e < 2; ++e) top = fmaxf(top, base + 8 * h + 2 * t4 + e < n_pos ? __fmul_rn(s[h][e], scale2) : -INFINITY);
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // A whole number at or above the maximum, so that rescaling sums is exact.  (No finite score so far: weights 0, or NaN
@@ -212,13 +212,18 @@ __global__ void __launch_bounds__(WARPS * 32, AM_SM_WARPS / WARPS) attn_decode_m
     const float keep = whole_pow2(m - ref);
     m = top;
     // weights times 2^15: the halves of their split then reach down to 2^-38 of the largest.  (One rounding between the score
-    // and the exponent, of the size of the exponent, not of the score.)
+    // and the exponent, of the size of the exponent, not of the score.  From 2^23 on the maximum is a rounded product itself, and
+    // the products that it is compared with are rounded alike: unrounded ones may lie a power of two and more above it, whose
+    // weights fp16 does not hold, or all of them far below.)
+    const bool coarse = fabsf(ref) >= 8388608.f;
     float w[2][2];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        w[h][e] = base + 8 * h + 2 * t4 + e < n_pos ? 32768.f * ex2(__fmaf_rn(s[h][e], scale2, -ref)) : 0.f;
+      for (int e = 0; e < 2; ++e) {
+        const float x = coarse ? __fsub_rn(__fmul_rn(s[h][e], scale2), ref) : __fmaf_rn(s[h][e], scale2, -ref);
+        w[h][e] = base + 8 * h + 2 * t4 + e < n_pos ? 32768.f * ex2(x) : 0.f;
+      }
     l = l * keep + ((w[0][0] + w[0][1]) + (w[1][0] + w[1][1]));
     const uint2 w0 = split_weights(w[0][0], w[0][1]), w1 = split_weights(w[1][0], w[1][1]);
 #pragma unroll
