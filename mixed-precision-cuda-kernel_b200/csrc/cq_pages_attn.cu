@@ -199,7 +199,8 @@ __device__ __noinline__ float4 infinities(const Pool<T> pool, const Table table,
 // with consecutive columns, meet different banks (one sequence of 32 heads, 256 slots: 5.4 us; in order 5.8).
 __device__ __forceinline__ int place_of(int f) { return 4 * (f ^ (f >> 3 & 3)); }
 // CLUSTER: a cluster of CTAs for the heads of a KV head and sequence, each with the same share of its tiles.  Otherwise all tiles of all
-// sequences and KV heads in a row, cut into equal ranges for the CTAs that the device holds at once.
+// sequences and KV heads in a row, cut into equal ranges for the CTAs that the device holds at once.  (168 registers a thread for 128 columns,
+// 122 to 128 for 64; with equal ranges 48 to 64 bytes are spilled, 12 without a step for 64 columns.)
 template <typename T, int D, bool STEP, bool CLUSTER>
 __global__ void __launch_bounds__(AT_WARPS * 32, per_sm(D)) pages_attend_kernel(const Rows<T> q, const Pool<T> pool, const Table table, const NewRow<T> fresh,
                                                                         const long long* __restrict__ length, T* __restrict__ out, void* ws, const Shape shape) {
@@ -606,8 +607,9 @@ const Held& held_by_device(int head_dim) {
 // CTAs of a cluster for each sequence and task, 0: equal ranges.  The least time by a model (us): waves of clusters, each its start and the
 // turns of a warp, which take longer the fuller the SMs are; joins; for ranges what all warps need together, a start for every task and
 // the second kernel.  It goes by the table's width: lengths are known to the device alone.  Its numbers are those with which it lost
-// least over 937 calls (1 to 128 sequences of 32 / 32, 64 / 8 and 16 / 4 heads, 60 to 65000 slots, equal and mixed lengths): the plan taken is 0.6 %
-// behind the best on average, 12 % at most.  (16 sequences of 64 / 8 heads up to 4001 slots: 1 CTA 83 us, 2 53, 3 41, 4 50, 8 49, ranges
+// least over 937 calls (1 to 128 sequences of 32 / 32, 64 / 8 and 16 / 4 heads, 60 to 65000 slots, equal and mixed lengths) with tables as wide as the
+// longest sequence: the plan taken is 0.6 % behind the best on average, 12 % at most.  In wider tables it is further behind: 16 sequences of
+// 32 / 32 heads with 110 slots take 8.7 us, in a table of 4096 slots 21.9, of 16384 15.4; 33 of 16 / 4 heads with 200 5.0, 5.0 and 10.2.  (16 sequences of 64 / 8 heads up to 4001 slots: 1 CTA 83 us, 2 53, 3 41, 4 50, 8 49, ranges
 // 44; 8 of 40 heads, window 1021: 1 32, 2 39, ranges 38; 2 of 64 / 8 heads up to 20000 slots: 8 53, ranges 33; 24 of 16 / 4 heads, 1500 slots: 5
 // 11.6, 6, of which the device does not hold 96, 16.8; 5 of them, 60 slots: 1 2.7, ranges 8.1.)
 int plan_of(const cq_pages* pages, const cq_table* table, int n_heads, int window, int sinks) {

@@ -400,7 +400,7 @@ class CherryDecoder:
     def control(self, repetition=None, presence=None, frequency=None, bias=None, grammar=None):
         """From here on tokens are picked from adjusted logits.  repetition, presence, frequency: a number for all sequences or
         one for each (repetition positive), from a sequence's next prompt on; presence and frequency count what was generated, repetition the prompt too.  bias:
-        {token: number}.  grammar: (masks (states, words) int32 with a bit for each token, follow (states, vocab) integers: the state
+        {token: number}.  (prefill's logits are adjusted ones then.)  grammar: (masks (states, words) int32 with a bit for each token, follow (states, vocab) integers: the state
         behind a token, -1 for none; kept in 32 bits, 128 KB a state for 32000 tokens); sequences start in state 0, here and with every
         prompt.  Without arguments: the bare logits again."""
         if all(x is None for x in (repetition, presence, frequency, bias, grammar)):
