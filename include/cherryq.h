@@ -394,7 +394,7 @@ int cq_pages_step(const cq_pages* pages, const cq_table* table, const cq_rows* q
  * out[b][v] = x, rounded to the type; next[b] = the lowest v of the largest x (before rounding; NaN counts as the largest).
  * Every pointer but logits, out and next may be NULL: without tokens no penalties, without length all `width` tokens, without prompt from the
  * first.  Numbers outside the vocabulary among tokens and bias_ids stand for nothing, a mask row outside the masks for no
- * mask (mask_rows NULL: row b of at least as many masks).  length and prompt are bounded by the row.  Strides in elements between rows,
+ * mask (mask_rows NULL: row b of at least as many masks).  Less than 2^30 tokens and biases a row, up to 2^30 logits.  length and prompt are bounded by the row.  Strides in elements between rows,
  * whose columns are contiguous; those of what is only read may be 0.  out is logits (with the same stride) or shares no memory with it.
  * tokens, length, prompt, bias_ids, mask_rows, next: device int64; repetition (positive), presence, frequency, bias: device fp32. */
 typedef struct cq_adjust {

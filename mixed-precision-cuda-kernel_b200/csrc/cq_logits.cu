@@ -443,7 +443,8 @@ size_t span(int64_t rows, int64_t cols, int64_t stride, size_t item) { return (s
 
 extern "C" int cq_adjust_logits(const cq_adjust* a, int rows, int vocab, cq_stream_t stream) {
   if (!a || !a->logits || !a->out || !a->next) return CQ_ERR_BAD_ARG;
-  if (rows < 1 || rows > 65535 || vocab < 1 || vocab > (1 << 30) || a->width >= (1 << 30)) return CQ_ERR_BAD_SHAPE;
+  // (indices, and their steps behind the last entry, in 32 bits)
+  if (rows < 1 || rows > 65535 || vocab < 1 || vocab > (1 << 30) || a->width >= (1 << 30) || a->biases >= (1 << 30)) return CQ_ERR_BAD_SHAPE;
   if (a->dtype < 0 || a->dtype > 2) return CQ_ERR_UNSUPPORTED;
   const size_t item = a->dtype == 1 ? 4 : 2;
   if (((uintptr_t)a->logits | (uintptr_t)a->out) & (item - 1)) return CQ_ERR_BAD_ARG;

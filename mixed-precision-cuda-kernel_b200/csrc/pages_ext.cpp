@@ -230,7 +230,7 @@ std::pair<torch::Tensor, torch::Tensor> adjust_logits(const torch::Tensor& logit
   if (bias.has_value()) {
     a.bias_ids_stride = matrix(*bias_ids, "bias_ids", torch::kInt64, device, rows);
     a.bias_stride = matrix(*bias, "bias", torch::kFloat32, device, rows);
-    TORCH_CHECK(bias->size(1) == bias_ids->size(1) && bias->size(1) <= INT32_MAX, "bias_ids and bias must have the same shape");
+    TORCH_CHECK(bias->size(1) == bias_ids->size(1) && bias->size(1) < (1 << 30), "bias_ids and bias must have the same shape, of less than 2^30 a row");
     a.biases = (int)bias->size(1);
     a.bias_ids = (const long long*)bias_ids->const_data_ptr();
     a.bias = bias->const_data_ptr<float>();
