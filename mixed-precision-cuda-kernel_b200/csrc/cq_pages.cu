@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(THREADS) pages_read_kernel(const Pool<T> pool,
   constexpr int LANES = D / 8, HEADS = THREADS / LANES / SLOTS;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int s = blockIdx.z, r = threadIdx.x / LANES, head = blockIdx.y * HEADS + r % HEADS, c = 8 * (threadIdx.x % LANES);
-  const int i = blockIdx.x * SLOTS + r / HEADS;
+  const long long i = (long long)blockIdx.x * SLOTS + r / HEADS;
   if (i >= count || head >= pool.heads) return;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const long long slot = first[s] + i;
@@ -102,7 +102,7 @@ int write(const cq_pages* pages, const cq_table* table, const cq_rows* q, void* 
           const float* sin_t, const long long* positions, int table_rows, const long long* first, const long long* starts, int rows, int H,
           cudaStream_t stream) {
   constexpr int HEADS = THREADS / (D / 16) / TOKENS;
-  CQ_CUDA_TRY(kv4_launch(pages_write_kernel<T, D>, dim3((rows + TOKENS - 1) / TOKENS, (H + 2 * pages->n_kv_heads + HEADS - 1) / HEADS), dim3(THREADS), 0, stream,
+  CQ_CUDA_TRY(kv4_launch(pages_write_kernel<T, D>, dim3((rows - 1) / TOKENS + 1, (H + 2 * pages->n_kv_heads + HEADS - 1) / HEADS), dim3(THREADS), 0, stream,
                          rows_of<T>(H ? q : nullptr), (T*)q_out, rows_of<T>(k), rows_of<T>(v), cos_t, sin_t, positions, table_rows, first, starts,
                          pool_of<T>(pages), table_of(table), table->sequences, rows, H));
   return CQ_OK;
@@ -110,7 +110,7 @@ int write(const cq_pages* pages, const cq_table* table, const cq_rows* q, void* 
 template <typename T, int D>
 int read(const cq_pages* pages, const cq_table* table, const long long* first, int count, void* k, void* v, cudaStream_t stream) {
   constexpr int HEADS = THREADS / (D / 8) / SLOTS;
-  CQ_CUDA_TRY(kv4_launch(pages_read_kernel<T, D>, dim3((count + SLOTS - 1) / SLOTS, (pages->n_kv_heads + HEADS - 1) / HEADS, table->sequences), dim3(THREADS), 0, stream,
+  CQ_CUDA_TRY(kv4_launch(pages_read_kernel<T, D>, dim3((count - 1) / SLOTS + 1, (pages->n_kv_heads + HEADS - 1) / HEADS, table->sequences), dim3(THREADS), 0, stream,
                          pool_of<T>(pages), table_of(table), first, count, (T*)k, (T*)v));
   return CQ_OK;
 }
