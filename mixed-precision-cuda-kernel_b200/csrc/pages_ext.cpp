@@ -81,7 +81,7 @@ struct KVPages {
   }
   cq_rows check_queries(const torch::Tensor& q, int64_t rows) const {
     const cq_rows r = check_rows(q, "q", rows, -1);
-    TORCH_CHECK(q.size(1) % c.n_kv_heads == 0, "the query heads must be a multiple of the ", c.n_kv_heads, " KV heads");
+    TORCH_CHECK(q.size(1) % c.n_kv_heads == 0 && q.size(1) <= INT32_MAX, "the query heads must be a multiple of the ", c.n_kv_heads, " KV heads");
     return r;
   }
   // the tables' rows; 0 without rotation

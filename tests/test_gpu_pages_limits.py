@@ -21,3 +21,13 @@ def test_as_many_rows_as_are_taken(qc):
     want = torch.zeros_like(cache.k)
     want[1, 0, 3:5] = row
     assert torch.equal(cache.k, want) and torch.equal(cache.v, -want)
+
+
+def test_more_heads_than_a_number_holds(qc):
+    cache = qc.KVPages.empty(2, 2, 16, 64)
+    table, one = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.long, device="cuda")
+    row = torch.zeros(1, 1, 64, dtype=torch.half, device="cuda")
+    for heads in (2 ** 31, 2 ** 32 + 2, 2 ** 17):
+        q = row.expand(1, heads, 64)
+        with pytest.raises(RuntimeError):
+            cache.write(q, row.expand(1, 2, 64), row.expand(1, 2, 64), table, one)
